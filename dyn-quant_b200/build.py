@@ -2,7 +2,7 @@
 
   dyn_quant/libdq_b200.so    the sm_100a kernels + the C ABI (include/dq_abi.h),
                              nvcc -gencode arch=compute_100a,code=sm_100a, static cudart
-  dyn_quant/_C.<abi>.so      the torch extension (csrc/torch_ext.cpp) over that ABI
+  dyn_quant/_C.<abi>.so      the torch extension (csrc/torch_ext.cpp, torch_kv.cpp) over that ABI
 
 usage: python dyn-quant_b200/build.py [--force]
 """
@@ -22,8 +22,9 @@ CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-LIB_SOURCES = ["dq_gemv.cu", "dq_stream.cu", "dq_batched.cu", "dq_moe.cu", "dq_abi.cu"]
-LIB_HEADERS = ["dq_common.cuh", "dq_internal.h", "dq_plan.cuh", "dq_gplan.cuh"]
+LIB_SOURCES = ["dq_gemv.cu", "dq_stream.cu", "dq_batched.cu", "dq_moe.cu", "dq_kv.cu", "dq_kv_attend.cu", "dq_abi.cu"]
+LIB_HEADERS = ["dq_common.cuh", "dq_internal.h", "dq_plan.cuh", "dq_gplan.cuh", "dq_kv.cuh"]
+EXT_SOURCES = ["torch_ext.cpp", "torch_kv.cpp"]
 LIB_PATH = os.path.join(PKG, "libdq_b200.so")
 EXT_SUFFIX = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
 EXT_PATH = os.path.join(PKG, "_C" + EXT_SUFFIX)
@@ -55,8 +56,8 @@ def build_ext(force: bool = False) -> str:
     import torch
     from torch.utils import cpp_extension as ce
 
-    src = os.path.join(CSRC, "torch_ext.cpp")
-    if not (force or _stale(EXT_PATH, [src, LIB_PATH, os.path.join(INCLUDE, "dq_abi.h"), __file__])):
+    srcs = [os.path.join(CSRC, s) for s in EXT_SOURCES]
+    if not (force or _stale(EXT_PATH, [*srcs, LIB_PATH, os.path.join(INCLUDE, "dq_abi.h"), __file__])):
         return EXT_PATH
     inc = ce.include_paths(device_type="cuda") if "device_type" in ce.include_paths.__code__.co_varnames \
         else ce.include_paths(cuda=True)
@@ -67,7 +68,7 @@ def build_ext(force: bool = False) -> str:
            f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
            f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}"]
     cmd += [f"-I{p}" for p in inc]
-    cmd += [src, "-o", EXT_PATH]
+    cmd += [*srcs, "-o", EXT_PATH]
     cmd += [f"-L{p}" for p in libdirs]
     cmd += [f"-L{PKG}", "-ldq_b200", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
             "-ltorch_python", "-Wl,-rpath,$ORIGIN"]

@@ -147,8 +147,11 @@ dq_status_t dq_read_device_error(uint32_t* word, int clear) {
     if (st != DQ_OK) return st;
     st = read_stream_error(&bs, clear != 0);
     if (st != DQ_OK) return st;
+    uint32_t kv = 0, ka = 0;
+    if ((st = read_kv_error(&kv, clear != 0)) != DQ_OK) return st;
+    if ((st = read_kv_attend_error(&ka, clear != 0)) != DQ_OK) return st;
     // streaming kernel: bit 0 of its word (its own copies) -> bit 5
-    *word = b1 | (bg << 8) | ((bs & 1u) ? (1u << 5) : 0u);
+    *word = b1 | (bg << 8) | ((bs & 1u) ? (1u << 5) : 0u) | (kv << 16) | (ka << 20);
     return DQ_OK;
 }
 
@@ -363,6 +366,110 @@ dq_status_t dq_detect_outliers(const uint16_t* x, int32_t d_in, float outlier_k,
     if (!aligned16(x)) return DQ_ERR_ALIGNMENT;
     return launch_detect(x, d_in, outlier_k, mask_words, indices, count, stats,
                          static_cast<cudaStream_t>(stream));
+}
+
+// ---------------------------------------------------------------------------
+// Paged 4-bit KV cache
+// ---------------------------------------------------------------------------
+static bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+// The sizes alone (what the workspace queries need).
+static dq_status_t check_kv_shape(const dq_kv_cache_t* c) {
+    if (!c) return DQ_ERR_INVALID_ARGUMENT;
+    if (c->n_seqs < 0 || c->n_pages < 0 || c->max_pages < 0 || c->page_size <= 0 || c->page_size % 16 != 0 ||
+        c->kv_heads <= 0)
+        return DQ_ERR_SHAPE;
+    if (c->head_dim != 64 && c->head_dim != 128) return DQ_ERR_UNSUPPORTED;
+    if (c->n_seqs > 2048 || c->kv_heads > 65535) return DQ_ERR_UNSUPPORTED;
+    // slots and positions are 32-bit
+    if (static_cast<long long>(c->max_pages) * c->page_size > (1ll << 30)) return DQ_ERR_UNSUPPORTED;
+    return DQ_OK;
+}
+
+static dq_status_t check_kv_cache(const dq_kv_cache_t* c) {
+    const dq_status_t st = check_kv_shape(c);
+    if (st != DQ_OK) return st;
+    if (c->n_seqs == 0) return DQ_OK;
+    if (!c->lengths || !c->evicted || !c->arrivals) return DQ_ERR_INVALID_ARGUMENT;
+    if (c->max_pages > 0 && !c->page_table) return DQ_ERR_INVALID_ARGUMENT;
+    if (c->n_pages > 0 && (!c->units || !c->mass || !c->pos)) return DQ_ERR_INVALID_ARGUMENT;
+    if (!aligned16(c->units) || !aligned4(c->mass) || !aligned4(c->pos) || !aligned4(c->lengths) ||
+        !aligned4(c->evicted) || !aligned4(c->page_table) || !aligned4(c->arrivals))
+        return DQ_ERR_ALIGNMENT;
+    return DQ_OK;
+}
+
+static bool strides_ok(const int64_t s[3]) {
+    for (int i = 0; i < 3; ++i)
+        if (s[i] < 0 || s[i] % 8 != 0) return false;
+    return true;
+}
+
+size_t dq_kv_unit_bytes(int32_t head_dim) {
+    return head_dim == 64 || head_dim == 128 ? static_cast<size_t>(16 * head_dim + 128) : 0;
+}
+
+dq_status_t dq_kv_append(const dq_kv_cache_t* cache, const uint16_t* k, const int64_t k_stride[3], const uint16_t* v,
+                         const int64_t v_stride[3], int32_t tokens, const int32_t* counts, const int32_t* at,
+                         uint16_t* k_values, uint16_t* v_values, void* stream) {
+    const dq_status_t st = check_kv_cache(cache);
+    if (st != DQ_OK) return st;
+    if (tokens < 0) return DQ_ERR_SHAPE;
+    if (cache->n_seqs == 0 || tokens == 0) return DQ_OK;
+    if (!k || !v || !k_stride || !v_stride || (k_values == nullptr) != (v_values == nullptr))
+        return DQ_ERR_INVALID_ARGUMENT;
+    if (!strides_ok(k_stride) || !strides_ok(v_stride)) return DQ_ERR_ALIGNMENT;
+    if (!aligned16(k) || !aligned16(v) || !aligned16(k_values) || !aligned16(v_values) || !aligned4(counts) ||
+        !aligned4(at))
+        return DQ_ERR_ALIGNMENT;
+    return launch_kv_append(*cache, k, k_stride, v, v_stride, tokens, counts, at, k_values, v_values,
+                            static_cast<cudaStream_t>(stream));
+}
+
+static dq_status_t check_kv_rows(const dq_kv_cache_t* c, int32_t tokens, int32_t q_heads) {
+    if (tokens < 0 || q_heads <= 0 || q_heads % c->kv_heads != 0) return DQ_ERR_SHAPE;
+    if (static_cast<long long>(tokens) * q_heads > (1ll << 28)) return DQ_ERR_UNSUPPORTED;
+    return DQ_OK;
+}
+
+size_t dq_kv_attend_workspace_bytes(const dq_kv_cache_t* cache, int32_t tokens, int32_t q_heads, int32_t accumulate) {
+    if (check_kv_shape(cache) != DQ_OK || check_kv_rows(cache, tokens, q_heads) != DQ_OK) return 0;
+    return kv_attend_workspace(*cache, tokens, q_heads, accumulate != 0);
+}
+
+dq_status_t dq_kv_attend(const dq_kv_cache_t* cache, const dq_kv_attend_t* r, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+    if (!r) return DQ_ERR_INVALID_ARGUMENT;
+    dq_status_t st = check_kv_cache(cache);
+    if (st != DQ_OK) return st;
+    if ((st = check_kv_rows(cache, r->tokens, r->q_heads)) != DQ_OK) return st;
+    if (cache->n_seqs == 0 || r->tokens == 0) return DQ_OK;
+    if (!r->q || !r->out) return DQ_ERR_INVALID_ARGUMENT;
+    if (!(r->scale == r->scale) || r->scale - r->scale != 0.f) return DQ_ERR_INVALID_ARGUMENT;  // NaN, infinity
+    if (!strides_ok(r->q_stride) || !strides_ok(r->out_stride)) return DQ_ERR_ALIGNMENT;
+    if (!aligned16(r->q) || !aligned16(r->out) || !aligned4(r->lse) || !aligned4(r->counts)) return DQ_ERR_ALIGNMENT;
+    if (!workspace || workspace_bytes < kv_attend_workspace(*cache, r->tokens, r->q_heads, r->accumulate != 0))
+        return DQ_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return DQ_ERR_ALIGNMENT;
+    return launch_kv_attend(*cache, *r, workspace, static_cast<cudaStream_t>(stream));
+}
+
+size_t dq_kv_evict_workspace_bytes(const dq_kv_cache_t* cache, int32_t keep) {
+    if (check_kv_shape(cache) != DQ_OK || keep < 1) return 0;
+    return kv_evict_workspace(*cache, keep);
+}
+
+dq_status_t dq_kv_evict(const dq_kv_cache_t* cache, int32_t keep, int32_t recent, int32_t sink, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+    const dq_status_t st = check_kv_cache(cache);
+    if (st != DQ_OK) return st;
+    if (keep < 1 || recent < 0 || sink < 0 || static_cast<long long>(recent) + sink > keep) return DQ_ERR_INVALID_ARGUMENT;
+    if (cache->n_seqs == 0) return DQ_OK;
+    const size_t need = kv_evict_workspace(*cache, keep);
+    if (need == 0) return DQ_OK;  // no sequence can have more than keep slots
+    if (!workspace || workspace_bytes < need) return DQ_ERR_WORKSPACE;
+    if (!aligned4(workspace)) return DQ_ERR_ALIGNMENT;
+    return launch_kv_evict(*cache, keep, recent, sink, workspace, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

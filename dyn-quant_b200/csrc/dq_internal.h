@@ -403,6 +403,18 @@ dq_status_t launch_silu_mul(const uint16_t* a, const uint16_t* b, uint16_t* h, l
 dq_status_t launch_combine(const uint16_t* y, const int32_t* rows, const float* weight, float* out, int m, int d,
                            cudaStream_t stream);
 
+// Paged 4-bit KV cache (dq_kv.cu, dq_kv_attend.cu); arguments validated by the C ABI layer.
+dq_status_t launch_kv_append(const dq_kv_cache_t& c, const uint16_t* k, const int64_t ks[3], const uint16_t* v,
+                             const int64_t vs[3], int tokens, const int32_t* counts, const int32_t* at,
+                             uint16_t* k_values, uint16_t* v_values, cudaStream_t stream);
+size_t kv_attend_workspace(const dq_kv_cache_t& c, int tokens, int q_heads, bool mass);
+dq_status_t launch_kv_attend(const dq_kv_cache_t& c, const dq_kv_attend_t& r, void* workspace, cudaStream_t stream);
+size_t kv_evict_workspace(const dq_kv_cache_t& c, int keep);
+dq_status_t launch_kv_evict(const dq_kv_cache_t& c, int keep, int recent, int sink, void* workspace,
+                            cudaStream_t stream);
+dq_status_t read_kv_error(uint32_t* word, bool clear);
+dq_status_t read_kv_attend_error(uint32_t* word, bool clear);
+
 // Largest d_in the single-pass kernels accept (x, its B fragments and the
 // outlier list live in shared memory next to the weight rings).
 constexpr int kMaxDIn = 30720;

@@ -2,7 +2,7 @@
 // bindings (csrc/bindings.cpp:184-193 of dyn-quant) with the same names,
 // argument meaning and RuntimeError behaviour, implemented over the C ABI of
 // libdq_b200.so.  Extra functions: build_colmajor, build_native, detect_outliers,
-// split_gemv_batched.
+// split_gemv_batched; the KV cache (torch_kv.cpp).
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -346,7 +346,10 @@ private:
 
 }  // namespace
 
+void bind_kv(py::module_& m);  // torch_kv.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    bind_kv(m);
     py::class_<SplitLinear>(m, "SplitLinear")
         .def(py::init<const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, const torch::Tensor&,
                       const torch::Tensor&, double>(),

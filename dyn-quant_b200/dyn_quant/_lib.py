@@ -54,6 +54,12 @@ EXPORTED_SYMBOLS = (
     "dq_ipc_handle",
     "dq_ipc_open",
     "dq_ipc_close",
+    "dq_kv_unit_bytes",
+    "dq_kv_append",
+    "dq_kv_attend_workspace_bytes",
+    "dq_kv_attend",
+    "dq_kv_evict_workspace_bytes",
+    "dq_kv_evict",
 )
 
 MAX_GATHER_RANKS = 8  # DQ_MAX_GATHER_RANKS
@@ -85,6 +91,43 @@ class DqGather(C.Structure):
         ("rows_per", C.c_int32),
         ("d_total", C.c_int32),
         ("region", C.c_void_p * MAX_GATHER_RANKS),
+    ]
+
+
+class DqKvCache(C.Structure):
+    """dq_kv_cache_t (include/dq_abi.h)."""
+
+    _fields_ = [
+        ("units", C.c_void_p),
+        ("mass", C.c_void_p),
+        ("pos", C.c_void_p),
+        ("lengths", C.c_void_p),
+        ("evicted", C.c_void_p),
+        ("page_table", C.c_void_p),
+        ("arrivals", C.c_void_p),
+        ("n_seqs", C.c_int32),
+        ("n_pages", C.c_int32),
+        ("max_pages", C.c_int32),
+        ("page_size", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+    ]
+
+
+class DqKvAttend(C.Structure):
+    """dq_kv_attend_t (include/dq_abi.h)."""
+
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("q_stride", C.c_int64 * 3),
+        ("out", C.c_void_p),
+        ("out_stride", C.c_int64 * 3),
+        ("lse", C.c_void_p),
+        ("counts", C.c_void_p),
+        ("tokens", C.c_int32),
+        ("q_heads", C.c_int32),
+        ("scale", C.c_float),
+        ("accumulate", C.c_int32),
     ]
 
 
@@ -171,6 +214,19 @@ def lib() -> C.CDLL:
         L.dq_ipc_open.argtypes = [C.c_char_p, C.POINTER(C.c_void_p)]
         L.dq_ipc_close.restype = st
         L.dq_ipc_close.argtypes = [P]
+        kv, i64x3 = C.POINTER(DqKvCache), C.POINTER(C.c_int64)
+        L.dq_kv_unit_bytes.restype = C.c_size_t
+        L.dq_kv_unit_bytes.argtypes = [i32]
+        L.dq_kv_append.restype = st
+        L.dq_kv_append.argtypes = [kv, P, i64x3, P, i64x3, i32, P, P, P, P, P]
+        L.dq_kv_attend_workspace_bytes.restype = C.c_size_t
+        L.dq_kv_attend_workspace_bytes.argtypes = [kv, i32, i32, i32]
+        L.dq_kv_attend.restype = st
+        L.dq_kv_attend.argtypes = [kv, C.POINTER(DqKvAttend), P, C.c_size_t, P]
+        L.dq_kv_evict_workspace_bytes.restype = C.c_size_t
+        L.dq_kv_evict_workspace_bytes.argtypes = [kv, i32]
+        L.dq_kv_evict.restype = st
+        L.dq_kv_evict.argtypes = [kv, i32, i32, i32, P, C.c_size_t, P]
         _lib = L
     return _lib
 

@@ -375,10 +375,118 @@ DQ_API dq_status_t dq_ipc_close(void* ptr);
  * bounded wait for another rank's rows gave up, bit 5 by the streaming kernel
  * (DQ_STREAM=1) whose bounded wait for its own bulk copies gave up (it
  * carries on; its output is not valid), bit 8 by a batched kernel
- * whose bounded wait for its own bulk copies gave up.  Synchronous; clear != 0
- * resets the word.  No reference counterpart.
+ * whose bounded wait for its own bulk copies gave up.  KV cache calls: bits
+ * 16 .. 18 (append, evict) and 20 .. 22 (attend), in this order a page index
+ * outside the pool, a length or count outside the sequence's pages, a bounded
+ * wait for the kernel's own copies that gave up (the attention's output is not
+ * valid then).  Synchronous; clear != 0 resets the word.  No reference
+ * counterpart.
  */
 DQ_API dq_status_t dq_read_device_error(uint32_t* word, int clear);
+
+/*
+ * Paged 4-bit KV cache of one attention layer.  No counterpart in the reference
+ * (its scope is the linear layers); rows are kept in its INT4 format
+ * (src/quant_format.cuh:12-97), one group per row of head_dim values.
+ *
+ * Sequence b's token slots 0 .. lengths[b] - 1 lie in the pages
+ * page_table[b][0], page_table[b][1], ..., page_size slots each.  16
+ * consecutive slots of one KV head are one unit of dq_kv_unit_bytes bytes:
+ *   K      16 rows of head_dim/2 bytes, as dq_quantize packs a row
+ *   V      [8 slot pairs][head_dim/4][2] uint16: the four codes of columns
+ *          4q .. 4q + 3 (lowest bits first) of the pair's even and odd slot
+ *   params [16][4] f16: K scale, K zero, V scale, V zero
+ * mass is the attention weight a slot has received (dq_kv_attend with
+ * accumulate), pos the position at which its token was appended; both move with
+ * the slot when dq_kv_evict moves it.  A page that two sequences share may be
+ * read by dq_kv_attend; append, accumulate and evict need it to be owned by one.
+ * Calls on one cache must be stream-ordered (each reads and writes lengths).
+ */
+typedef struct dq_kv_cache_t {
+    uint8_t* units;            /* [n_pages][kv_heads][page_size / 16][dq_kv_unit_bytes], 16-byte aligned */
+    float* mass;               /* [n_pages][kv_heads][page_size] */
+    int32_t* pos;              /* [n_pages][kv_heads][page_size] */
+    int32_t* lengths;          /* [n_seqs] slots in use */
+    int32_t* evicted;          /* [n_seqs] tokens evicted so far (positions seen = lengths + evicted) */
+    const int32_t* page_table; /* [n_seqs][max_pages]; entries past a sequence's last page are not read */
+    uint32_t* arrivals;        /* [n_seqs] zero-filled once; every call leaves it at zero */
+    int32_t n_seqs;            /* 1 .. 2048 */
+    int32_t n_pages;
+    int32_t max_pages;
+    int32_t page_size;         /* a multiple of 16 */
+    int32_t kv_heads;
+    int32_t head_dim;          /* 64 or 128 */
+} dq_kv_cache_t;
+
+/* Bytes of one unit: 16 head_dim + 128 (0 for an unsupported head_dim). */
+DQ_API size_t dq_kv_unit_bytes(int32_t head_dim);
+
+/*
+ * Quantize new keys and values into the cache: for every sequence b the tokens
+ * k[b][i], v[b][i], i < counts[b] (counts NULL: all `tokens`), go to slots
+ * at[b] + i (at NULL: lengths[b] + i), mass 0, pos evicted[b] + slot, and
+ * lengths[b] becomes at[b] + counts[b].  at below lengths rewinds the sequence
+ * (drafted tokens that were rejected); it must not reach below what an eviction
+ * has rearranged.  Bytes and scales are those of dq_quantize for rows of 128.
+ * k, v: f16, 16-byte aligned, head_dim values contiguous, strides (sequence,
+ * token, head) in values, multiples of 8.  k_values, v_values: both NULL, or
+ * f16 [n_seqs][tokens][kv_heads][head_dim], which receive the values that the
+ * cache now holds, scale * (code - zero) rounded to f16, zero for i >= counts[b].
+ * A start outside the pages leaves the sequence as it is, tokens past its last
+ * page are dropped, a page index outside the pool drops its tokens; each sets a
+ * bit of the device error word.  One kernel.
+ */
+DQ_API dq_status_t dq_kv_append(const dq_kv_cache_t* cache, const uint16_t* k, const int64_t k_stride[3],
+                                const uint16_t* v, const int64_t v_stride[3], int32_t tokens,
+                                const int32_t* counts, const int32_t* at, uint16_t* k_values,
+                                uint16_t* v_values, void* stream);
+
+/* Arguments of dq_kv_attend.  Strides (sequence, token, head) in values, multiples of 8. */
+typedef struct dq_kv_attend_t {
+    const uint16_t* q;      /* f16 [n_seqs][tokens][q_heads][head_dim], head_dim contiguous, 16-byte aligned */
+    int64_t q_stride[3];
+    uint16_t* out;          /* f16, q's shape, 16-byte aligned */
+    int64_t out_stride[3];
+    float* lse;             /* [n_seqs][tokens][q_heads] natural log of the softmax's sum, or NULL */
+    const int32_t* counts;  /* [n_seqs] query tokens of each sequence, or NULL: all of them */
+    int32_t tokens;
+    int32_t q_heads;        /* a multiple of kv_heads; query heads g h .. g h + g - 1 read KV head h */
+    float scale;            /* of the scores, e.g. 1 / sqrt(head_dim) */
+    int32_t accumulate;     /* != 0: add each slot's weight, summed over query tokens and heads, to mass */
+} dq_kv_attend_t;
+
+/* Workspace of dq_kv_attend (16-byte aligned scratch, no initial contents); 0 on invalid arguments. */
+DQ_API size_t dq_kv_attend_workspace_bytes(const dq_kv_cache_t* cache, int32_t tokens, int32_t q_heads,
+                                           int32_t accumulate);
+
+/*
+ * Attention of the newest tokens over the cache: the counts[b] query tokens of
+ * sequence b are its last slots (append them first), query i sees slots
+ * 0 .. lengths[b] - counts[b] + i.  out = softmax(scale q K^T) V; scores, the
+ * softmax's maximum and sum and the output are FP32, the weights times the V
+ * scales are rounded to f16 for the product.  Rows without keys (an empty
+ * sequence, i >= counts[b]) give out 0 and lse -infinity.  Units of a page
+ * index outside the pool count as absent and set a bit of the device error
+ * word.  Slots behind lengths[b] are not read into any result.  Results are
+ * bit-reproducible.  Two kernels, three with accumulate.
+ */
+DQ_API dq_status_t dq_kv_attend(const dq_kv_cache_t* cache, const dq_kv_attend_t* args, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
+/* Workspace of dq_kv_evict (4-byte aligned scratch, no initial contents). */
+DQ_API size_t dq_kv_evict_workspace_bytes(const dq_kv_cache_t* cache, int32_t keep);
+
+/*
+ * Cut every sequence with more than `keep` slots to `keep`, head by head: the
+ * slots of the last `recent` positions and of the first `sink` positions stay
+ * (recent + sink <= keep), of the others those with the largest mass, equal
+ * ones lowest slot first.  Survivors below slot `keep` stay where they are; the
+ * k-th survivor beyond moves into the k-th freed slot below, with its mass and
+ * position.  evicted[b] grows by what lengths[b] loses; slots from `keep` on are
+ * left as they were.  Attention does not depend on the order of slots.  One kernel.
+ */
+DQ_API dq_status_t dq_kv_evict(const dq_kv_cache_t* cache, int32_t keep, int32_t recent, int32_t sink,
+                               void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
