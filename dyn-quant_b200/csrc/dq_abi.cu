@@ -380,9 +380,11 @@ static dq_status_t check_kv_shape(const dq_kv_cache_t* c) {
         c->kv_heads <= 0)
         return DQ_ERR_SHAPE;
     if (c->head_dim != 64 && c->head_dim != 128) return DQ_ERR_UNSUPPORTED;
-    if (c->n_seqs > 2048 || c->kv_heads > 65535) return DQ_ERR_UNSUPPORTED;
-    // slots and positions are 32-bit
-    if (static_cast<long long>(c->max_pages) * c->page_size > (1ll << 30)) return DQ_ERR_UNSUPPORTED;
+    if (c->n_seqs > kKvMaxSeqs || c->kv_heads > 65535 || c->page_size > (1 << 20)) return DQ_ERR_UNSUPPORTED;
+    // slots, positions, a sequence's steps and the pool's units are counted in 32 bits
+    const long long cap = static_cast<long long>(c->max_pages) * c->page_size;
+    if (cap > (1ll << 30) || cap * (c->n_seqs > 0 ? c->n_seqs : 1) > (1ll << 35)) return DQ_ERR_UNSUPPORTED;
+    if (static_cast<double>(c->n_pages) * c->kv_heads * (c->page_size / 16) > 2147483647.0) return DQ_ERR_UNSUPPORTED;
     return DQ_OK;
 }
 

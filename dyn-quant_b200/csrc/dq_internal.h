@@ -404,6 +404,7 @@ dq_status_t launch_combine(const uint16_t* y, const int32_t* rows, const float* 
                            cudaStream_t stream);
 
 // Paged 4-bit KV cache (dq_kv.cu, dq_kv_attend.cu); arguments validated by the C ABI layer.
+constexpr int kKvMaxSeqs = 1024;  // sequences of one cache (the attention's plan lives in shared memory)
 dq_status_t launch_kv_append(const dq_kv_cache_t& c, const uint16_t* k, const int64_t ks[3], const uint16_t* v,
                              const int64_t vs[3], int tokens, const int32_t* counts, const int32_t* at,
                              uint16_t* k_values, uint16_t* v_values, cudaStream_t stream);

@@ -18,7 +18,6 @@
 namespace dq {
 
 constexpr int kKvTokens = 16;       // slots of one unit
-constexpr int kKvMaxSeqs = 2048;    // sequences of one cache (their unit prefix sums live in shared memory)
 constexpr uint32_t kKvErrPage = 1u; // a page index outside the pool
 constexpr uint32_t kKvErrLen = 2u;  // a length or count outside the sequence's pages
 constexpr uint32_t kKvErrWait = 4u; // a bounded wait for the kernel's own copies gave up

@@ -6,13 +6,15 @@
 // One pass over the cache with the running maximum and sum of the softmax.
 // Rows r = (query token, query head of the KV head) share the KV head's units.
 //
-// Work split: the units of all (sequence, KV head, row tile) jobs form one
-// list, cut into equal runs, one per warp of a persistent grid, so ragged
-// lengths, few sequences and long ones all fill the GPU.  Each warp streams
-// its run through a ring of bulk copies of its own; job borders do not
-// interrupt the stream.  A job inside one run is finished there; the others
-// leave their partial sums (maximum, sum, unnormalised output) in the
-// workspace, which kv_combine_kernel joins in warp order.
+// Work split: the steps (32 slots, two units) of all (sequence, KV head, row
+// tile) jobs form one list, cut into equal runs, one per warp of a persistent
+// grid, so ragged lengths, few sequences and long ones all fill the GPU.  Each
+// warp streams its run through a ring of bulk copies of its own; job borders do
+// not interrupt the stream.  A job inside one run is finished there.  The pieces
+// of the others meet in shared memory when their CTA's warps (neighbouring
+// runs) are done, and what a CTA's border still cuts leaves its partial sums
+// (maximum, sum, unnormalised output) in the workspace for kv_combine_kernel.
+// All sums have a fixed order.
 //
 // Products (mma.sync.m16n8k16, f16 x f16 -> f32) are transposed, so that the 16
 // slots of a unit are the MMA's rows and the query rows its 8 columns:
@@ -21,8 +23,10 @@
 // A decode step has at most 8 rows per KV head, so nothing of an MMA is idle,
 // and a lane's S values (slots g, g + 8; rows 2t, 2t + 1) lie in the lanes that
 // hold its O columns' rows: maxima, sums and rescaling stay in the lane.
-// Codes become f16 integers c - 8 exactly: (bits 4..7 | 0x5400) is 64 + c, one
-// f16x2 subtraction takes 72.  Scales and zeros are applied in FP32:
+// Codes become f16 integers c - 8 exactly: (bits 0..3 | 0x6400) is 1024 + c and
+// (bits 4..7 | 0x5400) is 64 + c, one f16x2 subtraction takes 1032 or 72; a word
+// of eight codes costs one shift, four lop3 and four subtractions.  Scales and
+// zeros are applied in FP32:
 //   S   = s_k (D - (z_k - 8) sum q),  D the MMA's sum of q (c - 8)
 //   O   = sum p' (c - 8) - sum p' (z_v - 8),  p' = p s_v w
 // p' is the only rounding to FP16 besides the output's: p <= 2^8 (the maximum
@@ -37,10 +41,15 @@ namespace {
 
 __device__ unsigned int g_kv_attend_error;
 
-constexpr int kAtWarps = 4;           // warps per CTA
 constexpr int kAtMaxWarps = 2560;     // bound on the grid's warps (workspace sizing)
 constexpr float kNone = -1e30f;       // running maximum of a row that has seen no key
 constexpr float kLazy = 8.0f;         // a score passes the running maximum by this much (log2) before it moves
+constexpr int kStep = 2 * kKvTokens;  // slots of one step of a run
+
+// Warps of a CTA and CTAs of an SM for row tiles of 8 NT rows: two row tiles
+// need 168 registers a thread, one tile 128.
+__host__ __device__ constexpr int at_warps(int nt) { return nt == 1 ? 8 : 12; }
+__host__ __device__ constexpr int at_ctas(int nt) { return nt == 1 ? 2 : 1; }
 
 struct KvAttendArgs {
     KvView c;
@@ -50,62 +59,66 @@ struct KvAttendArgs {
     float* lse;              // [n_seqs][tokens][q_heads] natural log, or null
     float* lse2;             // workspace: the same in log2 (mass pass), or null
     const int32_t* counts;
-    float* part;             // [warps][2][rows][D]
-    float* part_ml;          // [warps][2][rows][2]
+    float* part;             // [CTAs][2][rows][D]
+    float* part_ml;          // [CTAs][2][rows][2]
+    int* pre;                // [n_seqs + 1] the plan's prefix sums, for the combining kernel
     int tokens, group, n_rt; // query tokens, query heads per KV head, row tiles
     float scale2;            // scale * log2(e)
     int depth;               // ring slots per warp
 };
 
-// The list of units: pre[b] = units of the sequences before b, a job being
-// ulen[b] units of one (sequence, KV head, row tile).
+// The list of steps: a job is steps_of(len[b]) steps of one (sequence, KV head,
+// row tile), a sequence has `jobs` of them one after another, pre[b] counts the
+// steps of one job of every sequence before b.  Warp w takes base steps, one
+// more if w < rem.
 struct Plan {
-    const long long* pre;
+    const int* pre;
     const int* len;
-    long long total;
-    long long base;  // units per warp; the first rem warps take one more
+    int jobs;
+    long long base;
     int rem;
-    int jobs;        // per sequence
 };
 
-// Bytes of the plan in shared memory.
-__host__ __device__ inline int plan_bytes(int n_seqs) { return ((n_seqs + 1) * 8 + n_seqs * 4 + 127) / 128 * 128; }
+__host__ __device__ inline int steps_of(int len) { return (len + kStep - 1) / kStep; }
 
-__device__ __forceinline__ long long warp_start(const Plan& p, long long w) {
-    return w * p.base + (w < p.rem ? w : p.rem);
+// Bytes of the plan in shared memory.
+__host__ __device__ inline int plan_bytes(int n_seqs) { return ((2 * n_seqs + 1) * 4 + 127) / 128 * 128; }
+
+__device__ __forceinline__ long long warp_start(long long base, int rem, long long w) {
+    return w * base + (w < rem ? w : rem);
 }
-__device__ __forceinline__ long long warp_of(const Plan& p, long long u) {
-    const long long cut = p.rem * (p.base + 1);
-    return u < cut ? u / (p.base + 1) : p.rem + (u - cut) / p.base;
+__device__ __forceinline__ long long warp_of(long long base, int rem, long long u) {
+    const long long cut = rem * (base + 1);
+    return u < cut ? u / (base + 1) : rem + (u - cut) / base;
 }
 
 // Built by every CTA from the lengths (a few KB from L2); all threads call it.
 template <int NT>
 __device__ Plan make_plan(const KvView& c, int jobs, int warps, char* smem, unsigned int* err) {
-    long long* pre = reinterpret_cast<long long*>(smem);
-    int* lens = reinterpret_cast<int*>(smem + (c.n_seqs + 1) * 8);
-    __shared__ long long wtot[NT / 32];
+    int* pre = reinterpret_cast<int*>(smem);
+    int* lens = pre + c.n_seqs + 1;
+    __shared__ int wtot[NT / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    long long run = 0;
+    int run = 0;
     for (int b0 = 0; b0 < c.n_seqs; b0 += NT) {
         const int b = b0 + tid;
-        long long v = 0;
+        int v = 0;
         if (b < c.n_seqs) {
             bool bad = false;
             const int n = kv_length(c, b, &bad);
             if (bad && err) atomicOr(err, kKvErrLen);
             lens[b] = n;
-            v = static_cast<long long>((n + kKvTokens - 1) / kKvTokens) * jobs;
+            v = steps_of(n);
         }
-        long long inc = v;
+        int inc = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long t = __shfl_up_sync(0xffffffffu, inc, o);
+            const int t = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += t;
         }
         if (lane == 31) wtot[warp] = inc;
         __syncthreads();
-        long long before = run;
+        int before = run;
         for (int w = 0; w < NT / 32; ++w) {
             if (w < warp) before += wtot[w];
             run += wtot[w];
@@ -118,26 +131,41 @@ __device__ Plan make_plan(const KvView& c, int jobs, int warps, char* smem, unsi
     Plan p;
     p.pre = pre;
     p.len = lens;
-    p.total = run;
-    p.base = run / warps;
-    p.rem = static_cast<int>(run - p.base * warps);
     p.jobs = jobs;
+    const long long total = static_cast<long long>(run) * jobs;
+    p.base = total / warps;
+    p.rem = static_cast<int>(total - p.base * warps);
     return p;
 }
 
-// The sequence of unit u (u < total): the last b with pre[b] <= u that has units.
-__device__ __forceinline__ int seq_of(const Plan& p, int n_seqs, long long u) {
-    int lo = 0, hi = n_seqs;  // pre[lo] <= u < pre[hi]
+// Where a step lies: sequence, its length, job and step of the job.
+struct StepAt {
+    int b, len, job, step;
+};
+
+__device__ __forceinline__ StepAt step_at(const Plan& p, int n_seqs, long long u) {
+    const int v = static_cast<int>(u / p.jobs);  // pre[b] <= v < pre[b + 1]: the last b with pre[b] <= v
+    int lo = 0, hi = n_seqs;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (p.pre[mid] <= u) lo = mid;
+        if (p.pre[mid] <= v) lo = mid;
         else hi = mid;
     }
-    return lo;
+    const int st = p.pre[lo + 1] - p.pre[lo];
+    const long long r = u - static_cast<long long>(p.pre[lo]) * p.jobs;
+    StepAt a;
+    a.b = lo;
+    a.len = p.len[lo];
+    a.job = static_cast<int>(r / st);
+    a.step = static_cast<int>(r - static_cast<long long>(a.job) * st);
+    return a;
 }
 
-// f16 pairs (c - 8) of the nibbles at bits 4..7 and 20..23.
-__device__ __forceinline__ uint32_t centred(uint32_t w) {
+// f16 pairs (c - 8) of the nibbles at bits 0..3 and 16..19, and at bits 4..7 and 20..23.
+__device__ __forceinline__ uint32_t low_codes(uint32_t w) {
+    return hsub2_u32(lop3_and_or(w, 0x000F000Fu, 0x64006400u), 0x64086408u);  // (1024 + c) - 1032
+}
+__device__ __forceinline__ uint32_t high_codes(uint32_t w) {
     return hsub2_u32(lop3_and_or(w, 0x00F000F0u, 0x54005400u), 0x54805480u);  // (64 + c) - 72
 }
 
@@ -169,6 +197,19 @@ __device__ __forceinline__ float lane_sum_g(float v) {
 #pragma unroll
     for (int o = 4; o <= 16; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
+}
+
+// 1 / sum of a row's weights; 0 where it has seen no key, not a number where the sum is not.
+__device__ __forceinline__ float row_norm(float sum) {
+    return sum > 0.f ? __fdiv_rn(1.f, sum) : (sum == 0.f ? 0.f : sum);
+}
+
+// lse of a row, in log2 and natural.
+__device__ __forceinline__ void store_lse(const KvAttendArgs& a, int b, int tok, int head, float m, float sum) {
+    const size_t i = (static_cast<size_t>(b) * a.tokens + tok) * (a.c.heads * a.group) + head;
+    const float l2 = sum == 0.f ? -INFINITY : m + log2f(sum);
+    if (a.lse) a.lse[i] = l2 * 0.693147180559945309f;
+    if (a.lse2) a.lse2[i] = l2;
 }
 
 // B fragments of 8 NT query rows and what the scores need of them.
@@ -223,86 +264,114 @@ struct QueryTile {
     }
 };
 
-// D of one unit: the MMA's sum of q (c - 8) for slots g, g + 8 and rows 2t, 2t + 1.
-template <int D, int NT>
-__device__ __forceinline__ void score_mma(uint32_t unit, const QueryTile<D, NT>& q, float (&s)[NT][4]) {
+// D of U units: the MMA's sums of q (c - 8) for slots g, g + 8 and rows 2t, 2t + 1.
+template <int D, int NT, int U>
+__device__ __forceinline__ void score_mma(uint32_t unit, const QueryTile<D, NT>& q, float (&s)[U][NT][4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    uint32_t k0[D / 32], k1[D / 32];
-    if (D == 128) {
-        const uint4 x = lds_v4(unit + g * 64 + t * 16), y = lds_v4(unit + (g + 8) * 64 + t * 16);
-        k0[0] = x.x; k0[1] = x.y; k0[D / 32 - 2] = x.z; k0[D / 32 - 1] = x.w;
-        k1[0] = y.x; k1[1] = y.y; k1[D / 32 - 2] = y.z; k1[D / 32 - 1] = y.w;
-    } else {
-        const uint2 x = lds_v2(unit + g * 32 + t * 8), y = lds_v2(unit + (g + 8) * 32 + t * 8);
-        k0[0] = x.x; k0[1] = x.y;
-        k1[0] = y.x; k1[1] = y.y;
-    }
+    uint32_t k0[U][D / 32], k1[U][D / 32];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-        const uint32_t a0 = centred(k0[i] << 4), a1 = centred(k1[i] << 4), a2 = centred(k0[i]), a3 = centred(k1[i]);
-        const uint32_t b0 = centred(k0[i] >> 4), b1 = centred(k1[i] >> 4), b2 = centred(k0[i] >> 8), b3 = centred(k1[i] >> 8);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            mma_16816(s[nt], a0, a1, a2, a3, q.f[nt][4 * i], q.f[nt][4 * i + 1]);
-            mma_16816(s[nt], b0, b1, b2, b3, q.f[nt][4 * i + 2], q.f[nt][4 * i + 3]);
+    for (int u = 0; u < U; ++u) {
+        const uint32_t at = unit + u * kv_unit_bytes(D) + g * (D / 2) + t * (D / 8);
+        if (D == 128) {
+            const uint4 x = lds_v4(at), y = lds_v4(at + 8 * (D / 2));
+            k0[u][0] = x.x; k0[u][1] = x.y; k0[u][D / 32 - 2] = x.z; k0[u][D / 32 - 1] = x.w;
+            k1[u][0] = y.x; k1[u][1] = y.y; k1[u][D / 32 - 2] = y.z; k1[u][D / 32 - 1] = y.w;
+        } else {
+            const uint2 x = lds_v2(at), y = lds_v2(at + 8 * (D / 2));
+            k0[u][0] = x.x; k0[u][1] = x.y;
+            k1[u][0] = y.x; k1[u][1] = y.y;
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[u][nt][e] = 0.f;
     }
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t w0 = k0[u][i], w1 = k1[u][i], x0 = w0 >> 8, x1 = w1 >> 8;
+            const uint32_t a0 = low_codes(w0), a1 = low_codes(w1), a2 = high_codes(w0), a3 = high_codes(w1);
+            const uint32_t b0 = low_codes(x0), b1 = low_codes(x1), b2 = high_codes(x0), b3 = high_codes(x1);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                mma_16816(s[u][nt], a0, a1, a2, a3, q.f[nt][4 * i], q.f[nt][4 * i + 1]);
+                mma_16816(s[u][nt], b0, b1, b2, b3, q.f[nt][4 * i + 2], q.f[nt][4 * i + 3]);
+            }
+        }
 }
 
-// A warp's run of units through its ring: lane u % 32 of each 32 units looks
-// the unit's page up and issues its copies.
+// A warp's run of steps through its ring: lane i % 32 of each 32 steps looks
+// the step's pages up and issues its copies.
 template <int D, bool kKeysOnly>
-struct UnitStream {
-    uint32_t ring, bars, flags;  // shared-memory addresses of this warp's slots, barriers, page-found words
+struct StepStream {
+    static constexpr int kUnit = kv_unit_bytes(D);
+    static constexpr int kSlot = 2 * kUnit;
+    uint32_t ring, bars, flags;  // shared-memory addresses of this warp's slots, barriers, units-found words
     int depth, n, issued, parity, slot;
+    bool absent;                 // some unit of the run lies in no page of the pool
     long long u0;
-    const uint8_t* src;
-    bool ok;
+    int src[2];                  // this lane's step: the units' indices in the pool, -1: none
 
-    __device__ __forceinline__ void init(char* smem, int warp, int depth_) {
+    // Bytes of `warps` rings behind `smem`.
+    static __host__ __device__ int bytes(int warps, int depth) { return (warps * depth * (kSlot + 12) + 127) / 128 * 128; }
+
+    __device__ __forceinline__ void init(char* smem, int warps, int warp, int depth_) {
         depth = depth_;
-        ring = smem_u32(smem) + warp * depth * kv_unit_bytes(D);
-        bars = smem_u32(smem) + kAtWarps * depth * kv_unit_bytes(D) + warp * depth * 8;
-        flags = smem_u32(smem) + kAtWarps * depth * (kv_unit_bytes(D) + 8) + warp * depth * 4;
+        ring = smem_u32(smem) + warp * depth * kSlot;
+        bars = smem_u32(smem) + warps * depth * kSlot + warp * depth * 8;
+        flags = smem_u32(smem) + warps * depth * (kSlot + 8) + warp * depth * 4;
         if ((threadIdx.x & 31) == 0)
             for (int i = 0; i < depth; ++i) mbar_init(bars + 8 * i, 1);
         fence_mbar_init();
         __syncwarp();
     }
     __device__ __forceinline__ void lookup(const KvAttendArgs& a, const Plan& p) {
-        src = nullptr;
+        src[0] = src[1] = -1;
+        bool bad = false;
         const int i = issued + (threadIdx.x & 31);
         if (i < n) {
-            const long long u = u0 + i;
-            const int b = seq_of(p, a.c.n_seqs, u);
-            const int ul = (p.len[b] + kKvTokens - 1) / kKvTokens;
-            const long long r = u - p.pre[b];
-            const int job = static_cast<int>(r / ul), ub = static_cast<int>(r - static_cast<long long>(job) * ul);
-            const int h = kKeysOnly ? job : job / a.n_rt;
-            const int page = kv_page(a.c, b, ub * kKvTokens);
-            if (page >= 0) src = kv_unit<D>(a.c, page, h, ub * kKvTokens % a.c.page_size);
+            const StepAt x = step_at(p, a.c.n_seqs, u0 + i);
+            const int h = kKeysOnly ? x.job : x.job / a.n_rt;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int s = x.step * kStep + e * kKvTokens;
+                if (s >= x.len) break;
+                const int page = kv_page(a.c, x.b, s);
+                if (page >= 0) src[e] = static_cast<int>((kv_line(a.c, page, h) + s % a.c.page_size) / kKvTokens);
+                else bad = true;
+            }
         }
+        if (__any_sync(0xffffffffu, bad)) absent = true;
     }
-    // Issue the copy of the next unit of the run (every lane calls it).
-    __device__ __forceinline__ void issue(const KvAttendArgs& a, const Plan& p) {
+    // Issue the copies of the run's next step into slot s (every lane calls it).
+    __device__ __forceinline__ void issue(const KvAttendArgs& a, const Plan& p, int s) {
         if ((issued & 31) == 0) lookup(a, p);
         if ((threadIdx.x & 31) == (issued & 31)) {
-            const int s = issued % depth;
-            const uint32_t bar = bars + 8 * s, dst = ring + s * kv_unit_bytes(D);
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(flags + 4 * s), "r"(src != nullptr ? 1u : 0u) : "memory");
-            if (src == nullptr) {
+            const uint32_t bar = bars + 8 * s, dst = ring + s * kSlot;
+            const bool f0 = src[0] >= 0, f1 = src[1] >= 0;
+            constexpr uint32_t kKeys = kKeysOnly ? 8 * D + kKvTokens * 8 : kUnit;
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(flags + 4 * s), "r"((f0 ? 1u : 0u) | (f1 ? 2u : 0u)) : "memory");
+            if (!f0 && !f1) {
                 mbar_arrive(bar);
-            } else if (kKeysOnly) {
-                mbar_arrive_expect_tx(bar, 8 * D + kKvTokens * 8);
-                bulk_g2s(dst, src, 8 * D, bar);
-                bulk_g2s(dst + kv_param_offset(D), src + kv_param_offset(D), kKvTokens * 8, bar);
             } else {
-                mbar_arrive_expect_tx(bar, kv_unit_bytes(D));
-                bulk_g2s(dst, src, kv_unit_bytes(D), bar);
+                mbar_arrive_expect_tx(bar, (f0 ? kKeys : 0u) + (f1 ? kKeys : 0u));
+                const uint8_t* from = a.c.units + static_cast<size_t>(f0 ? src[0] : src[1]) * kUnit;
+                if (!kKeysOnly && f0 && src[1] == src[0] + 1) {
+                    bulk_g2s(dst, from, kSlot, bar);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        if (src[e] < 0) continue;
+                        if (e == 1) from = a.c.units + static_cast<size_t>(src[1]) * kUnit;
+                        if (kKeysOnly) {
+                            bulk_g2s(dst + e * kUnit, from, 8 * D, bar);
+                            bulk_g2s(dst + e * kUnit + kv_param_offset(D), from + kv_param_offset(D), kKvTokens * 8, bar);
+                        } else {
+                            bulk_g2s(dst + e * kUnit, from, kUnit, bar);
+                        }
+                    }
+                }
             }
         }
         ++issued;
@@ -311,27 +380,27 @@ struct UnitStream {
         u0 = first;
         n = count;
         issued = parity = slot = 0;
-        ok = true;
+        absent = false;
         const int m = min(depth, n);
-        for (int i = 0; i < m; ++i) issue(a, p);
+        for (int i = 0; i < m; ++i) issue(a, p, i);
     }
-    // Wait for the unit in the current slot; false when the bounded wait gave up.
+    // Wait for the step in the current slot; false when the bounded wait gave up.
     __device__ __forceinline__ bool wait() {
         const bool got = mbar_wait_bounded(bars + 8 * slot, parity);
-        ok = __all_sync(0xffffffffu, got);
-        return ok;
+        return __all_sync(0xffffffffu, got);
     }
-    __device__ __forceinline__ uint32_t unit() const { return ring + slot * kv_unit_bytes(D); }
-    __device__ __forceinline__ bool found() const { return lds_u32(flags + 4 * slot) != 0; }
+    __device__ __forceinline__ uint32_t unit() const { return ring + slot * kSlot; }
+    // Bit e: unit e of the step was copied (only asked for when some unit of the run is absent).
+    __device__ __forceinline__ uint32_t found() const { return lds_u32(flags + 4 * slot); }
     // The current slot is read: refill it, go to the next.
     __device__ __forceinline__ void next(const KvAttendArgs& a, const Plan& p) {
         __syncwarp();
-        if (issued < n) issue(a, p);
+        if (issued < n) issue(a, p, slot);
         if (++slot == depth) { slot = 0; parity ^= 1; }
     }
     // After a wait that gave up: no copy may still be in flight when the CTA's shared memory is released.
-    __device__ __forceinline__ void drain(int consumed, unsigned int* err) {
-        if ((threadIdx.x & 31) == 0) atomicOr(err, kKvErrWait);
+    __device__ __forceinline__ void drain(int consumed) {
+        if ((threadIdx.x & 31) == 0) atomicOr(&g_kv_attend_error, kKvErrWait);
         for (int i = consumed; i < issued; ++i) {
             mbar_wait_bounded(bars + 8 * slot, parity);
             if (++slot == depth) { slot = 0; parity ^= 1; }
@@ -339,47 +408,20 @@ struct UnitStream {
     }
 };
 
-// ---------------------------------------------------------------------------
-// The pass over the cache
-// ---------------------------------------------------------------------------
-template <int D, int NT>
-__global__ void __launch_bounds__(32 * kAtWarps, NT == 1 ? 4 : 3) kv_attend_kernel(const KvAttendArgs a) {
-    extern __shared__ __align__(128) char smem[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const KvView& c = a.c;
-    UnitStream<D, false> st;
-    st.init(smem + plan_bytes(c.n_seqs), warp, a.depth);
-    pdl_launch_dependents();
-    pdl_wait();
-    const int warps = gridDim.x * kAtWarps;
-    const Plan p = make_plan<32 * kAtWarps>(c, c.heads * a.n_rt, warps, smem, blockIdx.x == 0 ? &g_kv_attend_error : nullptr);
-    const int w = warp * gridDim.x + blockIdx.x;  // neighbouring runs on different SMs
-    const long long u0 = warp_start(p, w), u1 = warp_start(p, w + 1);
-    const int n = static_cast<int>(u1 - u0);
-    if (n == 0) return;
-    st.start(a, p, u0, n);
+// A unit's scale and zero for slots g and g + 8 of keys, ready for the scores.
+struct KeyParams {
+    float s0, z0, s1, z1;
+    __device__ __forceinline__ KeyParams(uint2 p0, uint2 p1, float scale2)
+        : s0(h2f_bits(lo16(p0.x)) * scale2), z0(h2f_bits(hi16(p0.x)) - 8.f),
+          s1(h2f_bits(lo16(p1.x)) * scale2), z1(h2f_bits(hi16(p1.x)) - 8.f) {}
+};
 
-    QueryTile<D, NT> q;
-    float o[NT][D / 16][4], m[NT][2], l[NT][2], zs[NT][2], vw = 0.f;
-    int b = 0, h = 0, rt = 0, len = 0, ub = 0, ul = 0, done = 0, seg = 0;
-    long long left = 0;  // units of the current sequence's jobs not yet begun
-    bool bad_page = false;
-    while (done < n) {
-        // a job, or the part of it in this run
-        if (done == 0 || left == 0) {
-            const long long u = u0 + done;
-            b = seq_of(p, c.n_seqs, u);
-            len = p.len[b];
-            ul = (len + kKvTokens - 1) / kKvTokens;
-            const long long r = u - p.pre[b];
-            const int job = static_cast<int>(r / ul);
-            ub = static_cast<int>(r - static_cast<long long>(job) * ul);
-            h = job / a.n_rt;
-            rt = job - h * a.n_rt;
-            left = p.pre[b + 1] - u;
-        }
-        const int first_ub = ub, take = min(ul - ub, n - done);
-        q.load(a, b, h, rt, len);
+// The running softmax of one job in one warp.
+template <int D, int NT>
+struct RowState {
+    float o[NT][D / 16][4], m[NT][2], l[NT][2], zs[NT][2], vw;
+
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -390,229 +432,384 @@ __global__ void __launch_bounds__(32 * kAtWarps, NT == 1 ? 4 : 3) kv_attend_kern
             for (int e = 0; e < 2; ++e) { m[nt][e] = kNone; l[nt][e] = 0.f; zs[nt][e] = 0.f; }
         }
         vw = 2147483648.0f;  // 2^31 brings the smallest FP16 scale, 2^-24, to 2^7
+    }
 
-        for (int i = 0; i < take; ++i, ++ub) {
-            if (!st.wait()) { st.drain(done + i, &g_kv_attend_error); return; }
-            const bool found = st.found();
-            if (!found) bad_page = true;
-            if (found && ub * kKvTokens < q.max_lim) {
-                const uint32_t unit = st.unit();
-                float s[NT][4];
-                score_mma<D, NT>(unit, q, s);
-                const uint2 p0 = lds_v2(unit + kv_param_offset(D) + 8 * g), p1 = lds_v2(unit + kv_param_offset(D) + 8 * (g + 8));
-                const float sk0 = h2f_bits(lo16(p0.x)) * a.scale2, zk0 = h2f_bits(hi16(p0.x)) - 8.f;
-                const float sk1 = h2f_bits(lo16(p1.x)) * a.scale2, zk1 = h2f_bits(hi16(p1.x)) - 8.f;
-                float sv0 = h2f_bits(lo16(p0.y)), zv0 = h2f_bits(hi16(p0.y)) - 8.f;
-                float sv1 = h2f_bits(lo16(p1.y)), zv1 = h2f_bits(hi16(p1.y)) - 8.f;
+    // U units from slot j of the sequence on.  found: bit u set where unit u is there.
+    template <int U>
+    __device__ __forceinline__ void add(const QueryTile<D, NT>& q, uint32_t unit, int j, int len, uint32_t found, float scale2) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        float s[U][NT][4], sv[U][2], zv[U][2];
+        score_mma<D, NT, U>(unit, q, s);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
+        for (int u = 0; u < U; ++u) {
+            const uint32_t pa = unit + u * kv_unit_bytes(D) + kv_param_offset(D) + 8 * g;
+            const uint2 p0 = lds_v2(pa), p1 = lds_v2(pa + 64);
+            const KeyParams k(p0, p1, scale2);
+            sv[u][0] = h2f_bits(lo16(p0.y)); zv[u][0] = h2f_bits(hi16(p0.y)) - 8.f;
+            sv[u][1] = h2f_bits(lo16(p1.y)); zv[u][1] = h2f_bits(hi16(p1.y)) - 8.f;
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        s[nt][e] = fmaf(-zk0, q.sum[nt][e], s[nt][e]) * sk0;
-                        s[nt][e + 2] = fmaf(-zk1, q.sum[nt][e], s[nt][e + 2]) * sk1;
-                    }
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    s[u][nt][e] = fmaf(-k.z0, q.sum[nt][e], s[u][nt][e]) * k.s0;
+                    s[u][nt][e + 2] = fmaf(-k.z1, q.sum[nt][e], s[u][nt][e + 2]) * k.s1;
                 }
-                if (ub * kKvTokens + kKvTokens > q.min_lim) {
-                    // the last unit of the sequence or of a query token: keys behind a row's own are
-                    // taken out, and what lies behind the last token is never multiplied
-                    const int j0 = ub * kKvTokens + g, j1 = j0 + 8;
-                    if (j0 >= len) { sv0 = 0.f; zv0 = 0.f; }
-                    if (j1 >= len) { sv1 = 0.f; zv1 = 0.f; }
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            if (j0 >= q.lim[nt][e]) s[nt][e] = -INFINITY;
-                            if (j1 >= q.lim[nt][e]) s[nt][e + 2] = -INFINITY;
-                        }
-                }
-                // a new maximum or a larger V scale: rare after the first units
-                bool up = fmaxf(sv0, sv1) * vw > 128.f;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) up |= fmaxf(s[nt][e], s[nt][e + 2]) > m[nt][e] + kLazy;
-                if (__any_sync(0xffffffffu, up)) {
-                    const float big = lane_max_g(fmaxf(sv0, sv1));
-                    float ratio = 1.f;
-                    if (big * vw > 128.f) {
-                        // 2^(7 - e) with 2^(e-1) <= big < 2^e
-                        const float nw = __uint_as_float((260u - (__float_as_uint(big) >> 23)) << 23);
-                        ratio = __uint_as_float(__float_as_uint(nw) - __float_as_uint(vw) + 0x3F800000u);  // nw / vw, powers of two
-                        vw = nw;
-                    }
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float top = fmaxf(m[nt][e], lane_max_g(fmaxf(s[nt][e], s[nt][e + 2])));
-                            const float f = (top == m[nt][e]) ? 1.f : ex2(m[nt][e] - top);
-                            m[nt][e] = top;
-                            l[nt][e] *= f;
-                            const float fr = f * ratio;
-                            zs[nt][e] *= fr;
-#pragma unroll
-                            for (int j = 0; j < D / 16; ++j) { o[nt][j][e] *= fr; o[nt][j][e + 2] *= fr; }
-                        }
-                }
-                const float w0 = sv0 * vw, w1 = sv1 * vw;
-                uint32_t pf[NT][2];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float x[4];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float e0 = ex2(s[nt][e] - m[nt][e]), e1 = ex2(s[nt][e + 2] - m[nt][e]);
-                        l[nt][e] += e0 + e1;
-                        x[e] = e0 * w0;
-                        x[e + 2] = e1 * w1;
-                        zs[nt][e] = fmaf(x[e], zv0, fmaf(x[e + 2], zv1, zs[nt][e]));
-                    }
-                    pf[nt][0] = movmatrix_trans(pack_f32(x[0], x[1]));
-                    pf[nt][1] = movmatrix_trans(pack_f32(x[2], x[3]));
-                }
-                uint32_t v0[D / 32], v1[D / 32];
-                const uint32_t vb = unit + kv_v_offset(D) + t * D + g * (D / 8);
-                if (D == 128) {
-                    const uint4 x = lds_v4(vb), y = lds_v4(vb + 4 * D);
-                    v0[0] = x.x; v0[1] = x.y; v0[D / 32 - 2] = x.z; v0[D / 32 - 1] = x.w;
-                    v1[0] = y.x; v1[1] = y.y; v1[D / 32 - 2] = y.z; v1[D / 32 - 1] = y.w;
-                } else {
-                    const uint2 x = lds_v2(vb), y = lds_v2(vb + 4 * D);
-                    v0[0] = x.x; v0[1] = x.y;
-                    v1[0] = y.x; v1[1] = y.y;
-                }
-#pragma unroll
-                for (int k = 0; k < D / 32; ++k) {
-                    const uint32_t a0 = centred(v0[k] << 4), a1 = centred(v0[k]), a2 = centred(v1[k] << 4), a3 = centred(v1[k]);
-                    const uint32_t b0 = centred(v0[k] >> 4), b1 = centred(v0[k] >> 8), b2 = centred(v1[k] >> 4), b3 = centred(v1[k] >> 8);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        mma_16816(o[nt][2 * k], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);
-                        mma_16816(o[nt][2 * k + 1], b0, b1, b2, b3, pf[nt][0], pf[nt][1]);
-                    }
-                }
-            }
-            st.next(a, p);
         }
-
-        // the lane's columns (D/8 g ..) of rows 2t and 2t + 1
-        const bool whole = first_ub == 0 && ub == ul;
-        const int rows = a.tokens * a.group;
-        const float inv_w = __uint_as_float(0x7F000000u - __float_as_uint(vw));  // 1 / vw, a power of two
+        if (j + U * kKvTokens > q.min_lim || found != (1u << U) - 1u) {
+            // the end of the sequence or of a query token's keys, or an absent page: slots behind a
+            // row's keys are taken out, and what lies behind the last token is never multiplied
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int jj = j + u * kKvTokens + g + 8 * x;
+                    const bool there = jj < len && (found >> u & 1u);
+                    if (!there) { sv[u][x] = 0.f; zv[u][x] = 0.f; }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (!there || jj >= q.lim[nt][e]) s[u][nt][e + 2 * x] = -INFINITY;
+                }
+        }
+        // a new maximum or a larger V scale: rare after the first steps
+        float big = fmaxf(sv[0][0], sv[0][1]), top[NT][2];
+#pragma unroll
+        for (int u = 1; u < U; ++u) big = fmaxf(big, fmaxf(sv[u][0], sv[u][1]));
+        bool up = big * vw > 128.f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float ls = lane_sum_g(l[nt][e]), z = lane_sum_g(zs[nt][e]);
-                const int rl = nt * 8 + 2 * t + e, r = rt * NT * 8 + rl;
-                if (r >= rows) continue;
-                float v[D / 8];
+                top[nt][e] = fmaxf(s[0][nt][e], s[0][nt][e + 2]);
 #pragma unroll
-                for (int j = 0; j < D / 16; ++j) {
-                    v[2 * j] = (o[nt][j][e] - z) * inv_w;
-                    v[2 * j + 1] = (o[nt][j][e + 2] - z) * inv_w;
+                for (int u = 1; u < U; ++u) top[nt][e] = fmaxf(top[nt][e], fmaxf(s[u][nt][e], s[u][nt][e + 2]));
+                up |= top[nt][e] > m[nt][e] + kLazy;
+            }
+        if (__any_sync(0xffffffffu, up)) rescale(top, big);
+        uint32_t pf[U][NT][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float w0 = sv[u][0] * vw, w1 = sv[u][1] * vw;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float e0 = ex2(s[u][nt][e] - m[nt][e]), e1 = ex2(s[u][nt][e + 2] - m[nt][e]);
+                    l[nt][e] += e0 + e1;
+                    x[e] = e0 * w0;
+                    x[e + 2] = e1 * w1;
+                    zs[nt][e] = fmaf(x[e], zv[u][0], fmaf(x[e + 2], zv[u][1], zs[nt][e]));
                 }
-                if (whole) {
-                    const int tok = r / a.group, head = h * a.group + r % a.group;
-                    const float f = ls > 0.f ? __fdiv_rn(1.f, ls) : (ls == 0.f ? 0.f : ls);
-                    uint16_t* dst = a.out + b * a.os[0] + tok * a.os[1] + head * a.os[2] + (D / 8) * g;
+                pf[u][nt][0] = movmatrix_trans(pack_f32(x[0], x[1]));
+                pf[u][nt][1] = movmatrix_trans(pack_f32(x[2], x[3]));
+            }
+        }
 #pragma unroll
-                    for (int j = 0; j < D / 8; j += 8)
-                        *reinterpret_cast<uint4*>(dst + j) =
-                            make_uint4(pack_f32(v[j] * f, v[j + 1] * f), pack_f32(v[j + 2] * f, v[j + 3] * f),
-                                       pack_f32(v[j + 4] * f, v[j + 5] * f), pack_f32(v[j + 6] * f, v[j + 7] * f));
-                    if (g == 0) {
-                        const size_t li = (static_cast<size_t>(b) * a.tokens + tok) * (c.heads * a.group) + head;
-                        const float l2 = ls == 0.f ? -INFINITY : m[nt][e] + log2f(ls);
-                        if (a.lse) a.lse[li] = l2 * 0.693147180559945309f;
-                        if (a.lse2) a.lse2[li] = l2;
-                    }
-                } else {
-                    const size_t pi = (static_cast<size_t>(w) * 2 + seg) * (NT * 8) + rl;
-                    float* dst = a.part + pi * D + (D / 8) * g;
+        for (int u = 0; u < U; ++u) {
+            uint32_t v0[D / 32], v1[D / 32];
+            const uint32_t vb = unit + u * kv_unit_bytes(D) + kv_v_offset(D) + t * D + g * (D / 8);
+            if (D == 128) {
+                const uint4 x = lds_v4(vb), y = lds_v4(vb + 4 * D);
+                v0[0] = x.x; v0[1] = x.y; v0[D / 32 - 2] = x.z; v0[D / 32 - 1] = x.w;
+                v1[0] = y.x; v1[1] = y.y; v1[D / 32 - 2] = y.z; v1[D / 32 - 1] = y.w;
+            } else {
+                const uint2 x = lds_v2(vb), y = lds_v2(vb + 4 * D);
+                v0[0] = x.x; v0[1] = x.y;
+                v1[0] = y.x; v1[1] = y.y;
+            }
 #pragma unroll
-                    for (int j = 0; j < D / 8; j += 4)
-                        *reinterpret_cast<float4*>(dst + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-                    if (g == 0) *reinterpret_cast<float2*>(a.part_ml + pi * 2) = make_float2(m[nt][e], ls);
+            for (int k = 0; k < D / 32; ++k) {
+                const uint32_t y0 = v0[k] >> 8, y1 = v1[k] >> 8;
+                const uint32_t a0 = low_codes(v0[k]), a1 = high_codes(v0[k]), a2 = low_codes(v1[k]), a3 = high_codes(v1[k]);
+                const uint32_t b0 = low_codes(y0), b1 = high_codes(y0), b2 = low_codes(y1), b3 = high_codes(y1);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma_16816(o[nt][2 * k], a0, a1, a2, a3, pf[u][nt][0], pf[u][nt][1]);
+                    mma_16816(o[nt][2 * k + 1], b0, b1, b2, b3, pf[u][nt][0], pf[u][nt][1]);
                 }
             }
-        done += take;
-        left -= take;
-        seg = 1;
-        if (ub == ul) {
-            ub = 0;
-            if (++rt == a.n_rt) { rt = 0; ++h; }
         }
     }
-    if (bad_page && lane == 0) atomicOr(&g_kv_attend_error, kKvErrPage);
+
+    __device__ __forceinline__ void rescale(const float (&top)[NT][2], float big) {
+        big = lane_max_g(big);
+        float ratio = 1.f;
+        if (big * vw > 128.f) {
+            // 2^(7 - e) with 2^(e-1) <= big < 2^e
+            const float nw = __uint_as_float((260u - (__float_as_uint(big) >> 23)) << 23);
+            ratio = __uint_as_float(__float_as_uint(nw) - __float_as_uint(vw) + 0x3F800000u);  // nw / vw, powers of two
+            vw = nw;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float now = fmaxf(m[nt][e], lane_max_g(top[nt][e]));
+                const float f = (now == m[nt][e]) ? 1.f : ex2(m[nt][e] - now);
+                m[nt][e] = now;
+                l[nt][e] *= f;
+                const float fr = f * ratio;
+                zs[nt][e] *= fr;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) { o[nt][k][e] *= fr; o[nt][k][e + 2] *= fr; }
+            }
+    }
+
+    // Row 2t + e of tile nt: its sum of weights and the lane's columns D/8 g .. of its unnormalised output.
+    __device__ __forceinline__ float finish(int nt, int e, float (&v)[D / 8]) const {
+        const float z = lane_sum_g(zs[nt][e]), inv = __uint_as_float(0x7F000000u - __float_as_uint(vw));  // 1 / vw
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+            v[2 * k] = (o[nt][k][e] - z) * inv;
+            v[2 * k + 1] = (o[nt][k][e + 2] - z) * inv;
+        }
+        return lane_sum_g(l[nt][e]);
+    }
+};
+
+// A piece of a job that its run cut: which job and which of its steps.
+struct Piece {
+    int b, job, first, end;  // job < 0: none
+};
+
+// ---------------------------------------------------------------------------
+// The pass over the cache
+// ---------------------------------------------------------------------------
+template <int D, int NT>
+__global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kernel(const KvAttendArgs a) {
+    constexpr int W = at_warps(NT), R = 8 * NT, kPiece = R * (D + 2);
+    extern __shared__ __align__(128) char smem[];
+    __shared__ Piece pieces[2 * W];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const KvView& c = a.c;
+    char* at = smem + plan_bytes(c.n_seqs);
+    StepStream<D, false> st;
+    char* rings = at + W * kPiece * 4;
+    st.init(rings, W, warp, a.depth);
+    // A piece is [R][D + 2] floats: output, maximum, sum.  A warp's first piece has room of its own, its
+    // last one takes the warp's ring, which has run dry by then.
+    auto piece_at = [&](int k) {
+        return reinterpret_cast<float*>((k & 1) ? rings + (k >> 1) * a.depth * StepStream<D, false>::kSlot : at + (k >> 1) * kPiece * 4);
+    };
+    pdl_launch_dependents();
+    pdl_wait();
+    const Plan p = make_plan<32 * W>(c, c.heads * a.n_rt, gridDim.x * W, smem, blockIdx.x == 0 ? &g_kv_attend_error : nullptr);
+    if (blockIdx.x == 0)
+        for (int b = threadIdx.x; b <= c.n_seqs; b += 32 * W) a.pre[b] = p.pre[b];
+    const long long w = static_cast<long long>(blockIdx.x) * W + warp;
+    const long long u0 = warp_start(p.base, p.rem, w);
+    const int n = static_cast<int>(warp_start(p.base, p.rem, w + 1) - u0);
+    if (lane < 2) pieces[2 * warp + lane].job = -1;
+    __syncwarp();
+    const int rows = a.tokens * a.group;
+    if (n > 0) {
+        st.start(a, p, u0, n);
+        QueryTile<D, NT> q;
+        RowState<D, NT> rs;
+        int b = 0, job = 0, len = 0, ub = 0, ul = 0, done = 0;
+        bool gave_up = false;
+        int left = 0;  // steps of the current sequence not yet begun, those of this run
+        while (done < n && !gave_up) {
+            if (left == 0) {
+                const long long u = u0 + done;
+                const StepAt x = step_at(p, c.n_seqs, u);
+                b = x.b;
+                len = x.len;
+                ul = steps_of(len);
+                job = x.job;
+                ub = x.step;
+                left = static_cast<int>(min(static_cast<long long>(p.pre[b + 1]) * p.jobs - u, static_cast<long long>(n - done)));
+            }
+            // a job, or the part of it in this run
+            const int first = ub, take = min(ul - ub, n - done);
+            const int h = job / a.n_rt, rt = job - h * a.n_rt;
+            q.load(a, b, h, rt, len);
+            rs.clear();
+            for (int i = 0; i < take; ++i, ++ub) {
+                if (!st.wait()) {
+                    st.drain(done + i);
+                    gave_up = true;
+                    break;
+                }
+                const int j = ub * kStep;
+                if (j < q.max_lim) {
+                    uint32_t found = 3u;
+                    if (st.absent) {
+                        found = st.found();
+                        if (j + kKvTokens >= len) found |= 2u;  // behind the last slot: not copied, and not missed
+                    }
+                    if constexpr (NT == 1) {
+                        rs.template add<2>(q, st.unit(), j, len, found, a.scale2);
+                    } else {
+                        rs.template add<1>(q, st.unit(), j, len, found & 1u, a.scale2);
+                        if (j + kKvTokens < q.max_lim)
+                            rs.template add<1>(q, st.unit() + kv_unit_bytes(D), j + kKvTokens, len, found >> 1, a.scale2);
+                    }
+                }
+                st.next(a, p);
+            }
+            if (gave_up) break;
+            const bool whole = first == 0 && ub == ul;
+            const int k = 2 * warp + (done == 0 ? 0 : 1);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float v[D / 8];
+                    const float sum = rs.finish(nt, e, v);
+                    const int rl = nt * 8 + 2 * t + e, r = rt * R + rl;
+                    if (r >= rows) continue;
+                    if (whole) {
+                        const int tok = r / a.group, head = h * a.group + r % a.group;
+                        const float f = row_norm(sum);
+                        uint16_t* dst = a.out + b * a.os[0] + tok * a.os[1] + head * a.os[2] + (D / 8) * g;
+#pragma unroll
+                        for (int i = 0; i < D / 8; i += 8)
+                            *reinterpret_cast<uint4*>(dst + i) =
+                                make_uint4(pack_f32(v[i] * f, v[i + 1] * f), pack_f32(v[i + 2] * f, v[i + 3] * f),
+                                           pack_f32(v[i + 4] * f, v[i + 5] * f), pack_f32(v[i + 6] * f, v[i + 7] * f));
+                        if (g == 0) store_lse(a, b, tok, head, rs.m[nt][e], sum);
+                    } else {
+                        float* dst = piece_at(k) + rl * (D + 2);
+#pragma unroll
+                        for (int i = 0; i < D / 8; i += 2)
+                            *reinterpret_cast<float2*>(dst + (D / 8) * g + i) = make_float2(v[i], v[i + 1]);
+                        if (g == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(rs.m[nt][e], sum);
+                    }
+                }
+            if (!whole && lane == 0) pieces[k] = Piece{b, job, first, ub};
+            done += take;
+            left -= take;
+            if (ub == ul) { ub = 0; ++job; }
+        }
+    }
+    __syncthreads();
+    // Neighbouring pieces of one job meet here, in order; a job that ends up whole is finished, the
+    // others (at most the CTA's first and last) go to the workspace.
+    int slot = 0;
+    for (int k = 0; k < 2 * W;) {
+        const Piece first = pieces[k];
+        if (first.job < 0) { ++k; continue; }
+        int end = first.end, k1 = k + 1;
+        for (; k1 < 2 * W; ++k1) {
+            const Piece x = pieces[k1];
+            if (x.job < 0) continue;
+            if (x.b != first.b || x.job != first.job) break;
+            end = x.end;
+        }
+        const bool whole = first.first == 0 && end == steps_of(p.len[first.b]);
+        const int h = first.job / a.n_rt, rt = first.job - h * a.n_rt;
+        constexpr int C = 8;  // columns of a thread
+        for (int i = threadIdx.x; i < R * (D / C); i += 32 * W) {
+            const int rl = i / (D / C), col = C * (i % (D / C)), r = rt * R + rl;
+            if (r >= rows) break;
+            float m = kNone, sum = 0.f, v[C];
+            for (int x = k; x < k1; ++x)
+                if (pieces[x].job >= 0) m = fmaxf(m, piece_at(x)[rl * (D + 2) + D]);
+#pragma unroll
+            for (int y = 0; y < C; ++y) v[y] = 0.f;
+            for (int x = k; x < k1; ++x) {
+                if (pieces[x].job < 0) continue;
+                const float* src = piece_at(x) + rl * (D + 2);
+                const float f = ex2(src[D] - m);
+                sum += src[D + 1] * f;
+#pragma unroll
+                for (int y = 0; y < C; y += 2) {
+                    const float2 z = *reinterpret_cast<const float2*>(src + col + y);
+                    v[y] += z.x * f;
+                    v[y + 1] += z.y * f;
+                }
+            }
+            if (whole) {
+                const int tok = r / a.group, head = h * a.group + r % a.group;
+                const float f = row_norm(sum);
+                *reinterpret_cast<uint4*>(a.out + first.b * a.os[0] + tok * a.os[1] + head * a.os[2] + col) =
+                    make_uint4(pack_f32(v[0] * f, v[1] * f), pack_f32(v[2] * f, v[3] * f), pack_f32(v[4] * f, v[5] * f),
+                               pack_f32(v[6] * f, v[7] * f));
+                if (col == 0) store_lse(a, first.b, tok, head, m, sum);
+            } else {
+                const size_t pi = (static_cast<size_t>(blockIdx.x) * 2 + slot) * R + rl;
+                float4* dst = reinterpret_cast<float4*>(a.part + pi * D + col);
+                dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+                dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+                if (col == 0) *reinterpret_cast<float2*>(a.part_ml + pi * 2) = make_float2(m, sum);
+            }
+        }
+        if (!whole) slot = 1;
+        k = k1;
+    }
+    if (lane == 0 && n > 0 && st.absent) atomicOr(&g_kv_attend_error, kKvErrPage);
 }
 
 // ---------------------------------------------------------------------------
-// Joins the partial sums of the jobs cut between runs, in run order; writes the
-// rows of sequences without keys.  One CTA per job, a warp per partial.
+// Joins the partial sums of the jobs cut between CTAs, in CTA order; writes the
+// rows of sequences without keys.  One warp per row: the maxima first, a lane
+// each, then the outputs with independent loads.
 // ---------------------------------------------------------------------------
-constexpr int kCbWarps = 8;
+constexpr int kCbWarps = 4;
 
 template <int D, int NT>
-__global__ void __launch_bounds__(32 * kCbWarps) kv_combine_kernel(const KvAttendArgs a, const int warps) {
-    extern __shared__ __align__(128) char smem[];
-    __shared__ float so[kCbWarps][D];
-    __shared__ float sml[kCbWarps][2];
+__global__ void __launch_bounds__(32 * kCbWarps) kv_combine_kernel(const KvAttendArgs a, const int ctas) {
+    constexpr int W = at_warps(NT), R = 8 * NT, V = D / 32;  // V columns of a lane
     const KvView& c = a.c;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int lane = threadIdx.x & 31, hq = c.heads * a.group;
     pdl_launch_dependents();
     pdl_wait();
-    const Plan p = make_plan<32 * kCbWarps>(c, c.heads * a.n_rt, warps, smem, nullptr);
-    const int b = blockIdx.y, job = blockIdx.x, h = job / a.n_rt, rt = job - h * a.n_rt;
-    const int ul = (p.len[b] + kKvTokens - 1) / kKvTokens;
-    const long long u0 = p.pre[b] + static_cast<long long>(job) * ul;
-    const long long w0 = ul ? warp_of(p, u0) : 0, w1 = ul ? warp_of(p, u0 + ul - 1) : 0;
-    if (ul && w0 == w1) return;  // finished by its warp
-    const int rows = min(a.tokens * a.group - rt * NT * 8, NT * 8);
-    const int np = ul ? static_cast<int>(w1 - w0 + 1) : 0;
-    const int seg0 = ul && warp_start(p, w0) == u0 ? 0 : 1;
-    constexpr int V = D / 32;  // columns of a lane
-    for (int rl = 0; rl < rows; ++rl) {
-        float m = kNone, l = 0.f, o[V];
-#pragma unroll
-        for (int k = 0; k < V; ++k) o[k] = 0.f;
-        for (int i = warp; i < np; i += kCbWarps) {
-            const size_t pi = (static_cast<size_t>(w0 + i) * 2 + (i == 0 ? seg0 : 0)) * (NT * 8) + rl;
-            const float mi = ldcg_f32(a.part_ml + 2 * pi), li = ldcg_f32(a.part_ml + 2 * pi + 1);
-            const float top = fmaxf(m, mi), f0 = ex2(m - top), f1 = ex2(mi - top);
-            m = top;
-            l = l * f0 + li * f1;
-#pragma unroll
-            for (int k = 0; k < V; ++k) o[k] = o[k] * f0 + ldcg_f32(a.part + pi * D + lane + 32 * k) * f1;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < V; ++k) so[warp][lane + 32 * k] = o[k];
-        if (lane == 0) { sml[warp][0] = m; sml[warp][1] = l; }
-        __syncthreads();
-        const int r = rt * NT * 8 + rl, tok = r / a.group, head = h * a.group + r % a.group;
-        if (tid < D) {
-            float top = kNone;
-#pragma unroll
-            for (int i = 0; i < kCbWarps; ++i) top = fmaxf(top, sml[i][0]);
-            float ls = 0.f, v = 0.f;
-#pragma unroll
-            for (int i = 0; i < kCbWarps; ++i) {
-                const float f = ex2(sml[i][0] - top);
-                ls += sml[i][1] * f;
-                v += so[i][tid] * f;
+    const long long item = static_cast<long long>(blockIdx.x) * kCbWarps + (threadIdx.x >> 5);
+    if (item >= static_cast<long long>(c.n_seqs) * a.tokens * hq) return;
+    const int head = static_cast<int>(item % hq);
+    const long long bt = item / hq;
+    const int b = static_cast<int>(bt / a.tokens), tok = static_cast<int>(bt % a.tokens);
+    const int h = head / a.group, r = tok * a.group + head % a.group, rt = r / R, rl = r % R;
+    const int jobs = c.heads * a.n_rt;
+    const int p0 = static_cast<int>(ldcg_u32(a.pre + b)), ul = static_cast<int>(ldcg_u32(a.pre + b + 1)) - p0;
+    const long long total = static_cast<long long>(static_cast<int>(ldcg_u32(a.pre + c.n_seqs))) * jobs;
+    const long long base = total / (static_cast<long long>(ctas) * W);
+    const int rem = static_cast<int>(total - base * ctas * W);
+    long long c0 = 0;
+    int np = 0, first_slot = 0;
+    if (ul > 0) {
+        const long long u0 = static_cast<long long>(p0) * jobs + static_cast<long long>(ul) * (h * a.n_rt + rt);
+        c0 = warp_of(base, rem, u0) / W;
+        np = static_cast<int>(warp_of(base, rem, u0 + ul - 1) / W - c0) + 1;
+        if (np == 1) return;  // finished by its CTA
+        // a CTA's first cut job is in its slot 0: this one, unless another reaches into the CTA from before
+        const long long start = warp_start(base, rem, c0 * W);
+        if (u0 > start) {
+            const int v = static_cast<int>(start / jobs);
+            int lo = 0, hi = b + 1;  // pre[lo] <= v < pre[hi]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (static_cast<int>(ldcg_u32(a.pre + mid)) <= v) lo = mid;
+                else hi = mid;
             }
-            const float f = ls > 0.f ? __fdiv_rn(1.f, ls) : (ls == 0.f ? 0.f : ls);
-            a.out[b * a.os[0] + tok * a.os[1] + head * a.os[2] + tid] = __half_as_ushort(__float2half_rn(v * f));
-            if (tid == 0) {
-                const size_t li = (static_cast<size_t>(b) * a.tokens + tok) * (c.heads * a.group) + head;
-                const float l2 = ls == 0.f ? -INFINITY : top + log2f(ls);
-                if (a.lse) a.lse[li] = l2 * 0.693147180559945309f;
-                if (a.lse2) a.lse2[li] = l2;
-            }
+            const int q0 = static_cast<int>(ldcg_u32(a.pre + lo)), qu = static_cast<int>(ldcg_u32(a.pre + lo + 1)) - q0;
+            first_slot = (start - static_cast<long long>(q0) * jobs) % qu != 0 ? 1 : 0;
         }
     }
+    float m = kNone;
+    for (int i = lane; i < np; i += 32)
+        m = fmaxf(m, ldcg_f32(a.part_ml + 2 * (((c0 + i) * 2 + (i == 0 ? first_slot : 0)) * R + rl)));
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float sum = 0.f, v[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < np; ++i) {
+        const size_t pi = ((c0 + i) * 2 + (i == 0 ? first_slot : 0)) * R + rl;
+        const float f = ex2(ldcg_f32(a.part_ml + 2 * pi) - m);
+        sum += ldcg_f32(a.part_ml + 2 * pi + 1) * f;
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] += ldcg_f32(a.part + pi * D + lane + 32 * k) * f;
+    }
+    const float f = row_norm(sum);
+    uint16_t* dst = a.out + b * a.os[0] + tok * a.os[1] + head * a.os[2];
+#pragma unroll
+    for (int k = 0; k < V; ++k) dst[lane + 32 * k] = __half_as_ushort(__float2half_rn(v[k] * f));
+    if (lane == 0) store_lse(a, b, tok, head, m, sum);
 }
 
 // ---------------------------------------------------------------------------
@@ -621,86 +818,103 @@ __global__ void __launch_bounds__(32 * kCbWarps) kv_combine_kernel(const KvAtten
 // every row's lse is known.  A slot's sum is one lane group's, in row order.
 // ---------------------------------------------------------------------------
 template <int D>
-__global__ void __launch_bounds__(32 * kAtWarps, 4) kv_mass_kernel(const KvAttendArgs a) {
+__global__ void __launch_bounds__(32 * at_warps(1), at_ctas(1)) kv_mass_kernel(const KvAttendArgs a) {
+    constexpr int W = at_warps(1);
     extern __shared__ __align__(128) char smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const KvView& c = a.c;
-    UnitStream<D, true> st;
-    st.init(smem + plan_bytes(c.n_seqs), warp, a.depth);
+    StepStream<D, true> st;
+    st.init(smem + plan_bytes(c.n_seqs), W, warp, a.depth);
     pdl_launch_dependents();
     pdl_wait();
-    const Plan p = make_plan<32 * kAtWarps>(c, c.heads, gridDim.x * kAtWarps, smem, nullptr);
-    const int w = warp * gridDim.x + blockIdx.x;
-    const long long u0 = warp_start(p, w);
-    const int n = static_cast<int>(warp_start(p, w + 1) - u0);
+    const Plan p = make_plan<32 * W>(c, c.heads, gridDim.x * W, smem, nullptr);
+    const long long w = static_cast<long long>(blockIdx.x) * W + warp;
+    const long long u0 = warp_start(p.base, p.rem, w);
+    const int n = static_cast<int>(warp_start(p.base, p.rem, w + 1) - u0);
     if (n == 0) return;
     st.start(a, p, u0, n);
     QueryTile<D, 1> q;
-    const int n_rt = (a.tokens * a.group + 7) / 8, rows = a.tokens * a.group;
-    int last_b = -1, last_h = -1;
+    const int rows = a.tokens * a.group, n_rt = (rows + 7) / 8;
+    int b = 0, h = 0, len = 0, ub = 0, ul = 0;
+    long long left = 0;
+    bool fresh = true;
     float lse[2] = {0.f, 0.f};
     for (int i = 0; i < n; ++i) {
-        const long long u = u0 + i;
-        const int b = seq_of(p, c.n_seqs, u), len = p.len[b], ul = (len + kKvTokens - 1) / kKvTokens;
-        const long long r = u - p.pre[b];
-        const int h = static_cast<int>(r / ul), ub = static_cast<int>(r - static_cast<long long>(h) * ul);
-        if (!st.wait()) { st.drain(i, &g_kv_attend_error); return; }
-        if (st.found()) {
-            const uint32_t unit = st.unit();
-            const uint2 p0 = lds_v2(unit + kv_param_offset(D) + 8 * g), p1 = lds_v2(unit + kv_param_offset(D) + 8 * (g + 8));
-            const float sk0 = h2f_bits(lo16(p0.x)) * a.scale2, zk0 = h2f_bits(hi16(p0.x)) - 8.f;
-            const float sk1 = h2f_bits(lo16(p1.x)) * a.scale2, zk1 = h2f_bits(hi16(p1.x)) - 8.f;
-            const int j0 = ub * kKvTokens + g, j1 = j0 + 8;
-            float add0 = 0.f, add1 = 0.f;
-            for (int rt = 0; rt < n_rt; ++rt) {
-                if (n_rt > 1 || b != last_b || h != last_h) {
-                    q.load(a, b, h, rt, len);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int row = rt * 8 + 2 * t + e;
-                        lse[e] = INFINITY;  // padding rows weigh nothing
-                        if (row < rows) {
-                            const int tok = row / a.group, head = h * a.group + row % a.group;
-                            lse[e] = ldcg_f32(a.lse2 + (static_cast<size_t>(b) * a.tokens + tok) * (c.heads * a.group) + head);
-                            if (lse[e] == -INFINITY) lse[e] = INFINITY;  // a row without keys
-                        }
-                    }
-                    last_b = b;
-                    last_h = h;
-                }
-                if (ub * kKvTokens >= q.max_lim) continue;
-                float s[1][4];
-                score_mma<D, 1>(unit, q, s);
+        if (left == 0) {
+            const long long u = u0 + i;
+            const StepAt x = step_at(p, c.n_seqs, u);
+            b = x.b;
+            len = x.len;
+            ul = steps_of(len);
+            h = x.job;
+            ub = x.step;
+            left = static_cast<long long>(p.pre[b + 1]) * p.jobs - u;
+            fresh = true;
+        }
+        if (!st.wait()) { st.drain(i); return; }
+        const uint32_t unit = st.unit(), found = st.found();
+        float add[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+        for (int rt = 0; rt < n_rt; ++rt) {
+            if (n_rt > 1 || fresh) {
+                q.load(a, b, h, rt, len);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float e0 = ex2(fmaf(-zk0, q.sum[0][e], s[0][e]) * sk0 - lse[e]);
-                    const float e1 = ex2(fmaf(-zk1, q.sum[0][e], s[0][e + 2]) * sk1 - lse[e]);
-                    if (j0 < q.lim[0][e]) add0 += e0;
-                    if (j1 < q.lim[0][e]) add1 += e1;
+                    const int row = rt * 8 + 2 * t + e;
+                    lse[e] = INFINITY;  // padding rows weigh nothing
+                    if (row < rows) {
+                        const int tok = row / a.group, head = h * a.group + row % a.group;
+                        lse[e] = ldcg_f32(a.lse2 + (static_cast<size_t>(b) * a.tokens + tok) * (c.heads * a.group) + head);
+                        if (lse[e] == -INFINITY) lse[e] = INFINITY;  // a row without keys
+                    }
+                }
+                fresh = false;
+            }
+            if (ub * kStep >= q.max_lim) continue;
+            float s[2][1][4];
+            score_mma<D, 1, 2>(unit, q, s);
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const uint32_t pa = unit + y * kv_unit_bytes(D) + kv_param_offset(D) + 8 * g;
+                const KeyParams k(lds_v2(pa), lds_v2(pa + 64), a.scale2);
+                const int j0 = ub * kStep + y * kKvTokens + g, j1 = j0 + 8;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float e0 = ex2(fmaf(-k.z0, q.sum[0][e], s[y][0][e]) * k.s0 - lse[e]);
+                    const float e1 = ex2(fmaf(-k.z1, q.sum[0][e], s[y][0][e + 2]) * k.s1 - lse[e]);
+                    if (j0 < q.lim[0][e]) add[y][0] += e0;
+                    if (j1 < q.lim[0][e]) add[y][1] += e1;
                 }
             }
+        }
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            float add0 = add[y][0], add1 = add[y][1];
             add0 += __shfl_xor_sync(0xffffffffu, add0, 1);
             add1 += __shfl_xor_sync(0xffffffffu, add1, 1);
             add0 += __shfl_xor_sync(0xffffffffu, add0, 2);
             add1 += __shfl_xor_sync(0xffffffffu, add1, 2);
-            const int page = kv_page(c, b, ub * kKvTokens);
-            if (page >= 0 && t < 2) {
-                const int j = t == 0 ? j0 : j1;
-                if (j < len) c.mass[kv_line(c, page, h) + j % c.page_size] += t == 0 ? add0 : add1;
+            const int s0 = ub * kStep + y * kKvTokens, jj = s0 + g + 8 * t;
+            if ((found >> y & 1u) && t < 2 && jj < len) {
+                const int page = kv_page(c, b, s0);
+                if (page >= 0) c.mass[kv_line(c, page, h) + jj % c.page_size] += t == 0 ? add0 : add1;
             }
         }
         st.next(a, p);
+        --left;
+        if (++ub == ul) { ub = 0; ++h; fresh = true; }
     }
 }
 
-constexpr int kAtSmemPerSm = 226 * 1024;
+constexpr int kSmemPerSm = 226 * 1024;
 
-// Shared memory of a CTA when `ctas` of them share an SM, and the ring depth that fits.
-int ring_depth(int n_seqs, int d, int ctas, int* smem) {
-    const int room = kAtSmemPerSm / ctas - 1024 - plan_bytes(n_seqs) - 256;
-    int depth = room / (kAtWarps * (kv_unit_bytes(d) + 12));
-    depth = depth > 12 ? 12 : depth;
-    *smem = plan_bytes(n_seqs) + (kAtWarps * depth * (kv_unit_bytes(d) + 12) + 127) / 128 * 128;
+// Ring slots per warp that fit next to the plan and `fixed` bytes when `ctas` CTAs share an SM, and the CTA's
+// shared memory.
+template <class Stream>
+int ring_depth(int n_seqs, int warps, int ctas, int fixed, int* smem) {
+    const int used = plan_bytes(n_seqs) + fixed, room = kSmemPerSm / ctas - 2048 - used;
+    int depth = room / (warps * (Stream::kSlot + 12));
+    depth = depth > 8 ? 8 : depth;
+    *smem = used + Stream::bytes(warps, depth);
     return depth;
 }
 
@@ -713,39 +927,42 @@ dq_status_t allow_smem(K kernel, int smem) {
 
 template <int D, int NT>
 dq_status_t attend(KvAttendArgs& a, cudaStream_t stream) {
+    constexpr int W = at_warps(NT);
     DeviceInfo di;
     dq_status_t st = device_info(&di);
     if (st != DQ_OK) return st;
-    const int ctas = NT == 1 ? 4 : 3;
-    int grid = di.sm_count * ctas;
-    if (grid * kAtWarps > kAtMaxWarps) grid = kAtMaxWarps / kAtWarps;
-    int smem = 0;
-    a.depth = ring_depth(a.c.n_seqs, D, ctas, &smem);
+    int grid = di.sm_count * at_ctas(NT), smem = 0;
+    if (grid * W > kAtMaxWarps) grid = kAtMaxWarps / W;
+    a.depth = ring_depth<StepStream<D, false>>(a.c.n_seqs, W, at_ctas(NT), W * 8 * NT * (D + 2) * 4, &smem);
+    // a piece fits in a ring of two slots
+    static_assert(8 * NT * (D + 2) * 4 <= 2 * StepStream<D, false>::kSlot, "ring too small for a piece");
+    if (a.depth < 2) return DQ_ERR_UNSUPPORTED;
     if ((st = allow_smem(kv_attend_kernel<D, NT>, smem)) != DQ_OK) return st;
-    if ((st = launch_pdl(kv_attend_kernel<D, NT>, dim3(grid), 32 * kAtWarps, smem, stream, a)) != DQ_OK) return st;
-    const dim3 jobs(a.c.heads * a.n_rt, a.c.n_seqs);
-    st = launch_pdl(kv_combine_kernel<D, NT>, jobs, 32 * kCbWarps, plan_bytes(a.c.n_seqs), stream, a, grid * kAtWarps);
+    if ((st = launch_pdl(kv_attend_kernel<D, NT>, dim3(grid), 32 * W, smem, stream, a)) != DQ_OK) return st;
+    const long long items = static_cast<long long>(a.c.n_seqs) * a.tokens * a.c.heads * a.group;
+    st = launch_pdl(kv_combine_kernel<D, NT>, dim3(static_cast<unsigned>((items + kCbWarps - 1) / kCbWarps)),
+                    32 * kCbWarps, 0, stream, a, grid);
     if (st != DQ_OK || !a.lse2) return st;
-    grid = di.sm_count * 4;
-    if (grid * kAtWarps > kAtMaxWarps) grid = kAtMaxWarps / kAtWarps;
-    a.depth = ring_depth(a.c.n_seqs, D, 4, &smem);
+    grid = di.sm_count * at_ctas(1);
+    a.depth = ring_depth<StepStream<D, true>>(a.c.n_seqs, at_warps(1), at_ctas(1), 0, &smem);
     if ((st = allow_smem(kv_mass_kernel<D>, smem)) != DQ_OK) return st;
-    return launch_pdl(kv_mass_kernel<D>, dim3(grid), 32 * kAtWarps, smem, stream, a);
+    return launch_pdl(kv_mass_kernel<D>, dim3(grid), 32 * at_warps(1), smem, stream, a);
 }
 
 // Row tiles of one warp: 8 rows when a KV head has no more, else 16.
 int row_tiles(int rows) { return rows <= 8 ? 1 : 2; }
 
 struct AttendWs {
-    size_t part, ml, lse2, total;
+    size_t part, ml, pre, lse2, total;
 };
 AttendWs attend_ws(const dq_kv_cache_t& c, int tokens, int q_heads, bool mass) {
     const int nt = row_tiles(tokens * (q_heads / c.kv_heads));
-    const size_t rows = static_cast<size_t>(kAtMaxWarps) * 2 * 8 * nt;
+    const size_t rows = static_cast<size_t>(kAtMaxWarps / at_warps(nt)) * 2 * 8 * nt;
     AttendWs w;
     w.part = 0;
     w.ml = align256(rows * c.head_dim * 4);
-    w.lse2 = w.ml + align256(rows * 8);
+    w.pre = w.ml + align256(rows * 8);
+    w.lse2 = w.pre + align256((static_cast<size_t>(c.n_seqs) + 1) * 4);
     w.total = w.lse2 + (mass ? align256(static_cast<size_t>(c.n_seqs) * tokens * q_heads * 4) : 0);
     return w;
 }
@@ -771,6 +988,7 @@ dq_status_t launch_kv_attend(const dq_kv_cache_t& c, const dq_kv_attend_t& r, vo
     char* base = static_cast<char*>(workspace);
     a.part = reinterpret_cast<float*>(base + w.part);
     a.part_ml = reinterpret_cast<float*>(base + w.ml);
+    a.pre = reinterpret_cast<int*>(base + w.pre);
     a.lse2 = r.accumulate ? reinterpret_cast<float*>(base + w.lse2) : nullptr;
     const int rows = r.tokens * a.group, nt = row_tiles(rows);
     a.n_rt = (rows + 8 * nt - 1) / (8 * nt);

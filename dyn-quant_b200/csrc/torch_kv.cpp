@@ -44,7 +44,7 @@ public:
         check(pos, "pos", at::kInt, {pages, heads, page});
         TORCH_CHECK(lengths.dim() == 1 && page_table.dim() == 2, "lengths must be 1D and page_table 2D");
         const int64_t seqs = lengths.size(0);
-        TORCH_CHECK(seqs <= 2048, "at most 2048 sequences per cache");
+        TORCH_CHECK(seqs <= 1024, "at most 1024 sequences per cache");
         check(lengths, "lengths", at::kInt, {seqs});
         check(evicted, "evicted", at::kInt, {seqs});
         check(arrivals, "arrivals", at::kInt, {seqs});

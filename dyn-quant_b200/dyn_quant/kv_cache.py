@@ -33,7 +33,7 @@ class Int4KVCache:
     """The 4-bit KV cache of one layer for a fixed set of sequence slots.
 
     Args:
-        n_seqs:     sequences (batch slots); at most 2048.
+        n_seqs:     sequences (batch slots); at most 1024.
         n_pages:    pages of the pool, shared out to the sequences by `page_table`.
         n_kv_heads: KV heads.
         head_dim:   64 or 128.

@@ -410,7 +410,7 @@ typedef struct dq_kv_cache_t {
     int32_t* evicted;          /* [n_seqs] tokens evicted so far (positions seen = lengths + evicted) */
     const int32_t* page_table; /* [n_seqs][max_pages]; entries past a sequence's last page are not read */
     uint32_t* arrivals;        /* [n_seqs] zero-filled once; every call leaves it at zero */
-    int32_t n_seqs;            /* 1 .. 2048 */
+    int32_t n_seqs;            /* 0 .. 1024 */
     int32_t n_pages;
     int32_t max_pages;
     int32_t page_size;         /* a multiple of 16 */

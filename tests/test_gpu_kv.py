@@ -489,7 +489,7 @@ def test_refusals():
     bad(cache.assign, 0, [0] * (cache.max_pages + 1))
     bad(Int4KVCache, 2, 4, 2, 96)
     bad(Int4KVCache, 2, 4, 2, 128, 24)
-    bad(Int4KVCache, 2049, 4, 2)
+    bad(Int4KVCache, 1025, 4, 2)
     bad(Int4KVCache, 2, 4, 2, 128, 64, units=torch.zeros(3, dtype=torch.uint8, device="cuda"))
     bad(Int4KVCache, 2, 4, 2, 128, 64, meta=torch.zeros(3, dtype=torch.int32, device="cuda"))
     bad(Int4KVCache, 2, 4, 2, 128, 64, page_table=torch.zeros(2, 9, dtype=torch.int32, device="cuda"))

@@ -64,7 +64,7 @@ def test_every_call_checks_the_cache(call):
     for bad in (dict(page_size=24), dict(page_size=0), dict(page_size=-16), dict(kv_heads=0), dict(n_seqs=-1),
                 dict(n_pages=-1), dict(max_pages=-1)):
         assert call(cache(**bad)) == shape, bad
-    for bad in (dict(head_dim=96), dict(head_dim=0), dict(n_seqs=2049), dict(max_pages=1 << 25), dict(kv_heads=1 << 17)):
+    for bad in (dict(head_dim=96), dict(head_dim=0), dict(n_seqs=1025), dict(max_pages=1 << 25), dict(kv_heads=1 << 17)):
         assert call(cache(**bad)) == unsup, bad
     assert call(cache(n_seqs=0, lengths=None, evicted=None, arrivals=None)) == _lib.DQ_OK
 
