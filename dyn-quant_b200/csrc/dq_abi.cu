@@ -430,7 +430,7 @@ dq_status_t dq_kv_append(const dq_kv_cache_t* cache, const uint16_t* k, const in
 
 static dq_status_t check_kv_rows(const dq_kv_cache_t* c, int32_t tokens, int32_t q_heads) {
     if (tokens < 0 || q_heads <= 0 || q_heads % c->kv_heads != 0) return DQ_ERR_SHAPE;
-    if (static_cast<long long>(tokens) * q_heads > (1ll << 28)) return DQ_ERR_UNSUPPORTED;
+    if (static_cast<long long>(tokens) * q_heads > (1ll << 26)) return DQ_ERR_UNSUPPORTED;
     return DQ_OK;
 }
 

@@ -12,23 +12,27 @@
 // warp streams its run through a ring of bulk copies of its own; job borders do
 // not interrupt the stream.  A job inside one run is finished there.  The pieces
 // of the others meet in shared memory when their CTA's warps (neighbouring
-// runs) are done, and what a CTA's border still cuts leaves its partial sums
-// (maximum, sum, unnormalised output) in the workspace for kv_combine_kernel.
-// All sums have a fixed order.
+// runs) are done.  What a CTA's border still cuts leaves its partial sums
+// (maximum, sum, unnormalised output) in the workspace, and the last of the
+// job's CTAs to arrive joins them (for several row tiles, kv_combine_kernel
+// does).  All sums have a fixed order.
 //
 // Products (mma.sync.m16n8k16, f16 x f16 -> f32) are transposed, so that the 16
 // slots of a unit are the MMA's rows and the query rows its 8 columns:
-//   S^T = K Q^T   A = 16 slots x 16 columns of K, B = Q^T
+//   S^T = K Q^T    A = 16 slots x 16 columns of K, B = Q^T
 //   O^T = V^T P^T A = 16 columns of V x 16 slots, B = P^T
 // A decode step has at most 8 rows per KV head, so nothing of an MMA is idle,
 // and a lane's S values (slots g, g + 8; rows 2t, 2t + 1) lie in the lanes that
 // hold its O columns' rows: maxima, sums and rescaling stay in the lane.
-// Codes become f16 integers c - 8 exactly: (bits 0..3 | 0x6400) is 1024 + c and
-// (bits 4..7 | 0x5400) is 64 + c, one f16x2 subtraction takes 1032 or 72; a word
-// of eight codes costs one shift, four lop3 and four subtractions.  Scales and
-// zeros are applied in FP32:
-//   S   = s_k (D - (z_k - 8) sum q),  D the MMA's sum of q (c - 8)
+// Codes are used as they lie: a nibble at bits 0..3 or 4..7 of a half word is the
+// subnormal f16 number c 2^-24 or c 2^-20, which an MMA multiplies exactly, so a
+// word of eight codes costs one shift and four masks.  Scores keep the two
+// weights in two accumulators; in the output they lie in different rows of the
+// MMA and are set right at the end.  Scales and zeros are applied in FP32:
+//   S   = s_k (D - z_k sum q),  D the MMAs' sum of q c
 //   O   = sum p' (c - 8) - sum p' (z_v - 8),  p' = p s_v w
+// The 8 is taken off by a second MMA with a constant A, which keeps the running
+// sums (FP32, and the rounding of p' in them) at the size of the centred values.
 // p' is the only rounding to FP16 besides the output's: p <= 2^8 (the maximum
 // is taken again only when a score passes it by 8) and w is the power of two
 // that brings the largest s_v seen to at most 2^7, so p' <= 2^15 and small
@@ -45,6 +49,7 @@ constexpr int kAtMaxWarps = 2560;     // bound on the grid's warps (workspace si
 constexpr float kNone = -1e30f;       // running maximum of a row that has seen no key
 constexpr float kLazy = 8.0f;         // a score passes the running maximum by this much (log2) before it moves
 constexpr int kStep = 2 * kKvTokens;  // slots of one step of a run
+constexpr float kCode = 16777216.0f;  // 2^24: a masked code is c / kCode
 
 // Warps of a CTA and CTAs of an SM for row tiles of 8 NT rows: two row tiles
 // need 168 registers a thread, one tile 128.
@@ -62,35 +67,50 @@ struct KvAttendArgs {
     float* part;             // [CTAs][2][rows][D]
     float* part_ml;          // [CTAs][2][rows][2]
     int* pre;                // [n_seqs + 1] the plan's prefix sums, for the combining kernel
+    uint32_t* done;          // [n_seqs][heads] CTAs of a cut job that have arrived (one row tile)
     int tokens, group, n_rt; // query tokens, query heads per KV head, row tiles
-    float scale2;            // scale * log2(e)
+    float scale2;            // scale * log2(e) * kCode
     int depth;               // ring slots per warp
 };
 
 // The list of steps: a job is steps_of(len[b]) steps of one (sequence, KV head,
 // row tile), a sequence has `jobs` of them one after another, pre[b] counts the
 // steps of one job of every sequence before b.  Warp w takes base steps, one
-// more if w < rem.
+// more if w < rem.  Short lists are cut into runs of up to 4 steps rather than
+// one: a job then needs fewer warps, and its pieces meet in one CTA.
+struct Runs {
+    long long base, total;
+    int rem;
+
+    __device__ __forceinline__ Runs() {}
+    __device__ __forceinline__ Runs(int job_steps, int n_seqs, int jobs, int warps) {
+        total = static_cast<long long>(job_steps) * jobs;
+        const int least = min(4, (job_steps + n_seqs - 1) / n_seqs);
+        if (total < static_cast<long long>(warps) * least) warps = max(1, static_cast<int>(total) / max(least, 1));
+        base = total / warps;
+        rem = static_cast<int>(total - base * warps);
+    }
+    __device__ __forceinline__ long long start(long long w) const {
+        return min(w * base + (w < rem ? w : rem), total);
+    }
+    // the warp whose run has step u
+    __device__ __forceinline__ long long warp_of(long long u) const {
+        const long long cut = rem * (base + 1);
+        return u < cut ? u / (base + 1) : rem + (u - cut) / base;
+    }
+};
+
 struct Plan {
     const int* pre;
     const int* len;
     int jobs;
-    long long base;
-    int rem;
+    Runs runs;
 };
 
 __host__ __device__ inline int steps_of(int len) { return (len + kStep - 1) / kStep; }
 
 // Bytes of the plan in shared memory.
 __host__ __device__ inline int plan_bytes(int n_seqs) { return ((2 * n_seqs + 1) * 4 + 127) / 128 * 128; }
-
-__device__ __forceinline__ long long warp_start(long long base, int rem, long long w) {
-    return w * base + (w < rem ? w : rem);
-}
-__device__ __forceinline__ long long warp_of(long long base, int rem, long long u) {
-    const long long cut = rem * (base + 1);
-    return u < cut ? u / (base + 1) : rem + (u - cut) / base;
-}
 
 // Built by every CTA from the lengths (a few KB from L2); all threads call it.
 template <int NT>
@@ -132,9 +152,7 @@ __device__ Plan make_plan(const KvView& c, int jobs, int warps, char* smem, unsi
     p.pre = pre;
     p.len = lens;
     p.jobs = jobs;
-    const long long total = static_cast<long long>(run) * jobs;
-    p.base = total / warps;
-    p.rem = static_cast<int>(total - p.base * warps);
+    p.runs = Runs(run, c.n_seqs, jobs, warps);
     return p;
 }
 
@@ -143,8 +161,13 @@ struct StepAt {
     int b, len, job, step;
 };
 
+// a / b for a >= 0, with the short division where it does.
+__device__ __forceinline__ int quotient(long long a, int b) {
+    return (a >> 32) == 0 ? static_cast<int>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : static_cast<int>(a / b);
+}
+
 __device__ __forceinline__ StepAt step_at(const Plan& p, int n_seqs, long long u) {
-    const int v = static_cast<int>(u / p.jobs);  // pre[b] <= v < pre[b + 1]: the last b with pre[b] <= v
+    const int v = quotient(u, p.jobs);  // pre[b] <= v < pre[b + 1]: the last b with pre[b] <= v
     int lo = 0, hi = n_seqs;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -156,17 +179,41 @@ __device__ __forceinline__ StepAt step_at(const Plan& p, int n_seqs, long long u
     StepAt a;
     a.b = lo;
     a.len = p.len[lo];
-    a.job = static_cast<int>(r / st);
+    a.job = quotient(r, st);
     a.step = static_cast<int>(r - static_cast<long long>(a.job) * st);
     return a;
 }
 
-// f16 pairs (c - 8) of the nibbles at bits 0..3 and 16..19, and at bits 4..7 and 20..23.
-__device__ __forceinline__ uint32_t low_codes(uint32_t w) {
-    return hsub2_u32(lop3_and_or(w, 0x000F000Fu, 0x64006400u), 0x64086408u);  // (1024 + c) - 1032
+// f16 pairs c 2^-24 of the nibbles at bits 0..3 and 16..19, c 2^-20 of those at bits 4..7 and 20..23.
+__device__ __forceinline__ uint32_t low_codes(uint32_t w) { return w & 0x000F000Fu; }
+__device__ __forceinline__ uint32_t high_codes(uint32_t w) { return w & 0x00F000F0u; }
+
+// mma_16816 that the compiler may move (it has no effect besides its result).
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t high_codes(uint32_t w) {
-    return hsub2_u32(lop3_and_or(w, 0x00F000F0u, 0x54005400u), 0x54805480u);  // (64 + c) - 72
+
+// Dynamic shared memory by its byte offset.
+template <class T>
+__device__ __forceinline__ T smem_at(int off) {
+    extern __shared__ __align__(128) char smem[];
+    return *reinterpret_cast<const T*>(smem + off);
+}
+
+// D/32 words at once: 16 or 8 bytes.
+template <int D>
+__device__ __forceinline__ void load_words(int off, uint32_t (&w)[D / 32]) {
+    if (D == 128) {
+        const uint4 x = smem_at<uint4>(off);
+        w[0] = x.x; w[1] = x.y; w[D / 32 - 2] = x.z; w[D / 32 - 1] = x.w;
+    } else {
+        const uint2 x = smem_at<uint2>(off);
+        w[0] = x.x; w[1] = x.y;
+    }
 }
 
 // An 8x8 matrix of b16 in the MMA layout, transposed across the warp.
@@ -216,7 +263,7 @@ __device__ __forceinline__ void store_lse(const KvAttendArgs& a, int b, int tok,
 template <int D, int NT>
 struct QueryTile {
     uint32_t f[NT][D / 8];  // per 8-column word: (0,4), (1,5), (2,6), (3,7)
-    float sum[NT][2];       // sum of q over the columns, rows 2t and 2t + 1
+    float sum[NT][2];       // sum of q over the columns / kCode, rows 2t and 2t + 1
     int lim[NT][2];         // keys that rows 2t and 2t + 1 see
     int min_lim, max_lim;   // over the tile's rows
 
@@ -255,7 +302,7 @@ struct QueryTile {
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                sum[nt][e] = __shfl_sync(0xffffffffu, s, 8 * t + 4 * e);
+                sum[nt][e] = __shfl_sync(0xffffffffu, s, 8 * t + 4 * e) * (1.f / kCode);
                 lim[nt][e] = __shfl_sync(0xffffffffu, l, 8 * t + 4 * e);
             }
         }
@@ -264,41 +311,40 @@ struct QueryTile {
     }
 };
 
-// D of U units: the MMA's sums of q (c - 8) for slots g, g + 8 and rows 2t, 2t + 1.
+// D / kCode of U units: the MMAs' sums of q c for slots g, g + 8 and rows 2t, 2t + 1.
 template <int D, int NT, int U>
-__device__ __forceinline__ void score_mma(uint32_t unit, const QueryTile<D, NT>& q, float (&s)[U][NT][4]) {
+__device__ __forceinline__ void score_mma(int unit, const QueryTile<D, NT>& q, float (&s)[U][NT][4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint32_t k0[U][D / 32], k1[U][D / 32];
+    float lo[U][NT][4], hi[U][NT][4];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const uint32_t at = unit + u * kv_unit_bytes(D) + g * (D / 2) + t * (D / 8);
-        if (D == 128) {
-            const uint4 x = lds_v4(at), y = lds_v4(at + 8 * (D / 2));
-            k0[u][0] = x.x; k0[u][1] = x.y; k0[u][D / 32 - 2] = x.z; k0[u][D / 32 - 1] = x.w;
-            k1[u][0] = y.x; k1[u][1] = y.y; k1[u][D / 32 - 2] = y.z; k1[u][D / 32 - 1] = y.w;
-        } else {
-            const uint2 x = lds_v2(at), y = lds_v2(at + 8 * (D / 2));
-            k0[u][0] = x.x; k0[u][1] = x.y;
-            k1[u][0] = y.x; k1[u][1] = y.y;
-        }
+        const int at = unit + u * kv_unit_bytes(D) + g * (D / 2) + t * (D / 8);
+        load_words<D>(at, k0[u]);
+        load_words<D>(at + 8 * (D / 2), k1[u]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[u][nt][e] = 0.f;
+            for (int e = 0; e < 4; ++e) lo[u][nt][e] = hi[u][nt][e] = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const uint32_t w0 = k0[u][i], w1 = k1[u][i], x0 = w0 >> 8, x1 = w1 >> 8;
-            const uint32_t a0 = low_codes(w0), a1 = low_codes(w1), a2 = high_codes(w0), a3 = high_codes(w1);
-            const uint32_t b0 = low_codes(x0), b1 = low_codes(x1), b2 = high_codes(x0), b3 = high_codes(x1);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                mma_16816(s[u][nt], a0, a1, a2, a3, q.f[nt][4 * i], q.f[nt][4 * i + 1]);
-                mma_16816(s[u][nt], b0, b1, b2, b3, q.f[nt][4 * i + 2], q.f[nt][4 * i + 3]);
+                mma(lo[u][nt], low_codes(w0), low_codes(w1), low_codes(x0), low_codes(x1), q.f[nt][4 * i], q.f[nt][4 * i + 2]);
+                mma(hi[u][nt], high_codes(w0), high_codes(w1), high_codes(x0), high_codes(x1), q.f[nt][4 * i + 1],
+                    q.f[nt][4 * i + 3]);
             }
         }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[u][nt][e] = fmaf(hi[u][nt][e], 0.0625f, lo[u][nt][e]);
 }
 
 // A warp's run of steps through its ring: lane i % 32 of each 32 steps looks
@@ -307,7 +353,7 @@ template <int D, bool kKeysOnly>
 struct StepStream {
     static constexpr int kUnit = kv_unit_bytes(D);
     static constexpr int kSlot = 2 * kUnit;
-    uint32_t ring, bars, flags;  // shared-memory addresses of this warp's slots, barriers, units-found words
+    int ring, bars, flags;       // offsets in shared memory of this warp's slots, barriers, units-found words
     int depth, n, issued, parity, slot;
     bool absent;                 // some unit of the run lies in no page of the pool
     long long u0;
@@ -316,13 +362,17 @@ struct StepStream {
     // Bytes of `warps` rings behind `smem`.
     static __host__ __device__ int bytes(int warps, int depth) { return (warps * depth * (kSlot + 12) + 127) / 128 * 128; }
 
-    __device__ __forceinline__ void init(char* smem, int warps, int warp, int depth_) {
+    static __device__ __forceinline__ uint32_t base() {
+        extern __shared__ __align__(128) char smem[];
+        return smem_u32(smem);
+    }
+    __device__ __forceinline__ void init(int off, int warps, int warp, int depth_) {
         depth = depth_;
-        ring = smem_u32(smem) + warp * depth * kSlot;
-        bars = smem_u32(smem) + warps * depth * kSlot + warp * depth * 8;
-        flags = smem_u32(smem) + warps * depth * (kSlot + 8) + warp * depth * 4;
+        ring = off + warp * depth * kSlot;
+        bars = off + warps * depth * kSlot + warp * depth * 8;
+        flags = off + warps * depth * (kSlot + 8) + warp * depth * 4;
         if ((threadIdx.x & 31) == 0)
-            for (int i = 0; i < depth; ++i) mbar_init(bars + 8 * i, 1);
+            for (int i = 0; i < depth; ++i) mbar_init(base() + bars + 8 * i, 1);
         fence_mbar_init();
         __syncwarp();
     }
@@ -348,10 +398,10 @@ struct StepStream {
     __device__ __forceinline__ void issue(const KvAttendArgs& a, const Plan& p, int s) {
         if ((issued & 31) == 0) lookup(a, p);
         if ((threadIdx.x & 31) == (issued & 31)) {
-            const uint32_t bar = bars + 8 * s, dst = ring + s * kSlot;
+            const uint32_t bar = base() + bars + 8 * s, dst = base() + ring + s * kSlot;
             const bool f0 = src[0] >= 0, f1 = src[1] >= 0;
             constexpr uint32_t kKeys = kKeysOnly ? 8 * D + kKvTokens * 8 : kUnit;
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(flags + 4 * s), "r"((f0 ? 1u : 0u) | (f1 ? 2u : 0u)) : "memory");
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(base() + flags + 4 * s), "r"((f0 ? 1u : 0u) | (f1 ? 2u : 0u)) : "memory");
             if (!f0 && !f1) {
                 mbar_arrive(bar);
             } else {
@@ -386,12 +436,12 @@ struct StepStream {
     }
     // Wait for the step in the current slot; false when the bounded wait gave up.
     __device__ __forceinline__ bool wait() {
-        const bool got = mbar_wait_bounded(bars + 8 * slot, parity);
+        const bool got = mbar_wait_bounded(base() + bars + 8 * slot, parity);
         return __all_sync(0xffffffffu, got);
     }
-    __device__ __forceinline__ uint32_t unit() const { return ring + slot * kSlot; }
+    __device__ __forceinline__ int unit() const { return ring + slot * kSlot; }
     // Bit e: unit e of the step was copied (only asked for when some unit of the run is absent).
-    __device__ __forceinline__ uint32_t found() const { return lds_u32(flags + 4 * slot); }
+    __device__ __forceinline__ uint32_t found() const { return smem_at<uint32_t>(flags + 4 * slot); }
     // The current slot is read: refill it, go to the next.
     __device__ __forceinline__ void next(const KvAttendArgs& a, const Plan& p) {
         __syncwarp();
@@ -402,7 +452,7 @@ struct StepStream {
     __device__ __forceinline__ void drain(int consumed) {
         if ((threadIdx.x & 31) == 0) atomicOr(&g_kv_attend_error, kKvErrWait);
         for (int i = consumed; i < issued; ++i) {
-            mbar_wait_bounded(bars + 8 * slot, parity);
+            mbar_wait_bounded(base() + bars + 8 * slot, parity);
             if (++slot == depth) { slot = 0; parity ^= 1; }
         }
     }
@@ -412,8 +462,8 @@ struct StepStream {
 struct KeyParams {
     float s0, z0, s1, z1;
     __device__ __forceinline__ KeyParams(uint2 p0, uint2 p1, float scale2)
-        : s0(h2f_bits(lo16(p0.x)) * scale2), z0(h2f_bits(hi16(p0.x)) - 8.f),
-          s1(h2f_bits(lo16(p1.x)) * scale2), z1(h2f_bits(hi16(p1.x)) - 8.f) {}
+        : s0(h2f_bits(lo16(p0.x)) * scale2), z0(h2f_bits(hi16(p0.x))),
+          s1(h2f_bits(lo16(p1.x)) * scale2), z1(h2f_bits(hi16(p1.x))) {}
 };
 
 // The running softmax of one job in one warp.
@@ -436,14 +486,14 @@ struct RowState {
 
     // U units from slot j of the sequence on.  found: bit u set where unit u is there.
     template <int U>
-    __device__ __forceinline__ void add(const QueryTile<D, NT>& q, uint32_t unit, int j, int len, uint32_t found, float scale2) {
+    __device__ __forceinline__ void add(const QueryTile<D, NT>& q, int unit, int j, int len, uint32_t found, float scale2) {
         const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
         float s[U][NT][4], sv[U][2], zv[U][2];
         score_mma<D, NT, U>(unit, q, s);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const uint32_t pa = unit + u * kv_unit_bytes(D) + kv_param_offset(D) + 8 * g;
-            const uint2 p0 = lds_v2(pa), p1 = lds_v2(pa + 64);
+            const int pa = unit + u * kv_unit_bytes(D) + kv_param_offset(D) + 8 * g;
+            const uint2 p0 = smem_at<uint2>(pa), p1 = smem_at<uint2>(pa + 64);
             const KeyParams k(p0, p1, scale2);
             sv[u][0] = h2f_bits(lo16(p0.y)); zv[u][0] = h2f_bits(hi16(p0.y)) - 8.f;
             sv[u][1] = h2f_bits(lo16(p1.y)); zv[u][1] = h2f_bits(hi16(p1.y)) - 8.f;
@@ -509,25 +559,21 @@ struct RowState {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             uint32_t v0[D / 32], v1[D / 32];
-            const uint32_t vb = unit + u * kv_unit_bytes(D) + kv_v_offset(D) + t * D + g * (D / 8);
-            if (D == 128) {
-                const uint4 x = lds_v4(vb), y = lds_v4(vb + 4 * D);
-                v0[0] = x.x; v0[1] = x.y; v0[D / 32 - 2] = x.z; v0[D / 32 - 1] = x.w;
-                v1[0] = y.x; v1[1] = y.y; v1[D / 32 - 2] = y.z; v1[D / 32 - 1] = y.w;
-            } else {
-                const uint2 x = lds_v2(vb), y = lds_v2(vb + 4 * D);
-                v0[0] = x.x; v0[1] = x.y;
-                v1[0] = y.x; v1[1] = y.y;
-            }
+            const int vb = unit + u * kv_unit_bytes(D) + kv_v_offset(D) + t * D + g * (D / 8);
+            load_words<D>(vb, v0);
+            load_words<D>(vb + 4 * D, v1);
+            // rows g of an MMA are columns of low nibbles, rows g + 8 of high ones: -8 in either
+            constexpr uint32_t kLow8 = 0x80088008u, kHigh8 = 0x80808080u;
 #pragma unroll
             for (int k = 0; k < D / 32; ++k) {
-                const uint32_t y0 = v0[k] >> 8, y1 = v1[k] >> 8;
-                const uint32_t a0 = low_codes(v0[k]), a1 = high_codes(v0[k]), a2 = low_codes(v1[k]), a3 = high_codes(v1[k]);
-                const uint32_t b0 = low_codes(y0), b1 = high_codes(y0), b2 = low_codes(y1), b3 = high_codes(y1);
+                const uint32_t w0 = v0[k], w1 = v1[k], y0 = w0 >> 8, y1 = w1 >> 8;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    mma_16816(o[nt][2 * k], a0, a1, a2, a3, pf[u][nt][0], pf[u][nt][1]);
-                    mma_16816(o[nt][2 * k + 1], b0, b1, b2, b3, pf[u][nt][0], pf[u][nt][1]);
+                    const uint32_t b0 = pf[u][nt][0], b1 = pf[u][nt][1];
+                    mma(o[nt][2 * k], low_codes(w0), high_codes(w0), low_codes(w1), high_codes(w1), b0, b1);
+                    mma(o[nt][2 * k + 1], low_codes(y0), high_codes(y0), low_codes(y1), high_codes(y1), b0, b1);
+                    mma(o[nt][2 * k], kLow8, kHigh8, kLow8, kHigh8, b0, b1);
+                    mma(o[nt][2 * k + 1], kLow8, kHigh8, kLow8, kHigh8, b0, b1);
                 }
             }
         }
@@ -562,12 +608,86 @@ struct RowState {
         const float z = lane_sum_g(zs[nt][e]), inv = __uint_as_float(0x7F000000u - __float_as_uint(vw));  // 1 / vw
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-            v[2 * k] = (o[nt][k][e] - z) * inv;
-            v[2 * k + 1] = (o[nt][k][e + 2] - z) * inv;
+            v[2 * k] = fmaf(o[nt][k][e], kCode, -z) * inv;
+            v[2 * k + 1] = fmaf(o[nt][k][e + 2], kCode / 16.f, -z) * inv;
         }
         return lane_sum_g(l[nt][e]);
     }
 };
+
+// Columns col .. col + N - 1 of row r of KV head h, normalised; the thread with column 0 stores the row's lse.
+template <int N>
+__device__ __forceinline__ void store_row(const KvAttendArgs& a, int b, int h, int r, int col, const float (&v)[N], float m,
+                                          float sum) {
+    const int tok = r / a.group, head = h * a.group + r - tok * a.group;
+    const float f = row_norm(sum);
+    uint16_t* dst = a.out + b * a.os[0] + tok * a.os[1] + head * a.os[2] + col;
+#pragma unroll
+    for (int i = 0; i < N; i += 8)
+        *reinterpret_cast<uint4*>(dst + i) =
+            make_uint4(pack_f32(v[i] * f, v[i + 1] * f), pack_f32(v[i + 2] * f, v[i + 3] * f),
+                       pack_f32(v[i + 4] * f, v[i + 5] * f), pack_f32(v[i + 6] * f, v[i + 7] * f));
+    if (col == 0) store_lse(a, b, tok, head, m, sum);
+}
+
+// The CTAs that share a job (c0 .. c0 + n - 1) and the workspace slot of the first; every later CTA begins
+// inside the job, which is its slot 0.
+struct Share {
+    long long c0;
+    int n, slot0;
+};
+
+template <int W>
+__device__ __forceinline__ Share share_of(const int* pre, int n_seqs, int jobs, const Runs& runs, int b, int job) {
+    Share s{0, 0, 0};
+    const int p0 = pre[b], ul = pre[b + 1] - p0;
+    if (ul == 0) return s;
+    const long long u0 = static_cast<long long>(p0) * jobs + static_cast<long long>(ul) * job;
+    s.c0 = runs.warp_of(u0) / W;
+    s.n = static_cast<int>(runs.warp_of(u0 + ul - 1) / W - s.c0) + 1;
+    const long long start = runs.start(s.c0 * W);
+    if (s.n > 1 && u0 > start) {
+        // the job at the CTA's start has slot 0 if the border cuts it
+        const int v = quotient(start, jobs);
+        int lo = 0, hi = b + 1;  // pre[lo] <= v < pre[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (pre[mid] <= v) lo = mid;
+            else hi = mid;
+        }
+        s.slot0 = (start - static_cast<long long>(pre[lo]) * jobs) % (pre[lo + 1] - pre[lo]) != 0 ? 1 : 0;
+    }
+    return s;
+}
+
+// One warp joins row r's partial sums: the maxima first, a lane each, then the outputs with independent loads.
+template <int D, int NT>
+__device__ __forceinline__ void join_row(const KvAttendArgs& a, const Share& s, int b, int h, int rt, int r) {
+    constexpr int R = 8 * NT, V = D / 32;  // V columns of a lane
+    const int lane = threadIdx.x & 31, rl = r - rt * R;
+    auto at = [&](int i) { return (static_cast<size_t>(s.c0 + i) * 2 + (i == 0 ? s.slot0 : 0)) * R + rl; };
+    float m = kNone;
+    for (int i = lane; i < s.n; i += 32) m = fmaxf(m, ldcg_f32(a.part_ml + 2 * at(i)));
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float sum = 0.f, v[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < s.n; ++i) {
+        const size_t pi = at(i);
+        const float f = ex2(ldcg_f32(a.part_ml + 2 * pi) - m);
+        sum += ldcg_f32(a.part_ml + 2 * pi + 1) * f;
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] += ldcg_f32(a.part + pi * D + lane + 32 * k) * f;
+    }
+    const int tok = r / a.group, head = h * a.group + r - tok * a.group;
+    const float f = row_norm(sum);
+    uint16_t* dst = a.out + b * a.os[0] + tok * a.os[1] + head * a.os[2];
+#pragma unroll
+    for (int k = 0; k < V; ++k) dst[lane + 32 * k] = __half_as_ushort(__float2half_rn(v[k] * f));
+    if (lane == 0) store_lse(a, b, tok, head, m, sum);
+}
 
 // A piece of a job that its run cut: which job and which of its steps.
 struct Piece {
@@ -584,10 +704,11 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
     __shared__ Piece pieces[2 * W];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const KvView& c = a.c;
+    __shared__ int last;
     char* at = smem + plan_bytes(c.n_seqs);
-    StepStream<D, false> st;
     char* rings = at + W * kPiece * 4;
-    st.init(rings, W, warp, a.depth);
+    StepStream<D, false> st;
+    st.init(static_cast<int>(rings - smem), W, warp, a.depth);
     // A piece is [R][D + 2] floats: output, maximum, sum.  A warp's first piece has room of its own, its
     // last one takes the warp's ring, which has run dry by then.
     auto piece_at = [&](int k) {
@@ -596,11 +717,11 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
     pdl_launch_dependents();
     pdl_wait();
     const Plan p = make_plan<32 * W>(c, c.heads * a.n_rt, gridDim.x * W, smem, blockIdx.x == 0 ? &g_kv_attend_error : nullptr);
-    if (blockIdx.x == 0)
+    if (a.n_rt > 1 && blockIdx.x == 0)
         for (int b = threadIdx.x; b <= c.n_seqs; b += 32 * W) a.pre[b] = p.pre[b];
     const long long w = static_cast<long long>(blockIdx.x) * W + warp;
-    const long long u0 = warp_start(p.base, p.rem, w);
-    const int n = static_cast<int>(warp_start(p.base, p.rem, w + 1) - u0);
+    const long long u0 = p.runs.start(w);
+    const int n = static_cast<int>(p.runs.start(w + 1) - u0);
     if (lane < 2) pieces[2 * warp + lane].job = -1;
     __syncwarp();
     const int rows = a.tokens * a.group;
@@ -662,15 +783,7 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
                     const int rl = nt * 8 + 2 * t + e, r = rt * R + rl;
                     if (r >= rows) continue;
                     if (whole) {
-                        const int tok = r / a.group, head = h * a.group + r % a.group;
-                        const float f = row_norm(sum);
-                        uint16_t* dst = a.out + b * a.os[0] + tok * a.os[1] + head * a.os[2] + (D / 8) * g;
-#pragma unroll
-                        for (int i = 0; i < D / 8; i += 8)
-                            *reinterpret_cast<uint4*>(dst + i) =
-                                make_uint4(pack_f32(v[i] * f, v[i + 1] * f), pack_f32(v[i + 2] * f, v[i + 3] * f),
-                                           pack_f32(v[i + 4] * f, v[i + 5] * f), pack_f32(v[i + 6] * f, v[i + 7] * f));
-                        if (g == 0) store_lse(a, b, tok, head, rs.m[nt][e], sum);
+                        store_row(a, b, h, r, (D / 8) * g, v, rs.m[nt][e], sum);
                     } else {
                         float* dst = piece_at(k) + rl * (D + 2);
 #pragma unroll
@@ -683,6 +796,16 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
             done += take;
             left -= take;
             if (ub == ul) { ub = 0; ++job; }
+        }
+    }
+    // rows of sequences without slots
+    for (int b = blockIdx.x; b < c.n_seqs; b += gridDim.x) {
+        if (p.len[b] != 0) continue;
+        const int hq = c.heads * a.group;
+        for (int i = threadIdx.x; i < a.tokens * hq * (D / 8); i += 32 * W) {
+            const int x = i / (D / 8), tok = x / hq, head = x - tok * hq, col = 8 * (i % (D / 8));
+            *reinterpret_cast<uint4*>(a.out + b * a.os[0] + tok * a.os[1] + head * a.os[2] + col) = make_uint4(0, 0, 0, 0);
+            if (col == 0) store_lse(a, b, tok, head, 0.f, 0.f);
         }
     }
     __syncthreads();
@@ -723,12 +846,7 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
                 }
             }
             if (whole) {
-                const int tok = r / a.group, head = h * a.group + r % a.group;
-                const float f = row_norm(sum);
-                *reinterpret_cast<uint4*>(a.out + first.b * a.os[0] + tok * a.os[1] + head * a.os[2] + col) =
-                    make_uint4(pack_f32(v[0] * f, v[1] * f), pack_f32(v[2] * f, v[3] * f), pack_f32(v[4] * f, v[5] * f),
-                               pack_f32(v[6] * f, v[7] * f));
-                if (col == 0) store_lse(a, first.b, tok, head, m, sum);
+                store_row(a, first.b, h, r, col, v, m, sum);
             } else {
                 const size_t pi = (static_cast<size_t>(blockIdx.x) * 2 + slot) * R + rl;
                 float4* dst = reinterpret_cast<float4*>(a.part + pi * D + col);
@@ -737,6 +855,21 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
                 if (col == 0) *reinterpret_cast<float2*>(a.part_ml + pi * 2) = make_float2(m, sum);
             }
         }
+        if (!whole && a.n_rt == 1) {
+            // one row tile: the last of the job's CTAs to arrive joins the partial sums, in CTA order
+            const Share s = share_of<W>(p.pre, c.n_seqs, p.jobs, p.runs, first.b, first.job);
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                __threadfence();
+                uint32_t* d = a.done + static_cast<size_t>(first.b) * c.heads + first.job;
+                last = atomicAdd(d, 1u) == static_cast<uint32_t>(s.n - 1);
+                if (last) *d = 0;
+                __threadfence();
+            }
+            __syncthreads();
+            if (last)
+                for (int r = warp; r < rows; r += W) join_row<D, NT>(a, s, first.b, h, 0, r);
+        }
         if (!whole) slot = 1;
         k = k1;
     }
@@ -744,72 +877,26 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
 }
 
 // ---------------------------------------------------------------------------
-// Joins the partial sums of the jobs cut between CTAs, in CTA order; writes the
-// rows of sequences without keys.  One warp per row: the maxima first, a lane
-// each, then the outputs with independent loads.
+// Joins the partial sums of the jobs cut between CTAs when a KV head's rows fill
+// several tiles (their jobs have no arrival counters).  One warp per row.
 // ---------------------------------------------------------------------------
 constexpr int kCbWarps = 4;
 
 template <int D, int NT>
 __global__ void __launch_bounds__(32 * kCbWarps) kv_combine_kernel(const KvAttendArgs a, const int ctas) {
-    constexpr int W = at_warps(NT), R = 8 * NT, V = D / 32;  // V columns of a lane
     const KvView& c = a.c;
-    const int lane = threadIdx.x & 31, hq = c.heads * a.group;
+    const int hq = c.heads * a.group, jobs = c.heads * a.n_rt;
     pdl_launch_dependents();
     pdl_wait();
     const long long item = static_cast<long long>(blockIdx.x) * kCbWarps + (threadIdx.x >> 5);
     if (item >= static_cast<long long>(c.n_seqs) * a.tokens * hq) return;
-    const int head = static_cast<int>(item % hq);
     const long long bt = item / hq;
-    const int b = static_cast<int>(bt / a.tokens), tok = static_cast<int>(bt % a.tokens);
-    const int h = head / a.group, r = tok * a.group + head % a.group, rt = r / R, rl = r % R;
-    const int jobs = c.heads * a.n_rt;
-    const int p0 = static_cast<int>(ldcg_u32(a.pre + b)), ul = static_cast<int>(ldcg_u32(a.pre + b + 1)) - p0;
-    const long long total = static_cast<long long>(static_cast<int>(ldcg_u32(a.pre + c.n_seqs))) * jobs;
-    const long long base = total / (static_cast<long long>(ctas) * W);
-    const int rem = static_cast<int>(total - base * ctas * W);
-    long long c0 = 0;
-    int np = 0, first_slot = 0;
-    if (ul > 0) {
-        const long long u0 = static_cast<long long>(p0) * jobs + static_cast<long long>(ul) * (h * a.n_rt + rt);
-        c0 = warp_of(base, rem, u0) / W;
-        np = static_cast<int>(warp_of(base, rem, u0 + ul - 1) / W - c0) + 1;
-        if (np == 1) return;  // finished by its CTA
-        // a CTA's first cut job is in its slot 0: this one, unless another reaches into the CTA from before
-        const long long start = warp_start(base, rem, c0 * W);
-        if (u0 > start) {
-            const int v = static_cast<int>(start / jobs);
-            int lo = 0, hi = b + 1;  // pre[lo] <= v < pre[hi]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (static_cast<int>(ldcg_u32(a.pre + mid)) <= v) lo = mid;
-                else hi = mid;
-            }
-            const int q0 = static_cast<int>(ldcg_u32(a.pre + lo)), qu = static_cast<int>(ldcg_u32(a.pre + lo + 1)) - q0;
-            first_slot = (start - static_cast<long long>(q0) * jobs) % qu != 0 ? 1 : 0;
-        }
-    }
-    float m = kNone;
-    for (int i = lane; i < np; i += 32)
-        m = fmaxf(m, ldcg_f32(a.part_ml + 2 * (((c0 + i) * 2 + (i == 0 ? first_slot : 0)) * R + rl)));
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float sum = 0.f, v[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < np; ++i) {
-        const size_t pi = ((c0 + i) * 2 + (i == 0 ? first_slot : 0)) * R + rl;
-        const float f = ex2(ldcg_f32(a.part_ml + 2 * pi) - m);
-        sum += ldcg_f32(a.part_ml + 2 * pi + 1) * f;
-#pragma unroll
-        for (int k = 0; k < V; ++k) v[k] += ldcg_f32(a.part + pi * D + lane + 32 * k) * f;
-    }
-    const float f = row_norm(sum);
-    uint16_t* dst = a.out + b * a.os[0] + tok * a.os[1] + head * a.os[2];
-#pragma unroll
-    for (int k = 0; k < V; ++k) dst[lane + 32 * k] = __half_as_ushort(__float2half_rn(v[k] * f));
-    if (lane == 0) store_lse(a, b, tok, head, m, sum);
+    const int head = static_cast<int>(item - bt * hq), b = static_cast<int>(bt / a.tokens);
+    const int tok = static_cast<int>(bt - static_cast<long long>(b) * a.tokens);
+    const int h = head / a.group, r = tok * a.group + head - h * a.group, rt = r / (8 * NT);
+    const Runs runs(a.pre[c.n_seqs], c.n_seqs, jobs, ctas * at_warps(NT));
+    const Share s = share_of<at_warps(NT)>(a.pre, c.n_seqs, jobs, runs, b, h * a.n_rt + rt);
+    if (s.n > 1) join_row<D, NT>(a, s, b, h, rt, r);  // else finished by its CTA, or empty
 }
 
 // ---------------------------------------------------------------------------
@@ -824,13 +911,13 @@ __global__ void __launch_bounds__(32 * at_warps(1), at_ctas(1)) kv_mass_kernel(c
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const KvView& c = a.c;
     StepStream<D, true> st;
-    st.init(smem + plan_bytes(c.n_seqs), W, warp, a.depth);
+    st.init(plan_bytes(c.n_seqs), W, warp, a.depth);
     pdl_launch_dependents();
     pdl_wait();
     const Plan p = make_plan<32 * W>(c, c.heads, gridDim.x * W, smem, nullptr);
     const long long w = static_cast<long long>(blockIdx.x) * W + warp;
-    const long long u0 = warp_start(p.base, p.rem, w);
-    const int n = static_cast<int>(warp_start(p.base, p.rem, w + 1) - u0);
+    const long long u0 = p.runs.start(w);
+    const int n = static_cast<int>(p.runs.start(w + 1) - u0);
     if (n == 0) return;
     st.start(a, p, u0, n);
     QueryTile<D, 1> q;
@@ -852,7 +939,8 @@ __global__ void __launch_bounds__(32 * at_warps(1), at_ctas(1)) kv_mass_kernel(c
             fresh = true;
         }
         if (!st.wait()) { st.drain(i); return; }
-        const uint32_t unit = st.unit(), found = st.found();
+        const int unit = st.unit();
+        const uint32_t found = st.found();
         float add[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
         for (int rt = 0; rt < n_rt; ++rt) {
             if (n_rt > 1 || fresh) {
@@ -874,8 +962,8 @@ __global__ void __launch_bounds__(32 * at_warps(1), at_ctas(1)) kv_mass_kernel(c
             score_mma<D, 1, 2>(unit, q, s);
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-                const uint32_t pa = unit + y * kv_unit_bytes(D) + kv_param_offset(D) + 8 * g;
-                const KeyParams k(lds_v2(pa), lds_v2(pa + 64), a.scale2);
+                const int pa = unit + y * kv_unit_bytes(D) + kv_param_offset(D) + 8 * g;
+                const KeyParams k(smem_at<uint2>(pa), smem_at<uint2>(pa + 64), a.scale2);
                 const int j0 = ub * kStep + y * kKvTokens + g, j1 = j0 + 8;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
@@ -940,7 +1028,8 @@ dq_status_t attend(KvAttendArgs& a, cudaStream_t stream) {
     if ((st = allow_smem(kv_attend_kernel<D, NT>, smem)) != DQ_OK) return st;
     if ((st = launch_pdl(kv_attend_kernel<D, NT>, dim3(grid), 32 * W, smem, stream, a)) != DQ_OK) return st;
     const long long items = static_cast<long long>(a.c.n_seqs) * a.tokens * a.c.heads * a.group;
-    st = launch_pdl(kv_combine_kernel<D, NT>, dim3(static_cast<unsigned>((items + kCbWarps - 1) / kCbWarps)),
+    if (a.n_rt > 1)
+        st = launch_pdl(kv_combine_kernel<D, NT>, dim3(static_cast<unsigned>((items + kCbWarps - 1) / kCbWarps)),
                     32 * kCbWarps, 0, stream, a, grid);
     if (st != DQ_OK || !a.lse2) return st;
     grid = di.sm_count * at_ctas(1);
@@ -983,7 +1072,8 @@ dq_status_t launch_kv_attend(const dq_kv_cache_t& c, const dq_kv_attend_t& r, vo
     a.counts = r.counts;
     a.tokens = r.tokens;
     a.group = r.q_heads / c.kv_heads;
-    a.scale2 = r.scale * 1.44269504088896341f;
+    a.scale2 = r.scale * (1.44269504088896341f * kCode);
+    a.done = c.arrivals + c.n_seqs;
     const AttendWs w = attend_ws(c, r.tokens, r.q_heads, r.accumulate != 0);
     char* base = static_cast<char*>(workspace);
     a.part = reinterpret_cast<float*>(base + w.part);

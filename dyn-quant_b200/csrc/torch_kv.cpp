@@ -47,7 +47,7 @@ public:
         TORCH_CHECK(seqs <= 1024, "at most 1024 sequences per cache");
         check(lengths, "lengths", at::kInt, {seqs});
         check(evicted, "evicted", at::kInt, {seqs});
-        check(arrivals, "arrivals", at::kInt, {seqs});
+        check(arrivals, "arrivals", at::kInt, {seqs * (1 + heads)});
         check(page_table, "page_table", at::kInt, {seqs, page_table.size(1)});
         TORCH_CHECK(pages <= INT32_MAX && heads <= 65535 && page_table.size(1) * page <= (int64_t{1} << 30),
                     "cache too large");
@@ -178,7 +178,7 @@ private:
         TORCH_CHECK(t.size(0) == c_.n_seqs && t.size(3) == c_.head_dim && (heads == 0 || t.size(2) == heads), name,
                     " does not fit the cache: n_seqs=", c_.n_seqs, " head_dim=", c_.head_dim, " kv_heads=", c_.kv_heads,
                     ", got ", t_in.sizes());
-        TORCH_CHECK(t.size(1) <= INT32_MAX && t.size(2) <= INT32_MAX && t.size(1) * t.size(2) <= (int64_t{1} << 28), name,
+        TORCH_CHECK(t.size(1) <= INT32_MAX && t.size(2) <= INT32_MAX && t.size(1) * t.size(2) <= (int64_t{1} << 26), name,
                     " has too many rows");
         if (t.scalar_type() != at::kHalf) t = t.to(at::kHalf);
         if (t.numel() && !direct(t)) t = t.contiguous();

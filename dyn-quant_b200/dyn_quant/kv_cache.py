@@ -92,7 +92,8 @@ class Int4KVCache:
             torch.full((n_seqs, max_pages), -1, dtype=torch.int32, device=dev)
         if tuple(self.page_table.shape) != (n_seqs, max_pages):
             raise RuntimeError(f"page_table must have shape {(n_seqs, max_pages)}, got {tuple(self.page_table.shape)}")
-        self._arrivals = torch.zeros(n_seqs, dtype=torch.int32, device=self.units.device)
+        self._arrivals = torch.zeros(n_seqs * (1 + n_kv_heads), dtype=torch.int32,
+                                     device=self.units.device)
         self._h = dyn_quant._C.KVCache(self.units, self.mass, self.pos, self.lengths, self.evicted, self.page_table,
                                        self._arrivals)
 
@@ -112,6 +113,8 @@ class Int4KVCache:
     def reset(self, seq: int | None = None) -> None:
         """Empty one sequence, or all of them (pages stay assigned)."""
         at = slice(None) if seq is None else seq
+        if seq is None:
+            self._arrivals.zero_()  # non-zero only after a call that reported a device error
         self.lengths[at] = 0
         self.evicted[at] = 0
 

@@ -409,7 +409,8 @@ typedef struct dq_kv_cache_t {
     int32_t* lengths;          /* [n_seqs] slots in use */
     int32_t* evicted;          /* [n_seqs] tokens evicted so far (positions seen = lengths + evicted) */
     const int32_t* page_table; /* [n_seqs][max_pages]; entries past a sequence's last page are not read */
-    uint32_t* arrivals;        /* [n_seqs] zero-filled once; every call leaves it at zero */
+    uint32_t* arrivals;        /* [n_seqs * (1 + kv_heads)] zero-filled once; every call leaves it at zero
+                                * (again after a call whose bounded wait gave up: dq_read_device_error) */
     int32_t n_seqs;            /* 0 .. 1024 */
     int32_t n_pages;
     int32_t max_pages;
@@ -468,7 +469,8 @@ DQ_API size_t dq_kv_attend_workspace_bytes(const dq_kv_cache_t* cache, int32_t t
  * sequence, i >= counts[b]) give out 0 and lse -infinity.  Units of a page
  * index outside the pool count as absent and set a bit of the device error
  * word.  Slots behind lengths[b] are not read into any result.  Results are
- * bit-reproducible.  Two kernels, three with accumulate.
+ * bit-reproducible.  One kernel when a KV head has at most 16 query rows (query
+ * tokens times its query heads), else two; one more with accumulate.
  */
 DQ_API dq_status_t dq_kv_attend(const dq_kv_cache_t* cache, const dq_kv_attend_t* args, void* workspace,
                                 size_t workspace_bytes, void* stream);

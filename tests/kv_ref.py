@@ -58,12 +58,12 @@ def attend(q, line, n, scale, count=None):
             out[i, a] = p @ v[e, :seen]
             lse[i, a] = m + np.log(w.sum())
             mass[e, :seen] += p
-            # Scores: the products q (c - 8) are exact; D/16 MMAs and the steps inside each add up FP32 sums
-            # (truncated at worst: a full ulp, 2^-23, of at most `terms`), then two FP32 operations.  A weight's
+            # Scores: the products q c are exact; D/16 MMAs and the steps inside each add up FP32 sums
+            # (truncated at worst: a full ulp, 2^-23, of at most `terms`), then three FP32 operations.  A weight's
             # relative error is twice the score's (the score and the sum's) plus the exponential's 2^-22 and the
             # subtraction of the maximum from a score of size |s|.
-            terms = abs(scale) * line["ks"][e, :seen] * (np.abs(q[i, a]) @ np.abs(line["kc"][e, :seen] - 8).T
-                                                   + np.abs(line["kz"][e, :seen] - 8) * np.abs(q[i, a]).sum())
+            terms = abs(scale) * line["ks"][e, :seen] * (np.abs(q[i, a]) @ line["kc"][e, :seen].T
+                                                         + np.abs(line["kz"][e, :seen]) * np.abs(q[i, a]).sum())
             rel = 2 * (24 * 2.0 ** -23 * terms.max() + 2.0 ** -22 + 2.0 ** -22 * np.abs(s).max()) + 2.0 ** -20
             # Output: p' = p s w is rounded to FP16 once (2^-11 of p s |c - 8|; below 2^-14 half of 2^-24, with
             # 1 / w <= 2^-6 max s), the sums are FP32 (one truncation per unit), the result is rounded to FP16.

@@ -62,7 +62,7 @@ def test_append_stores_the_quantizers_rows(dim, heads, page, t, starts, counts):
     cn = counts or [t] * n
     kv, vv = cache.append(k.cuda(), v.cuda(), counts=None if counts is None else ints(*counts), at=at, values=True)
     assert cache.lengths.tolist() == [s + c for s, c in zip(starts, cn)]
-    assert cache._arrivals.tolist() == [0] * n
+    assert not cache._arrivals.any()
     table = cache.page_table.cpu().numpy()
     written = torch.zeros(cache.units.shape[:2] + (page,), dtype=torch.bool)
     for b in range(n):
@@ -207,6 +207,7 @@ def test_attend_is_reproducible_and_ignores_what_lies_behind():
     cache = R.make_cache([2000, 3, 777], 4, 128, 64)
     q = R.queries(cache, 1, 8)
     a, la = cache.attend(q, return_lse=True)
+    assert not cache._arrivals.any()
     for _ in range(3):
         b, lb = cache.attend(q, return_lse=True)
         assert torch.equal(a, b) and torch.equal(la, lb)
@@ -289,7 +290,7 @@ def test_lengths_outside_the_pages_are_cut_and_reported():
     torch.cuda.synchronize()
     assert _C.read_device_error(True) == 3 << 16
     cache.lengths.copy_(ints(40, 0))
-    assert cache._arrivals.tolist() == [0, 0]
+    assert not cache._arrivals.any()
 
 
 # ---------------------------------------------------------------------------
@@ -319,7 +320,7 @@ def _evict_and_check(cache, keep, recent, sink):
     assert cache.lengths.tolist() == new_len and cache.evicted.tolist() == new_ev
     assert torch.equal(cache.pos.cpu(), pos) and torch.equal(cache.mass.cpu(), mass)
     assert torch.equal(cache.units.cpu(), units)
-    assert cache._arrivals.tolist() == [0] * cache.n_seqs
+    assert not cache._arrivals.any()
     return sum(len(p) for p in moves.values())
 
 
