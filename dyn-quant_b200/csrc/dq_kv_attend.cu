@@ -52,8 +52,8 @@ constexpr int kStep = 2 * kKvTokens;  // slots of one step of a run
 constexpr float kCode = 16777216.0f;  // 2^24: a masked code is c / kCode
 
 // Warps of a CTA and CTAs of an SM for row tiles of 8 NT rows: two row tiles
-// need 168 registers a thread, one tile 128.
-__host__ __device__ constexpr int at_warps(int nt) { return nt == 1 ? 8 : 12; }
+// need about 200 registers a thread, one tile 128.
+__host__ __device__ constexpr int at_warps(int nt) { return nt == 1 ? 8 : 10; }
 __host__ __device__ constexpr int at_ctas(int nt) { return nt == 1 ? 2 : 1; }
 
 struct KvAttendArgs {
@@ -66,6 +66,7 @@ struct KvAttendArgs {
     const int32_t* counts;
     float* part;             // [CTAs][2][rows][D]
     float* part_ml;          // [CTAs][2][rows][2]
+    float* first;            // [warps][rows][D + 2] pieces of jobs that end inside a run
     int* pre;                // [n_seqs + 1] the plan's prefix sums, for the combining kernel
     uint32_t* done;          // [n_seqs][heads] CTAs of a cut job that have arrived (one row tile)
     int tokens, group, n_rt; // query tokens, query heads per KV head, row tiles
@@ -197,6 +198,14 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 // Dynamic shared memory by its byte offset.
 template <class T>
 __device__ __forceinline__ T smem_at(int off) {
@@ -226,6 +235,35 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
 __device__ __forceinline__ float ex2(float v) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// Two FP32 operations in one instruction, on the pair of a lane's rows 2t, 2t + 1.
+struct f2 {
+    unsigned long long v;
+    __device__ __forceinline__ f2() {}
+    __device__ __forceinline__ f2(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
+    __device__ __forceinline__ explicit f2(float x) : f2(x, x) {}
+    __device__ __forceinline__ float x() const {
+        return __uint_as_float(static_cast<uint32_t>(v));
+    }
+    __device__ __forceinline__ float y() const {
+        return __uint_as_float(static_cast<uint32_t>(v >> 32));
+    }
+};
+__device__ __forceinline__ f2 operator+(f2 a, f2 b) {
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ f2 operator*(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
     return r;
 }
 
@@ -263,26 +301,39 @@ __device__ __forceinline__ void store_lse(const KvAttendArgs& a, int b, int tok,
 template <int D, int NT>
 struct QueryTile {
     uint32_t f[NT][D / 8];  // per 8-column word: (0,4), (1,5), (2,6), (3,7)
-    float sum[NT][2];       // sum of q over the columns / kCode, rows 2t and 2t + 1
+    f2 sum[NT];             // - sum of q over the columns / kCode, rows 2t and 2t + 1
     int lim[NT][2];         // keys that rows 2t and 2t + 1 see
     int min_lim, max_lim;   // over the tile's rows
 
-    // row r of the job: query token r / group, head h * group + r % group
-    __device__ __forceinline__ void load(const KvAttendArgs& a, int b, int h, int rt, int len) {
+    int cnt;
+    // Request row r of the job, query token r / group, head h * group + r % group, ...
+    __device__ __forceinline__ void request(const KvAttendArgs& a, int b, int h, int rt, uint4 (&raw)[NT][D / 32]) {
         const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
         const int rows = a.tokens * a.group;
-        const int cnt = a.counts ? min(max(static_cast<int>(ldcg_u32(a.counts + b)), 0), a.tokens) : a.tokens;
+        cnt = a.counts ? min(max(static_cast<int>(ldcg_u32(a.counts + b)), 0), a.tokens) : a.tokens;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = (rt * NT + nt) * 8 + g, tok = r / a.group;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                raw[nt][i] = make_uint4(0, 0, 0, 0);
+                if (r < rows && tok < cnt)
+                    raw[nt][i] = ldcg_v4(a.q + b * a.qs[0] + tok * a.qs[1] + (h * a.group + r - tok * a.group) * a.qs[2] + (D / 4) * t + 8 * i);
+            }
+        }
+    }
+    // ... and arrange it.
+    __device__ __forceinline__ void arrange(const KvAttendArgs& a, int rt, int len, const uint4 (&raw)[NT][D / 32]) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        const int rows = a.tokens * a.group;
         int lo = len, hi = 0;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int r = (rt * NT + nt) * 8 + g;
-            const int tok = r / a.group;
+            const int r = (rt * NT + nt) * 8 + g, tok = r / a.group;
             float s = 0.f;
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (r < rows && tok < cnt)
-                    w = ldcg_v4(a.q + b * a.qs[0] + tok * a.qs[1] + (h * a.group + r % a.group) * a.qs[2] + (D / 4) * t + 8 * i);
+                const uint4 w = raw[nt][i];
                 f[nt][4 * i] = __byte_perm(w.x, w.z, 0x5410);
                 f[nt][4 * i + 1] = __byte_perm(w.x, w.z, 0x7632);
                 f[nt][4 * i + 2] = __byte_perm(w.y, w.w, 0x5410);
@@ -300,20 +351,24 @@ struct QueryTile {
                 lo = min(lo, l);
                 hi = max(hi, l);
             }
+            s *= -1.f / kCode;
+            sum[nt] = f2(__shfl_sync(0xffffffffu, s, 8 * t), __shfl_sync(0xffffffffu, s, 8 * t + 4));
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                sum[nt][e] = __shfl_sync(0xffffffffu, s, 8 * t + 4 * e) * (1.f / kCode);
-                lim[nt][e] = __shfl_sync(0xffffffffu, l, 8 * t + 4 * e);
-            }
+            for (int e = 0; e < 2; ++e) lim[nt][e] = __shfl_sync(0xffffffffu, l, 8 * t + 4 * e);
         }
         min_lim = __reduce_min_sync(0xffffffffu, lo);
         max_lim = __reduce_max_sync(0xffffffffu, hi);
+    }
+    __device__ __forceinline__ void load(const KvAttendArgs& a, int b, int h, int rt, int len) {
+        uint4 raw[NT][D / 32];
+        request(a, b, h, rt, raw);
+        arrange(a, rt, len, raw);
     }
 };
 
 // D / kCode of U units: the MMAs' sums of q c for slots g, g + 8 and rows 2t, 2t + 1.
 template <int D, int NT, int U>
-__device__ __forceinline__ void score_mma(int unit, const QueryTile<D, NT>& q, float (&s)[U][NT][4]) {
+__device__ __forceinline__ void score_mma(int unit, const QueryTile<D, NT>& q, f2 (&s)[U][NT][2]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint32_t k0[U][D / 32], k1[U][D / 32];
     float lo[U][NT][4], hi[U][NT][4];
@@ -322,10 +377,6 @@ __device__ __forceinline__ void score_mma(int unit, const QueryTile<D, NT>& q, f
         const int at = unit + u * kv_unit_bytes(D) + g * (D / 2) + t * (D / 8);
         load_words<D>(at, k0[u]);
         load_words<D>(at + 8 * (D / 2), k1[u]);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) lo[u][nt][e] = hi[u][nt][e] = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
@@ -334,9 +385,14 @@ __device__ __forceinline__ void score_mma(int unit, const QueryTile<D, NT>& q, f
             const uint32_t w0 = k0[u][i], w1 = k1[u][i], x0 = w0 >> 8, x1 = w1 >> 8;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                mma(lo[u][nt], low_codes(w0), low_codes(w1), low_codes(x0), low_codes(x1), q.f[nt][4 * i], q.f[nt][4 * i + 2]);
-                mma(hi[u][nt], high_codes(w0), high_codes(w1), high_codes(x0), high_codes(x1), q.f[nt][4 * i + 1],
-                    q.f[nt][4 * i + 3]);
+                if (i == 0) {
+                    mma_first(lo[u][nt], low_codes(w0), low_codes(w1), low_codes(x0), low_codes(x1), q.f[nt][0], q.f[nt][2]);
+                    mma_first(hi[u][nt], high_codes(w0), high_codes(w1), high_codes(x0), high_codes(x1), q.f[nt][1], q.f[nt][3]);
+                } else {
+                    mma(lo[u][nt], low_codes(w0), low_codes(w1), low_codes(x0), low_codes(x1), q.f[nt][4 * i], q.f[nt][4 * i + 2]);
+                    mma(hi[u][nt], high_codes(w0), high_codes(w1), high_codes(x0), high_codes(x1), q.f[nt][4 * i + 1],
+                        q.f[nt][4 * i + 3]);
+                }
             }
         }
 #pragma unroll
@@ -344,7 +400,8 @@ __device__ __forceinline__ void score_mma(int unit, const QueryTile<D, NT>& q, f
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[u][nt][e] = fmaf(hi[u][nt][e], 0.0625f, lo[u][nt][e]);
+            for (int x = 0; x < 2; ++x)
+                s[u][nt][x] = fma2(f2(hi[u][nt][2 * x], hi[u][nt][2 * x + 1]), f2(0.0625f), f2(lo[u][nt][2 * x], lo[u][nt][2 * x + 1]));
 }
 
 // A warp's run of steps through its ring: lane i % 32 of each 32 steps looks
@@ -397,34 +454,43 @@ struct StepStream {
     // Issue the copies of the run's next step into slot s (every lane calls it).
     __device__ __forceinline__ void issue(const KvAttendArgs& a, const Plan& p, int s) {
         if ((issued & 31) == 0) lookup(a, p);
-        if ((threadIdx.x & 31) == (issued & 31)) {
+        const int i0 = __shfl_sync(0xffffffffu, src[0], issued), i1 = __shfl_sync(0xffffffffu, src[1], issued);
+        if ((threadIdx.x & 31) == 0) {
             const uint32_t bar = base() + bars + 8 * s, dst = base() + ring + s * kSlot;
-            const bool f0 = src[0] >= 0, f1 = src[1] >= 0;
-            constexpr uint32_t kKeys = kKeysOnly ? 8 * D + kKvTokens * 8 : kUnit;
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(base() + flags + 4 * s), "r"((f0 ? 1u : 0u) | (f1 ? 2u : 0u)) : "memory");
-            if (!f0 && !f1) {
-                mbar_arrive(bar);
+            if (!kKeysOnly && i0 >= 0 && i1 == i0 + 1) {
+                set_found(s, 3u);
+                mbar_arrive_expect_tx(bar, kSlot);
+                bulk_g2s(dst, a.c.units + static_cast<size_t>(i0) * kUnit, kSlot, bar);
             } else {
-                mbar_arrive_expect_tx(bar, (f0 ? kKeys : 0u) + (f1 ? kKeys : 0u));
-                const uint8_t* from = a.c.units + static_cast<size_t>(f0 ? src[0] : src[1]) * kUnit;
-                if (!kKeysOnly && f0 && src[1] == src[0] + 1) {
-                    bulk_g2s(dst, from, kSlot, bar);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        if (src[e] < 0) continue;
-                        if (e == 1) from = a.c.units + static_cast<size_t>(src[1]) * kUnit;
-                        if (kKeysOnly) {
-                            bulk_g2s(dst + e * kUnit, from, 8 * D, bar);
-                            bulk_g2s(dst + e * kUnit + kv_param_offset(D), from + kv_param_offset(D), kKvTokens * 8, bar);
-                        } else {
-                            bulk_g2s(dst + e * kUnit, from, kUnit, bar);
-                        }
-                    }
-                }
+                issue_units(a, s, bar, dst, i0, i1);
             }
         }
         ++issued;
+    }
+    __device__ __forceinline__ void set_found(int s, uint32_t v) {
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(base() + flags + 4 * s), "r"(v) : "memory");
+    }
+    // A step's units one by one: from different pages, one of them missing, or their keys alone.
+    __device__ __forceinline__ void issue_units(const KvAttendArgs& a, int s, uint32_t bar, uint32_t dst, int i0, int i1) {
+        constexpr uint32_t kBytes = kKeysOnly ? 8 * D + kKvTokens * 8 : kUnit;
+        set_found(s, (i0 >= 0 ? 1u : 0u) | (i1 >= 0 ? 2u : 0u));
+        if (i0 < 0 && i1 < 0) {
+            mbar_arrive(bar);
+            return;
+        }
+        mbar_arrive_expect_tx(bar, (i0 >= 0 ? kBytes : 0u) + (i1 >= 0 ? kBytes : 0u));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int i = e ? i1 : i0;
+            if (i < 0) continue;
+            const uint8_t* from = a.c.units + static_cast<size_t>(i) * kUnit;
+            if (kKeysOnly) {
+                bulk_g2s(dst + e * kUnit, from, 8 * D, bar);
+                bulk_g2s(dst + e * kUnit + kv_param_offset(D), from + kv_param_offset(D), kKvTokens * 8, bar);
+            } else {
+                bulk_g2s(dst + e * kUnit, from, kUnit, bar);
+            }
+        }
     }
     __device__ __forceinline__ void start(const KvAttendArgs& a, const Plan& p, long long first, int count) {
         u0 = first;
@@ -458,18 +524,11 @@ struct StepStream {
     }
 };
 
-// A unit's scale and zero for slots g and g + 8 of keys, ready for the scores.
-struct KeyParams {
-    float s0, z0, s1, z1;
-    __device__ __forceinline__ KeyParams(uint2 p0, uint2 p1, float scale2)
-        : s0(h2f_bits(lo16(p0.x)) * scale2), z0(h2f_bits(hi16(p0.x))),
-          s1(h2f_bits(lo16(p1.x)) * scale2), z1(h2f_bits(hi16(p1.x))) {}
-};
-
-// The running softmax of one job in one warp.
+// The running softmax of one job in one warp: rows 2t, 2t + 1 of each row tile.
 template <int D, int NT>
 struct RowState {
-    float o[NT][D / 16][4], m[NT][2], l[NT][2], zs[NT][2], vw;
+    float o[NT][D / 16][4], vw;
+    f2 m[NT], l[NT], zs[NT];  // m: minus the running maximum
 
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -478,32 +537,33 @@ struct RowState {
             for (int j = 0; j < D / 16; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[nt][j][e] = 0.f;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) { m[nt][e] = kNone; l[nt][e] = 0.f; zs[nt][e] = 0.f; }
+            m[nt] = f2(-kNone);
+            l[nt] = zs[nt] = f2(0.f);
         }
         vw = 2147483648.0f;  // 2^31 brings the smallest FP16 scale, 2^-24, to 2^7
     }
 
-    // U units from slot j of the sequence on.  found: bit u set where unit u is there.
+    // Scores and weights of U units from slot j of the sequence on, the weights as the B operands of their
+    // output product, and the units' V codes.  found: bit u set where unit u is there.
     template <int U>
-    __device__ __forceinline__ void add(const QueryTile<D, NT>& q, int unit, int j, int len, uint32_t found, float scale2) {
+    __device__ __forceinline__ void weigh(const QueryTile<D, NT>& q, int unit, int j, int len, uint32_t found, float scale2,
+                                          uint32_t (&pf)[U][NT][2], uint32_t (&v)[U][2][D / 32]) {
         const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-        float s[U][NT][4], sv[U][2], zv[U][2];
+        f2 s[U][NT][2];
+        float sv[U][2], zv[U][2];
         score_mma<D, NT, U>(unit, q, s);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int pa = unit + u * kv_unit_bytes(D) + kv_param_offset(D) + 8 * g;
-            const uint2 p0 = smem_at<uint2>(pa), p1 = smem_at<uint2>(pa + 64);
-            const KeyParams k(p0, p1, scale2);
-            sv[u][0] = h2f_bits(lo16(p0.y)); zv[u][0] = h2f_bits(hi16(p0.y)) - 8.f;
-            sv[u][1] = h2f_bits(lo16(p1.y)); zv[u][1] = h2f_bits(hi16(p1.y)) - 8.f;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int x = 0; x < 2; ++x) {
+                const uint2 p = smem_at<uint2>(pa + 64 * x);
+                const f2 sk(h2f_bits(lo16(p.x)) * scale2), zk(h2f_bits(hi16(p.x)));
+                sv[u][x] = h2f_bits(lo16(p.y));
+                zv[u][x] = h2f_bits(hi16(p.y)) - 8.f;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    s[u][nt][e] = fmaf(-k.z0, q.sum[nt][e], s[u][nt][e]) * k.s0;
-                    s[u][nt][e + 2] = fmaf(-k.z1, q.sum[nt][e], s[u][nt][e + 2]) * k.s1;
-                }
+                for (int nt = 0; nt < NT; ++nt) s[u][nt][x] = fma2(zk, q.sum[nt], s[u][nt][x]) * sk;
+            }
         }
         if (j + U * kKvTokens > q.min_lim || found != (1u << U) - 1u) {
             // the end of the sequence or of a query token's keys, or an absent page: slots behind a
@@ -517,9 +577,8 @@ struct RowState {
                     if (!there) { sv[u][x] = 0.f; zv[u][x] = 0.f; }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            if (!there || jj >= q.lim[nt][e]) s[u][nt][e + 2 * x] = -INFINITY;
+                        s[u][nt][x] = f2(there && jj < q.lim[nt][0] ? s[u][nt][x].x() : -INFINITY,
+                                         there && jj < q.lim[nt][1] ? s[u][nt][x].y() : -INFINITY);
                 }
         }
         // a new maximum or a larger V scale: rare after the first steps
@@ -528,52 +587,58 @@ struct RowState {
         for (int u = 1; u < U; ++u) big = fmaxf(big, fmaxf(sv[u][0], sv[u][1]));
         bool up = big * vw > 128.f;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
+            top[nt][0] = fmaxf(s[0][nt][0].x(), s[0][nt][1].x());
+            top[nt][1] = fmaxf(s[0][nt][0].y(), s[0][nt][1].y());
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                top[nt][e] = fmaxf(s[0][nt][e], s[0][nt][e + 2]);
-#pragma unroll
-                for (int u = 1; u < U; ++u) top[nt][e] = fmaxf(top[nt][e], fmaxf(s[u][nt][e], s[u][nt][e + 2]));
-                up |= top[nt][e] > m[nt][e] + kLazy;
+            for (int u = 1; u < U; ++u) {
+                top[nt][0] = fmaxf(top[nt][0], fmaxf(s[u][nt][0].x(), s[u][nt][1].x()));
+                top[nt][1] = fmaxf(top[nt][1], fmaxf(s[u][nt][0].y(), s[u][nt][1].y()));
             }
+            up |= top[nt][0] + m[nt].x() > kLazy;
+            up |= top[nt][1] + m[nt].y() > kLazy;
+        }
         if (__any_sync(0xffffffffu, up)) rescale(top, big);
-        uint32_t pf[U][NT][2];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const float w0 = sv[u][0] * vw, w1 = sv[u][1] * vw;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float x[4];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float e0 = ex2(s[u][nt][e] - m[nt][e]), e1 = ex2(s[u][nt][e + 2] - m[nt][e]);
-                    l[nt][e] += e0 + e1;
-                    x[e] = e0 * w0;
-                    x[e + 2] = e1 * w1;
-                    zs[nt][e] = fmaf(x[e], zv[u][0], fmaf(x[e + 2], zv[u][1], zs[nt][e]));
-                }
-                pf[u][nt][0] = movmatrix_trans(pack_f32(x[0], x[1]));
-                pf[u][nt][1] = movmatrix_trans(pack_f32(x[2], x[3]));
-            }
+            const int vb = unit + u * kv_unit_bytes(D) + kv_v_offset(D) + t * D + g * (D / 8);
+            load_words<D>(vb, v[u][0]);
+            load_words<D>(vb + 4 * D, v[u][1]);
         }
 #pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const f2 w(sv[u][x] * vw), z(zv[u][x]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const f2 d = s[u][nt][x] + m[nt], e(ex2(d.x()), ex2(d.y())), p = e * w;
+                    l[nt] = l[nt] + e;
+                    zs[nt] = fma2(p, z, zs[nt]);
+                    pf[u][nt][x] = movmatrix_trans(pack_f32(p.x(), p.y()));
+                }
+            }
+    }
+
+    // The output product of what weigh() left.  Rows g of an MMA are columns of low nibbles, rows g + 8 of
+    // high ones; the constants are -8 in either.
+    template <int U>
+    __device__ __forceinline__ void output(const uint32_t (&pf)[U][NT][2], const uint32_t (&v)[U][2][D / 32]) {
+        constexpr uint32_t kLow8 = 0x80088008u, kHigh8 = 0x80808080u;
+#pragma unroll
         for (int u = 0; u < U; ++u) {
-            uint32_t v0[D / 32], v1[D / 32];
-            const int vb = unit + u * kv_unit_bytes(D) + kv_v_offset(D) + t * D + g * (D / 8);
-            load_words<D>(vb, v0);
-            load_words<D>(vb + 4 * D, v1);
-            // rows g of an MMA are columns of low nibbles, rows g + 8 of high ones: -8 in either
-            constexpr uint32_t kLow8 = 0x80088008u, kHigh8 = 0x80808080u;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) mma(o[nt][k], kLow8, kHigh8, kLow8, kHigh8, pf[u][nt][0], pf[u][nt][1]);
 #pragma unroll
             for (int k = 0; k < D / 32; ++k) {
-                const uint32_t w0 = v0[k], w1 = v1[k], y0 = w0 >> 8, y1 = w1 >> 8;
+                const uint32_t w0 = v[u][0][k], w1 = v[u][1][k], y0 = w0 >> 8, y1 = w1 >> 8;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     const uint32_t b0 = pf[u][nt][0], b1 = pf[u][nt][1];
                     mma(o[nt][2 * k], low_codes(w0), high_codes(w0), low_codes(w1), high_codes(w1), b0, b1);
                     mma(o[nt][2 * k + 1], low_codes(y0), high_codes(y0), low_codes(y1), high_codes(y1), b0, b1);
-                    mma(o[nt][2 * k], kLow8, kHigh8, kLow8, kHigh8, b0, b1);
-                    mma(o[nt][2 * k + 1], kLow8, kHigh8, kLow8, kHigh8, b0, b1);
                 }
             }
         }
@@ -589,30 +654,37 @@ struct RowState {
             vw = nw;
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
+            float now[2], f[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float now = fmaxf(m[nt][e], lane_max_g(top[nt][e]));
-                const float f = (now == m[nt][e]) ? 1.f : ex2(m[nt][e] - now);
-                m[nt][e] = now;
-                l[nt][e] *= f;
-                const float fr = f * ratio;
-                zs[nt][e] *= fr;
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k) { o[nt][k][e] *= fr; o[nt][k][e + 2] *= fr; }
+                const float old = -(e ? m[nt].y() : m[nt].x());
+                now[e] = fmaxf(old, lane_max_g(top[nt][e]));
+                f[e] = (now[e] == old) ? 1.f : ex2(old - now[e]);
             }
+            m[nt] = f2(-now[0], -now[1]);
+            l[nt] = l[nt] * f2(f[0], f[1]);
+            const f2 fr(f[0] * ratio, f[1] * ratio);
+            zs[nt] = zs[nt] * fr;
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[nt][k][x] *= (x & 1) ? fr.y() : fr.x();
+        }
     }
 
     // Row 2t + e of tile nt: its sum of weights and the lane's columns D/8 g .. of its unnormalised output.
     __device__ __forceinline__ float finish(int nt, int e, float (&v)[D / 8]) const {
-        const float z = lane_sum_g(zs[nt][e]), inv = __uint_as_float(0x7F000000u - __float_as_uint(vw));  // 1 / vw
+        const float z = lane_sum_g(e ? zs[nt].y() : zs[nt].x());
+        const float inv = __uint_as_float(0x7F000000u - __float_as_uint(vw));  // 1 / vw
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
             v[2 * k] = fmaf(o[nt][k][e], kCode, -z) * inv;
             v[2 * k + 1] = fmaf(o[nt][k][e + 2], kCode / 16.f, -z) * inv;
         }
-        return lane_sum_g(l[nt][e]);
+        return lane_sum_g(e ? l[nt].y() : l[nt].x());
     }
+    __device__ __forceinline__ float top(int nt, int e) const { return -(e ? m[nt].y() : m[nt].x()); }
 };
 
 // Columns col .. col + N - 1 of row r of KV head h, normalised; the thread with column 0 stores the row's lse.
@@ -704,15 +776,16 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
     __shared__ Piece pieces[2 * W];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const KvView& c = a.c;
-    __shared__ int last;
-    char* at = smem + plan_bytes(c.n_seqs);
-    char* rings = at + W * kPiece * 4;
+    __shared__ Piece cut[2];
+    __shared__ Share share[2];
     StepStream<D, false> st;
-    st.init(static_cast<int>(rings - smem), W, warp, a.depth);
-    // A piece is [R][D + 2] floats: output, maximum, sum.  A warp's first piece has room of its own, its
-    // last one takes the warp's ring, which has run dry by then.
+    st.init(plan_bytes(c.n_seqs), W, warp, a.depth);
+    // A piece is [R][D + 2] floats: output, maximum, sum.  A warp's last piece takes its ring, which has run
+    // dry by then; one of a job that ends inside the run goes to the workspace, so that the rings have all
+    // of the shared memory.
     auto piece_at = [&](int k) {
-        return reinterpret_cast<float*>((k & 1) ? rings + (k >> 1) * a.depth * StepStream<D, false>::kSlot : at + (k >> 1) * kPiece * 4);
+        return (k & 1) ? reinterpret_cast<float*>(smem + plan_bytes(c.n_seqs) + (k >> 1) * a.depth * StepStream<D, false>::kSlot)
+                       : a.first + (static_cast<size_t>(blockIdx.x) * W + (k >> 1)) * kPiece;
     };
     pdl_launch_dependents();
     pdl_wait();
@@ -726,27 +799,35 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
     __syncwarp();
     const int rows = a.tokens * a.group;
     if (n > 0) {
-        st.start(a, p, u0, n);
         QueryTile<D, NT> q;
         RowState<D, NT> rs;
         int b = 0, job = 0, len = 0, ub = 0, ul = 0, done = 0;
         bool gave_up = false;
         int left = 0;  // steps of the current sequence not yet begun, those of this run
+        auto next_seq = [&]() {
+            const long long u = u0 + done;
+            const StepAt x = step_at(p, c.n_seqs, u);
+            b = x.b;
+            len = x.len;
+            ul = steps_of(len);
+            job = x.job;
+            ub = x.step;
+            left = static_cast<int>(min(static_cast<long long>(p.pre[b + 1]) * p.jobs - u, static_cast<long long>(n - done)));
+        };
+        {
+            // the first queries are asked for before the whole GPU's first copies
+            next_seq();
+            uint4 raw[NT][D / 32];
+            q.request(a, b, job / a.n_rt, job % a.n_rt, raw);
+            st.start(a, p, u0, n);
+            q.arrange(a, job % a.n_rt, len, raw);
+        }
         while (done < n && !gave_up) {
-            if (left == 0) {
-                const long long u = u0 + done;
-                const StepAt x = step_at(p, c.n_seqs, u);
-                b = x.b;
-                len = x.len;
-                ul = steps_of(len);
-                job = x.job;
-                ub = x.step;
-                left = static_cast<int>(min(static_cast<long long>(p.pre[b + 1]) * p.jobs - u, static_cast<long long>(n - done)));
-            }
+            if (left == 0) next_seq();
             // a job, or the part of it in this run
             const int first = ub, take = min(ul - ub, n - done);
             const int h = job / a.n_rt, rt = job - h * a.n_rt;
-            q.load(a, b, h, rt, len);
+            if (done > 0) q.load(a, b, h, rt, len);
             rs.clear();
             for (int i = 0; i < take; ++i, ++ub) {
                 if (!st.wait()) {
@@ -761,19 +842,28 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
                         found = st.found();
                         if (j + kKvTokens >= len) found |= 2u;  // behind the last slot: not copied, and not missed
                     }
+                    // the slot is refilled as soon as its V codes are in registers
                     if constexpr (NT == 1) {
-                        rs.template add<2>(q, st.unit(), j, len, found, a.scale2);
+                        uint32_t pf[2][NT][2], v[2][2][D / 32];
+                        rs.template weigh<2>(q, st.unit(), j, len, found, a.scale2, pf, v);
+                        st.next(a, p);
+                        rs.template output<2>(pf, v);
                     } else {
-                        rs.template add<1>(q, st.unit(), j, len, found & 1u, a.scale2);
-                        if (j + kKvTokens < q.max_lim)
-                            rs.template add<1>(q, st.unit() + kv_unit_bytes(D), j + kKvTokens, len, found >> 1, a.scale2);
+                        uint32_t pf[1][NT][2], v[1][2][D / 32];
+                        rs.template weigh<1>(q, st.unit(), j, len, found & 1u, a.scale2, pf, v);
+                        rs.template output<1>(pf, v);
+                        const bool second = j + kKvTokens < q.max_lim;
+                        if (second) rs.template weigh<1>(q, st.unit() + kv_unit_bytes(D), j + kKvTokens, len, found >> 1, a.scale2, pf, v);
+                        st.next(a, p);
+                        if (second) rs.template output<1>(pf, v);
                     }
+                } else {
+                    st.next(a, p);
                 }
-                st.next(a, p);
             }
             if (gave_up) break;
             const bool whole = first == 0 && ub == ul;
-            const int k = 2 * warp + (done == 0 ? 0 : 1);
+            const int k = 2 * warp + (done + take == n ? 1 : 0);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -783,13 +873,13 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
                     const int rl = nt * 8 + 2 * t + e, r = rt * R + rl;
                     if (r >= rows) continue;
                     if (whole) {
-                        store_row(a, b, h, r, (D / 8) * g, v, rs.m[nt][e], sum);
+                        store_row(a, b, h, r, (D / 8) * g, v, rs.top(nt, e), sum);
                     } else {
                         float* dst = piece_at(k) + rl * (D + 2);
 #pragma unroll
                         for (int i = 0; i < D / 8; i += 2)
                             *reinterpret_cast<float2*>(dst + (D / 8) * g + i) = make_float2(v[i], v[i + 1]);
-                        if (g == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(rs.m[nt][e], sum);
+                        if (g == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(rs.top(nt, e), sum);
                     }
                 }
             if (!whole && lane == 0) pieces[k] = Piece{b, job, first, ub};
@@ -809,9 +899,9 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
         }
     }
     __syncthreads();
-    // Neighbouring pieces of one job meet here, in order; a job that ends up whole is finished, the
-    // others (at most the CTA's first and last) go to the workspace.
-    int slot = 0;
+    // Neighbouring pieces of one job meet here, in order, its rows dealt to the warps; a job that ends up
+    // whole is finished, the others (at most the CTA's first and last) go to the workspace.
+    int turn = 0, cuts = 0;
     for (int k = 0; k < 2 * W;) {
         const Piece first = pieces[k];
         if (first.job < 0) { ++k; continue; }
@@ -823,55 +913,64 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
             end = x.end;
         }
         const bool whole = first.first == 0 && end == steps_of(p.len[first.b]);
-        const int h = first.job / a.n_rt, rt = first.job - h * a.n_rt;
-        constexpr int C = 8;  // columns of a thread
-        for (int i = threadIdx.x; i < R * (D / C); i += 32 * W) {
-            const int rl = i / (D / C), col = C * (i % (D / C)), r = rt * R + rl;
-            if (r >= rows) break;
-            float m = kNone, sum = 0.f, v[C];
-            for (int x = k; x < k1; ++x)
-                if (pieces[x].job >= 0) m = fmaxf(m, piece_at(x)[rl * (D + 2) + D]);
+        {
+            const int h = first.job / a.n_rt, rt = first.job - h * a.n_rt, n_rows = min(R, rows - rt * R);
+            constexpr int C = 8, L = D / C, P = 32 / L;  // columns of a lane, lanes of a row, rows of a turn
+            for (int r0 = 0; r0 < n_rows; r0 += P, ++turn) {
+                const int rl = r0 + lane / L, col = C * (lane % L);
+                if (turn % W != warp || rl >= n_rows) continue;
+                float m = kNone, sum = 0.f, v[C];
+                for (int x = k; x < k1; ++x)
+                    if (pieces[x].job >= 0) m = fmaxf(m, piece_at(x)[rl * (D + 2) + D]);
 #pragma unroll
-            for (int y = 0; y < C; ++y) v[y] = 0.f;
-            for (int x = k; x < k1; ++x) {
-                if (pieces[x].job < 0) continue;
-                const float* src = piece_at(x) + rl * (D + 2);
-                const float f = ex2(src[D] - m);
-                sum += src[D + 1] * f;
+                for (int y = 0; y < C; ++y) v[y] = 0.f;
+                for (int x = k; x < k1; ++x) {
+                    if (pieces[x].job < 0) continue;
+                    const float* src = piece_at(x) + rl * (D + 2);
+                    const float f = ex2(src[D] - m);
+                    sum += src[D + 1] * f;
 #pragma unroll
-                for (int y = 0; y < C; y += 2) {
-                    const float2 z = *reinterpret_cast<const float2*>(src + col + y);
-                    v[y] += z.x * f;
-                    v[y + 1] += z.y * f;
+                    for (int y = 0; y < C; y += 2) {
+                        const float2 z = *reinterpret_cast<const float2*>(src + col + y);
+                        v[y] += z.x * f;
+                        v[y + 1] += z.y * f;
+                    }
+                }
+                if (whole) {
+                    store_row(a, first.b, h, rt * R + rl, col, v, m, sum);
+                } else {
+                    const size_t pi = (static_cast<size_t>(blockIdx.x) * 2 + cuts) * R + rl;
+                    float4* dst = reinterpret_cast<float4*>(a.part + pi * D + col);
+                    dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+                    dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+                    if (col == 0) *reinterpret_cast<float2*>(a.part_ml + pi * 2) = make_float2(m, sum);
                 }
             }
-            if (whole) {
-                store_row(a, first.b, h, r, col, v, m, sum);
-            } else {
-                const size_t pi = (static_cast<size_t>(blockIdx.x) * 2 + slot) * R + rl;
-                float4* dst = reinterpret_cast<float4*>(a.part + pi * D + col);
-                dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-                dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-                if (col == 0) *reinterpret_cast<float2*>(a.part_ml + pi * 2) = make_float2(m, sum);
-            }
         }
-        if (!whole && a.n_rt == 1) {
-            // one row tile: the last of the job's CTAs to arrive joins the partial sums, in CTA order
-            const Share s = share_of<W>(p.pre, c.n_seqs, p.jobs, p.runs, first.b, first.job);
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                __threadfence();
-                uint32_t* d = a.done + static_cast<size_t>(first.b) * c.heads + first.job;
-                last = atomicAdd(d, 1u) == static_cast<uint32_t>(s.n - 1);
-                if (last) *d = 0;
-                __threadfence();
-            }
-            __syncthreads();
-            if (last)
-                for (int r = warp; r < rows; r += W) join_row<D, NT>(a, s, first.b, h, 0, r);
+        if (!whole) {
+            if (threadIdx.x == 0) cut[cuts] = first;
+            ++cuts;
         }
-        if (!whole) slot = 1;
         k = k1;
+    }
+    if (cuts > 0 && a.n_rt == 1) {
+        // one row tile: the last of a job's CTAs to arrive joins the partial sums, in CTA order
+        __syncthreads();
+        if (threadIdx.x < cuts) {
+            const Piece x = cut[threadIdx.x];
+            const Share s = share_of<W>(p.pre, c.n_seqs, p.jobs, p.runs, x.b, x.job);
+            __threadfence();
+            uint32_t* d = a.done + static_cast<size_t>(x.b) * c.heads + x.job;
+            const bool last = atomicAdd(d, 1u) == static_cast<uint32_t>(s.n - 1);
+            if (last) *d = 0;
+            __threadfence();
+            share[threadIdx.x] = last ? s : Share{0, 0, 0};
+        }
+        __syncthreads();
+        for (int i = warp; i < cuts * rows; i += W) {
+            const Share s = share[i / rows];
+            if (s.n > 0) join_row<D, NT>(a, s, cut[i / rows].b, cut[i / rows].job, 0, i % rows);
+        }
     }
     if (lane == 0 && n > 0 && st.absent) atomicOr(&g_kv_attend_error, kKvErrPage);
 }
@@ -925,7 +1024,7 @@ __global__ void __launch_bounds__(32 * at_warps(1), at_ctas(1)) kv_mass_kernel(c
     int b = 0, h = 0, len = 0, ub = 0, ul = 0;
     long long left = 0;
     bool fresh = true;
-    float lse[2] = {0.f, 0.f};
+    f2 lse(0.f);  // minus the rows' lse
     for (int i = 0; i < n; ++i) {
         if (left == 0) {
             const long long u = u0 + i;
@@ -945,34 +1044,33 @@ __global__ void __launch_bounds__(32 * at_warps(1), at_ctas(1)) kv_mass_kernel(c
         for (int rt = 0; rt < n_rt; ++rt) {
             if (n_rt > 1 || fresh) {
                 q.load(a, b, h, rt, len);
+                float v[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int row = rt * 8 + 2 * t + e;
-                    lse[e] = INFINITY;  // padding rows weigh nothing
+                    v[e] = -INFINITY;  // padding rows and rows without keys weigh nothing
                     if (row < rows) {
                         const int tok = row / a.group, head = h * a.group + row % a.group;
-                        lse[e] = ldcg_f32(a.lse2 + (static_cast<size_t>(b) * a.tokens + tok) * (c.heads * a.group) + head);
-                        if (lse[e] == -INFINITY) lse[e] = INFINITY;  // a row without keys
+                        const float x = ldcg_f32(a.lse2 + (static_cast<size_t>(b) * a.tokens + tok) * (c.heads * a.group) + head);
+                        if (x != -INFINITY) v[e] = -x;
                     }
                 }
+                lse = f2(v[0], v[1]);
                 fresh = false;
             }
             if (ub * kStep >= q.max_lim) continue;
-            float s[2][1][4];
+            f2 s[2][1][2];
             score_mma<D, 1, 2>(unit, q, s);
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                const int pa = unit + y * kv_unit_bytes(D) + kv_param_offset(D) + 8 * g;
-                const KeyParams k(smem_at<uint2>(pa), smem_at<uint2>(pa + 64), a.scale2);
-                const int j0 = ub * kStep + y * kKvTokens + g, j1 = j0 + 8;
+            for (int y = 0; y < 2; ++y)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float e0 = ex2(fmaf(-k.z0, q.sum[0][e], s[y][0][e]) * k.s0 - lse[e]);
-                    const float e1 = ex2(fmaf(-k.z1, q.sum[0][e], s[y][0][e + 2]) * k.s1 - lse[e]);
-                    if (j0 < q.lim[0][e]) add[y][0] += e0;
-                    if (j1 < q.lim[0][e]) add[y][1] += e1;
+                for (int x = 0; x < 2; ++x) {
+                    const uint2 p = smem_at<uint2>(unit + y * kv_unit_bytes(D) + kv_param_offset(D) + 8 * g + 64 * x);
+                    const int jj = ub * kStep + y * kKvTokens + g + 8 * x;
+                    const f2 d = fma2(f2(h2f_bits(hi16(p.x))), q.sum[0], s[y][0][x]) * f2(h2f_bits(lo16(p.x)) * a.scale2) + lse;
+                    if (jj < q.lim[0][0]) add[y][x] += ex2(d.x());
+                    if (jj < q.lim[0][1]) add[y][x] += ex2(d.y());
                 }
-            }
         }
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
@@ -995,11 +1093,10 @@ __global__ void __launch_bounds__(32 * at_warps(1), at_ctas(1)) kv_mass_kernel(c
 
 constexpr int kSmemPerSm = 226 * 1024;
 
-// Ring slots per warp that fit next to the plan and `fixed` bytes when `ctas` CTAs share an SM, and the CTA's
-// shared memory.
+// Ring slots per warp that fit next to the plan when `ctas` CTAs share an SM, and the CTA's shared memory.
 template <class Stream>
-int ring_depth(int n_seqs, int warps, int ctas, int fixed, int* smem) {
-    const int used = plan_bytes(n_seqs) + fixed, room = kSmemPerSm / ctas - 2048 - used;
+int ring_depth(int n_seqs, int warps, int ctas, int* smem) {
+    const int used = plan_bytes(n_seqs), room = kSmemPerSm / ctas - 2048 - used;
     int depth = room / (warps * (Stream::kSlot + 12));
     depth = depth > 8 ? 8 : depth;
     *smem = used + Stream::bytes(warps, depth);
@@ -1021,7 +1118,7 @@ dq_status_t attend(KvAttendArgs& a, cudaStream_t stream) {
     if (st != DQ_OK) return st;
     int grid = di.sm_count * at_ctas(NT), smem = 0;
     if (grid * W > kAtMaxWarps) grid = kAtMaxWarps / W;
-    a.depth = ring_depth<StepStream<D, false>>(a.c.n_seqs, W, at_ctas(NT), W * 8 * NT * (D + 2) * 4, &smem);
+    a.depth = ring_depth<StepStream<D, false>>(a.c.n_seqs, W, at_ctas(NT), &smem);
     // a piece fits in a ring of two slots
     static_assert(8 * NT * (D + 2) * 4 <= 2 * StepStream<D, false>::kSlot, "ring too small for a piece");
     if (a.depth < 2) return DQ_ERR_UNSUPPORTED;
@@ -1033,7 +1130,7 @@ dq_status_t attend(KvAttendArgs& a, cudaStream_t stream) {
                     32 * kCbWarps, 0, stream, a, grid);
     if (st != DQ_OK || !a.lse2) return st;
     grid = di.sm_count * at_ctas(1);
-    a.depth = ring_depth<StepStream<D, true>>(a.c.n_seqs, at_warps(1), at_ctas(1), 0, &smem);
+    a.depth = ring_depth<StepStream<D, true>>(a.c.n_seqs, at_warps(1), at_ctas(1), &smem);
     if ((st = allow_smem(kv_mass_kernel<D>, smem)) != DQ_OK) return st;
     return launch_pdl(kv_mass_kernel<D>, dim3(grid), 32 * at_warps(1), smem, stream, a);
 }
@@ -1042,7 +1139,7 @@ dq_status_t attend(KvAttendArgs& a, cudaStream_t stream) {
 int row_tiles(int rows) { return rows <= 8 ? 1 : 2; }
 
 struct AttendWs {
-    size_t part, ml, pre, lse2, total;
+    size_t part, ml, first, pre, lse2, total;
 };
 AttendWs attend_ws(const dq_kv_cache_t& c, int tokens, int q_heads, bool mass) {
     const int nt = row_tiles(tokens * (q_heads / c.kv_heads));
@@ -1050,7 +1147,8 @@ AttendWs attend_ws(const dq_kv_cache_t& c, int tokens, int q_heads, bool mass) {
     AttendWs w;
     w.part = 0;
     w.ml = align256(rows * c.head_dim * 4);
-    w.pre = w.ml + align256(rows * 8);
+    w.first = w.ml + align256(rows * 8);
+    w.pre = w.first + align256(static_cast<size_t>(kAtMaxWarps) * 8 * nt * (c.head_dim + 2) * 4);
     w.lse2 = w.pre + align256((static_cast<size_t>(c.n_seqs) + 1) * 4);
     w.total = w.lse2 + (mass ? align256(static_cast<size_t>(c.n_seqs) * tokens * q_heads * 4) : 0);
     return w;
@@ -1078,6 +1176,7 @@ dq_status_t launch_kv_attend(const dq_kv_cache_t& c, const dq_kv_attend_t& r, vo
     char* base = static_cast<char*>(workspace);
     a.part = reinterpret_cast<float*>(base + w.part);
     a.part_ml = reinterpret_cast<float*>(base + w.ml);
+    a.first = reinterpret_cast<float*>(base + w.first);
     a.pre = reinterpret_cast<int*>(base + w.pre);
     a.lse2 = r.accumulate ? reinterpret_cast<float*>(base + w.lse2) : nullptr;
     const int rows = r.tokens * a.group, nt = row_tiles(rows);
