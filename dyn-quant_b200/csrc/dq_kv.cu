@@ -7,11 +7,15 @@
 #include <cfloat>
 #include <climits>
 
+#include <cooperative_groups.h>
+
 #include "dq_kv.cuh"
 
 namespace dq {
 
 namespace {
+
+namespace cg = cooperative_groups;
 
 __device__ unsigned int g_kv_error;
 
@@ -20,12 +24,15 @@ __device__ unsigned int g_kv_error;
 //
 // A row of D values becomes lo = min, s = (max - lo) / 15 (1 for a row flatter
 // than 1e-8), z = -lo / s and codes trunc((v - lo) / s + 1/2), with the
-// operations and roundings of quantize_kernel, so a row's bytes are those of
-// dq_quantize.  D/4 lanes hold one (slot pair, head): both slots' K and V rows
-// are requested at once, four columns a lane, and min / max meet in shuffles.
-// A pair is the granule because V words hold two neighbouring slots: with both
-// slots new a lane stores whole words, else its 16-bit half.  Bound by the rows
-// read and the codes written (prompts) or by one launch (a decode step).
+// operations and roundings of quantize_kernel, so a finite row's bytes are
+// those of dq_quantize.  D/8 lanes hold one (slot pair, head), eight columns
+// each: both slots' K and V rows are requested at once in 16-byte loads.  Min
+// and max of a row meet as one f16 pair (min, -max), a shuffle a step; the
+// conversion to a code is one addition of 2^23 rounded down, whose low bits are
+// gathered by shifted additions.  A pair is the granule because V words hold
+// two neighbouring slots: with both slots new a lane stores whole words, else
+// its 16-bit halves.  Bound by instructions, then by the rows read and written
+// (prompts), or by one launch (a decode step).
 // ---------------------------------------------------------------------------
 struct KvAppendArgs {
     KvView c;
@@ -40,56 +47,54 @@ struct KvAppendArgs {
 };
 
 struct KvRow {
-    uint32_t codes;  // four codes of this lane, 4 bits each
-    uint16_t s, z;
+    uint32_t codes;  // eight codes of this lane
+    uint32_t sz;     // scale | zero << 16
 };
 
-template <int LPR>
-__device__ __forceinline__ KvRow kv_quant_row(uint2 raw) {
-    const float v[4] = {h2f_bits(lo16(raw.x)), h2f_bits(hi16(raw.x)), h2f_bits(lo16(raw.y)), h2f_bits(hi16(raw.y))};
-    float lo = FLT_MAX, hi = -FLT_MAX;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (v[i] < lo) lo = v[i];
-        if (v[i] > hi) hi = v[i];
-    }
-#pragma unroll
-    for (int o = LPR / 2; o >= 1; o >>= 1) {
-        const float l2 = __shfl_xor_sync(0xffffffffu, lo, o), h2 = __shfl_xor_sync(0xffffffffu, hi, o);
-        if (l2 < lo) lo = l2;
-        if (h2 > hi) hi = h2;
-    }
-    const float range = __fsub_rn(hi, lo);
-    const float step = (range < 1e-8f) ? 1.0f : __fdiv_rn(range, 15.0f);
-    const float inv = __fdiv_rn(1.0f, step);
-    KvRow r;
-    r.s = __half_as_ushort(__float2half_rn(step));
-    r.z = __half_as_ushort(__float2half_rn(__fmul_rn(-lo, inv)));
-    r.codes = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float t = __fadd_rn(__fmul_rn(__fsub_rn(v[i], lo), inv), 0.5f);
-        // out-of-range and NaN give code 0, as quantize_kernel's conversion does
-        int q = (t >= -2147483648.0f && t < 2147483648.0f) ? __float2int_rz(t) : INT_MIN;
-        q = q < 0 ? 0 : (q > 15 ? 15 : q);
-        r.codes |= static_cast<uint32_t>(q) << (4 * i);
-    }
+__device__ __forceinline__ uint32_t min_h2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("min.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
 
-// The four values that the cache now holds for this lane's columns.
-__device__ __forceinline__ uint2 kv_values(const KvRow& r) {
-    const float s = h2f_bits(r.s), z = h2f_bits(r.z);
-    uint16_t h[4];
+// LPR lanes' row, eight columns each; with kValues the values that the cache now holds come back in raw.
+template <int LPR, bool kValues>
+__device__ __forceinline__ KvRow kv_quant_row(uint4& raw) {
+    uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    const uint32_t lo2 = min_h2(min_h2(w[0], w[1]), min_h2(w[2], w[3]));
+    const uint32_t hi2 = min_h2(min_h2(w[0] ^ 0x80008000u, w[1] ^ 0x80008000u), min_h2(w[2] ^ 0x80008000u, w[3] ^ 0x80008000u));
+    uint32_t mm = min_h2(__byte_perm(lo2, hi2, 0x5410), __byte_perm(lo2, hi2, 0x7632));  // (min, -max)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        h[i] = __half_as_ushort(__float2half_rn(__fmul_rn(s, __fsub_rn(static_cast<float>((r.codes >> (4 * i)) & 15u), z))));
-    return make_uint2(pack_h2(h[0], h[1]), pack_h2(h[2], h[3]));
+    for (int o = LPR / 2; o >= 1; o >>= 1) mm = min_h2(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+    const float lo = h2f_bits(lo16(mm)), range = __fsub_rn(-h2f_bits(hi16(mm)), lo);
+    const float step = (range < 1e-8f) ? 1.0f : __fdiv_rn(range, 15.0f);
+    const float inv = __fdiv_rn(1.0f, step);
+    KvRow r;
+    r.sz = pack_h2(__half_as_ushort(__float2half_rn(step)), __half_as_ushort(__float2half_rn(__fmul_rn(-lo, inv))));
+    const float s16 = h2f_bits(lo16(r.sz)), z16 = h2f_bits(hi16(r.sz));
+    uint32_t acc = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float val[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float v = h2f_bits(e ? hi16(w[i]) : lo16(w[i]));
+            // at least 0.5 (v >= lo); 15.5 at most also where the row is not finite
+            const float t = fminf(__fadd_rn(__fmul_rn(__fsub_rn(v, lo), inv), 0.5f), 15.5f);
+            const float c = __fadd_rz(t, 8388608.0f);  // 2^23 + trunc(t)
+            acc += __float_as_uint(c) << (4 * (2 * i + e));
+            if (kValues) val[e] = __fmul_rn(s16, __fsub_rn(__fsub_rn(c, 8388608.0f), z16));
+        }
+        if (kValues) w[i] = pack_h2(__half_as_ushort(__float2half_rn(val[0])), __half_as_ushort(__float2half_rn(val[1])));
+    }
+    r.codes = acc - (0x4B000000u + 0xB0000000u);  // the bits of 2^23 itself, of the terms that do not shift them out
+    if (kValues) raw = make_uint4(w[0], w[1], w[2], w[3]);
+    return r;
 }
 
-template <int D>
+template <int D, bool kValues>
 __global__ void __launch_bounds__(128) kv_append_kernel(const KvAppendArgs a, const int items_per_cta) {
-    constexpr int LPR = D / 4;  // lanes of one row
+    constexpr int LPR = D / 8;  // lanes of one row
     const KvView& c = a.c;
     const int b = blockIdx.y;
     pdl_launch_dependents();
@@ -112,71 +117,70 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const KvAppendArgs a, co
     bool bad_page = false;
     // All lanes of a warp stay in the loop together (the row reductions are shuffles of the whole warp).
     const long long first = static_cast<long long>(blockIdx.x) * items_per_cta;
-    const long long last = first + items_per_cta < items ? first + items_per_cta : items;
-    for (long long i0 = first; i0 < last; i0 += subs) {
-        const long long it = i0 + sub;
-        const bool mine = it < last;
-        const int pair = pair0 + static_cast<int>(mine ? it / c.heads : 0), h = static_cast<int>(mine ? it % c.heads : 0);
+    const int count = static_cast<int>(first >= items ? 0 : (items - first < items_per_cta ? items - first : items_per_cta));
+    int pair = pair0 + static_cast<int>((first + sub) / c.heads), h = static_cast<int>((first + sub) % c.heads);
+    for (int i0 = 0; i0 < count; i0 += subs) {
+        const bool mine = i0 + sub < count;
         bool on[2];
-        uint2 kr[2], vr[2];
-        int tok[2];
+        uint4 kr[2], vr[2];
+        KvRow kq[2], vq[2];
+        const int tok = 2 * pair - start;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const int slot = 2 * pair + e;
-            tok[e] = slot - start;
-            on[e] = mine && tok[e] >= 0 && tok[e] < n;
-            kr[e] = vr[e] = make_uint2(0, 0);
+            on[e] = mine && tok + e >= 0 && tok + e < n;
+            kr[e] = vr[e] = make_uint4(0, 0, 0, 0);
             if (on[e]) {
-                const uint16_t* kp = a.k + b * a.ks[0] + tok[e] * a.ks[1] + h * a.ks[2] + 4 * col;
-                const uint16_t* vp = a.v + b * a.vs[0] + tok[e] * a.vs[1] + h * a.vs[2] + 4 * col;
-                kr[e] = *reinterpret_cast<const uint2*>(kp);
-                vr[e] = *reinterpret_cast<const uint2*>(vp);
+                kr[e] = ldg_stream_v4(a.k + b * a.ks[0] + (tok + e) * a.ks[1] + h * a.ks[2] + 8 * col);
+                vr[e] = ldg_stream_v4(a.v + b * a.vs[0] + (tok + e) * a.vs[1] + h * a.vs[2] + 8 * col);
             }
         }
         const int page = mine ? kv_page(c, b, 2 * pair) : 0;  // a pair never crosses a page
-        KvRow kq[2], vq[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            kq[e] = kv_quant_row<LPR>(kr[e]);
-            vq[e] = kv_quant_row<LPR>(vr[e]);
-            if (on[e] && a.k_values) {
-                const size_t o = ((static_cast<size_t>(b) * a.tokens + tok[e]) * c.heads + h) * D + 4 * col;
-                *reinterpret_cast<uint2*>(a.k_values + o) = kv_values(kq[e]);
-                *reinterpret_cast<uint2*>(a.v_values + o) = kv_values(vq[e]);
+            kq[e] = kv_quant_row<LPR, kValues>(kr[e]);
+            vq[e] = kv_quant_row<LPR, kValues>(vr[e]);
+            if (kValues && on[e]) {
+                const size_t o = ((static_cast<size_t>(b) * a.tokens + tok + e) * c.heads + h) * D + 8 * col;
+                *reinterpret_cast<uint4*>(a.k_values + o) = kr[e];
+                *reinterpret_cast<uint4*>(a.v_values + o) = vr[e];
             }
         }
-        if (!mine) continue;
-        if (page < 0) { bad_page = true; continue; }
-        const int off = (2 * pair) % c.page_size, row = off % kKvTokens;
-        uint8_t* u = kv_unit<D>(c, page, h, off);
+        if (mine && page < 0) bad_page = true;
+        if (mine && page >= 0) {
+            const int off = (2 * pair) % c.page_size, row = off % kKvTokens;
+            uint8_t* u = kv_unit<D>(c, page, h, off);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            if (!on[e]) continue;
-            *reinterpret_cast<uint16_t*>(u + (row + e) * (D / 2) + 2 * col) = static_cast<uint16_t>(kq[e].codes);
-            if (col == 0) {
-                *reinterpret_cast<uint2*>(u + kv_param_offset(D) + 8 * (row + e)) =
-                    make_uint2(pack_h2(kq[e].s, kq[e].z), pack_h2(vq[e].s, vq[e].z));
-                const size_t line = kv_line(c, page, h) + off + e;
-                c.mass[line] = 0.f;
-                c.pos[line] = gone + 2 * pair + e;
+            for (int e = 0; e < 2; ++e) {
+                if (!on[e]) continue;
+                *reinterpret_cast<uint32_t*>(u + (row + e) * (D / 2) + 4 * col) = kq[e].codes;
+                if (col == 0) {
+                    *reinterpret_cast<uint2*>(u + kv_param_offset(D) + 8 * (row + e)) = make_uint2(kq[e].sz, vq[e].sz);
+                    const size_t line = kv_line(c, page, h) + off + e;
+                    c.mass[line] = 0.f;
+                    c.pos[line] = gone + 2 * pair + e;
+                }
+            }
+            uint8_t* vw = u + kv_v_offset(D) + (row / 2) * D + 8 * col;  // column quads 2 col, 2 col + 1
+            if (on[0] && on[1]) {
+                *reinterpret_cast<uint2*>(vw) = make_uint2(__byte_perm(vq[0].codes, vq[1].codes, 0x5410),
+                                                           __byte_perm(vq[0].codes, vq[1].codes, 0x7632));
+            } else if (on[0] || on[1]) {
+                const uint32_t x = on[0] ? vq[0].codes : vq[1].codes;
+                uint16_t* half = reinterpret_cast<uint16_t*>(vw) + (on[0] ? 0 : 1);
+                half[0] = lo16(x);
+                half[2] = hi16(x);
             }
         }
-        uint8_t* vw = u + kv_v_offset(D) + (row / 2) * D + 4 * col;
-        if (on[0] && on[1])
-            *reinterpret_cast<uint32_t*>(vw) = vq[0].codes | (vq[1].codes << 16);
-        else if (on[0])
-            *reinterpret_cast<uint16_t*>(vw) = static_cast<uint16_t>(vq[0].codes);
-        else if (on[1])
-            *reinterpret_cast<uint16_t*>(vw + 2) = static_cast<uint16_t>(vq[1].codes);
+        for (h += subs; h >= c.heads; h -= c.heads) ++pair;
     }
     // padding tokens of the returned values are zero
-    if (a.k_values) {
+    if (kValues) {
         const long long pad = static_cast<long long>(a.tokens - n) * c.heads * LPR;
         const size_t o = (static_cast<size_t>(b) * a.tokens + n) * c.heads * D;
         for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < pad;
              i += static_cast<long long>(gridDim.x) * blockDim.x) {
-            *reinterpret_cast<uint2*>(a.k_values + o + 4 * i) = make_uint2(0, 0);
-            *reinterpret_cast<uint2*>(a.v_values + o + 4 * i) = make_uint2(0, 0);
+            *reinterpret_cast<uint4*>(a.k_values + o + 8 * i) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(a.v_values + o + 8 * i) = make_uint4(0, 0, 0, 0);
         }
     }
     if (bad_page) atomicOr(&g_kv_error, kKvErrPage);
@@ -195,31 +199,64 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const KvAppendArgs a, co
 // ---------------------------------------------------------------------------
 // Evict
 //
-// One CTA per (sequence, head) with more than keep slots.  Slots are ranked by
-// an order-preserving integer of their weight (protected slots first), the
-// keep-th largest found by four 8-bit radix passes; ties stay in slot order.
-// Survivors keep their slot unless it lies at keep or beyond: the k-th of those
-// moves into the k-th hole below keep.  Sources and holes are disjoint, so the
-// moves need no order among themselves, and a step that drops one slot moves
-// at most one.
+// One cluster of CTAs per (sequence, head) with more than keep slots, a thread
+// per unit of 16 slots: one page lookup, then its weights and positions in
+// 16-byte loads.  Slots are ranked by an order-preserving integer of their
+// weight (protected slots first), kept in registers.  The keep-th largest is
+// found by three radix passes of 11, 11 and 10 bits over shared-memory
+// histograms, summed over the cluster through distributed shared memory; ties
+// stay in slot order (a scan of the threads' counts).  Survivors keep their slot
+// unless it lies at keep or beyond: the k-th of those moves into the k-th hole
+// below keep.  Sources and holes are disjoint, so the moves, dealt to all
+// threads of the cluster, need no order among themselves, and a step that drops
+// one slot moves at most one.  Bound by the chain of passes (short lists) or by
+// the moves' bytes.
 // ---------------------------------------------------------------------------
 constexpr int kEvThreads = 1024;
+constexpr int kEvRadix = 2048;  // bins of a pass
+constexpr int kEvBatch = 4;     // moves that a group of lanes has in flight
 
 struct KvEvictArgs {
     KvView c;
     int keep, recent, sink;
     int32_t* lists;  // per (sequence, head): list_cap holes, then list_cap sources
-    int list_cap;
+    int list_cap;    // a multiple of kEvBatch
 };
+
+// Exclusive scan of one value per thread over the CTA, and the total.
+__device__ __forceinline__ uint32_t cta_scan(uint32_t v, uint32_t* wsum, uint32_t* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t t = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += t;
+    }
+    __syncthreads();  // the last scan's sums have been read
+    if (lane == 31) wsum[warp] = inc;
+    __syncthreads();
+    const uint32_t w = wsum[lane];
+    uint32_t wi = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t t = __shfl_up_sync(0xffffffffu, wi, o);
+        if (lane >= o) wi += t;
+    }
+    *total = __shfl_sync(0xffffffffu, wi, 31);
+    return __shfl_sync(0xffffffffu, wi - w, warp) + inc - v;
+}
 
 template <int D>
 __global__ void __launch_bounds__(kEvThreads) kv_evict_kernel(const KvEvictArgs a) {
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t sel[2];  // chosen digit, slots above it
-    __shared__ unsigned long long wsum[kEvThreads / 32 + 1];
+    __shared__ uint32_t hist[kEvRadix];
+    __shared__ uint32_t sel[2];   // chosen digit, slots above it
+    __shared__ uint32_t sums[3];  // of this CTA: slots equal to the threshold, holes, sources
+    __shared__ uint32_t wsum[32];
     __shared__ int bad_any;
     const KvView& c = a.c;
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int cs = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+    const int h = blockIdx.x / cs, b = blockIdx.y, tid = threadIdx.x;
     pdl_launch_dependents();
     pdl_wait();
     bool bad = false;
@@ -227,135 +264,209 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_kernel(const KvEvictArgs 
     const int gone = static_cast<int>(ldcg_u32(c.evicted + b));
     if (bad && tid == 0) atomicOr(&g_kv_error, kKvErrLen);
     if (tid == 0) bad_any = 0;
-    __syncthreads();
     const bool work = len > a.keep;
     if (work) {
         const int newest = gone + len;
+        const int units = (len + kKvTokens - 1) / kKvTokens, share = (units + cs - 1) / cs, rounds = (share + kEvThreads - 1) / kEvThreads;
         bool bad_page = false;
-        auto key = [&](int slot) -> uint32_t {
-            const int page = kv_page(c, b, slot);
-            if (page < 0) { bad_page = true; return 0u; }
-            const size_t line = kv_line(c, page, h) + slot % c.page_size;
-            const int p = static_cast<int>(ldcg_u32(c.pos + line));
-            if (p >= newest - a.recent || p < a.sink) return 0xFFFFFFFFu;
-            uint32_t u = __float_as_uint(__fadd_rn(ldcg_f32(c.mass + line), 0.f));  // -0 counts as 0
-            u ^= (u >> 31) ? 0xFFFFFFFFu : 0x80000000u;
-            return u < 0xFFFFFFFEu ? u : 0xFFFFFFFEu;
+        uint32_t k[kKvTokens];
+        int n = 0, slot0 = 0;  // this thread's unit of the round: its slots in use, the first of them
+        auto fetch = [&](int round) {
+            const int i = round * kEvThreads + tid;
+            slot0 = (rank * share + i) * kKvTokens;
+            n = i >= share || len - slot0 < 0 ? 0 : (len - slot0 > kKvTokens ? kKvTokens : len - slot0);
+            const int page = n > 0 ? kv_page(c, b, slot0) : 0;
+            if (n > 0 && page < 0) {
+                bad_page = true;  // the slots of an absent page weigh least
+#pragma unroll
+                for (int i = 0; i < kKvTokens; ++i) k[i] = 0u;
+            } else if (n > 0) {
+                const size_t line = kv_line(c, page, h) + slot0 % c.page_size;
+                uint32_t w[kKvTokens], p[kKvTokens];
+                const bool wide = ((reinterpret_cast<uintptr_t>(c.mass) | reinterpret_cast<uintptr_t>(c.pos)) & 15u) == 0;
+#pragma unroll
+                for (int i = 0; i < kKvTokens; i += 4) {
+                    if (wide) {
+                        const uint4 x = ldcg_v4(c.mass + line + i), y = ldcg_v4(c.pos + line + i);
+                        w[i] = x.x; w[i + 1] = x.y; w[i + 2] = x.z; w[i + 3] = x.w;
+                        p[i] = y.x; p[i + 1] = y.y; p[i + 2] = y.z; p[i + 3] = y.w;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            w[i + e] = ldcg_u32(c.mass + line + i + e);
+                            p[i + e] = ldcg_u32(c.pos + line + i + e);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kKvTokens; ++i) {
+                    uint32_t u = __float_as_uint(__fadd_rn(__uint_as_float(w[i]), 0.f));  // -0 counts as 0
+                    u ^= (u >> 31) ? 0xFFFFFFFFu : 0x80000000u;
+                    const int at = static_cast<int>(p[i]);
+                    k[i] = (at >= newest - a.recent || at < a.sink) ? 0xFFFFFFFFu : (u < 0xFFFFFFFEu ? u : 0xFFFFFFFEu);
+                }
+            }
         };
+        if (rounds == 1) fetch(0);
         // the keep-th largest key
         uint32_t prefix = 0, mask = 0;
         int need = a.keep;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
+#pragma unroll
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
+            const uint32_t bins = pass == 2 ? 1023u : 2047u;
+            hist[tid] = hist[tid + kEvThreads] = 0;
             __syncthreads();
-            for (int s = tid; s < len; s += kEvThreads) {
-                const uint32_t k = key(s);
-                if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1u);
+            for (int r = 0; r < rounds; ++r) {
+                if (rounds > 1) fetch(r);
+#pragma unroll
+                for (int i = 0; i < kKvTokens; ++i)
+                    if (i < n && (k[i] & mask) == prefix) atomicAdd(&hist[(k[i] >> shift) & bins], 1u);
             }
-            __syncthreads();
-            if (warp == 0) {
-                // lane l covers digits 255 - 8l .. 248 - 8l, from the top
-                uint32_t sum = 0;
+            cluster.sync();
+            // bins top and top + 1 of the whole cluster, threads counted from the largest bin
+            const int top = kEvRadix - 2 - 2 * tid;
+            uint32_t n0 = 0, n1 = 0;
+            for (int r = 0; r < cs; ++r) {
+                const uint2 v = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(&hist[0], r) + top);
+                n0 += v.x;
+                n1 += v.y;
+            }
+            uint32_t total;
+            const uint32_t before = cta_scan(n0 + n1, wsum, &total), want = static_cast<uint32_t>(need);
+            if (before < want && want <= before + n0 + n1) {
+                const bool high = want <= before + n1;
+                sel[0] = static_cast<uint32_t>(high ? top + 1 : top);
+                sel[1] = high ? before : before + n1;
+            }
+            cluster.sync();
+            prefix |= sel[0] << shift;
+            mask |= bins << shift;
+            need -= static_cast<int>(sel[1]);
+        }
+        // slots equal to the threshold before this CTA's
+        auto equal = [&]() {
+            uint32_t e = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum += hist[255 - 8 * lane - i];
-                uint32_t inc = sum;
+            for (int i = 0; i < kKvTokens; ++i) e += i < n && k[i] == prefix;
+            return e;
+        };
+        uint32_t total, acc = 0;
+        for (int r = 0; r < rounds; ++r) {
+            if (rounds > 1) fetch(r);
+            cta_scan(equal(), wsum, &total);
+            acc += total;
+        }
+        if (tid == 0) sums[0] = acc;
+        cluster.sync();
+        uint32_t eq0 = 0;
+        for (int r = 0; r < rank; ++r) eq0 += *cluster.map_shared_rank(&sums[0], r);
+        // bit i: slot i of the thread's unit stays; its holes | sources << 16
+        uint32_t stay = 0, mine = 0, eq_run = eq0;
+        auto decide = [&]() {
+            uint32_t e = eq_run + cta_scan(equal(), wsum, &total);
+            eq_run += total;
+            stay = 0;
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
-                    if (lane >= o) inc += v;
+            for (int i = 0; i < kKvTokens; ++i) {
+                const bool same = k[i] == prefix;
+                if (i < n && (k[i] > prefix || (same && e < static_cast<uint32_t>(need)))) stay |= 1u << i;
+                e += same && i < n;
+            }
+            const int low = a.keep - slot0 < 0 ? 0 : (a.keep - slot0 > kKvTokens ? kKvTokens : a.keep - slot0);
+            const uint32_t below = (1u << low) - 1u, used = (1u << n) - 1u;
+            mine = __popc(~stay & below & used) | (__popc(stay & ~below) << 16);
+        };
+        uint32_t holes_n = 0, from_n = 0;
+        for (int r = 0; r < rounds; ++r) {
+            if (rounds > 1) fetch(r);
+            decide();
+            cta_scan(mine, wsum, &total);  // at most 16 x 1024 of either: no carry between the halves
+            holes_n += total & 0xFFFFu;
+            from_n += total >> 16;
+        }
+        if (tid == 0) { sums[1] = holes_n; sums[2] = from_n; }
+        cluster.sync();
+        uint32_t holes_at = 0, from_at = 0;
+        int n_moves = 0;
+        for (int r = 0; r < cs; ++r) {
+            const uint32_t* s = cluster.map_shared_rank(&sums[0], r);
+            const uint32_t x = s[1], y = s[2];
+            if (r < rank) { holes_at += x; from_at += y; }
+            n_moves += static_cast<int>(x);
+        }
+        int32_t* holes = a.lists + (static_cast<size_t>(b) * c.heads + h) * 2 * a.list_cap;
+        int32_t* from = holes + a.list_cap;
+        eq_run = eq0;
+        for (int r = 0; r < rounds; ++r) {
+            if (rounds > 1) { fetch(r); decide(); }
+            const uint32_t at = cta_scan(mine, wsum, &total);
+            uint32_t x = holes_at + (at & 0xFFFFu), y = from_at + (at >> 16);
+            for (int i = 0; i < n; ++i) {
+                const bool st = stay >> i & 1u;
+                if (slot0 + i < a.keep) {
+                    if (!st && x < static_cast<uint32_t>(a.list_cap)) holes[x++] = slot0 + i;
+                } else if (st && y < static_cast<uint32_t>(a.list_cap)) {
+                    from[y++] = slot0 + i;
                 }
-                const uint32_t before = inc - sum, want = static_cast<uint32_t>(need);
-                if (before < want && want <= inc) {
-                    uint32_t acc = before;
-                    for (int i = 0; i < 8; ++i) {
-                        const uint32_t n = hist[255 - 8 * lane - i];
-                        if (acc + n >= want) { sel[0] = 255 - 8 * lane - i; sel[1] = acc; break; }
-                        acc += n;
+            }
+            holes_at += total & 0xFFFFu;
+            from_at += total >> 16;
+        }
+        cluster.sync();
+        // moves: L lanes a slot, each 8 bytes of K codes and the 16 bytes of V words that hold its 16 columns
+        constexpr int L = D / 16;
+        const int l = tid % L, groups = cs * kEvThreads / L;
+        for (int m0 = (rank * kEvThreads + tid) / L * kEvBatch; m0 < n_moves; m0 += groups * kEvBatch) {
+            uint2 kc[kEvBatch], par[kEvBatch];
+            uint4 vc[kEvBatch];
+            uint32_t w[kEvBatch], p[kEvBatch];
+            int to[kEvBatch], pt[kEvBatch];
+            bool on[kEvBatch];
+#pragma unroll
+            for (int j = 0; j < kEvBatch; ++j) {
+                to[j] = 0;
+                int src = a.keep;
+                on[j] = m0 + j < n_moves;
+                if (on[j]) {
+                    to[j] = static_cast<int>(ldcg_u32(holes + m0 + j));
+                    src = static_cast<int>(ldcg_u32(from + m0 + j));
+                    if (to[j] < 0 || to[j] >= a.keep || src < a.keep || src >= len) on[j] = false;  // this call's lists: never
+                }
+                const int ps = on[j] ? kv_page(c, b, src) : -1;
+                pt[j] = on[j] ? kv_page(c, b, to[j]) : -1;
+                if (on[j] && (ps < 0 || pt[j] < 0)) { bad_page = true; on[j] = false; }
+                if (on[j]) {
+                    const int os = src % c.page_size, rs = os % kKvTokens;
+                    const uint8_t* us = kv_unit<D>(c, ps, h, os);
+                    kc[j] = *reinterpret_cast<const uint2*>(us + rs * (D / 2) + 8 * l);
+                    vc[j] = *reinterpret_cast<const uint4*>(us + kv_v_offset(D) + (rs / 2) * D + 16 * l);
+                    if (rs & 1) vc[j] = make_uint4(vc[j].x >> 16, vc[j].y >> 16, vc[j].z >> 16, vc[j].w >> 16);
+                    if (l == 0) {
+                        par[j] = *reinterpret_cast<const uint2*>(us + kv_param_offset(D) + 8 * rs);
+                        const size_t ls = kv_line(c, ps, h) + os;
+                        w[j] = ldcg_u32(c.mass + ls);
+                        p[j] = ldcg_u32(c.pos + ls);
                     }
                 }
             }
-            __syncthreads();
-            prefix |= sel[0] << shift;
-            mask |= 255u << shift;
-            need -= static_cast<int>(sel[1]);
-            __syncthreads();
-        }
-        // exclusive scan over the CTA of one 64-bit value per thread
-        auto scan = [&](unsigned long long v, unsigned long long* total) {
-            unsigned long long inc = v;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const unsigned long long t = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += t;
-            }
-            __syncthreads();
-            if (lane == 31) wsum[warp] = inc;
-            __syncthreads();
-            if (warp == 0) {
-                const unsigned long long w = wsum[lane];
-                unsigned long long wi = w;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const unsigned long long t = __shfl_up_sync(0xffffffffu, wi, o);
-                    if (lane >= o) wi += t;
+            for (int j = 0; j < kEvBatch; ++j) {
+                if (!on[j]) continue;
+                const int ot = to[j] % c.page_size, rt = ot % kKvTokens;
+                uint8_t* ut = kv_unit<D>(c, pt[j], h, ot);
+                *reinterpret_cast<uint2*>(ut + rt * (D / 2) + 8 * l) = kc[j];
+                uint16_t* vt = reinterpret_cast<uint16_t*>(ut + kv_v_offset(D) + (rt / 2) * D + 16 * l) + (rt & 1);
+                vt[0] = static_cast<uint16_t>(vc[j].x);
+                vt[2] = static_cast<uint16_t>(vc[j].y);
+                vt[4] = static_cast<uint16_t>(vc[j].z);
+                vt[6] = static_cast<uint16_t>(vc[j].w);
+                if (l == 0) {
+                    *reinterpret_cast<uint2*>(ut + kv_param_offset(D) + 8 * rt) = par[j];
+                    const size_t lt = kv_line(c, pt[j], h) + ot;
+                    c.mass[lt] = __uint_as_float(w[j]);
+                    c.pos[lt] = static_cast<int>(p[j]);
                 }
-                wsum[lane] = wi - w;
-                if (lane == 31) wsum[32] = wi;
-            }
-            __syncthreads();
-            *total = wsum[32];
-            return wsum[warp] + inc - v;
-        };
-        // slots in contiguous chunks per thread, so that ranks follow the slot order
-        const int per = (len + kEvThreads - 1) / kEvThreads;
-        const int s0 = min(tid * per, len), s1 = min(s0 + per, len);
-        unsigned long long total = 0, eq = 0;
-        for (int s = s0; s < s1; ++s) eq += key(s) == prefix;
-        const unsigned long long eq0 = scan(eq, &total);
-        unsigned long long cnt = 0, e = eq0;
-        for (int s = s0; s < s1; ++s) {
-            const uint32_t k = key(s);
-            const bool stays = k > prefix || (k == prefix && e < static_cast<unsigned long long>(need));
-            e += k == prefix;
-            if (s < a.keep && !stays) cnt += 1ull;
-            if (s >= a.keep && stays) cnt += 1ull << 32;
-        }
-        const unsigned long long base = scan(cnt, &total);
-        const int n_moves = static_cast<int>(total & 0xFFFFFFFFull);
-        int32_t* holes = a.lists + (static_cast<size_t>(b) * c.heads + h) * 2 * a.list_cap;
-        int32_t* from = holes + a.list_cap;
-        int hi = static_cast<int>(base & 0xFFFFFFFFull), fi = static_cast<int>(base >> 32);
-        e = eq0;
-        for (int s = s0; s < s1; ++s) {
-            const uint32_t k = key(s);
-            const bool stays = k > prefix || (k == prefix && e < static_cast<unsigned long long>(need));
-            e += k == prefix;
-            if (s < a.keep && !stays && hi < a.list_cap) holes[hi++] = s;
-            if (s >= a.keep && stays && fi < a.list_cap) from[fi++] = s;
-        }
-        __syncthreads();
-        // moves: D/16 lanes a slot, each 8 bytes of K and 4 half words of V
-        constexpr int L = D / 16;
-        for (int m = tid / L; m < n_moves; m += kEvThreads / L) {
-            const int l = tid % L, to = holes[m], src = from[m];
-            if (to < 0 || to >= a.keep || src < a.keep || src >= len) continue;  // lists are this call's: never taken
-            const int pt = kv_page(c, b, to), ps = kv_page(c, b, src);
-            if (pt < 0 || ps < 0) { bad_page = true; continue; }
-            const int ot = to % c.page_size, os = src % c.page_size;
-            uint8_t* ut = kv_unit<D>(c, pt, h, ot);
-            const uint8_t* us = kv_unit<D>(c, ps, h, os);
-            const int rt = ot % kKvTokens, rs = os % kKvTokens;
-            *reinterpret_cast<uint2*>(ut + rt * (D / 2) + 8 * l) = *reinterpret_cast<const uint2*>(us + rs * (D / 2) + 8 * l);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<uint16_t*>(ut + kv_v_offset(D) + (rt / 2) * D + 4 * (4 * l + i) + 2 * (rt & 1)) =
-                    *reinterpret_cast<const uint16_t*>(us + kv_v_offset(D) + (rs / 2) * D + 4 * (4 * l + i) + 2 * (rs & 1));
-            if (l == 0) {
-                *reinterpret_cast<uint2*>(ut + kv_param_offset(D) + 8 * rt) =
-                    *reinterpret_cast<const uint2*>(us + kv_param_offset(D) + 8 * rs);
-                const size_t lt = kv_line(c, pt, h) + ot, ls = kv_line(c, ps, h) + os;
-                c.mass[lt] = c.mass[ls];
-                c.pos[lt] = c.pos[ls];
             }
         }
         if (bad_page) bad_any = 1;
@@ -363,6 +474,7 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_kernel(const KvEvictArgs 
     __syncthreads();
     if (tid == 0) {
         if (bad_any) atomicOr(&g_kv_error, kKvErrPage);
+        // every CTA of the sequence has read its length: the last one to arrive writes the new one
         if (atomicAdd(c.arrivals + b, 1u) == gridDim.x - 1) {
             c.arrivals[b] = 0;
             if (work) {
@@ -371,6 +483,15 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_kernel(const KvEvictArgs 
             }
         }
     }
+}
+
+// CTAs per (sequence, head): as many as fill the GPU once (two of 1024 threads on an SM), at most 8 and no more
+// than give every CTA 4096 slots of a full sequence.
+int evict_cluster(const dq_kv_cache_t& c, int sm_count) {
+    const long long pairs = static_cast<long long>(c.n_seqs) * c.kv_heads, cap = static_cast<long long>(c.max_pages) * c.page_size;
+    int cs = 1;
+    while (cs < 8 && pairs * cs * 2 <= 2ll * sm_count && cap >= 4096ll * cs * 2) cs *= 2;
+    return cs;
 }
 
 }  // namespace
@@ -388,35 +509,44 @@ dq_status_t launch_kv_append(const dq_kv_cache_t& c, const uint16_t* k, const in
     a.counts = counts;
     a.at = at;
     a.tokens = tokens;
-    const int threads = 128, subs = threads / (c.head_dim / 4);
+    const int threads = 128, subs = threads / (c.head_dim / 8);
     const long long items = (static_cast<long long>(tokens) / 2 + 1) * c.kv_heads;
-    const int rounds = 4;  // items a sub-warp takes, one after another
-    const int per = subs * rounds;
+    const int per = subs * 4;  // a sub-warp takes four items, one after another
     const dim3 grid(static_cast<unsigned>((items + per - 1) / per), c.n_seqs);
-    if (c.head_dim == 128) return launch_pdl(kv_append_kernel<128>, grid, threads, 0, stream, a, per);
-    return launch_pdl(kv_append_kernel<64>, grid, threads, 0, stream, a, per);
+    const bool values = k_values != nullptr;
+    if (c.head_dim == 128)
+        return values ? launch_pdl(kv_append_kernel<128, true>, grid, threads, 0, stream, 1, a, per)
+                      : launch_pdl(kv_append_kernel<128, false>, grid, threads, 0, stream, 1, a, per);
+    return values ? launch_pdl(kv_append_kernel<64, true>, grid, threads, 0, stream, 1, a, per)
+                  : launch_pdl(kv_append_kernel<64, false>, grid, threads, 0, stream, 1, a, per);
+}
+
+// Holes and sources of one head, at most, rounded up to a batch.
+static long long evict_list_cap(const dq_kv_cache_t& c, int keep) {
+    const long long cap = static_cast<long long>(c.max_pages) * c.page_size, n = keep < cap - keep ? keep : cap - keep;
+    return n <= 0 ? 0 : (n + kEvBatch - 1) / kEvBatch * kEvBatch;
 }
 
 size_t kv_evict_workspace(const dq_kv_cache_t& c, int keep) {
-    const long long cap = static_cast<long long>(c.max_pages) * c.page_size;
-    const long long n = keep < cap - keep ? keep : cap - keep;  // holes and sources of one head, at most
-    if (n <= 0) return 0;
-    return align256(static_cast<size_t>(c.n_seqs) * c.kv_heads * 2 * static_cast<size_t>(n) * sizeof(int32_t));
+    return align256(static_cast<size_t>(c.n_seqs) * c.kv_heads * 2 * static_cast<size_t>(evict_list_cap(c, keep)) * sizeof(int32_t));
 }
 
 dq_status_t launch_kv_evict(const dq_kv_cache_t& c, int keep, int recent, int sink, void* workspace,
                             cudaStream_t stream) {
+    DeviceInfo di;
+    const dq_status_t st = device_info(&di);
+    if (st != DQ_OK) return st;
     KvEvictArgs a{};
     a.c = kv_view(c);
     a.keep = keep;
     a.recent = recent;
     a.sink = sink;
     a.lists = static_cast<int32_t*>(workspace);
-    const long long cap = static_cast<long long>(c.max_pages) * c.page_size;
-    a.list_cap = static_cast<int>(keep < cap - keep ? keep : cap - keep);
-    const dim3 grid(c.kv_heads, c.n_seqs);
-    if (c.head_dim == 128) return launch_pdl(kv_evict_kernel<128>, grid, kEvThreads, 0, stream, a);
-    return launch_pdl(kv_evict_kernel<64>, grid, kEvThreads, 0, stream, a);
+    a.list_cap = static_cast<int>(evict_list_cap(c, keep));
+    const int cs = evict_cluster(c, di.sm_count);
+    const dim3 grid(c.kv_heads * cs, c.n_seqs);
+    if (c.head_dim == 128) return launch_pdl(kv_evict_kernel<128>, grid, kEvThreads, 0, stream, cs, a);
+    return launch_pdl(kv_evict_kernel<64>, grid, kEvThreads, 0, stream, cs, a);
 }
 
 dq_status_t read_kv_error(uint32_t* word, bool clear) {

@@ -66,19 +66,23 @@ __device__ __forceinline__ int kv_length(const KvView& c, int b, bool* bad) {
     return n < 0 ? 0 : (n > cap ? cap : n);
 }
 
-// A launch as a programmatic dependent of the preceding work on the stream.
+// A launch as a programmatic dependent of the preceding work on the stream, in clusters of cluster x 1 CTAs.
 template <class K, class... A>
-inline dq_status_t launch_pdl(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t stream, A... args) {
+inline dq_status_t launch_pdl(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t stream, int cluster, A... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e != cudaSuccess) { set_cuda_error(e); return DQ_ERR_CUDA; }

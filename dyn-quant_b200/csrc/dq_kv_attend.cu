@@ -31,7 +31,8 @@
 // MMA and are set right at the end.  Scales and zeros are applied in FP32:
 //   S   = s_k (D - z_k sum q),  D the MMAs' sum of q c
 //   O   = sum p' (c - 8) - sum p' (z_v - 8),  p' = p s_v w
-// The 8 is taken off by a second MMA with a constant A, which keeps the running
+// The 8 is the same for all columns: one MMA a unit with a constant A collects
+// 8 sum p' and every 8 steps it is taken off all of O, which keeps the running
 // sums (FP32, and the rounding of p' in them) at the size of the centred values.
 // p' is the only rounding to FP16 besides the output's: p <= 2^8 (the maximum
 // is taken again only when a score passes it by 8) and w is the power of two
@@ -72,6 +73,7 @@ struct KvAttendArgs {
     int tokens, group, n_rt; // query tokens, query heads per KV head, row tiles
     float scale2;            // scale * log2(e) * kCode
     int depth;               // ring slots per warp
+    int first_off;           // offset in shared memory of those pieces, 0: they are in the workspace
 };
 
 // The list of steps: a job is steps_of(len[b]) steps of one (sequence, KV head,
@@ -433,12 +435,13 @@ struct StepStream {
         fence_mbar_init();
         __syncwarp();
     }
-    __device__ __forceinline__ void lookup(const KvAttendArgs& a, const Plan& p) {
+    __device__ __forceinline__ StepAt lookup(const KvAttendArgs& a, const Plan& p) {
         src[0] = src[1] = -1;
         bool bad = false;
         const int i = issued + (threadIdx.x & 31);
+        StepAt x{0, 0, 0, 0};
         if (i < n) {
-            const StepAt x = step_at(p, a.c.n_seqs, u0 + i);
+            x = step_at(p, a.c.n_seqs, u0 + i);
             const int h = kKeysOnly ? x.job : x.job / a.n_rt;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -450,10 +453,11 @@ struct StepStream {
             }
         }
         if (__any_sync(0xffffffffu, bad)) absent = true;
+        return x;
     }
     // Issue the copies of the run's next step into slot s (every lane calls it).
     __device__ __forceinline__ void issue(const KvAttendArgs& a, const Plan& p, int s) {
-        if ((issued & 31) == 0) lookup(a, p);
+        if (issued > 0 && (issued & 31) == 0) lookup(a, p);
         const int i0 = __shfl_sync(0xffffffffu, src[0], issued), i1 = __shfl_sync(0xffffffffu, src[1], issued);
         if ((threadIdx.x & 31) == 0) {
             const uint32_t bar = base() + bars + 8 * s, dst = base() + ring + s * kSlot;
@@ -492,20 +496,33 @@ struct StepStream {
             }
         }
     }
-    __device__ __forceinline__ void start(const KvAttendArgs& a, const Plan& p, long long first, int count) {
+    // Where the run begins; then fill() asks for its first steps.
+    __device__ __forceinline__ StepAt start(const KvAttendArgs& a, const Plan& p, long long first, int count) {
         u0 = first;
         n = count;
         issued = parity = slot = 0;
         absent = false;
+        StepAt x = lookup(a, p);
+        x.b = __shfl_sync(0xffffffffu, x.b, 0);
+        x.len = __shfl_sync(0xffffffffu, x.len, 0);
+        x.job = __shfl_sync(0xffffffffu, x.job, 0);
+        x.step = __shfl_sync(0xffffffffu, x.step, 0);
+        return x;
+    }
+    __device__ __forceinline__ void fill(const KvAttendArgs& a, const Plan& p) {
         const int m = min(depth, n);
         for (int i = 0; i < m; ++i) issue(a, p, i);
     }
-    // Wait for the step in the current slot; false when the bounded wait gave up.
-    __device__ __forceinline__ bool wait() {
-        const bool got = mbar_wait_bounded(base() + bars + 8 * slot, parity);
+    // Wait for the step `ahead` slots on; false when the bounded wait gave up.
+    __device__ __forceinline__ bool wait(int ahead = 0) {
+        const bool wrap = slot + ahead >= depth;
+        const bool got = mbar_wait_bounded(base() + bars + 8 * (slot + ahead - (wrap ? depth : 0)), parity ^ (wrap ? 1 : 0));
         return __all_sync(0xffffffffu, got);
     }
     __device__ __forceinline__ int unit() const { return ring + slot * kSlot; }
+    __device__ __forceinline__ int unit(int ahead) const {
+        return ring + (slot + ahead - (slot + ahead >= depth ? depth : 0)) * kSlot;
+    }
     // Bit e: unit e of the step was copied (only asked for when some unit of the run is absent).
     __device__ __forceinline__ uint32_t found() const { return smem_at<uint32_t>(flags + 4 * slot); }
     // The current slot is read: refill it, go to the next.
@@ -527,7 +544,7 @@ struct StepStream {
 // The running softmax of one job in one warp: rows 2t, 2t + 1 of each row tile.
 template <int D, int NT>
 struct RowState {
-    float o[NT][D / 16][4], vw;
+    float o[NT][D / 16][4], c8[NT][4], vw;  // c8: - 8 sum p' since the last settle(), in either scale of o
     f2 m[NT], l[NT], zs[NT];  // m: minus the running maximum
 
     __device__ __forceinline__ void clear() {
@@ -537,6 +554,8 @@ struct RowState {
             for (int j = 0; j < D / 16; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[nt][j][e] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c8[nt][e] = 0.f;
             m[nt] = f2(-kNone);
             l[nt] = zs[nt] = f2(0.f);
         }
@@ -628,9 +647,7 @@ struct RowState {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k) mma(o[nt][k], kLow8, kHigh8, kLow8, kHigh8, pf[u][nt][0], pf[u][nt][1]);
+            for (int nt = 0; nt < NT; ++nt) mma(c8[nt], kLow8, kHigh8, kLow8, kHigh8, pf[u][nt][0], pf[u][nt][1]);
 #pragma unroll
             for (int k = 0; k < D / 32; ++k) {
                 const uint32_t w0 = v[u][0][k], w1 = v[u][1][k], y0 = w0 >> 8, y1 = w1 >> 8;
@@ -642,6 +659,17 @@ struct RowState {
                 }
             }
         }
+    }
+
+    __device__ __forceinline__ void settle() {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) o[nt][k][x] += c8[nt][x];
+                c8[nt][x] = 0.f;
+            }
     }
 
     __device__ __forceinline__ void rescale(const float (&top)[NT][2], float big) {
@@ -670,6 +698,8 @@ struct RowState {
             for (int k = 0; k < D / 16; ++k)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) o[nt][k][x] *= (x & 1) ? fr.y() : fr.x();
+#pragma unroll
+            for (int x = 0; x < 4; ++x) c8[nt][x] *= (x & 1) ? fr.y() : fr.x();
         }
     }
 
@@ -771,21 +801,26 @@ struct Piece {
 // ---------------------------------------------------------------------------
 template <int D, int NT>
 __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kernel(const KvAttendArgs a) {
-    constexpr int W = at_warps(NT), R = 8 * NT, kPiece = R * (D + 2);
+    constexpr int W = at_warps(NT), R = 8 * NT;
+    static_assert(2 * W <= 32, "a lane per piece");
     extern __shared__ __align__(128) char smem[];
     __shared__ Piece pieces[2 * W];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const KvView& c = a.c;
     __shared__ Piece cut[2];
     __shared__ Share share[2];
+    __shared__ bool join[2];
     StepStream<D, false> st;
     st.init(plan_bytes(c.n_seqs), W, warp, a.depth);
-    // A piece is [R][D + 2] floats: output, maximum, sum.  A warp's last piece takes its ring, which has run
-    // dry by then; one of a job that ends inside the run goes to the workspace, so that the rings have all
-    // of the shared memory.
+    // A piece is a row of D + 2 floats for each row of the job: output, maximum, sum.  A warp's last piece
+    // takes its ring, which has run dry by then; one of a job that ends inside the run goes behind the rings
+    // if it is small, else to the workspace, so that the rings have the shared memory.
+    const int piece = min(a.tokens * a.group, R) * (D + 2);
     auto piece_at = [&](int k) {
-        return (k & 1) ? reinterpret_cast<float*>(smem + plan_bytes(c.n_seqs) + (k >> 1) * a.depth * StepStream<D, false>::kSlot)
-                       : a.first + (static_cast<size_t>(blockIdx.x) * W + (k >> 1)) * kPiece;
+        const int i = k >> 1;
+        if (k & 1) return reinterpret_cast<float*>(smem + plan_bytes(c.n_seqs) + i * a.depth * StepStream<D, false>::kSlot);
+        if (a.first_off > 0) return reinterpret_cast<float*>(smem + a.first_off) + i * piece;
+        return a.first + (static_cast<size_t>(blockIdx.x) * W + i) * piece;
     };
     pdl_launch_dependents();
     pdl_wait();
@@ -804,26 +839,31 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
         int b = 0, job = 0, len = 0, ub = 0, ul = 0, done = 0;
         bool gave_up = false;
         int left = 0;  // steps of the current sequence not yet begun, those of this run
-        auto next_seq = [&]() {
-            const long long u = u0 + done;
-            const StepAt x = step_at(p, c.n_seqs, u);
+        auto begin = [&](const StepAt& x) {
             b = x.b;
             len = x.len;
             ul = steps_of(len);
             job = x.job;
             ub = x.step;
-            left = static_cast<int>(min(static_cast<long long>(p.pre[b + 1]) * p.jobs - u, static_cast<long long>(n - done)));
+            left = static_cast<int>(min(static_cast<long long>(p.pre[b + 1]) * p.jobs - (u0 + done), static_cast<long long>(n - done)));
         };
         {
             // the first queries are asked for before the whole GPU's first copies
-            next_seq();
+            begin(st.start(a, p, u0, n));
             uint4 raw[NT][D / 32];
             q.request(a, b, job / a.n_rt, job % a.n_rt, raw);
-            st.start(a, p, u0, n);
+            st.fill(a, p);
+            if (a.n_rt == 1 && warp == 0 && lane < 2) {
+                // while the copies travel: the jobs at the CTA's two ends, and who shares them
+                const StepAt x = step_at(p, c.n_seqs, lane == 0 ? u0 : p.runs.start(w + W) - 1);
+                cut[lane] = Piece{x.b, x.job, 0, 0};
+                share[lane] = share_of<W>(p.pre, c.n_seqs, p.jobs, p.runs, x.b, x.job);
+            }
+            __syncwarp();
             q.arrange(a, job % a.n_rt, len, raw);
         }
         while (done < n && !gave_up) {
-            if (left == 0) next_seq();
+            if (left == 0) begin(step_at(p, c.n_seqs, u0 + done));
             // a job, or the part of it in this run
             const int first = ub, take = min(ul - ub, n - done);
             const int h = job / a.n_rt, rt = job - h * a.n_rt;
@@ -842,6 +882,7 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
                         found = st.found();
                         if (j + kKvTokens >= len) found |= 2u;  // behind the last slot: not copied, and not missed
                     }
+                    if ((ub & 7) == 7) rs.settle();
                     // the slot is refilled as soon as its V codes are in registers
                     if constexpr (NT == 1) {
                         uint32_t pf[2][NT][2], v[2][2][D / 32];
@@ -862,6 +903,7 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
                 }
             }
             if (gave_up) break;
+            rs.settle();
             const bool whole = first == 0 && ub == ul;
             const int k = 2 * warp + (done + take == n ? 1 : 0);
 #pragma unroll
@@ -901,75 +943,72 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
     __syncthreads();
     // Neighbouring pieces of one job meet here, in order, its rows dealt to the warps; a job that ends up
     // whole is finished, the others (at most the CTA's first and last) go to the workspace.
-    int turn = 0, cuts = 0;
-    for (int k = 0; k < 2 * W;) {
-        const Piece first = pieces[k];
-        if (first.job < 0) { ++k; continue; }
-        int end = first.end, k1 = k + 1;
-        for (; k1 < 2 * W; ++k1) {
-            const Piece x = pieces[k1];
-            if (x.job < 0) continue;
-            if (x.b != first.b || x.job != first.job) break;
-            end = x.end;
-        }
-        const bool whole = first.first == 0 && end == steps_of(p.len[first.b]);
-        {
-            const int h = first.job / a.n_rt, rt = first.job - h * a.n_rt, n_rows = min(R, rows - rt * R);
-            constexpr int C = 8, L = D / C, P = 32 / L;  // columns of a lane, lanes of a row, rows of a turn
-            for (int r0 = 0; r0 < n_rows; r0 += P, ++turn) {
-                const int rl = r0 + lane / L, col = C * (lane % L);
-                if (turn % W != warp || rl >= n_rows) continue;
-                float m = kNone, sum = 0.f, v[C];
-                for (int x = k; x < k1; ++x)
-                    if (pieces[x].job >= 0) m = fmaxf(m, piece_at(x)[rl * (D + 2) + D]);
+    Piece mine{0, -1, 0, 0};  // lane k: piece k
+    if (lane < 2 * W) mine = pieces[lane];
+    const uint32_t valid = __ballot_sync(0xffffffffu, mine.job >= 0);
+    const uint32_t lower = valid & ((1u << lane) - 1u);
+    const int prev = lower ? 31 - __clz(lower) : 0;
+    const int pb = __shfl_sync(0xffffffffu, mine.b, prev), pj = __shfl_sync(0xffffffffu, mine.job, prev);
+    uint32_t heads = __ballot_sync(0xffffffffu, mine.job >= 0 && (!lower || pb != mine.b || pj != mine.job));
+    int turn = 0, cuts = 0, ends = 0;  // bit i of ends: cut job i is the CTA's last and not its first
+    while (heads) {
+        const int k = __ffs(heads) - 1;
+        heads &= heads - 1;
+        const uint32_t members = valid & ~((1u << k) - 1u) & (heads ? (heads & (0u - heads)) - 1u : 0xffffffffu);
+        const int jb = __shfl_sync(0xffffffffu, mine.b, k), jj = __shfl_sync(0xffffffffu, mine.job, k);
+        const bool whole = __shfl_sync(0xffffffffu, mine.first, k) == 0 &&
+                           __shfl_sync(0xffffffffu, mine.end, 31 - __clz(members)) == steps_of(p.len[jb]);
+        const int h = jj / a.n_rt, rt = jj - h * a.n_rt, n_rows = min(R, rows - rt * R);
+        constexpr int C = 8, L = D / C, P = 32 / L;  // columns of a lane, lanes of a row, rows of a turn
+        for (int r0 = 0; r0 < n_rows; r0 += P, ++turn) {
+            const int rl = r0 + lane / L, col = C * (lane % L);
+            if (turn % W != warp || rl >= n_rows) continue;
+            float m = kNone, sum = 0.f, v[C];
+            for (uint32_t x = members; x; x &= x - 1) m = fmaxf(m, piece_at(__ffs(x) - 1)[rl * (D + 2) + D]);
 #pragma unroll
-                for (int y = 0; y < C; ++y) v[y] = 0.f;
-                for (int x = k; x < k1; ++x) {
-                    if (pieces[x].job < 0) continue;
-                    const float* src = piece_at(x) + rl * (D + 2);
-                    const float f = ex2(src[D] - m);
-                    sum += src[D + 1] * f;
+            for (int y = 0; y < C; ++y) v[y] = 0.f;
+            for (uint32_t x = members; x; x &= x - 1) {
+                const float* src = piece_at(__ffs(x) - 1) + rl * (D + 2);
+                const float f = ex2(src[D] - m);
+                sum += src[D + 1] * f;
 #pragma unroll
-                    for (int y = 0; y < C; y += 2) {
-                        const float2 z = *reinterpret_cast<const float2*>(src + col + y);
-                        v[y] += z.x * f;
-                        v[y + 1] += z.y * f;
-                    }
+                for (int y = 0; y < C; y += 2) {
+                    const float2 z = *reinterpret_cast<const float2*>(src + col + y);
+                    v[y] += z.x * f;
+                    v[y + 1] += z.y * f;
                 }
-                if (whole) {
-                    store_row(a, first.b, h, rt * R + rl, col, v, m, sum);
-                } else {
-                    const size_t pi = (static_cast<size_t>(blockIdx.x) * 2 + cuts) * R + rl;
-                    float4* dst = reinterpret_cast<float4*>(a.part + pi * D + col);
-                    dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-                    dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-                    if (col == 0) *reinterpret_cast<float2*>(a.part_ml + pi * 2) = make_float2(m, sum);
-                }
+            }
+            if (whole) {
+                store_row(a, jb, h, rt * R + rl, col, v, m, sum);
+            } else {
+                const size_t pi = (static_cast<size_t>(blockIdx.x) * 2 + cuts) * R + rl;
+                float4* dst = reinterpret_cast<float4*>(a.part + pi * D + col);
+                dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+                dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+                if (col == 0) *reinterpret_cast<float2*>(a.part_ml + pi * 2) = make_float2(m, sum);
             }
         }
         if (!whole) {
-            if (threadIdx.x == 0) cut[cuts] = first;
+            if (a.n_rt == 1 && (cut[0].b != jb || cut[0].job != jj)) ends |= 1 << cuts;
             ++cuts;
         }
-        k = k1;
     }
     if (cuts > 0 && a.n_rt == 1) {
         // one row tile: the last of a job's CTAs to arrive joins the partial sums, in CTA order
         __syncthreads();
         if (threadIdx.x < cuts) {
-            const Piece x = cut[threadIdx.x];
-            const Share s = share_of<W>(p.pre, c.n_seqs, p.jobs, p.runs, x.b, x.job);
+            const int i = ends >> threadIdx.x & 1;
             __threadfence();
-            uint32_t* d = a.done + static_cast<size_t>(x.b) * c.heads + x.job;
-            const bool last = atomicAdd(d, 1u) == static_cast<uint32_t>(s.n - 1);
+            uint32_t* d = a.done + static_cast<size_t>(cut[i].b) * c.heads + cut[i].job;
+            const bool last = atomicAdd(d, 1u) == static_cast<uint32_t>(share[i].n - 1);
             if (last) *d = 0;
             __threadfence();
-            share[threadIdx.x] = last ? s : Share{0, 0, 0};
+            join[threadIdx.x] = last;
         }
         __syncthreads();
         for (int i = warp; i < cuts * rows; i += W) {
-            const Share s = share[i / rows];
-            if (s.n > 0) join_row<D, NT>(a, s, cut[i / rows].b, cut[i / rows].job, 0, i % rows);
+            const int x = i / rows, e = ends >> x & 1;
+            if (join[x]) join_row<D, NT>(a, share[e], cut[e].b, cut[e].job, 0, i - x * rows);
         }
     }
     if (lane == 0 && n > 0 && st.absent) atomicOr(&g_kv_attend_error, kKvErrPage);
@@ -1001,11 +1040,17 @@ __global__ void __launch_bounds__(32 * kCbWarps) kv_combine_kernel(const KvAtten
 // ---------------------------------------------------------------------------
 // Accumulated weight: mass_j += sum over the rows of exp2(score - lse), a second
 // pass over the keys alone (8 D + 128 of a unit's 16 D + 128 bytes) now that
-// every row's lse is known.  A slot's sum is one lane group's, in row order.
+// every row's lse is known.  Up to 8 rows stay in registers for a whole job;
+// more are taken 32 at a time over up to four steps that wait in the ring, so a
+// tile of queries is arranged once for 128 slots.  A slot's sum is one lane
+// group's, in row order.
 // ---------------------------------------------------------------------------
-template <int D>
-__global__ void __launch_bounds__(32 * at_warps(1), at_ctas(1)) kv_mass_kernel(const KvAttendArgs a) {
-    constexpr int W = at_warps(1);
+__host__ __device__ constexpr int ms_warps(int nt) { return nt == 1 ? 8 : 12; }
+__host__ __device__ constexpr int ms_ctas(int nt) { return nt == 1 ? 2 : 1; }
+
+template <int D, int NT>
+__global__ void __launch_bounds__(32 * ms_warps(NT), ms_ctas(NT)) kv_mass_kernel(const KvAttendArgs a) {
+    constexpr int W = ms_warps(NT), G = NT == 1 ? 1 : 4, U = NT == 1 ? 2 : 1;
     extern __shared__ __align__(128) char smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const KvView& c = a.c;
@@ -1018,85 +1063,99 @@ __global__ void __launch_bounds__(32 * at_warps(1), at_ctas(1)) kv_mass_kernel(c
     const long long u0 = p.runs.start(w);
     const int n = static_cast<int>(p.runs.start(w + 1) - u0);
     if (n == 0) return;
-    st.start(a, p, u0, n);
-    QueryTile<D, 1> q;
-    const int rows = a.tokens * a.group, n_rt = (rows + 7) / 8;
-    int b = 0, h = 0, len = 0, ub = 0, ul = 0;
-    long long left = 0;
+    const int rows = a.tokens * a.group, n_rt = (rows + 8 * NT - 1) / (8 * NT);
+    StepAt at = st.start(a, p, u0, n);
+    st.fill(a, p);
+    QueryTile<D, NT> q;
+    f2 lse[NT];  // minus the rows' lse
     bool fresh = true;
-    f2 lse(0.f);  // minus the rows' lse
-    for (int i = 0; i < n; ++i) {
-        if (left == 0) {
-            const long long u = u0 + i;
-            const StepAt x = step_at(p, c.n_seqs, u);
-            b = x.b;
-            len = x.len;
-            ul = steps_of(len);
-            h = x.job;
-            ub = x.step;
-            left = static_cast<long long>(p.pre[b + 1]) * p.jobs - u;
-            fresh = true;
-        }
-        if (!st.wait()) { st.drain(i); return; }
-        const int unit = st.unit();
-        const uint32_t found = st.found();
-        float add[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+    for (int done = 0; done < n;) {
+        const int ul = steps_of(at.len), take = min(min(G, a.depth), min(ul - at.step, n - done));
+        for (int e = 0; e < take; ++e)
+            if (!st.wait(e)) { st.drain(done); return; }
+        float add[G][2][2];
+#pragma unroll
+        for (int e = 0; e < G; ++e) add[e][0][0] = add[e][0][1] = add[e][1][0] = add[e][1][1] = 0.f;
         for (int rt = 0; rt < n_rt; ++rt) {
             if (n_rt > 1 || fresh) {
-                q.load(a, b, h, rt, len);
-                float v[2];
+                q.load(a, at.b, at.job, rt, at.len);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int row = rt * 8 + 2 * t + e;
-                    v[e] = -INFINITY;  // padding rows and rows without keys weigh nothing
-                    if (row < rows) {
-                        const int tok = row / a.group, head = h * a.group + row % a.group;
-                        const float x = ldcg_f32(a.lse2 + (static_cast<size_t>(b) * a.tokens + tok) * (c.heads * a.group) + head);
-                        if (x != -INFINITY) v[e] = -x;
+                for (int nt = 0; nt < NT; ++nt) {
+                    float v[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int row = (rt * NT + nt) * 8 + 2 * t + e;
+                        v[e] = -INFINITY;  // padding rows and rows without keys weigh nothing
+                        if (row < rows) {
+                            const int tok = row / a.group, head = at.job * a.group + row - tok * a.group;
+                            const float x = ldcg_f32(a.lse2 + (static_cast<size_t>(at.b) * a.tokens + tok) * (c.heads * a.group) + head);
+                            if (x != -INFINITY) v[e] = -x;
+                        }
                     }
+                    lse[nt] = f2(v[0], v[1]);
                 }
-                lse = f2(v[0], v[1]);
                 fresh = false;
             }
-            if (ub * kStep >= q.max_lim) continue;
-            f2 s[2][1][2];
-            score_mma<D, 1, 2>(unit, q, s);
 #pragma unroll
-            for (int y = 0; y < 2; ++y)
+            for (int e = 0; e < G; ++e) {
+                if (e >= take || (at.step + e) * kStep >= q.max_lim) continue;
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const uint2 p = smem_at<uint2>(unit + y * kv_unit_bytes(D) + kv_param_offset(D) + 8 * g + 64 * x);
-                    const int jj = ub * kStep + y * kKvTokens + g + 8 * x;
-                    const f2 d = fma2(f2(h2f_bits(hi16(p.x))), q.sum[0], s[y][0][x]) * f2(h2f_bits(lo16(p.x)) * a.scale2) + lse;
-                    if (jj < q.lim[0][0]) add[y][x] += ex2(d.x());
-                    if (jj < q.lim[0][1]) add[y][x] += ex2(d.y());
+                for (int y0 = 0; y0 < 2; y0 += U) {
+                    const int unit = st.unit(e) + y0 * kv_unit_bytes(D);
+                    f2 s[U][NT][2];
+                    score_mma<D, NT, U>(unit, q, s);
+#pragma unroll
+                    for (int y = 0; y < U; ++y)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const uint2 pr = smem_at<uint2>(unit + y * kv_unit_bytes(D) + kv_param_offset(D) + 8 * g + 64 * x);
+                            const f2 zk(h2f_bits(hi16(pr.x))), sk(h2f_bits(lo16(pr.x)) * a.scale2);
+                            const int j = (at.step + e) * kStep + (y0 + y) * kKvTokens + g + 8 * x;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                const f2 d = fma2(zk, q.sum[nt], s[y][nt][x]) * sk + lse[nt];
+                                if (j < q.lim[nt][0]) add[e][y0 + y][x] += ex2(d.x());
+                                if (j < q.lim[nt][1]) add[e][y0 + y][x] += ex2(d.y());
+                            }
+                        }
                 }
-        }
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-            float add0 = add[y][0], add1 = add[y][1];
-            add0 += __shfl_xor_sync(0xffffffffu, add0, 1);
-            add1 += __shfl_xor_sync(0xffffffffu, add1, 1);
-            add0 += __shfl_xor_sync(0xffffffffu, add0, 2);
-            add1 += __shfl_xor_sync(0xffffffffu, add1, 2);
-            const int s0 = ub * kStep + y * kKvTokens, jj = s0 + g + 8 * t;
-            if ((found >> y & 1u) && t < 2 && jj < len) {
-                const int page = kv_page(c, b, s0);
-                if (page >= 0) c.mass[kv_line(c, page, h) + jj % c.page_size] += t == 0 ? add0 : add1;
             }
         }
-        st.next(a, p);
-        --left;
-        if (++ub == ul) { ub = 0; ++h; fresh = true; }
+#pragma unroll
+        for (int e = 0; e < G; ++e) {
+            if (e >= take) continue;
+            const uint32_t found = st.found();
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                float add0 = add[e][y][0], add1 = add[e][y][1];
+                add0 += __shfl_xor_sync(0xffffffffu, add0, 1);
+                add1 += __shfl_xor_sync(0xffffffffu, add1, 1);
+                add0 += __shfl_xor_sync(0xffffffffu, add0, 2);
+                add1 += __shfl_xor_sync(0xffffffffu, add1, 2);
+                const int s0 = (at.step + e) * kStep + y * kKvTokens, j = s0 + g + 8 * t;
+                if ((found >> y & 1u) && t < 2 && j < at.len) {
+                    const int page = kv_page(c, at.b, s0);
+                    if (page >= 0) c.mass[kv_line(c, page, at.job) + j % c.page_size] += t == 0 ? add0 : add1;
+                }
+            }
+            st.next(a, p);
+        }
+        done += take;
+        at.step += take;
+        if (at.step == ul && done < n) {
+            at = step_at(p, c.n_seqs, u0 + done);
+            fresh = true;
+        }
     }
 }
 
 constexpr int kSmemPerSm = 226 * 1024;
 
-// Ring slots per warp that fit next to the plan when `ctas` CTAs share an SM, and the CTA's shared memory.
+// Ring slots per warp that fit next to the plan and `fixed` bytes when `ctas` CTAs share an SM, and the CTA's
+// shared memory.
 template <class Stream>
-int ring_depth(int n_seqs, int warps, int ctas, int* smem) {
-    const int used = plan_bytes(n_seqs), room = kSmemPerSm / ctas - 2048 - used;
+int ring_depth(int n_seqs, int warps, int ctas, int fixed, int* smem) {
+    const int used = plan_bytes(n_seqs) + fixed, room = kSmemPerSm / ctas - 2048 - used;
     int depth = room / (warps * (Stream::kSlot + 12));
     depth = depth > 8 ? 8 : depth;
     *smem = used + Stream::bytes(warps, depth);
@@ -1110,6 +1169,19 @@ dq_status_t allow_smem(K kernel, int smem) {
     return DQ_OK;
 }
 
+// Pieces of jobs that end inside a run stay in shared memory up to this size: one row of a KV head, where nearly
+// every warp has such a piece, needs 4 KB; eight rows would take a slot of every ring.
+constexpr int kMaxKept = 8192;
+
+template <int D, int NT>
+dq_status_t mass(KvAttendArgs& a, int sm_count, cudaStream_t stream) {
+    int smem = 0;
+    a.depth = ring_depth<StepStream<D, true>>(a.c.n_seqs, ms_warps(NT), ms_ctas(NT), 0, &smem);
+    const dq_status_t st = allow_smem(kv_mass_kernel<D, NT>, smem);
+    if (st != DQ_OK) return st;
+    return launch_pdl(kv_mass_kernel<D, NT>, dim3(sm_count * ms_ctas(NT)), 32 * ms_warps(NT), smem, stream, 1, a);
+}
+
 template <int D, int NT>
 dq_status_t attend(KvAttendArgs& a, cudaStream_t stream) {
     constexpr int W = at_warps(NT);
@@ -1118,21 +1190,21 @@ dq_status_t attend(KvAttendArgs& a, cudaStream_t stream) {
     if (st != DQ_OK) return st;
     int grid = di.sm_count * at_ctas(NT), smem = 0;
     if (grid * W > kAtMaxWarps) grid = kAtMaxWarps / W;
-    a.depth = ring_depth<StepStream<D, false>>(a.c.n_seqs, W, at_ctas(NT), &smem);
+    const int rows = a.tokens * a.group, pieces = (W * (rows < 8 * NT ? rows : 8 * NT) * (D + 2) * 4 + 127) / 128 * 128;
+    const int kept = pieces <= kMaxKept ? pieces : 0;
+    a.depth = ring_depth<StepStream<D, false>>(a.c.n_seqs, W, at_ctas(NT), kept, &smem);
+    a.first_off = kept > 0 ? smem - kept : 0;
     // a piece fits in a ring of two slots
     static_assert(8 * NT * (D + 2) * 4 <= 2 * StepStream<D, false>::kSlot, "ring too small for a piece");
     if (a.depth < 2) return DQ_ERR_UNSUPPORTED;
     if ((st = allow_smem(kv_attend_kernel<D, NT>, smem)) != DQ_OK) return st;
-    if ((st = launch_pdl(kv_attend_kernel<D, NT>, dim3(grid), 32 * W, smem, stream, a)) != DQ_OK) return st;
+    if ((st = launch_pdl(kv_attend_kernel<D, NT>, dim3(grid), 32 * W, smem, stream, 1, a)) != DQ_OK) return st;
     const long long items = static_cast<long long>(a.c.n_seqs) * a.tokens * a.c.heads * a.group;
     if (a.n_rt > 1)
         st = launch_pdl(kv_combine_kernel<D, NT>, dim3(static_cast<unsigned>((items + kCbWarps - 1) / kCbWarps)),
-                    32 * kCbWarps, 0, stream, a, grid);
+                    32 * kCbWarps, 0, stream, 1, a, grid);
     if (st != DQ_OK || !a.lse2) return st;
-    grid = di.sm_count * at_ctas(1);
-    a.depth = ring_depth<StepStream<D, true>>(a.c.n_seqs, at_warps(1), at_ctas(1), &smem);
-    if ((st = allow_smem(kv_mass_kernel<D>, smem)) != DQ_OK) return st;
-    return launch_pdl(kv_mass_kernel<D>, dim3(grid), 32 * at_warps(1), smem, stream, a);
+    return rows <= 8 ? mass<D, 1>(a, di.sm_count, stream) : mass<D, 4>(a, di.sm_count, stream);
 }
 
 // Row tiles of one warp: 8 rows when a KV head has no more, else 16.
