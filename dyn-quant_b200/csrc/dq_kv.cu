@@ -207,24 +207,28 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const KvAppendArgs a, co
 // histograms, summed over the cluster through distributed shared memory; ties
 // stay in slot order (a scan of the threads' counts).  Survivors keep their slot
 // unless it lies at keep or beyond: the k-th of those moves into the k-th hole
-// below keep.  Sources and holes are disjoint, so the moves, dealt to all
-// threads of the cluster, need no order among themselves, and a step that drops
-// one slot moves at most one.  Bound by the chain of passes (short lists) or by
-// the moves' bytes.
+// below keep.  Sources and holes are disjoint, so the moves need no order among
+// themselves, and a step that drops one slot moves at most one.  Few moves (a
+// step at the cache's bound) are made by the cluster itself, many by a second
+// kernel over the whole GPU.  Bound by the chain of passes, then by the moves.
 // ---------------------------------------------------------------------------
-constexpr int kEvThreads = 1024;
-constexpr int kEvRadix = 2048;  // bins of a pass
-constexpr int kEvBatch = 4;     // moves that a group of lanes has in flight
+constexpr int kEvThreads = 256;
+constexpr int kEvRadix = 2048;    // bins of a pass
+constexpr int kEvBatch = 4;       // moves that a group of lanes has in flight
+constexpr int kEvInline = 256;    // moves of one head, at most, that the selecting kernel makes itself
+constexpr int kMvThreads = 256;
 
 struct KvEvictArgs {
     KvView c;
     int keep, recent, sink;
-    int32_t* lists;  // per (sequence, head): list_cap holes, then list_cap sources
-    int list_cap;    // a multiple of kEvBatch
+    int32_t* counts;  // [n_seqs][heads] moves
+    int32_t* lists;   // per (sequence, head): list_cap holes, then list_cap sources
+    int list_cap;
 };
 
 // Exclusive scan of one value per thread over the CTA, and the total.
 __device__ __forceinline__ uint32_t cta_scan(uint32_t v, uint32_t* wsum, uint32_t* total) {
+    constexpr int W = kEvThreads / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t inc = v;
 #pragma unroll
@@ -235,40 +239,106 @@ __device__ __forceinline__ uint32_t cta_scan(uint32_t v, uint32_t* wsum, uint32_
     __syncthreads();  // the last scan's sums have been read
     if (lane == 31) wsum[warp] = inc;
     __syncthreads();
-    const uint32_t w = wsum[lane];
-    uint32_t wi = w;
+    uint32_t before = 0, all = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t t = __shfl_up_sync(0xffffffffu, wi, o);
-        if (lane >= o) wi += t;
+    for (int w = 0; w < W; ++w) {
+        const uint32_t x = wsum[w];
+        if (w < warp) before += x;
+        all += x;
     }
-    *total = __shfl_sync(0xffffffffu, wi, 31);
-    return __shfl_sync(0xffffffffu, wi - w, warp) + inc - v;
+    *total = all;
+    return before + inc - v;
+}
+
+// Moves first, first + step, ... (in batches) of one (sequence, head): L lanes a slot, each 8 bytes of K codes and
+// the 16 bytes of V words that hold its 16 columns.  False where a page was outside the pool.
+template <int D>
+__device__ __forceinline__ bool move_slots(const KvEvictArgs& a, int b, int h, int n_moves, int first, int step) {
+    constexpr int L = D / 16;
+    const KvView& c = a.c;
+    const int32_t* holes = a.lists + (static_cast<size_t>(b) * c.heads + h) * 2 * a.list_cap;
+    const int32_t* from = holes + a.list_cap;
+    const int l = threadIdx.x % L, cap = c.max_pages * c.page_size;
+    bool ok = true;
+    for (int m0 = first; m0 < n_moves; m0 += step) {
+        uint2 kc[kEvBatch], par[kEvBatch];
+        uint4 vc[kEvBatch];
+        uint32_t w[kEvBatch], p[kEvBatch];
+        int to[kEvBatch], pt[kEvBatch], src[kEvBatch];
+        bool on[kEvBatch];
+#pragma unroll
+        for (int j = 0; j < kEvBatch; ++j) {
+            on[j] = m0 + j < n_moves;
+            to[j] = on[j] ? static_cast<int>(ldcg_u32(holes + m0 + j)) : 0;
+            src[j] = on[j] ? static_cast<int>(ldcg_u32(from + m0 + j)) : a.keep;
+        }
+#pragma unroll
+        for (int j = 0; j < kEvBatch; ++j) {
+            on[j] = on[j] && to[j] >= 0 && to[j] < a.keep && src[j] >= a.keep && src[j] < cap;  // (lists of this call: always)
+            const int ps = on[j] ? kv_page(c, b, src[j]) : -1;
+            pt[j] = on[j] ? kv_page(c, b, to[j]) : -1;
+            if (on[j] && (ps < 0 || pt[j] < 0)) { ok = false; on[j] = false; }
+            if (on[j]) {
+                const int os = src[j] % c.page_size, rs = os % kKvTokens;
+                const uint8_t* us = kv_unit<D>(c, ps, h, os);
+                kc[j] = *reinterpret_cast<const uint2*>(us + rs * (D / 2) + 8 * l);
+                vc[j] = *reinterpret_cast<const uint4*>(us + kv_v_offset(D) + (rs / 2) * D + 16 * l);
+                if (rs & 1) vc[j] = make_uint4(vc[j].x >> 16, vc[j].y >> 16, vc[j].z >> 16, vc[j].w >> 16);
+                if (l == 0) {
+                    par[j] = *reinterpret_cast<const uint2*>(us + kv_param_offset(D) + 8 * rs);
+                    const size_t ls = kv_line(c, ps, h) + os;
+                    w[j] = ldcg_u32(c.mass + ls);
+                    p[j] = ldcg_u32(c.pos + ls);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kEvBatch; ++j) {
+            if (!on[j]) continue;
+            const int ot = to[j] % c.page_size, rt = ot % kKvTokens;
+            uint8_t* ut = kv_unit<D>(c, pt[j], h, ot);
+            *reinterpret_cast<uint2*>(ut + rt * (D / 2) + 8 * l) = kc[j];
+            uint16_t* vt = reinterpret_cast<uint16_t*>(ut + kv_v_offset(D) + (rt / 2) * D + 16 * l) + (rt & 1);
+            vt[0] = static_cast<uint16_t>(vc[j].x);
+            vt[2] = static_cast<uint16_t>(vc[j].y);
+            vt[4] = static_cast<uint16_t>(vc[j].z);
+            vt[6] = static_cast<uint16_t>(vc[j].w);
+            if (l == 0) {
+                *reinterpret_cast<uint2*>(ut + kv_param_offset(D) + 8 * rt) = par[j];
+                const size_t lt = kv_line(c, pt[j], h) + ot;
+                c.mass[lt] = __uint_as_float(w[j]);
+                c.pos[lt] = static_cast<int>(p[j]);
+            }
+        }
+    }
+    return ok;
 }
 
 template <int D>
 __global__ void __launch_bounds__(kEvThreads) kv_evict_kernel(const KvEvictArgs a) {
-    __shared__ uint32_t hist[kEvRadix];
+    __shared__ __align__(16) uint32_t hist[kEvRadix];
     __shared__ uint32_t sel[2];   // chosen digit, slots above it
     __shared__ uint32_t sums[3];  // of this CTA: slots equal to the threshold, holes, sources
-    __shared__ uint32_t wsum[32];
-    __shared__ int bad_any;
+    __shared__ uint32_t wsum[kEvThreads / 32];
     const KvView& c = a.c;
     const cg::cluster_group cluster = cg::this_cluster();
     const int cs = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
     const int h = blockIdx.x / cs, b = blockIdx.y, tid = threadIdx.x;
+    auto meet = [&]() {
+        if (cs > 1) cluster.sync();
+        else __syncthreads();
+    };
     pdl_launch_dependents();
     pdl_wait();
-    bool bad = false;
+    bool bad = false, page_ok = true;
     const int len = kv_length(c, b, &bad);
     const int gone = static_cast<int>(ldcg_u32(c.evicted + b));
     if (bad && tid == 0) atomicOr(&g_kv_error, kKvErrLen);
-    if (tid == 0) bad_any = 0;
     const bool work = len > a.keep;
+    int n_moves = 0;
     if (work) {
         const int newest = gone + len;
         const int units = (len + kKvTokens - 1) / kKvTokens, share = (units + cs - 1) / cs, rounds = (share + kEvThreads - 1) / kEvThreads;
-        bool bad_page = false;
         uint32_t k[kKvTokens];
         int n = 0, slot0 = 0;  // this thread's unit of the round: its slots in use, the first of them
         auto fetch = [&](int round) {
@@ -277,33 +347,33 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_kernel(const KvEvictArgs 
             n = i >= share || len - slot0 < 0 ? 0 : (len - slot0 > kKvTokens ? kKvTokens : len - slot0);
             const int page = n > 0 ? kv_page(c, b, slot0) : 0;
             if (n > 0 && page < 0) {
-                bad_page = true;  // the slots of an absent page weigh least
+                page_ok = false;  // the slots of an absent page weigh least
 #pragma unroll
-                for (int i = 0; i < kKvTokens; ++i) k[i] = 0u;
+                for (int j = 0; j < kKvTokens; ++j) k[j] = 0u;
             } else if (n > 0) {
                 const size_t line = kv_line(c, page, h) + slot0 % c.page_size;
                 uint32_t w[kKvTokens], p[kKvTokens];
                 const bool wide = ((reinterpret_cast<uintptr_t>(c.mass) | reinterpret_cast<uintptr_t>(c.pos)) & 15u) == 0;
 #pragma unroll
-                for (int i = 0; i < kKvTokens; i += 4) {
+                for (int j = 0; j < kKvTokens; j += 4) {
                     if (wide) {
-                        const uint4 x = ldcg_v4(c.mass + line + i), y = ldcg_v4(c.pos + line + i);
-                        w[i] = x.x; w[i + 1] = x.y; w[i + 2] = x.z; w[i + 3] = x.w;
-                        p[i] = y.x; p[i + 1] = y.y; p[i + 2] = y.z; p[i + 3] = y.w;
+                        const uint4 x = ldcg_v4(c.mass + line + j), y = ldcg_v4(c.pos + line + j);
+                        w[j] = x.x; w[j + 1] = x.y; w[j + 2] = x.z; w[j + 3] = x.w;
+                        p[j] = y.x; p[j + 1] = y.y; p[j + 2] = y.z; p[j + 3] = y.w;
                     } else {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            w[i + e] = ldcg_u32(c.mass + line + i + e);
-                            p[i + e] = ldcg_u32(c.pos + line + i + e);
+                            w[j + e] = ldcg_u32(c.mass + line + j + e);
+                            p[j + e] = ldcg_u32(c.pos + line + j + e);
                         }
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < kKvTokens; ++i) {
-                    uint32_t u = __float_as_uint(__fadd_rn(__uint_as_float(w[i]), 0.f));  // -0 counts as 0
+                for (int j = 0; j < kKvTokens; ++j) {
+                    uint32_t u = __float_as_uint(__fadd_rn(__uint_as_float(w[j]), 0.f));  // -0 counts as 0
                     u ^= (u >> 31) ? 0xFFFFFFFFu : 0x80000000u;
-                    const int at = static_cast<int>(p[i]);
-                    k[i] = (at >= newest - a.recent || at < a.sink) ? 0xFFFFFFFFu : (u < 0xFFFFFFFEu ? u : 0xFFFFFFFEu);
+                    const int at = static_cast<int>(p[j]);
+                    k[j] = (at >= newest - a.recent || at < a.sink) ? 0xFFFFFFFFu : (u < 0xFFFFFFFEu ? u : 0xFFFFFFFEu);
                 }
             }
         };
@@ -311,11 +381,13 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_kernel(const KvEvictArgs 
         // the keep-th largest key
         uint32_t prefix = 0, mask = 0;
         int need = a.keep;
-#pragma unroll
+        constexpr int B = kEvRadix / kEvThreads;  // bins of a thread
+#pragma unroll 1
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
             const uint32_t bins = pass == 2 ? 1023u : 2047u;
-            hist[tid] = hist[tid + kEvThreads] = 0;
+#pragma unroll
+            for (int i = 0; i < B; i += 4) *reinterpret_cast<uint4*>(hist + B * tid + i) = make_uint4(0, 0, 0, 0);
             __syncthreads();
             for (int r = 0; r < rounds; ++r) {
                 if (rounds > 1) fetch(r);
@@ -323,49 +395,60 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_kernel(const KvEvictArgs 
                 for (int i = 0; i < kKvTokens; ++i)
                     if (i < n && (k[i] & mask) == prefix) atomicAdd(&hist[(k[i] >> shift) & bins], 1u);
             }
-            cluster.sync();
-            // bins top and top + 1 of the whole cluster, threads counted from the largest bin
-            const int top = kEvRadix - 2 - 2 * tid;
-            uint32_t n0 = 0, n1 = 0;
+            meet();
+            // bins top .. top + B - 1 of the whole cluster, threads counted from the largest bin
+            const int top = kEvRadix - B - B * tid;
+            uint32_t cnt[B], sum = 0;
+#pragma unroll
+            for (int i = 0; i < B; ++i) cnt[i] = 0;
             for (int r = 0; r < cs; ++r) {
-                const uint2 v = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(&hist[0], r) + top);
-                n0 += v.x;
-                n1 += v.y;
+                const uint32_t* other = cs > 1 ? cluster.map_shared_rank(&hist[0], r) : hist;
+#pragma unroll
+                for (int i = 0; i < B; i += 4) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(other + top + i);
+                    cnt[i] += v.x; cnt[i + 1] += v.y; cnt[i + 2] += v.z; cnt[i + 3] += v.w;
+                }
             }
+#pragma unroll
+            for (int i = 0; i < B; ++i) sum += cnt[i];
             uint32_t total;
-            const uint32_t before = cta_scan(n0 + n1, wsum, &total), want = static_cast<uint32_t>(need);
-            if (before < want && want <= before + n0 + n1) {
-                const bool high = want <= before + n1;
-                sel[0] = static_cast<uint32_t>(high ? top + 1 : top);
-                sel[1] = high ? before : before + n1;
+            const uint32_t before = cta_scan(sum, wsum, &total), want = static_cast<uint32_t>(need);
+            if (before < want && want <= before + sum) {
+                uint32_t acc = before;
+                bool open = true;
+#pragma unroll
+                for (int i = B - 1; i >= 0; --i) {
+                    if (open && acc + cnt[i] >= want) { sel[0] = top + i; sel[1] = acc; open = false; }
+                    acc += cnt[i];
+                }
             }
-            cluster.sync();
+            meet();
             prefix |= sel[0] << shift;
             mask |= bins << shift;
             need -= static_cast<int>(sel[1]);
         }
-        // slots equal to the threshold before this CTA's
+        // slots equal to the threshold: how many before this thread's (in the round, then before the CTA)
+        uint32_t total, acc = 0, eq_at = 0;
         auto equal = [&]() {
             uint32_t e = 0;
 #pragma unroll
             for (int i = 0; i < kKvTokens; ++i) e += i < n && k[i] == prefix;
             return e;
         };
-        uint32_t total, acc = 0;
         for (int r = 0; r < rounds; ++r) {
             if (rounds > 1) fetch(r);
-            cta_scan(equal(), wsum, &total);
+            eq_at = cta_scan(equal(), wsum, &total);
             acc += total;
         }
-        if (tid == 0) sums[0] = acc;
-        cluster.sync();
         uint32_t eq0 = 0;
-        for (int r = 0; r < rank; ++r) eq0 += *cluster.map_shared_rank(&sums[0], r);
-        // bit i: slot i of the thread's unit stays; its holes | sources << 16
-        uint32_t stay = 0, mine = 0, eq_run = eq0;
-        auto decide = [&]() {
-            uint32_t e = eq_run + cta_scan(equal(), wsum, &total);
-            eq_run += total;
+        if (cs > 1) {
+            if (tid == 0) sums[0] = acc;
+            meet();
+            for (int r = 0; r < rank; ++r) eq0 += *cluster.map_shared_rank(&sums[0], r);
+        }
+        // bit i of stay: slot i of the unit stays; holes | sources << 16 of the unit
+        uint32_t stay = 0;
+        auto decide = [&](uint32_t e) -> uint32_t {
             stay = 0;
 #pragma unroll
             for (int i = 0; i < kKvTokens; ++i) {
@@ -375,105 +458,65 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_kernel(const KvEvictArgs 
             }
             const int low = a.keep - slot0 < 0 ? 0 : (a.keep - slot0 > kKvTokens ? kKvTokens : a.keep - slot0);
             const uint32_t below = (1u << low) - 1u, used = (1u << n) - 1u;
-            mine = __popc(~stay & below & used) | (__popc(stay & ~below) << 16);
+            return __popc(~stay & below & used) | (__popc(stay & ~below) << 16);
         };
-        uint32_t holes_n = 0, from_n = 0;
+        uint32_t holes_n = 0, from_n = 0, at = 0, eq_run = eq0;
         for (int r = 0; r < rounds; ++r) {
-            if (rounds > 1) fetch(r);
-            decide();
-            cta_scan(mine, wsum, &total);  // at most 16 x 1024 of either: no carry between the halves
+            if (rounds > 1) {
+                fetch(r);
+                eq_at = cta_scan(equal(), wsum, &total);
+            }
+            const uint32_t mine = decide(eq_run + eq_at);
+            if (rounds > 1) eq_run += total;
+            at = cta_scan(mine, wsum, &total);  // at most 16 x 256 of either: no carry between the halves
             holes_n += total & 0xFFFFu;
             from_n += total >> 16;
         }
-        if (tid == 0) { sums[1] = holes_n; sums[2] = from_n; }
-        cluster.sync();
         uint32_t holes_at = 0, from_at = 0;
-        int n_moves = 0;
-        for (int r = 0; r < cs; ++r) {
-            const uint32_t* s = cluster.map_shared_rank(&sums[0], r);
-            const uint32_t x = s[1], y = s[2];
-            if (r < rank) { holes_at += x; from_at += y; }
-            n_moves += static_cast<int>(x);
+        n_moves = static_cast<int>(holes_n);
+        if (cs > 1) {
+            if (tid == 0) { sums[1] = holes_n; sums[2] = from_n; }
+            meet();
+            n_moves = 0;
+            for (int r = 0; r < cs; ++r) {
+                const uint32_t* s = cluster.map_shared_rank(&sums[0], r);
+                const uint32_t x = s[1], y = s[2];
+                if (r < rank) { holes_at += x; from_at += y; }
+                n_moves += static_cast<int>(x);
+            }
         }
         int32_t* holes = a.lists + (static_cast<size_t>(b) * c.heads + h) * 2 * a.list_cap;
         int32_t* from = holes + a.list_cap;
         eq_run = eq0;
         for (int r = 0; r < rounds; ++r) {
-            if (rounds > 1) { fetch(r); decide(); }
-            const uint32_t at = cta_scan(mine, wsum, &total);
-            uint32_t x = holes_at + (at & 0xFFFFu), y = from_at + (at >> 16);
-            for (int i = 0; i < n; ++i) {
-                const bool st = stay >> i & 1u;
-                if (slot0 + i < a.keep) {
-                    if (!st && x < static_cast<uint32_t>(a.list_cap)) holes[x++] = slot0 + i;
-                } else if (st && y < static_cast<uint32_t>(a.list_cap)) {
-                    from[y++] = slot0 + i;
-                }
+            if (rounds > 1) {
+                fetch(r);
+                eq_at = cta_scan(equal(), wsum, &total);
+                const uint32_t mine = decide(eq_run + eq_at);
+                eq_run += total;
+                at = cta_scan(mine, wsum, &total);
             }
+            uint32_t x = holes_at + (at & 0xFFFFu), y = from_at + (at >> 16);
+            const int low = a.keep - slot0 < 0 ? 0 : (a.keep - slot0 > kKvTokens ? kKvTokens : a.keep - slot0);
+            const uint32_t below = (1u << low) - 1u, used = (1u << n) - 1u;
+            for (uint32_t m = ~stay & below & used; m; m &= m - 1, ++x)
+                if (x < static_cast<uint32_t>(a.list_cap)) holes[x] = slot0 + __ffs(m) - 1;
+            for (uint32_t m = stay & ~below; m; m &= m - 1, ++y)
+                if (y < static_cast<uint32_t>(a.list_cap)) from[y] = slot0 + __ffs(m) - 1;
             holes_at += total & 0xFFFFu;
             from_at += total >> 16;
         }
-        cluster.sync();
-        // moves: L lanes a slot, each 8 bytes of K codes and the 16 bytes of V words that hold its 16 columns
-        constexpr int L = D / 16;
-        const int l = tid % L, groups = cs * kEvThreads / L;
-        for (int m0 = (rank * kEvThreads + tid) / L * kEvBatch; m0 < n_moves; m0 += groups * kEvBatch) {
-            uint2 kc[kEvBatch], par[kEvBatch];
-            uint4 vc[kEvBatch];
-            uint32_t w[kEvBatch], p[kEvBatch];
-            int to[kEvBatch], pt[kEvBatch];
-            bool on[kEvBatch];
-#pragma unroll
-            for (int j = 0; j < kEvBatch; ++j) {
-                to[j] = 0;
-                int src = a.keep;
-                on[j] = m0 + j < n_moves;
-                if (on[j]) {
-                    to[j] = static_cast<int>(ldcg_u32(holes + m0 + j));
-                    src = static_cast<int>(ldcg_u32(from + m0 + j));
-                    if (to[j] < 0 || to[j] >= a.keep || src < a.keep || src >= len) on[j] = false;  // this call's lists: never
-                }
-                const int ps = on[j] ? kv_page(c, b, src) : -1;
-                pt[j] = on[j] ? kv_page(c, b, to[j]) : -1;
-                if (on[j] && (ps < 0 || pt[j] < 0)) { bad_page = true; on[j] = false; }
-                if (on[j]) {
-                    const int os = src % c.page_size, rs = os % kKvTokens;
-                    const uint8_t* us = kv_unit<D>(c, ps, h, os);
-                    kc[j] = *reinterpret_cast<const uint2*>(us + rs * (D / 2) + 8 * l);
-                    vc[j] = *reinterpret_cast<const uint4*>(us + kv_v_offset(D) + (rs / 2) * D + 16 * l);
-                    if (rs & 1) vc[j] = make_uint4(vc[j].x >> 16, vc[j].y >> 16, vc[j].z >> 16, vc[j].w >> 16);
-                    if (l == 0) {
-                        par[j] = *reinterpret_cast<const uint2*>(us + kv_param_offset(D) + 8 * rs);
-                        const size_t ls = kv_line(c, ps, h) + os;
-                        w[j] = ldcg_u32(c.mass + ls);
-                        p[j] = ldcg_u32(c.pos + ls);
-                    }
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < kEvBatch; ++j) {
-                if (!on[j]) continue;
-                const int ot = to[j] % c.page_size, rt = ot % kKvTokens;
-                uint8_t* ut = kv_unit<D>(c, pt[j], h, ot);
-                *reinterpret_cast<uint2*>(ut + rt * (D / 2) + 8 * l) = kc[j];
-                uint16_t* vt = reinterpret_cast<uint16_t*>(ut + kv_v_offset(D) + (rt / 2) * D + 16 * l) + (rt & 1);
-                vt[0] = static_cast<uint16_t>(vc[j].x);
-                vt[2] = static_cast<uint16_t>(vc[j].y);
-                vt[4] = static_cast<uint16_t>(vc[j].z);
-                vt[6] = static_cast<uint16_t>(vc[j].w);
-                if (l == 0) {
-                    *reinterpret_cast<uint2*>(ut + kv_param_offset(D) + 8 * rt) = par[j];
-                    const size_t lt = kv_line(c, pt[j], h) + ot;
-                    c.mass[lt] = __uint_as_float(w[j]);
-                    c.pos[lt] = static_cast<int>(p[j]);
-                }
-            }
+        meet();
+        if (a.list_cap <= kEvInline) {
+            constexpr int L = D / 16;
+            if (!move_slots<D>(a, b, h, n_moves, (rank * kEvThreads + tid) / L * kEvBatch, cs * kEvThreads / L * kEvBatch))
+                page_ok = false;
         }
-        if (bad_page) bad_any = 1;
     }
+    if (!page_ok) atomicOr(&g_kv_error, kKvErrPage);
     __syncthreads();
     if (tid == 0) {
-        if (bad_any) atomicOr(&g_kv_error, kKvErrPage);
+        if (rank == 0 && a.list_cap > kEvInline) a.counts[b * c.heads + h] = n_moves;
         // every CTA of the sequence has read its length: the last one to arrive writes the new one
         if (atomicAdd(c.arrivals + b, 1u) == gridDim.x - 1) {
             c.arrivals[b] = 0;
@@ -485,13 +528,34 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_kernel(const KvEvictArgs 
     }
 }
 
-// CTAs per (sequence, head): as many as fill the GPU once (two of 1024 threads on an SM), at most 8 and no more
-// than give every CTA 4096 slots of a full sequence.
+template <int D>
+__global__ void __launch_bounds__(kMvThreads) kv_move_kernel(const KvEvictArgs a) {
+    constexpr int L = D / 16;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int h = blockIdx.y, b = blockIdx.z, n = static_cast<int>(ldcg_u32(a.counts + b * a.c.heads + h));
+    const int first = (static_cast<int>(blockIdx.x * kMvThreads + threadIdx.x)) / L * kEvBatch;
+    if (first < n && !move_slots<D>(a, b, h, n, first, static_cast<int>(gridDim.x) * kMvThreads / L * kEvBatch))
+        atomicOr(&g_kv_error, kKvErrPage);
+}
+
+// CTAs per (sequence, head): as many as fill the GPU (four on an SM), at most 8 and no more than give every CTA
+// 2048 slots of a full sequence.
 int evict_cluster(const dq_kv_cache_t& c, int sm_count) {
     const long long pairs = static_cast<long long>(c.n_seqs) * c.kv_heads, cap = static_cast<long long>(c.max_pages) * c.page_size;
     int cs = 1;
-    while (cs < 8 && pairs * cs * 2 <= 2ll * sm_count && cap >= 4096ll * cs * 2) cs *= 2;
+    while (cs < 8 && pairs * cs * 2 <= 4ll * sm_count && cap >= 2048ll * cs * 2) cs *= 2;
     return cs;
+}
+
+template <int D>
+dq_status_t evict(const dq_kv_cache_t& c, const KvEvictArgs& a, int sm_count, cudaStream_t stream) {
+    const int cs = evict_cluster(c, sm_count);
+    const dq_status_t st = launch_pdl(kv_evict_kernel<D>, dim3(c.kv_heads * cs, c.n_seqs), kEvThreads, 0, stream, cs, a);
+    if (st != DQ_OK || a.list_cap <= kEvInline) return st;
+    // a CTA for every 1024 moves: eight batches of a group of lanes
+    constexpr int kPer = kMvThreads / (D / 16) * kEvBatch * 8;
+    return launch_pdl(kv_move_kernel<D>, dim3((a.list_cap + kPer - 1) / kPer, c.kv_heads, c.n_seqs), kMvThreads, 0, stream, 1, a);
 }
 
 }  // namespace
@@ -521,14 +585,19 @@ dq_status_t launch_kv_append(const dq_kv_cache_t& c, const uint16_t* k, const in
                   : launch_pdl(kv_append_kernel<64, false>, grid, threads, 0, stream, 1, a, per);
 }
 
-// Holes and sources of one head, at most, rounded up to a batch.
+// Holes and sources of one head, at most.
 static long long evict_list_cap(const dq_kv_cache_t& c, int keep) {
     const long long cap = static_cast<long long>(c.max_pages) * c.page_size, n = keep < cap - keep ? keep : cap - keep;
-    return n <= 0 ? 0 : (n + kEvBatch - 1) / kEvBatch * kEvBatch;
+    return n < 0 ? 0 : n;
+}
+
+static size_t evict_lists_bytes(const dq_kv_cache_t& c, int keep) {
+    return align256(static_cast<size_t>(c.n_seqs) * c.kv_heads * 2 * static_cast<size_t>(evict_list_cap(c, keep)) * sizeof(int32_t));
 }
 
 size_t kv_evict_workspace(const dq_kv_cache_t& c, int keep) {
-    return align256(static_cast<size_t>(c.n_seqs) * c.kv_heads * 2 * static_cast<size_t>(evict_list_cap(c, keep)) * sizeof(int32_t));
+    const size_t lists = evict_lists_bytes(c, keep);
+    return lists == 0 ? 0 : lists + align256(static_cast<size_t>(c.n_seqs) * c.kv_heads * sizeof(int32_t));
 }
 
 dq_status_t launch_kv_evict(const dq_kv_cache_t& c, int keep, int recent, int sink, void* workspace,
@@ -542,11 +611,9 @@ dq_status_t launch_kv_evict(const dq_kv_cache_t& c, int keep, int recent, int si
     a.recent = recent;
     a.sink = sink;
     a.lists = static_cast<int32_t*>(workspace);
+    a.counts = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + evict_lists_bytes(c, keep));
     a.list_cap = static_cast<int>(evict_list_cap(c, keep));
-    const int cs = evict_cluster(c, di.sm_count);
-    const dim3 grid(c.kv_heads * cs, c.n_seqs);
-    if (c.head_dim == 128) return launch_pdl(kv_evict_kernel<128>, grid, kEvThreads, 0, stream, cs, a);
-    return launch_pdl(kv_evict_kernel<64>, grid, kEvThreads, 0, stream, cs, a);
+    return c.head_dim == 128 ? evict<128>(c, a, di.sm_count, stream) : evict<64>(c, a, di.sm_count, stream);
 }
 
 dq_status_t read_kv_error(uint32_t* word, bool clear) {

@@ -46,8 +46,8 @@ def test_sizes():
     assert L.dq_kv_attend_workspace_bytes(C.byref(c), 1, 7, 0) == 0
     assert L.dq_kv_attend_workspace_bytes(C.byref(cache(head_dim=96)), 1, 8, 0) == 0
     assert L.dq_kv_attend_workspace_bytes(None, 1, 8, 0) == 0
-    # two lists of at most min(keep, capacity - keep) entries per sequence and head
-    assert L.dq_kv_evict_workspace_bytes(C.byref(c), 200) == 2 * 2 * 2 * 56 * 4 + (-2 * 2 * 2 * 56 * 4) % 256
+    # two lists of at most min(keep, capacity - keep) entries per sequence and head, and a count
+    assert L.dq_kv_evict_workspace_bytes(C.byref(c), 200) == 2 * 2 * 2 * 56 * 4 + (-2 * 2 * 2 * 56 * 4) % 256 + 256
     assert L.dq_kv_evict_workspace_bytes(C.byref(c), 256) == 0
     assert L.dq_kv_evict_workspace_bytes(C.byref(c), 0) == 0
 
