@@ -316,9 +316,11 @@ __device__ __forceinline__ bool move_slots(const KvEvictArgs& a, int b, int h, i
 
 template <int D>
 __global__ void __launch_bounds__(kEvThreads) kv_evict_kernel(const KvEvictArgs a) {
-    __shared__ __align__(16) uint32_t hist[kEvRadix];
+    __shared__ __align__(16) uint32_t local[2][kEvRadix];  // this CTA's counts: of the first two passes, of the last
+    __shared__ __align__(16) uint32_t hists[3][kEvRadix];  // the cluster's counts, one a pass
     __shared__ uint32_t sel[2];   // chosen digit, slots above it
-    __shared__ uint32_t sums[3];  // of this CTA: slots equal to the threshold, holes, sources
+    __shared__ __align__(8) uint32_t sums[2];  // of this CTA: holes, sources
+    __shared__ uint32_t got[3];    // what the cluster's other CTAs say
     __shared__ uint32_t wsum[kEvThreads / 32];
     const KvView& c = a.c;
     const cg::cluster_group cluster = cg::this_cluster();
@@ -377,7 +379,10 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_kernel(const KvEvictArgs 
                 }
             }
         };
+        for (int i = 4 * tid; i < 2 * kEvRadix; i += 4 * kEvThreads) *reinterpret_cast<uint4*>(&local[0][0] + i) = make_uint4(0, 0, 0, 0);
+        for (int i = 4 * tid; i < 3 * kEvRadix; i += 4 * kEvThreads) *reinterpret_cast<uint4*>(&hists[0][0] + i) = make_uint4(0, 0, 0, 0);
         if (rounds == 1) fetch(0);
+        meet();
         // the keep-th largest key
         uint32_t prefix = 0, mask = 0;
         int need = a.keep;
@@ -386,27 +391,34 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_kernel(const KvEvictArgs 
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
             const uint32_t bins = pass == 2 ? 1023u : 2047u;
-#pragma unroll
-            for (int i = 0; i < B; i += 4) *reinterpret_cast<uint4*>(hist + B * tid + i) = make_uint4(0, 0, 0, 0);
-            __syncthreads();
+            uint32_t* mine = local[pass == 2 ? 1 : 0];
             for (int r = 0; r < rounds; ++r) {
                 if (rounds > 1) fetch(r);
 #pragma unroll
                 for (int i = 0; i < kKvTokens; ++i)
-                    if (i < n && (k[i] & mask) == prefix) atomicAdd(&hist[(k[i] >> shift) & bins], 1u);
+                    if (i < n && (k[i] & mask) == prefix) atomicAdd(&mine[(k[i] >> shift) & bins], 1u);
             }
-            meet();
-            // bins top .. top + B - 1 of the whole cluster, threads counted from the largest bin
+            __syncthreads();
+            // bins top .. top + B - 1, threads counted from the largest bin; the few that are not empty go to
+            // every CTA of the cluster
             const int top = kEvRadix - B - B * tid;
             uint32_t cnt[B], sum = 0;
 #pragma unroll
-            for (int i = 0; i < B; ++i) cnt[i] = 0;
-            for (int r = 0; r < cs; ++r) {
-                const uint32_t* other = cs > 1 ? cluster.map_shared_rank(&hist[0], r) : hist;
+            for (int i = 0; i < B; i += 4) {
+                const uint4 v = *reinterpret_cast<const uint4*>(mine + top + i);
+                cnt[i] = v.x; cnt[i + 1] = v.y; cnt[i + 2] = v.z; cnt[i + 3] = v.w;
+                if (pass == 0) *reinterpret_cast<uint4*>(mine + top + i) = make_uint4(0, 0, 0, 0);
+            }
+            if (cs > 1) {
+#pragma unroll
+                for (int i = 0; i < B; ++i)
+                    if (cnt[i] != 0)
+                        for (int r = 0; r < cs; ++r) atomicAdd(cluster.map_shared_rank(&hists[pass][top + i], r), cnt[i]);
+                meet();
 #pragma unroll
                 for (int i = 0; i < B; i += 4) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(other + top + i);
-                    cnt[i] += v.x; cnt[i + 1] += v.y; cnt[i + 2] += v.z; cnt[i + 3] += v.w;
+                    const uint4 v = *reinterpret_cast<const uint4*>(&hists[pass][top + i]);
+                    cnt[i] = v.x; cnt[i + 1] = v.y; cnt[i + 2] = v.z; cnt[i + 3] = v.w;
                 }
             }
 #pragma unroll
@@ -422,29 +434,29 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_kernel(const KvEvictArgs 
                     acc += cnt[i];
                 }
             }
-            meet();
+            __syncthreads();
             prefix |= sel[0] << shift;
             mask |= bins << shift;
             need -= static_cast<int>(sel[1]);
         }
         // slots equal to the threshold: how many before this thread's (in the round, then before the CTA)
-        uint32_t total, acc = 0, eq_at = 0;
+        uint32_t total, eq_at = 0;
         auto equal = [&]() {
             uint32_t e = 0;
 #pragma unroll
             for (int i = 0; i < kKvTokens; ++i) e += i < n && k[i] == prefix;
             return e;
         };
-        for (int r = 0; r < rounds; ++r) {
-            if (rounds > 1) fetch(r);
-            eq_at = cta_scan(equal(), wsum, &total);
-            acc += total;
-        }
+        if (rounds == 1) eq_at = cta_scan(equal(), wsum, &total);
         uint32_t eq0 = 0;
-        if (cs > 1) {
-            if (tid == 0) sums[0] = acc;
-            meet();
-            for (int r = 0; r < rank; ++r) eq0 += *cluster.map_shared_rank(&sums[0], r);
+        if (cs > 1) {  // the last pass counted them: the threshold's bin in the CTAs before
+            if (tid < 32) {
+                const uint32_t x = tid < rank ? cluster.map_shared_rank(&local[1][0], tid)[prefix & 1023u] : 0u;
+                const uint32_t all = __reduce_add_sync(0xffffffffu, x);
+                if (tid == 0) got[0] = all;
+            }
+            __syncthreads();
+            eq0 = got[0];
         }
         // bit i of stay: slot i of the unit stays; holes | sources << 16 of the unit
         uint32_t stay = 0;
@@ -475,15 +487,20 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_kernel(const KvEvictArgs 
         uint32_t holes_at = 0, from_at = 0;
         n_moves = static_cast<int>(holes_n);
         if (cs > 1) {
-            if (tid == 0) { sums[1] = holes_n; sums[2] = from_n; }
+            if (tid == 0) { sums[0] = holes_n; sums[1] = from_n; }
             meet();
-            n_moves = 0;
-            for (int r = 0; r < cs; ++r) {
-                const uint32_t* s = cluster.map_shared_rank(&sums[0], r);
-                const uint32_t x = s[1], y = s[2];
-                if (r < rank) { holes_at += x; from_at += y; }
-                n_moves += static_cast<int>(x);
+            if (tid < 32) {
+                uint2 x = make_uint2(0u, 0u);
+                if (tid < cs) x = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(&sums[0], tid));
+                const uint32_t all = __reduce_add_sync(0xffffffffu, x.x);
+                const uint32_t h0 = __reduce_add_sync(0xffffffffu, tid < rank ? x.x : 0u);
+                const uint32_t f0 = __reduce_add_sync(0xffffffffu, tid < rank ? x.y : 0u);
+                if (tid == 0) { got[0] = all; got[1] = h0; got[2] = f0; }
             }
+            __syncthreads();
+            n_moves = static_cast<int>(got[0]);
+            holes_at = got[1];
+            from_at = got[2];
         }
         int32_t* holes = a.lists + (static_cast<size_t>(b) * c.heads + h) * 2 * a.list_cap;
         int32_t* from = holes + a.list_cap;
@@ -529,7 +546,7 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_kernel(const KvEvictArgs 
 }
 
 template <int D>
-__global__ void __launch_bounds__(kMvThreads) kv_move_kernel(const KvEvictArgs a) {
+__global__ void __launch_bounds__(kMvThreads, 4) kv_move_kernel(const KvEvictArgs a) {
     constexpr int L = D / 16;
     pdl_launch_dependents();
     pdl_wait();
@@ -553,8 +570,8 @@ dq_status_t evict(const dq_kv_cache_t& c, const KvEvictArgs& a, int sm_count, cu
     const int cs = evict_cluster(c, sm_count);
     const dq_status_t st = launch_pdl(kv_evict_kernel<D>, dim3(c.kv_heads * cs, c.n_seqs), kEvThreads, 0, stream, cs, a);
     if (st != DQ_OK || a.list_cap <= kEvInline) return st;
-    // a CTA for every 1024 moves: eight batches of a group of lanes
-    constexpr int kPer = kMvThreads / (D / 16) * kEvBatch * 8;
+    // a batch per group of lanes: heads differ in their moves, and most CTAs of the grid find none
+    constexpr int kPer = kMvThreads / (D / 16) * kEvBatch;
     return launch_pdl(kv_move_kernel<D>, dim3((a.list_cap + kPer - 1) / kPer, c.kv_heads, c.n_seqs), kMvThreads, 0, stream, 1, a);
 }
 
