@@ -100,9 +100,9 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const KvAppendArgs a, co
     pdl_launch_dependents();
     pdl_wait();
     const int cap = c.max_pages * c.page_size;
-    const int start = static_cast<int>(ldcg_u32((a.at ? a.at : c.lengths) + b));
-    const int gone = static_cast<int>(ldcg_u32(c.evicted + b));
-    int n = a.counts ? static_cast<int>(ldcg_u32(a.counts + b)) : a.tokens;
+    const int start = ld_l2((a.at ? a.at : c.lengths) + b);
+    const int gone = ld_l2(c.evicted + b);
+    int n = a.counts ? ld_l2(a.counts + b) : a.tokens;
     bool bad_len = start < 0 || start > cap || n < 0 || n > a.tokens;
     const bool skip = start < 0 || start > cap;
     n = n < 0 ? 0 : (n > a.tokens ? a.tokens : n);
@@ -263,32 +263,35 @@ __device__ __forceinline__ bool move_slots(const KvEvictArgs& a, int b, int h, i
     for (int m0 = first; m0 < n_moves; m0 += step) {
         uint2 kc[kEvBatch], par[kEvBatch];
         uint4 vc[kEvBatch];
-        uint32_t w[kEvBatch], p[kEvBatch];
-        int to[kEvBatch], pt[kEvBatch], src[kEvBatch];
+        float w[kEvBatch];
+        int p[kEvBatch], to[kEvBatch], pt[kEvBatch], src[kEvBatch], ps[kEvBatch];
         bool on[kEvBatch];
 #pragma unroll
         for (int j = 0; j < kEvBatch; ++j) {
             on[j] = m0 + j < n_moves;
-            to[j] = on[j] ? static_cast<int>(ldcg_u32(holes + m0 + j)) : 0;
-            src[j] = on[j] ? static_cast<int>(ldcg_u32(from + m0 + j)) : a.keep;
+            to[j] = on[j] ? ld_l2(holes + m0 + j) : 0;
+            src[j] = on[j] ? ld_l2(from + m0 + j) : a.keep;
         }
 #pragma unroll
         for (int j = 0; j < kEvBatch; ++j) {
             on[j] = on[j] && to[j] >= 0 && to[j] < a.keep && src[j] >= a.keep && src[j] < cap;  // (lists of this call: always)
-            const int ps = on[j] ? kv_page(c, b, src[j]) : -1;
-            pt[j] = on[j] ? kv_page(c, b, to[j]) : -1;
-            if (on[j] && (ps < 0 || pt[j] < 0)) { ok = false; on[j] = false; }
+            ps[j] = on[j] ? kv_page(c, b, src[j]) : 0;
+            pt[j] = on[j] ? kv_page(c, b, to[j]) : 0;
+        }
+#pragma unroll
+        for (int j = 0; j < kEvBatch; ++j) {
+            if (ps[j] < 0 || pt[j] < 0) { ok = false; on[j] = false; }
             if (on[j]) {
                 const int os = src[j] % c.page_size, rs = os % kKvTokens;
-                const uint8_t* us = kv_unit<D>(c, ps, h, os);
+                const uint8_t* us = kv_unit<D>(c, ps[j], h, os);
                 kc[j] = *reinterpret_cast<const uint2*>(us + rs * (D / 2) + 8 * l);
                 vc[j] = *reinterpret_cast<const uint4*>(us + kv_v_offset(D) + (rs / 2) * D + 16 * l);
                 if (rs & 1) vc[j] = make_uint4(vc[j].x >> 16, vc[j].y >> 16, vc[j].z >> 16, vc[j].w >> 16);
                 if (l == 0) {
                     par[j] = *reinterpret_cast<const uint2*>(us + kv_param_offset(D) + 8 * rs);
-                    const size_t ls = kv_line(c, ps, h) + os;
-                    w[j] = ldcg_u32(c.mass + ls);
-                    p[j] = ldcg_u32(c.pos + ls);
+                    const size_t ls = kv_line(c, ps[j], h) + os;
+                    w[j] = ld_l2(c.mass + ls);
+                    p[j] = ld_l2(c.pos + ls);
                 }
             }
         }
@@ -306,8 +309,8 @@ __device__ __forceinline__ bool move_slots(const KvEvictArgs& a, int b, int h, i
             if (l == 0) {
                 *reinterpret_cast<uint2*>(ut + kv_param_offset(D) + 8 * rt) = par[j];
                 const size_t lt = kv_line(c, pt[j], h) + ot;
-                c.mass[lt] = __uint_as_float(w[j]);
-                c.pos[lt] = static_cast<int>(p[j]);
+                c.mass[lt] = w[j];
+                c.pos[lt] = p[j];
             }
         }
     }
@@ -334,7 +337,7 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_kernel(const KvEvictArgs 
     pdl_wait();
     bool bad = false, page_ok = true;
     const int len = kv_length(c, b, &bad);
-    const int gone = static_cast<int>(ldcg_u32(c.evicted + b));
+    const int gone = ld_l2(c.evicted + b);
     if (bad && tid == 0) atomicOr(&g_kv_error, kKvErrLen);
     const bool work = len > a.keep;
     int n_moves = 0;
@@ -359,14 +362,14 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_kernel(const KvEvictArgs 
 #pragma unroll
                 for (int j = 0; j < kKvTokens; j += 4) {
                     if (wide) {
-                        const uint4 x = ldcg_v4(c.mass + line + j), y = ldcg_v4(c.pos + line + j);
+                        const uint4 x = ld_l2_v4(c.mass + line + j), y = ld_l2_v4(c.pos + line + j);
                         w[j] = x.x; w[j + 1] = x.y; w[j + 2] = x.z; w[j + 3] = x.w;
                         p[j] = y.x; p[j + 1] = y.y; p[j + 2] = y.z; p[j + 3] = y.w;
                     } else {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            w[j + e] = ldcg_u32(c.mass + line + j + e);
-                            p[j + e] = ldcg_u32(c.pos + line + j + e);
+                            w[j + e] = __float_as_uint(ld_l2(c.mass + line + j + e));
+                            p[j + e] = static_cast<uint32_t>(ld_l2(c.pos + line + j + e));
                         }
                     }
                 }
@@ -550,7 +553,7 @@ __global__ void __launch_bounds__(kMvThreads, 4) kv_move_kernel(const KvEvictArg
     constexpr int L = D / 16;
     pdl_launch_dependents();
     pdl_wait();
-    const int h = blockIdx.y, b = blockIdx.z, n = static_cast<int>(ldcg_u32(a.counts + b * a.c.heads + h));
+    const int h = blockIdx.y, b = blockIdx.z, n = ld_l2(a.counts + b * a.c.heads + h);
     const int first = (static_cast<int>(blockIdx.x * kMvThreads + threadIdx.x)) / L * kEvBatch;
     if (first < n && !move_slots<D>(a, b, h, n, first, static_cast<int>(gridDim.x) * kMvThreads / L * kEvBatch))
         atomicOr(&g_kv_error, kKvErrPage);

@@ -43,9 +43,16 @@ inline KvView kv_view(const dq_kv_cache_t& c) {
                   c.n_seqs, c.n_pages, c.max_pages, c.page_size, c.kv_heads};
 }
 
+// Loads from L2 of what earlier kernels or other CTAs wrote.  Unlike the volatile forms of dq_common.cuh the
+// compiler may move them past one another, so a run of them is in flight at once.
+__device__ __forceinline__ int ld_l2(const int* p) { return __ldcg(p); }
+__device__ __forceinline__ uint32_t ld_l2(const uint32_t* p) { return __ldcg(p); }
+__device__ __forceinline__ float ld_l2(const float* p) { return __ldcg(p); }
+__device__ __forceinline__ uint4 ld_l2_v4(const void* p) { return __ldcg(static_cast<const uint4*>(p)); }
+
 // The page of a slot, or -1 where the table has none inside the pool.
 __device__ __forceinline__ int kv_page(const KvView& c, int b, int slot) {
-    const int p = static_cast<int>(ldcg_u32(c.table + static_cast<size_t>(b) * c.max_pages + slot / c.page_size));
+    const int p = ld_l2(c.table + static_cast<size_t>(b) * c.max_pages + slot / c.page_size);
     return (p >= 0 && p < c.n_pages) ? p : -1;
 }
 
@@ -61,7 +68,7 @@ __device__ __forceinline__ uint8_t* kv_unit(const KvView& c, int page, int h, in
 
 // Tokens of sequence b, kept inside its pages.
 __device__ __forceinline__ int kv_length(const KvView& c, int b, bool* bad) {
-    const int n = static_cast<int>(ldcg_u32(c.lengths + b)), cap = c.max_pages * c.page_size;
+    const int n = ld_l2(c.lengths + b), cap = c.max_pages * c.page_size;
     if (n < 0 || n > cap) *bad = true;
     return n < 0 ? 0 : (n > cap ? cap : n);
 }

@@ -64,6 +64,8 @@ struct KvAttendArgs {
     long long qs[3], os[3];  // strides in values: sequence, token, head
     float* lse;              // [n_seqs][tokens][q_heads] natural log, or null
     float* lse2;             // workspace: the same in log2 (mass pass), or null
+    float* scores;           // workspace: [units of the pool][16][pitch] scores in log2 for the mass pass, or null
+    int pitch;               // rows of a KV head, rounded up to 1, 2, 4 or 8
     const int32_t* counts;
     float* part;             // [CTAs][2][rows][D]
     float* part_ml;          // [CTAs][2][rows][2]
@@ -312,7 +314,7 @@ struct QueryTile {
     __device__ __forceinline__ void request(const KvAttendArgs& a, int b, int h, int rt, uint4 (&raw)[NT][D / 32]) {
         const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
         const int rows = a.tokens * a.group;
-        cnt = a.counts ? min(max(static_cast<int>(ldcg_u32(a.counts + b)), 0), a.tokens) : a.tokens;
+        cnt = a.counts ? min(max(ld_l2(a.counts + b), 0), a.tokens) : a.tokens;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int r = (rt * NT + nt) * 8 + g, tok = r / a.group;
@@ -320,7 +322,7 @@ struct QueryTile {
             for (int i = 0; i < D / 32; ++i) {
                 raw[nt][i] = make_uint4(0, 0, 0, 0);
                 if (r < rows && tok < cnt)
-                    raw[nt][i] = ldcg_v4(a.q + b * a.qs[0] + tok * a.qs[1] + (h * a.group + r - tok * a.group) * a.qs[2] + (D / 4) * t + 8 * i);
+                    raw[nt][i] = ld_l2_v4(a.q + b * a.qs[0] + tok * a.qs[1] + (h * a.group + r - tok * a.group) * a.qs[2] + (D / 4) * t + 8 * i);
             }
         }
     }
@@ -412,14 +414,14 @@ template <int D, bool kKeysOnly>
 struct StepStream {
     static constexpr int kUnit = kv_unit_bytes(D);
     static constexpr int kSlot = 2 * kUnit;
-    int ring, bars, flags;       // offsets in shared memory of this warp's slots, barriers, units-found words
+    int ring, bars, units;       // offsets in shared memory of this warp's slots, barriers, the slots' unit indices
     int depth, n, issued, parity, slot;
     bool absent;                 // some unit of the run lies in no page of the pool
     long long u0;
     int src[2];                  // this lane's step: the units' indices in the pool, -1: none
 
     // Bytes of `warps` rings behind `smem`.
-    static __host__ __device__ int bytes(int warps, int depth) { return (warps * depth * (kSlot + 12) + 127) / 128 * 128; }
+    static __host__ __device__ int bytes(int warps, int depth) { return (warps * depth * (kSlot + 16) + 127) / 128 * 128; }
 
     static __device__ __forceinline__ uint32_t base() {
         extern __shared__ __align__(128) char smem[];
@@ -429,7 +431,7 @@ struct StepStream {
         depth = depth_;
         ring = off + warp * depth * kSlot;
         bars = off + warps * depth * kSlot + warp * depth * 8;
-        flags = off + warps * depth * (kSlot + 8) + warp * depth * 4;
+        units = off + warps * depth * (kSlot + 8) + warp * depth * 8;
         if ((threadIdx.x & 31) == 0)
             for (int i = 0; i < depth; ++i) mbar_init(base() + bars + 8 * i, 1);
         fence_mbar_init();
@@ -461,23 +463,19 @@ struct StepStream {
         const int i0 = __shfl_sync(0xffffffffu, src[0], issued), i1 = __shfl_sync(0xffffffffu, src[1], issued);
         if ((threadIdx.x & 31) == 0) {
             const uint32_t bar = base() + bars + 8 * s, dst = base() + ring + s * kSlot;
+            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(base() + units + 8 * s), "r"(i0), "r"(i1) : "memory");
             if (!kKeysOnly && i0 >= 0 && i1 == i0 + 1) {
-                set_found(s, 3u);
                 mbar_arrive_expect_tx(bar, kSlot);
                 bulk_g2s(dst, a.c.units + static_cast<size_t>(i0) * kUnit, kSlot, bar);
             } else {
-                issue_units(a, s, bar, dst, i0, i1);
+                issue_units(a, bar, dst, i0, i1);
             }
         }
         ++issued;
     }
-    __device__ __forceinline__ void set_found(int s, uint32_t v) {
-        asm volatile("st.shared.u32 [%0], %1;" ::"r"(base() + flags + 4 * s), "r"(v) : "memory");
-    }
     // A step's units one by one: from different pages, one of them missing, or their keys alone.
-    __device__ __forceinline__ void issue_units(const KvAttendArgs& a, int s, uint32_t bar, uint32_t dst, int i0, int i1) {
+    __device__ __forceinline__ void issue_units(const KvAttendArgs& a, uint32_t bar, uint32_t dst, int i0, int i1) {
         constexpr uint32_t kBytes = kKeysOnly ? 8 * D + kKvTokens * 8 : kUnit;
-        set_found(s, (i0 >= 0 ? 1u : 0u) | (i1 >= 0 ? 2u : 0u));
         if (i0 < 0 && i1 < 0) {
             mbar_arrive(bar);
             return;
@@ -523,8 +521,13 @@ struct StepStream {
     __device__ __forceinline__ int unit(int ahead) const {
         return ring + (slot + ahead - (slot + ahead >= depth ? depth : 0)) * kSlot;
     }
+    // The step's units in the pool, -1: not copied.
+    __device__ __forceinline__ int2 unit_index() const { return smem_at<int2>(units + 8 * slot); }
     // Bit e: unit e of the step was copied (only asked for when some unit of the run is absent).
-    __device__ __forceinline__ uint32_t found() const { return smem_at<uint32_t>(flags + 4 * slot); }
+    __device__ __forceinline__ uint32_t found() const {
+        const int2 i = unit_index();
+        return (i.x >= 0 ? 1u : 0u) | (i.y >= 0 ? 2u : 0u);
+    }
     // The current slot is read: refill it, go to the next.
     __device__ __forceinline__ void next(const KvAttendArgs& a, const Plan& p) {
         __syncwarp();
@@ -564,9 +567,10 @@ struct RowState {
 
     // Scores and weights of U units from slot j of the sequence on, the weights as the B operands of their
     // output product, and the units' V codes.  found: bit u set where unit u is there.
-    template <int U>
+    template <int U, bool kScores>
     __device__ __forceinline__ void weigh(const QueryTile<D, NT>& q, int unit, int j, int len, uint32_t found, float scale2,
-                                          uint32_t (&pf)[U][NT][2], uint32_t (&v)[U][2][D / 32]) {
+                                          uint32_t (&pf)[U][NT][2], uint32_t (&v)[U][2][D / 32], float* scores, int pitch,
+                                          int2 index) {
         const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
         f2 s[U][NT][2];
         float sv[U][2], zv[U][2];
@@ -599,6 +603,20 @@ struct RowState {
                         s[u][nt][x] = f2(there && jj < q.lim[nt][0] ? s[u][nt][x].x() : -INFINITY,
                                          there && jj < q.lim[nt][1] ? s[u][nt][x].y() : -INFINITY);
                 }
+        }
+        if (kScores) {
+            // kept for the mass pass: [unit][slot][pitch], the lane's rows 2t, 2t + 1
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = u ? index.y : index.x;
+                if (i < 0 || 2 * t >= pitch) continue;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    float* dst = scores + (static_cast<size_t>(i) * kKvTokens + g + 8 * x) * pitch + 2 * t;
+                    if (pitch == 1) *dst = s[u][0][x].x();
+                    else *reinterpret_cast<float2*>(dst) = make_float2(s[u][0][x].x(), s[u][0][x].y());
+                }
+            }
         }
         // a new maximum or a larger V scale: rare after the first steps
         float big = fmaxf(sv[0][0], sv[0][1]), top[NT][2];
@@ -762,32 +780,50 @@ __device__ __forceinline__ Share share_of(const int* pre, int n_seqs, int jobs, 
     return s;
 }
 
-// One warp joins row r's partial sums: the maxima first, a lane each, then the outputs with independent loads.
+// One warp joins row r's partial sums: maxima and weights a lane each, then the outputs eight partials at a time.
 template <int D, int NT>
 __device__ __forceinline__ void join_row(const KvAttendArgs& a, const Share& s, int b, int h, int rt, int r) {
-    constexpr int R = 8 * NT, V = D / 32;  // V columns of a lane
+    constexpr int R = 8 * NT, V = D / 32;  // V columns of a lane, side by side
     const int lane = threadIdx.x & 31, rl = r - rt * R;
     auto at = [&](int i) { return (static_cast<size_t>(s.c0 + i) * 2 + (i == 0 ? s.slot0 : 0)) * R + rl; };
-    float m = kNone;
-    for (int i = lane; i < s.n; i += 32) m = fmaxf(m, ldcg_f32(a.part_ml + 2 * at(i)));
+    float m = kNone, sum = 0.f, v[V];
+    for (int i = lane; i < s.n; i += 32) m = fmaxf(m, ld_l2(a.part_ml + 2 * at(i)));
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float sum = 0.f, v[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) v[k] = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < s.n; ++i) {
-        const size_t pi = at(i);
-        const float f = ex2(ldcg_f32(a.part_ml + 2 * pi) - m);
-        sum += ldcg_f32(a.part_ml + 2 * pi + 1) * f;
+    for (int i0 = 0; i0 < s.n; i0 += 32) {
+        const bool on = i0 + lane < s.n;
+        const float2 ml = on ? __ldcg(reinterpret_cast<const float2*>(a.part_ml) + at(i0 + lane)) : make_float2(kNone, 0.f);
+        const float f = on ? ex2(ml.x - m) : 0.f;
+        sum += ml.y * f;
+        for (int j0 = 0; j0 < min(32, s.n - i0); j0 += 8) {
+            float x[8][V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[k] += ldcg_f32(a.part + pi * D + lane + 32 * k) * f;
+            for (int j = 0; j < 8; ++j) {
+                const float* src = a.part + at(min(i0 + j0 + j, s.n - 1)) * D + V * lane;  // past the end: weight 0
+                if constexpr (V == 4) {
+                    const float4 y = __ldcg(reinterpret_cast<const float4*>(src));
+                    x[j][0] = y.x; x[j][1] = y.y; x[j][2] = y.z; x[j][3] = y.w;
+                } else {
+                    const float2 y = __ldcg(reinterpret_cast<const float2*>(src));
+                    x[j][0] = y.x; x[j][1] = y.y;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float fj = __shfl_sync(0xffffffffu, f, j0 + j);
+#pragma unroll
+                for (int k = 0; k < V; ++k) v[k] = fmaf(x[j][k], fj, v[k]);
+            }
+        }
     }
+    sum = warp_sum(sum);
     const int tok = r / a.group, head = h * a.group + r - tok * a.group;
     const float f = row_norm(sum);
-    uint16_t* dst = a.out + b * a.os[0] + tok * a.os[1] + head * a.os[2];
+    uint16_t* dst = a.out + b * a.os[0] + tok * a.os[1] + head * a.os[2] + V * lane;
 #pragma unroll
-    for (int k = 0; k < V; ++k) dst[lane + 32 * k] = __half_as_ushort(__float2half_rn(v[k] * f));
+    for (int k = 0; k < V; k += 2) *reinterpret_cast<uint32_t*>(dst + k) = pack_f32(v[k] * f, v[k + 1] * f);
     if (lane == 0) store_lse(a, b, tok, head, m, sum);
 }
 
@@ -799,7 +835,7 @@ struct Piece {
 // ---------------------------------------------------------------------------
 // The pass over the cache
 // ---------------------------------------------------------------------------
-template <int D, int NT>
+template <int D, int NT, bool kScores>
 __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kernel(const KvAttendArgs a) {
     constexpr int W = at_warps(NT), R = 8 * NT;
     static_assert(2 * W <= 32, "a lane per piece");
@@ -886,15 +922,19 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
                     // the slot is refilled as soon as its V codes are in registers
                     if constexpr (NT == 1) {
                         uint32_t pf[2][NT][2], v[2][2][D / 32];
-                        rs.template weigh<2>(q, st.unit(), j, len, found, a.scale2, pf, v);
+                        int2 index = make_int2(-1, -1);
+                        if (kScores) index = st.unit_index();
+                        rs.template weigh<2, kScores>(q, st.unit(), j, len, found, a.scale2, pf, v, a.scores, a.pitch, index);
                         st.next(a, p);
                         rs.template output<2>(pf, v);
                     } else {
                         uint32_t pf[1][NT][2], v[1][2][D / 32];
-                        rs.template weigh<1>(q, st.unit(), j, len, found & 1u, a.scale2, pf, v);
+                        rs.template weigh<1, false>(q, st.unit(), j, len, found & 1u, a.scale2, pf, v, nullptr, 0, make_int2(-1, -1));
                         rs.template output<1>(pf, v);
                         const bool second = j + kKvTokens < q.max_lim;
-                        if (second) rs.template weigh<1>(q, st.unit() + kv_unit_bytes(D), j + kKvTokens, len, found >> 1, a.scale2, pf, v);
+                        if (second)
+                            rs.template weigh<1, false>(q, st.unit() + kv_unit_bytes(D), j + kKvTokens, len, found >> 1, a.scale2, pf, v,
+                                                 nullptr, 0, make_int2(-1, -1));
                         st.next(a, p);
                         if (second) rs.template output<1>(pf, v);
                     }
@@ -948,6 +988,7 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
     const uint32_t valid = __ballot_sync(0xffffffffu, mine.job >= 0);
     const uint32_t lower = valid & ((1u << lane) - 1u);
     const int prev = lower ? 31 - __clz(lower) : 0;
+    const int my_h = a.n_rt == 1 ? mine.job : mine.job / a.n_rt, my_steps = mine.job >= 0 ? steps_of(p.len[mine.b]) : 0;
     const int pb = __shfl_sync(0xffffffffu, mine.b, prev), pj = __shfl_sync(0xffffffffu, mine.job, prev);
     uint32_t heads = __ballot_sync(0xffffffffu, mine.job >= 0 && (!lower || pb != mine.b || pj != mine.job));
     int turn = 0, cuts = 0, ends = 0;  // bit i of ends: cut job i is the CTA's last and not its first
@@ -957,26 +998,47 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
         const uint32_t members = valid & ~((1u << k) - 1u) & (heads ? (heads & (0u - heads)) - 1u : 0xffffffffu);
         const int jb = __shfl_sync(0xffffffffu, mine.b, k), jj = __shfl_sync(0xffffffffu, mine.job, k);
         const bool whole = __shfl_sync(0xffffffffu, mine.first, k) == 0 &&
-                           __shfl_sync(0xffffffffu, mine.end, 31 - __clz(members)) == steps_of(p.len[jb]);
-        const int h = jj / a.n_rt, rt = jj - h * a.n_rt, n_rows = min(R, rows - rt * R);
+                           __shfl_sync(0xffffffffu, mine.end, 31 - __clz(members)) == __shfl_sync(0xffffffffu, my_steps, k);
+        const int h = __shfl_sync(0xffffffffu, my_h, k), rt = jj - h * a.n_rt, n_rows = min(R, rows - rt * R);
         constexpr int C = 8, L = D / C, P = 32 / L;  // columns of a lane, lanes of a row, rows of a turn
         for (int r0 = 0; r0 < n_rows; r0 += P, ++turn) {
             const int rl = r0 + lane / L, col = C * (lane % L);
             if (turn % W != warp || rl >= n_rows) continue;
-            float m = kNone, sum = 0.f, v[C];
-            for (uint32_t x = members; x; x &= x - 1) m = fmaxf(m, piece_at(__ffs(x) - 1)[rl * (D + 2) + D]);
+            // the warps' last pieces with loads that do not wait for one another; first pieces are few
+            float m = kNone, sum = 0.f, v[C], pm[W];
+            const int ring0 = plan_bytes(c.n_seqs) + rl * (D + 2) * 4, ring_step = a.depth * StepStream<D, false>::kSlot;
+            constexpr uint32_t kFirst = 0x55555555u;
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                pm[i] = (members >> (2 * i + 1) & 1u) ? smem_at<float>(ring0 + i * ring_step + 4 * D) : kNone;
+                m = fmaxf(m, pm[i]);
+            }
+            for (uint32_t x = members & kFirst; x; x &= x - 1) m = fmaxf(m, piece_at(__ffs(x) - 1)[rl * (D + 2) + D]);
 #pragma unroll
             for (int y = 0; y < C; ++y) v[y] = 0.f;
-            for (uint32_t x = members; x; x &= x - 1) {
-                const float* src = piece_at(__ffs(x) - 1) + rl * (D + 2);
-                const float f = ex2(src[D] - m);
-                sum += src[D + 1] * f;
+            auto take = [&](float f, const float2 (&z)[C / 2], float l) {
+                sum += l * f;
 #pragma unroll
                 for (int y = 0; y < C; y += 2) {
-                    const float2 z = *reinterpret_cast<const float2*>(src + col + y);
-                    v[y] += z.x * f;
-                    v[y + 1] += z.y * f;
+                    v[y] += z[y / 2].x * f;
+                    v[y + 1] += z[y / 2].y * f;
                 }
+            };
+            for (uint32_t x = members & kFirst; x; x &= x - 1) {
+                const float* src = piece_at(__ffs(x) - 1) + rl * (D + 2);
+                float2 z[C / 2];
+#pragma unroll
+                for (int y = 0; y < C / 2; ++y) z[y] = *reinterpret_cast<const float2*>(src + col + 2 * y);
+                take(ex2(src[D] - m), z, src[D + 1]);
+            }
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const bool on = members >> (2 * i + 1) & 1u;
+                float2 z[C / 2];
+#pragma unroll
+                for (int y = 0; y < C / 2; ++y)
+                    z[y] = on ? smem_at<float2>(ring0 + i * ring_step + 4 * (col + 2 * y)) : make_float2(0.f, 0.f);
+                take(ex2(pm[i] - m), z, on ? smem_at<float>(ring0 + i * ring_step + 4 * D + 4) : 0.f);
             }
             if (whole) {
                 store_row(a, jb, h, rt * R + rl, col, v, m, sum);
@@ -1088,7 +1150,7 @@ __global__ void __launch_bounds__(32 * ms_warps(NT), ms_ctas(NT)) kv_mass_kernel
                         v[e] = -INFINITY;  // padding rows and rows without keys weigh nothing
                         if (row < rows) {
                             const int tok = row / a.group, head = at.job * a.group + row - tok * a.group;
-                            const float x = ldcg_f32(a.lse2 + (static_cast<size_t>(at.b) * a.tokens + tok) * (c.heads * a.group) + head);
+                            const float x = ld_l2(a.lse2 + (static_cast<size_t>(at.b) * a.tokens + tok) * (c.heads * a.group) + head);
                             if (x != -INFINITY) v[e] = -x;
                         }
                     }
@@ -1149,6 +1211,65 @@ __global__ void __launch_bounds__(32 * ms_warps(NT), ms_ctas(NT)) kv_mass_kernel
     }
 }
 
+// The same from the scores that the pass over the cache has kept: a lane a slot, 32 slots a step.
+constexpr int kSmWarps = 8;
+
+template <int P>
+__global__ void __launch_bounds__(32 * kSmWarps) kv_score_mass_kernel(const KvAttendArgs a) {
+    extern __shared__ __align__(128) char smem[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const KvView& c = a.c;
+    pdl_launch_dependents();
+    pdl_wait();
+    const Plan p = make_plan<32 * kSmWarps>(c, c.heads, gridDim.x * kSmWarps, smem, nullptr);
+    const long long w = static_cast<long long>(blockIdx.x) * kSmWarps + warp, u0 = p.runs.start(w);
+    const int n = static_cast<int>(p.runs.start(w + 1) - u0);
+    if (n == 0) return;
+    const int rows = a.tokens * a.group;
+    StepAt at = step_at(p, c.n_seqs, u0);
+    float lse[P];
+    for (int done = 0; done < n;) {
+        const int ul = steps_of(at.len), take = min(ul - at.step, n - done);
+        const bool none = a.counts && ld_l2(a.counts + at.b) <= 0;  // no query: no scores
+#pragma unroll
+        for (int r = 0; r < P; ++r) {
+            lse[r] = INFINITY;  // padding rows and rows without keys weigh nothing
+            if (r < rows) {
+                const int tok = r / a.group, head = at.job * a.group + r - tok * a.group;
+                const float x = ld_l2(a.lse2 + (static_cast<size_t>(at.b) * a.tokens + tok) * (c.heads * a.group) + head);
+                if (x != -INFINITY) lse[r] = x;
+            }
+        }
+#pragma unroll 2
+        for (int i = 0; i < take; ++i) {
+            const int slot = (at.step + i) * kStep + lane;
+            if (slot >= at.len || none) continue;
+            const int page = kv_page(c, at.b, slot);
+            if (page < 0) continue;
+            const size_t line = kv_line(c, page, at.job) + slot % c.page_size;
+            float s[P];
+            if constexpr (P >= 4) {
+#pragma unroll
+                for (int r = 0; r < P; r += 4) {
+                    const uint4 x = ld_l2_v4(a.scores + line * P + r);
+                    s[r] = __uint_as_float(x.x); s[r + 1] = __uint_as_float(x.y);
+                    s[r + 2] = __uint_as_float(x.z); s[r + 3] = __uint_as_float(x.w);
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < P; ++r) s[r] = ld_l2(a.scores + line * P + r);
+            }
+            float add = 0.f;
+#pragma unroll
+            for (int r = 0; r < P; ++r)
+                if (r < rows) add += ex2(s[r] - lse[r]);
+            c.mass[line] = ld_l2(c.mass + line) + add;
+        }
+        done += take;
+        if (done < n) at = step_at(p, c.n_seqs, u0 + done);
+    }
+}
+
 constexpr int kSmemPerSm = 226 * 1024;
 
 // Ring slots per warp that fit next to the plan and `fixed` bytes when `ctas` CTAs share an SM, and the CTA's
@@ -1156,7 +1277,7 @@ constexpr int kSmemPerSm = 226 * 1024;
 template <class Stream>
 int ring_depth(int n_seqs, int warps, int ctas, int fixed, int* smem) {
     const int used = plan_bytes(n_seqs) + fixed, room = kSmemPerSm / ctas - 2048 - used;
-    int depth = room / (warps * (Stream::kSlot + 12));
+    int depth = room / (warps * (Stream::kSlot + 16));
     depth = depth > 8 ? 8 : depth;
     *smem = used + Stream::bytes(warps, depth);
     return depth;
@@ -1197,21 +1318,37 @@ dq_status_t attend(KvAttendArgs& a, cudaStream_t stream) {
     // a piece fits in a ring of two slots
     static_assert(8 * NT * (D + 2) * 4 <= 2 * StepStream<D, false>::kSlot, "ring too small for a piece");
     if (a.depth < 2) return DQ_ERR_UNSUPPORTED;
-    if ((st = allow_smem(kv_attend_kernel<D, NT>, smem)) != DQ_OK) return st;
-    if ((st = launch_pdl(kv_attend_kernel<D, NT>, dim3(grid), 32 * W, smem, stream, 1, a)) != DQ_OK) return st;
+    const auto kernel = NT == 1 && a.scores ? kv_attend_kernel<D, NT, NT == 1> : kv_attend_kernel<D, NT, false>;
+    if ((st = allow_smem(kernel, smem)) != DQ_OK) return st;
+    if ((st = launch_pdl(kernel, dim3(grid), 32 * W, smem, stream, 1, a)) != DQ_OK) return st;
     const long long items = static_cast<long long>(a.c.n_seqs) * a.tokens * a.c.heads * a.group;
     if (a.n_rt > 1)
         st = launch_pdl(kv_combine_kernel<D, NT>, dim3(static_cast<unsigned>((items + kCbWarps - 1) / kCbWarps)),
                     32 * kCbWarps, 0, stream, 1, a, grid);
     if (st != DQ_OK || !a.lse2) return st;
+    if (a.scores) {
+        const dim3 g(di.sm_count * 4);
+        const int threads = 32 * kSmWarps, bytes = plan_bytes(a.c.n_seqs);
+        switch (a.pitch) {
+            case 1: return launch_pdl(kv_score_mass_kernel<1>, g, threads, bytes, stream, 1, a);
+            case 2: return launch_pdl(kv_score_mass_kernel<2>, g, threads, bytes, stream, 1, a);
+            case 4: return launch_pdl(kv_score_mass_kernel<4>, g, threads, bytes, stream, 1, a);
+            default: return launch_pdl(kv_score_mass_kernel<8>, g, threads, bytes, stream, 1, a);
+        }
+    }
     return rows <= 8 ? mass<D, 1>(a, di.sm_count, stream) : mass<D, 4>(a, di.sm_count, stream);
 }
 
 // Row tiles of one warp: 8 rows when a KV head has no more, else 16.
 int row_tiles(int rows) { return rows <= 8 ? 1 : 2; }
 
+// Scores that the mass pass may keep in the workspace; a larger cache's keys are read a second time.
+constexpr size_t kMaxScores = size_t{1} << 30;
+
+int score_pitch(int rows) { return rows <= 2 ? rows : (rows <= 4 ? 4 : 8); }
+
 struct AttendWs {
-    size_t part, ml, first, pre, lse2, total;
+    size_t part, ml, first, pre, lse2, scores, total;
 };
 AttendWs attend_ws(const dq_kv_cache_t& c, int tokens, int q_heads, bool mass) {
     const int nt = row_tiles(tokens * (q_heads / c.kv_heads));
@@ -1222,7 +1359,10 @@ AttendWs attend_ws(const dq_kv_cache_t& c, int tokens, int q_heads, bool mass) {
     w.first = w.ml + align256(rows * 8);
     w.pre = w.first + align256(static_cast<size_t>(kAtMaxWarps) * 8 * nt * (c.head_dim + 2) * 4);
     w.lse2 = w.pre + align256((static_cast<size_t>(c.n_seqs) + 1) * 4);
-    w.total = w.lse2 + (mass ? align256(static_cast<size_t>(c.n_seqs) * tokens * q_heads * 4) : 0);
+    w.scores = w.lse2 + (mass ? align256(static_cast<size_t>(c.n_seqs) * tokens * q_heads * 4) : 0);
+    const int group_rows = tokens * (q_heads / c.kv_heads);
+    const size_t kept = static_cast<size_t>(c.n_pages) * c.kv_heads * c.page_size * score_pitch(group_rows) * sizeof(float);
+    w.total = w.scores + (mass && nt == 1 && group_rows > 0 && kept <= kMaxScores ? align256(kept) : 0);
     return w;
 }
 
@@ -1251,7 +1391,9 @@ dq_status_t launch_kv_attend(const dq_kv_cache_t& c, const dq_kv_attend_t& r, vo
     a.first = reinterpret_cast<float*>(base + w.first);
     a.pre = reinterpret_cast<int*>(base + w.pre);
     a.lse2 = r.accumulate ? reinterpret_cast<float*>(base + w.lse2) : nullptr;
+    a.scores = w.total > w.scores ? reinterpret_cast<float*>(base + w.scores) : nullptr;
     const int rows = r.tokens * a.group, nt = row_tiles(rows);
+    a.pitch = score_pitch(rows);
     a.n_rt = (rows + 8 * nt - 1) / (8 * nt);
     if (c.head_dim == 128) return nt == 1 ? attend<128, 1>(a, stream) : attend<128, 2>(a, stream);
     return nt == 1 ? attend<64, 1>(a, stream) : attend<64, 2>(a, stream);

@@ -41,7 +41,7 @@ def test_sizes():
     c = cache()
     base = L.dq_kv_attend_workspace_bytes(C.byref(c), 1, 8, 0)
     assert base > 0 and base % 256 == 0
-    assert L.dq_kv_attend_workspace_bytes(C.byref(c), 1, 8, 1) == base + 256  # 2 x 8 log-sums
+    assert L.dq_kv_attend_workspace_bytes(C.byref(c), 1, 8, 1) == base + 256 + 8 * 2 * 64 * 4 * 4  # 2 x 8 log-sums, 4 scores a slot
     assert L.dq_kv_attend_workspace_bytes(C.byref(c), 4, 8, 0) > base        # 16 rows per KV head
     assert L.dq_kv_attend_workspace_bytes(C.byref(c), 1, 7, 0) == 0
     assert L.dq_kv_attend_workspace_bytes(C.byref(cache(head_dim=96)), 1, 8, 0) == 0
