@@ -26,6 +26,24 @@ __host__ __device__ constexpr int kv_unit_bytes(int d) { return kKvTokens * d + 
 __host__ __device__ constexpr int kv_v_offset(int d) { return kKvTokens * d / 2; }
 __host__ __device__ constexpr int kv_param_offset(int d) { return kKvTokens * d; }
 
+// Division of 0 <= n < 2^31 by a launch constant: n / d = (umulhi(n, mul) + n) >> shift with
+// mul = floor(2^32 (2^shift - d) / d) + 1 and shift = ceil(log2 d).  A handful of cycles where the division by a
+// variable is dozens of dependent instructions, in code that a single warp waits for.
+struct Div {
+    int d = 1;
+    uint32_t mul = 1, shift = 0;
+    Div() = default;
+    explicit Div(int v) : d(v) {
+        while ((1u << shift) < static_cast<uint32_t>(v)) ++shift;
+        mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - static_cast<uint64_t>(v))) / static_cast<uint64_t>(v) + 1);
+    }
+    __host__ __device__ operator int() const { return d; }
+};
+__device__ __forceinline__ int operator/(int n, const Div& d) {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), d.mul) + static_cast<uint32_t>(n)) >> d.shift);
+}
+__device__ __forceinline__ int operator%(int n, const Div& d) { return n - (n / d) * d.d; }
+
 // dq_kv_cache_t as the kernels take it (validated).
 struct KvView {
     uint8_t* units;
@@ -35,12 +53,13 @@ struct KvView {
     int32_t* evicted;
     const int32_t* table;
     uint32_t* arrivals;
-    int n_seqs, n_pages, max_pages, page_size, heads;
+    int n_seqs, n_pages, max_pages, heads;
+    Div page_size;
 };
 
 inline KvView kv_view(const dq_kv_cache_t& c) {
     return KvView{c.units, c.mass, c.pos, c.lengths, c.evicted, c.page_table, c.arrivals,
-                  c.n_seqs, c.n_pages, c.max_pages, c.page_size, c.kv_heads};
+                  c.n_seqs, c.n_pages, c.max_pages, c.kv_heads, Div(c.page_size)};
 }
 
 // Loads from L2 of what earlier kernels or other CTAs wrote.  Unlike the volatile forms of dq_common.cuh the

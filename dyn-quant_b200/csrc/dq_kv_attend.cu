@@ -72,10 +72,11 @@ struct KvAttendArgs {
     float* first;            // [warps][rows][D + 2] pieces of jobs that end inside a run
     int* pre;                // [n_seqs + 1] the plan's prefix sums, for the combining kernel
     uint32_t* done;          // [n_seqs][heads] CTAs of a cut job that have arrived (one row tile)
-    int tokens, group, n_rt; // query tokens, query heads per KV head, row tiles
+    int tokens;              // query tokens
+    Div group, n_rt, jobs;   // query heads per KV head, row tiles, jobs of a sequence
     float scale2;            // scale * log2(e) * kCode
     int depth;               // ring slots per warp
-    int first_off;           // offset in shared memory of those pieces, 0: they are in the workspace
+    int first_off, places;   // shared memory for some of those pieces: its offset, how many
 };
 
 // The list of steps: a job is steps_of(len[b]) steps of one (sequence, KV head,
@@ -83,6 +84,14 @@ struct KvAttendArgs {
 // steps of one job of every sequence before b.  Warp w takes base steps, one
 // more if w < rem.  Short lists are cut into runs of up to 4 steps rather than
 // one: a job then needs fewer warps, and its pieces meet in one CTA.
+// a / b for 0 <= a, 0 < b, with the short division where it does.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    return ((a | b) >> 31) == 0 ? static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
+__device__ __forceinline__ int quotient(long long a, const Div& b) {
+    return (a >> 31) == 0 ? static_cast<int>(a) / b : static_cast<int>(a / b.d);
+}
+
 struct Runs {
     long long base, total;
     int rem;
@@ -92,7 +101,7 @@ struct Runs {
         total = static_cast<long long>(job_steps) * jobs;
         const int least = min(4, (job_steps + n_seqs - 1) / n_seqs);
         if (total < static_cast<long long>(warps) * least) warps = max(1, static_cast<int>(total) / max(least, 1));
-        base = total / warps;
+        base = quotient(total, warps);
         rem = static_cast<int>(total - base * warps);
     }
     __device__ __forceinline__ long long start(long long w) const {
@@ -101,14 +110,14 @@ struct Runs {
     // the warp whose run has step u
     __device__ __forceinline__ long long warp_of(long long u) const {
         const long long cut = rem * (base + 1);
-        return u < cut ? u / (base + 1) : rem + (u - cut) / base;
+        return u < cut ? quotient(u, base + 1) : rem + quotient(u - cut, base);
     }
 };
 
 struct Plan {
     const int* pre;
     const int* len;
-    int jobs;
+    Div jobs;
     Runs runs;
 };
 
@@ -119,7 +128,7 @@ __host__ __device__ inline int plan_bytes(int n_seqs) { return ((2 * n_seqs + 1)
 
 // Built by every CTA from the lengths (a few KB from L2); all threads call it.
 template <int NT>
-__device__ Plan make_plan(const KvView& c, int jobs, int warps, char* smem, unsigned int* err) {
+__device__ Plan make_plan(const KvView& c, const Div& jobs, int warps, char* smem, unsigned int* err) {
     int* pre = reinterpret_cast<int*>(smem);
     int* lens = pre + c.n_seqs + 1;
     __shared__ int wtot[NT / 32];
@@ -166,11 +175,6 @@ struct StepAt {
     int b, len, job, step;
 };
 
-// a / b for a >= 0, with the short division where it does.
-__device__ __forceinline__ int quotient(long long a, int b) {
-    return (a >> 32) == 0 ? static_cast<int>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : static_cast<int>(a / b);
-}
-
 __device__ __forceinline__ StepAt step_at(const Plan& p, int n_seqs, long long u) {
     const int v = quotient(u, p.jobs);  // pre[b] <= v < pre[b + 1]: the last b with pre[b] <= v
     int lo = 0, hi = n_seqs;
@@ -184,7 +188,7 @@ __device__ __forceinline__ StepAt step_at(const Plan& p, int n_seqs, long long u
     StepAt a;
     a.b = lo;
     a.len = p.len[lo];
-    a.job = quotient(r, st);
+    a.job = static_cast<int>(quotient(r, static_cast<long long>(st)));
     a.step = static_cast<int>(r - static_cast<long long>(a.job) * st);
     return a;
 }
@@ -290,13 +294,13 @@ __device__ __forceinline__ float lane_sum_g(float v) {
 
 // 1 / sum of a row's weights; 0 where it has seen no key, not a number where the sum is not.
 __device__ __forceinline__ float row_norm(float sum) {
-    return sum > 0.f ? __fdiv_rn(1.f, sum) : (sum == 0.f ? 0.f : sum);
+    return sum > 0.f ? __fdividef(1.f, sum) : (sum == 0.f ? 0.f : sum);  // sum < 2^31
 }
 
 // lse of a row, in log2 and natural.
 __device__ __forceinline__ void store_lse(const KvAttendArgs& a, int b, int tok, int head, float m, float sum) {
     const size_t i = (static_cast<size_t>(b) * a.tokens + tok) * (a.c.heads * a.group) + head;
-    const float l2 = sum == 0.f ? -INFINITY : m + log2f(sum);
+    const float l2 = sum == 0.f ? -INFINITY : m + __log2f(sum);  // absolute error 2^-21
     if (a.lse) a.lse[i] = l2 * 0.693147180559945309f;
     if (a.lse2) a.lse2[i] = l2;
 }
@@ -758,7 +762,7 @@ struct Share {
 };
 
 template <int W>
-__device__ __forceinline__ Share share_of(const int* pre, int n_seqs, int jobs, const Runs& runs, int b, int job) {
+__device__ __forceinline__ Share share_of(const int* pre, int n_seqs, const Div& jobs, const Runs& runs, int b, int job) {
     Share s{0, 0, 0};
     const int p0 = pre[b], ul = pre[b + 1] - p0;
     if (ul == 0) return s;
@@ -775,48 +779,56 @@ __device__ __forceinline__ Share share_of(const int* pre, int n_seqs, int jobs, 
             if (pre[mid] <= v) lo = mid;
             else hi = mid;
         }
-        s.slot0 = (start - static_cast<long long>(pre[lo]) * jobs) % (pre[lo + 1] - pre[lo]) != 0 ? 1 : 0;
+        const long long in = start - static_cast<long long>(pre[lo]) * jobs, st = pre[lo + 1] - pre[lo];
+        s.slot0 = in != quotient(in, st) * st ? 1 : 0;
     }
     return s;
 }
 
-// One warp joins row r's partial sums: maxima and weights a lane each, then the outputs eight partials at a time.
+// One warp joins row r's partial sums: maxima and sums a lane each, then the outputs eight partials at a time.
 template <int D, int NT>
 __device__ __forceinline__ void join_row(const KvAttendArgs& a, const Share& s, int b, int h, int rt, int r) {
-    constexpr int R = 8 * NT, V = D / 32;  // V columns of a lane, side by side
-    const int lane = threadIdx.x & 31, rl = r - rt * R;
-    auto at = [&](int i) { return (static_cast<size_t>(s.c0 + i) * 2 + (i == 0 ? s.slot0 : 0)) * R + rl; };
-    float m = kNone, sum = 0.f, v[V];
-    for (int i = lane; i < s.n; i += 32) m = fmaxf(m, ld_l2(a.part_ml + 2 * at(i)));
+    constexpr int R = 8 * NT, V = D / 32, N = 8;  // V columns of a lane, side by side; partials at a time
+    const int lane = threadIdx.x & 31, rl = r - rt * R, first = s.slot0 * R;  // only the first CTA's may be its slot 1
+    const size_t row0 = static_cast<size_t>(s.c0) * 2 * R + rl;
+    const float2* ml0 = reinterpret_cast<const float2*>(a.part_ml) + row0;
+    const float* o0 = a.part + row0 * D + V * lane;
+    auto ml_at = [&](int i) { return i < s.n ? __ldcg(ml0 + (i == 0 ? first : i * 2 * R)) : make_float2(kNone, 0.f); };
+    float x[N][V];
+    auto fetch = [&](int i0) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float* src = o0 + static_cast<size_t>(i0) * 2 * R * D + j * 2 * R * D + (i0 + j == 0 ? first * D : 0);
+            const bool on = i0 + j < s.n;
+            if constexpr (V == 4) {
+                const float4 y = on ? __ldcg(reinterpret_cast<const float4*>(src)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                x[j][0] = y.x; x[j][1] = y.y; x[j][2] = y.z; x[j][3] = y.w;
+            } else {
+                const float2 y = on ? __ldcg(reinterpret_cast<const float2*>(src)) : make_float2(0.f, 0.f);
+                x[j][0] = y.x; x[j][1] = y.y;
+            }
+        }
+    };
+    float2 ml = ml_at(lane);
+    fetch(0);
+    float m = ml.x, sum = 0.f, v[V];
+    for (int i = lane + 32; i < s.n; i += 32) m = fmaxf(m, ml_at(i).x);
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
 #pragma unroll
     for (int k = 0; k < V; ++k) v[k] = 0.f;
-    for (int i0 = 0; i0 < s.n; i0 += 32) {
-        const bool on = i0 + lane < s.n;
-        const float2 ml = on ? __ldcg(reinterpret_cast<const float2*>(a.part_ml) + at(i0 + lane)) : make_float2(kNone, 0.f);
-        const float f = on ? ex2(ml.x - m) : 0.f;
-        sum += ml.y * f;
-        for (int j0 = 0; j0 < min(32, s.n - i0); j0 += 8) {
-            float x[8][V];
+#pragma unroll 1
+    for (int i0 = 0; i0 < s.n; i0 += N) {
+        if (i0 > 0 && i0 % 32 == 0) ml = ml_at(i0 + lane);
+        const float f = ml.x > kNone ? ex2(ml.x - m) : (ml.x == kNone ? 0.f : ml.x);
+        if (i0 % 32 == 0) sum += ml.y * f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float* src = a.part + at(min(i0 + j0 + j, s.n - 1)) * D + V * lane;  // past the end: weight 0
-                if constexpr (V == 4) {
-                    const float4 y = __ldcg(reinterpret_cast<const float4*>(src));
-                    x[j][0] = y.x; x[j][1] = y.y; x[j][2] = y.z; x[j][3] = y.w;
-                } else {
-                    const float2 y = __ldcg(reinterpret_cast<const float2*>(src));
-                    x[j][0] = y.x; x[j][1] = y.y;
-                }
-            }
+        for (int j = 0; j < N; ++j) {
+            const float fj = __shfl_sync(0xffffffffu, f, i0 % 32 + j);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float fj = __shfl_sync(0xffffffffu, f, j0 + j);
-#pragma unroll
-                for (int k = 0; k < V; ++k) v[k] = fmaf(x[j][k], fj, v[k]);
-            }
+            for (int k = 0; k < V; ++k) v[k] = fmaf(x[j][k], fj, v[k]);
         }
+        if (i0 + N < s.n) fetch(i0 + N);
     }
     sum = warp_sum(sum);
     const int tok = r / a.group, head = h * a.group + r - tok * a.group;
@@ -846,21 +858,23 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
     __shared__ Piece cut[2];
     __shared__ Share share[2];
     __shared__ bool join[2];
+    __shared__ int kept, place[W];
     StepStream<D, false> st;
     st.init(plan_bytes(c.n_seqs), W, warp, a.depth);
     // A piece is a row of D + 2 floats for each row of the job: output, maximum, sum.  A warp's last piece
-    // takes its ring, which has run dry by then; one of a job that ends inside the run goes behind the rings
-    // if it is small, else to the workspace, so that the rings have the shared memory.
+    // takes its ring, which has run dry by then; one of a job that ends inside the run takes one of the
+    // CTA's few places behind the rings, or the workspace when they are gone.
     const int piece = min(a.tokens * a.group, R) * (D + 2);
+    if (threadIdx.x == 0) kept = 0;
     auto piece_at = [&](int k) {
         const int i = k >> 1;
         if (k & 1) return reinterpret_cast<float*>(smem + plan_bytes(c.n_seqs) + i * a.depth * StepStream<D, false>::kSlot);
-        if (a.first_off > 0) return reinterpret_cast<float*>(smem + a.first_off) + i * piece;
+        if (place[i] < a.places) return reinterpret_cast<float*>(smem + a.first_off) + place[i] * piece;
         return a.first + (static_cast<size_t>(blockIdx.x) * W + i) * piece;
     };
     pdl_launch_dependents();
     pdl_wait();
-    const Plan p = make_plan<32 * W>(c, c.heads * a.n_rt, gridDim.x * W, smem, blockIdx.x == 0 ? &g_kv_attend_error : nullptr);
+    const Plan p = make_plan<32 * W>(c, a.jobs, gridDim.x * W, smem, blockIdx.x == 0 ? &g_kv_attend_error : nullptr);
     if (a.n_rt > 1 && blockIdx.x == 0)
         for (int b = threadIdx.x; b <= c.n_seqs; b += 32 * W) a.pre[b] = p.pre[b];
     const long long w = static_cast<long long>(blockIdx.x) * W + warp;
@@ -946,6 +960,10 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
             rs.settle();
             const bool whole = first == 0 && ub == ul;
             const int k = 2 * warp + (done + take == n ? 1 : 0);
+            if (!whole && (k & 1) == 0) {
+                if (lane == 0) place[warp] = atomicAdd(&kept, 1);
+                __syncwarp();
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -990,20 +1008,38 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
     const int prev = lower ? 31 - __clz(lower) : 0;
     const int my_h = a.n_rt == 1 ? mine.job : mine.job / a.n_rt, my_steps = mine.job >= 0 ? steps_of(p.len[mine.b]) : 0;
     const int pb = __shfl_sync(0xffffffffu, mine.b, prev), pj = __shfl_sync(0xffffffffu, mine.job, prev);
-    uint32_t heads = __ballot_sync(0xffffffffu, mine.job >= 0 && (!lower || pb != mine.b || pj != mine.job));
-    int turn = 0, cuts = 0, ends = 0;  // bit i of ends: cut job i is the CTA's last and not its first
-    while (heads) {
-        const int k = __ffs(heads) - 1;
-        heads &= heads - 1;
-        const uint32_t members = valid & ~((1u << k) - 1u) & (heads ? (heads & (0u - heads)) - 1u : 0xffffffffu);
-        const int jb = __shfl_sync(0xffffffffu, mine.b, k), jj = __shfl_sync(0xffffffffu, mine.job, k);
-        const bool whole = __shfl_sync(0xffffffffu, mine.first, k) == 0 &&
-                           __shfl_sync(0xffffffffu, mine.end, 31 - __clz(members)) == __shfl_sync(0xffffffffu, my_steps, k);
-        const int h = __shfl_sync(0xffffffffu, my_h, k), rt = jj - h * a.n_rt, n_rows = min(R, rows - rt * R);
+    const uint32_t heads = __ballot_sync(0xffffffffu, mine.job >= 0 && (!lower || pb != mine.b || pj != mine.job));
+    // the groups of pieces of one job each: only the first and the last can be cut by the CTA's borders
+    const int groups = __popc(heads), k_last = groups > 0 ? 31 - __clz(heads) : 0, k_first = groups > 0 ? __ffs(heads) - 1 : 0;
+    auto members_of = [&](int k) {
+        const uint32_t above = heads & ~((2u << k) - 1u);
+        return valid & ~((1u << k) - 1u) & (above ? (above & (0u - above)) - 1u : 0xffffffffu);
+    };
+    auto is_cut = [&](int k) {
+        return __shfl_sync(0xffffffffu, mine.first, k) != 0 ||
+               __shfl_sync(0xffffffffu, mine.end, 31 - __clz(members_of(k))) != __shfl_sync(0xffffffffu, my_steps, k);
+    };
+    const bool cut_first = groups > 0 && is_cut(k_first), cut_last = groups > 1 && is_cut(k_last);
+    const int cuts = cut_first + cut_last;
+    // which of the CTA's two end jobs a cut group is: bit i of ends for cut i
+    auto end_of = [&](int k) {
+        return __shfl_sync(0xffffffffu, mine.b, k) != cut[0].b || __shfl_sync(0xffffffffu, mine.job, k) != cut[0].job;
+    };
+    const int ends = (cut_first && end_of(k_first) ? 1 : 0) | (cut_last && end_of(k_last) ? 1 << (cuts - 1) : 0);
+    {
         constexpr int C = 8, L = D / C, P = 32 / L;  // columns of a lane, lanes of a row, rows of a turn
-        for (int r0 = 0; r0 < n_rows; r0 += P, ++turn) {
+        const int turns = (min(rows, R) + P - 1) / P;
+        for (int item = warp; item < groups * turns; item += W) {
+            const int gi = item / turns, r0 = (item - gi * turns) * P;
+            uint32_t hs = heads;
+            for (int i = 0; i < gi; ++i) hs &= hs - 1;
+            const int k = __ffs(hs) - 1;
+            const uint32_t members = members_of(k);
+            const int jb = __shfl_sync(0xffffffffu, mine.b, k), jj = __shfl_sync(0xffffffffu, mine.job, k);
+            const int h = __shfl_sync(0xffffffffu, my_h, k), rt = jj - h * a.n_rt;
+            const bool whole = !(gi == 0 ? cut_first : (gi == groups - 1 && cut_last));
             const int rl = r0 + lane / L, col = C * (lane % L);
-            if (turn % W != warp || rl >= n_rows) continue;
+            if (rl >= min(R, rows - rt * R)) continue;
             // the warps' last pieces with loads that do not wait for one another; first pieces are few
             float m = kNone, sum = 0.f, v[C], pm[W];
             const int ring0 = plan_bytes(c.n_seqs) + rl * (D + 2) * 4, ring_step = a.depth * StepStream<D, false>::kSlot;
@@ -1043,16 +1079,12 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
             if (whole) {
                 store_row(a, jb, h, rt * R + rl, col, v, m, sum);
             } else {
-                const size_t pi = (static_cast<size_t>(blockIdx.x) * 2 + cuts) * R + rl;
+                const size_t pi = (static_cast<size_t>(blockIdx.x) * 2 + (gi > 0 && cut_first ? 1 : 0)) * R + rl;
                 float4* dst = reinterpret_cast<float4*>(a.part + pi * D + col);
                 dst[0] = make_float4(v[0], v[1], v[2], v[3]);
                 dst[1] = make_float4(v[4], v[5], v[6], v[7]);
                 if (col == 0) *reinterpret_cast<float2*>(a.part_ml + pi * 2) = make_float2(m, sum);
             }
-        }
-        if (!whole) {
-            if (a.n_rt == 1 && (cut[0].b != jb || cut[0].job != jj)) ends |= 1 << cuts;
-            ++cuts;
         }
     }
     if (cuts > 0 && a.n_rt == 1) {
@@ -1085,7 +1117,7 @@ constexpr int kCbWarps = 4;
 template <int D, int NT>
 __global__ void __launch_bounds__(32 * kCbWarps) kv_combine_kernel(const KvAttendArgs a, const int ctas) {
     const KvView& c = a.c;
-    const int hq = c.heads * a.group, jobs = c.heads * a.n_rt;
+    const int hq = c.heads * a.group;
     pdl_launch_dependents();
     pdl_wait();
     const long long item = static_cast<long long>(blockIdx.x) * kCbWarps + (threadIdx.x >> 5);
@@ -1094,8 +1126,8 @@ __global__ void __launch_bounds__(32 * kCbWarps) kv_combine_kernel(const KvAtten
     const int head = static_cast<int>(item - bt * hq), b = static_cast<int>(bt / a.tokens);
     const int tok = static_cast<int>(bt - static_cast<long long>(b) * a.tokens);
     const int h = head / a.group, r = tok * a.group + head - h * a.group, rt = r / (8 * NT);
-    const Runs runs(a.pre[c.n_seqs], c.n_seqs, jobs, ctas * at_warps(NT));
-    const Share s = share_of<at_warps(NT)>(a.pre, c.n_seqs, jobs, runs, b, h * a.n_rt + rt);
+    const Runs runs(a.pre[c.n_seqs], c.n_seqs, a.jobs, ctas * at_warps(NT));
+    const Share s = share_of<at_warps(NT)>(a.pre, c.n_seqs, a.jobs, runs, b, h * a.n_rt + rt);
     if (s.n > 1) join_row<D, NT>(a, s, b, h, rt, r);  // else finished by its CTA, or empty
 }
 
@@ -1120,7 +1152,7 @@ __global__ void __launch_bounds__(32 * ms_warps(NT), ms_ctas(NT)) kv_mass_kernel
     st.init(plan_bytes(c.n_seqs), W, warp, a.depth);
     pdl_launch_dependents();
     pdl_wait();
-    const Plan p = make_plan<32 * W>(c, c.heads, gridDim.x * W, smem, nullptr);
+    const Plan p = make_plan<32 * W>(c, a.jobs, gridDim.x * W, smem, nullptr);
     const long long w = static_cast<long long>(blockIdx.x) * W + warp;
     const long long u0 = p.runs.start(w);
     const int n = static_cast<int>(p.runs.start(w + 1) - u0);
@@ -1221,7 +1253,7 @@ __global__ void __launch_bounds__(32 * kSmWarps) kv_score_mass_kernel(const KvAt
     const KvView& c = a.c;
     pdl_launch_dependents();
     pdl_wait();
-    const Plan p = make_plan<32 * kSmWarps>(c, c.heads, gridDim.x * kSmWarps, smem, nullptr);
+    const Plan p = make_plan<32 * kSmWarps>(c, a.jobs, gridDim.x * kSmWarps, smem, nullptr);
     const long long w = static_cast<long long>(blockIdx.x) * kSmWarps + warp, u0 = p.runs.start(w);
     const int n = static_cast<int>(p.runs.start(w + 1) - u0);
     if (n == 0) return;
@@ -1290,9 +1322,9 @@ dq_status_t allow_smem(K kernel, int smem) {
     return DQ_OK;
 }
 
-// Pieces of jobs that end inside a run stay in shared memory up to this size: one row of a KV head, where nearly
-// every warp has such a piece, needs 4 KB; eight rows would take a slot of every ring.
-constexpr int kMaxKept = 8192;
+// Shared memory for pieces of jobs that end inside a run: two of eight rows, all of a CTA's with one row (where
+// nearly every warp has one).  Room for eight of eight rows would take a slot of every ring.
+constexpr int kKeptBytes = 8448;
 
 template <int D, int NT>
 dq_status_t mass(KvAttendArgs& a, int sm_count, cudaStream_t stream) {
@@ -1311,10 +1343,10 @@ dq_status_t attend(KvAttendArgs& a, cudaStream_t stream) {
     if (st != DQ_OK) return st;
     int grid = di.sm_count * at_ctas(NT), smem = 0;
     if (grid * W > kAtMaxWarps) grid = kAtMaxWarps / W;
-    const int rows = a.tokens * a.group, pieces = (W * (rows < 8 * NT ? rows : 8 * NT) * (D + 2) * 4 + 127) / 128 * 128;
-    const int kept = pieces <= kMaxKept ? pieces : 0;
-    a.depth = ring_depth<StepStream<D, false>>(a.c.n_seqs, W, at_ctas(NT), kept, &smem);
-    a.first_off = kept > 0 ? smem - kept : 0;
+    const int rows = a.tokens * a.group, piece = (rows < 8 * NT ? rows : 8 * NT) * (D + 2) * 4;
+    a.places = kKeptBytes / piece < W ? kKeptBytes / piece : W;
+    a.depth = ring_depth<StepStream<D, false>>(a.c.n_seqs, W, at_ctas(NT), (a.places * piece + 127) / 128 * 128, &smem);
+    a.first_off = smem - (a.places * piece + 127) / 128 * 128;
     // a piece fits in a ring of two slots
     static_assert(8 * NT * (D + 2) * 4 <= 2 * StepStream<D, false>::kSlot, "ring too small for a piece");
     if (a.depth < 2) return DQ_ERR_UNSUPPORTED;
@@ -1326,6 +1358,7 @@ dq_status_t attend(KvAttendArgs& a, cudaStream_t stream) {
         st = launch_pdl(kv_combine_kernel<D, NT>, dim3(static_cast<unsigned>((items + kCbWarps - 1) / kCbWarps)),
                     32 * kCbWarps, 0, stream, 1, a, grid);
     if (st != DQ_OK || !a.lse2) return st;
+    a.jobs = Div(a.c.heads);
     if (a.scores) {
         const dim3 g(di.sm_count * 4);
         const int threads = 32 * kSmWarps, bytes = plan_bytes(a.c.n_seqs);
@@ -1381,7 +1414,7 @@ dq_status_t launch_kv_attend(const dq_kv_cache_t& c, const dq_kv_attend_t& r, vo
     a.lse = r.lse;
     a.counts = r.counts;
     a.tokens = r.tokens;
-    a.group = r.q_heads / c.kv_heads;
+    a.group = Div(r.q_heads / c.kv_heads);
     a.scale2 = r.scale * (1.44269504088896341f * kCode);
     a.done = c.arrivals + c.n_seqs;
     const AttendWs w = attend_ws(c, r.tokens, r.q_heads, r.accumulate != 0);
@@ -1394,7 +1427,8 @@ dq_status_t launch_kv_attend(const dq_kv_cache_t& c, const dq_kv_attend_t& r, vo
     a.scores = w.total > w.scores ? reinterpret_cast<float*>(base + w.scores) : nullptr;
     const int rows = r.tokens * a.group, nt = row_tiles(rows);
     a.pitch = score_pitch(rows);
-    a.n_rt = (rows + 8 * nt - 1) / (8 * nt);
+    a.n_rt = Div((rows + 8 * nt - 1) / (8 * nt));
+    a.jobs = Div(c.kv_heads * a.n_rt);
     if (c.head_dim == 128) return nt == 1 ? attend<128, 1>(a, stream) : attend<128, 2>(a, stream);
     return nt == 1 ? attend<64, 1>(a, stream) : attend<64, 2>(a, stream);
 }
