@@ -22,8 +22,8 @@ CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-LIB_SOURCES = ["dq_gemv.cu", "dq_stream.cu", "dq_batched.cu", "dq_moe.cu", "dq_kv.cu", "dq_kv_attend.cu", "dq_abi.cu"]
-LIB_HEADERS = ["dq_common.cuh", "dq_internal.h", "dq_plan.cuh", "dq_gplan.cuh", "dq_kv.cuh"]
+LIB_SOURCES = ["dq_gemv.cu", "dq_stream.cu", "dq_batched.cu", "dq_moe.cu", "dq_kv.cu", "dq_kv_attend.cu", "dq_kv_chunk.cu", "dq_abi.cu"]
+LIB_HEADERS = ["dq_common.cuh", "dq_internal.h", "dq_plan.cuh", "dq_gplan.cuh", "dq_kv.cuh", "dq_kv_plan.cuh"]
 EXT_SOURCES = ["torch_ext.cpp", "torch_kv.cpp"]
 LIB_PATH = os.path.join(PKG, "libdq_b200.so")
 EXT_SUFFIX = sysconfig.get_config_var("EXT_SUFFIX") or ".so"

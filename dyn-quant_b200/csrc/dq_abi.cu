@@ -150,6 +150,9 @@ dq_status_t dq_read_device_error(uint32_t* word, int clear) {
     uint32_t kv = 0, ka = 0;
     if ((st = read_kv_error(&kv, clear != 0)) != DQ_OK) return st;
     if ((st = read_kv_attend_error(&ka, clear != 0)) != DQ_OK) return st;
+    uint32_t kc = 0;
+    if ((st = read_kv_chunk_error(&kc, clear != 0)) != DQ_OK) return st;
+    ka |= kc;
     // streaming kernel: bit 0 of its word (its own copies) -> bit 5
     *word = b1 | (bg << 8) | ((bs & 1u) ? (1u << 5) : 0u) | (kv << 16) | (ka << 20);
     return DQ_OK;

@@ -415,6 +415,7 @@ dq_status_t launch_kv_evict(const dq_kv_cache_t& c, int keep, int recent, int si
                             cudaStream_t stream);
 dq_status_t read_kv_error(uint32_t* word, bool clear);
 dq_status_t read_kv_attend_error(uint32_t* word, bool clear);
+dq_status_t read_kv_chunk_error(uint32_t* word, bool clear);
 
 // Largest d_in the single-pass kernels accept (x, its B fragments and the
 // outlier list live in shared memory next to the weight rings).

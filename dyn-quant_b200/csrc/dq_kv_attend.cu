@@ -38,7 +38,7 @@
 // is taken again only when a score passes it by 8) and w is the power of two
 // that brings the largest s_v seen to at most 2^7, so p' <= 2^15 and small
 // weights keep their 11 bits down to 2^-29 of the largest.
-#include "dq_kv.cuh"
+#include "dq_kv_plan.cuh"
 
 namespace dq {
 
@@ -47,151 +47,12 @@ namespace {
 __device__ unsigned int g_kv_attend_error;
 
 constexpr int kAtMaxWarps = 2560;     // bound on the grid's warps (workspace sizing)
-constexpr float kNone = -1e30f;       // running maximum of a row that has seen no key
-constexpr float kLazy = 8.0f;         // a score passes the running maximum by this much (log2) before it moves
-constexpr int kStep = 2 * kKvTokens;  // slots of one step of a run
 constexpr float kCode = 16777216.0f;  // 2^24: a masked code is c / kCode
 
 // Warps of a CTA and CTAs of an SM for row tiles of 8 NT rows: two row tiles
 // need about 200 registers a thread, one tile 128.
 __host__ __device__ constexpr int at_warps(int nt) { return nt == 1 ? 8 : 10; }
 __host__ __device__ constexpr int at_ctas(int nt) { return nt == 1 ? 2 : 1; }
-
-struct KvAttendArgs {
-    KvView c;
-    const uint16_t* q;
-    uint16_t* out;
-    long long qs[3], os[3];  // strides in values: sequence, token, head
-    float* lse;              // [n_seqs][tokens][q_heads] natural log, or null
-    float* lse2;             // workspace: the same in log2 (mass pass), or null
-    float* scores;           // workspace: [units of the pool][16][pitch] scores in log2 for the mass pass, or null
-    int pitch;               // rows of a KV head, rounded up to 1, 2, 4 or 8
-    const int32_t* counts;
-    float* part;             // [CTAs][2][rows][D]
-    float* part_ml;          // [CTAs][2][rows][2]
-    float* first;            // [warps][rows][D + 2] pieces of jobs that end inside a run
-    int* pre;                // [n_seqs + 1] the plan's prefix sums, for the combining kernel
-    uint32_t* done;          // [n_seqs][heads] CTAs of a cut job that have arrived (one row tile)
-    int tokens;              // query tokens
-    Div group, n_rt, jobs;   // query heads per KV head, row tiles, jobs of a sequence
-    float scale2;            // scale * log2(e) * kCode
-    int depth;               // ring slots per warp
-    int first_off, places;   // shared memory for some of those pieces: its offset, how many
-};
-
-// The list of steps: a job is steps_of(len[b]) steps of one (sequence, KV head,
-// row tile), a sequence has `jobs` of them one after another, pre[b] counts the
-// steps of one job of every sequence before b.  Warp w takes base steps, one
-// more if w < rem.  Short lists are cut into runs of up to 4 steps rather than
-// one: a job then needs fewer warps, and its pieces meet in one CTA.
-// a / b for 0 <= a, 0 < b, with the short division where it does.
-__device__ __forceinline__ long long quotient(long long a, long long b) {
-    return ((a | b) >> 31) == 0 ? static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
-}
-__device__ __forceinline__ int quotient(long long a, const Div& b) {
-    return (a >> 31) == 0 ? static_cast<int>(a) / b : static_cast<int>(a / b.d);
-}
-
-struct Runs {
-    long long base, total;
-    int rem;
-
-    __device__ __forceinline__ Runs() {}
-    __device__ __forceinline__ Runs(int job_steps, int n_seqs, int jobs, int warps) {
-        total = static_cast<long long>(job_steps) * jobs;
-        const int least = min(4, (job_steps + n_seqs - 1) / n_seqs);
-        if (total < static_cast<long long>(warps) * least) warps = max(1, static_cast<int>(total) / max(least, 1));
-        base = quotient(total, warps);
-        rem = static_cast<int>(total - base * warps);
-    }
-    __device__ __forceinline__ long long start(long long w) const {
-        return min(w * base + (w < rem ? w : rem), total);
-    }
-    // the warp whose run has step u
-    __device__ __forceinline__ long long warp_of(long long u) const {
-        const long long cut = rem * (base + 1);
-        return u < cut ? quotient(u, base + 1) : rem + quotient(u - cut, base);
-    }
-};
-
-struct Plan {
-    const int* pre;
-    const int* len;
-    Div jobs;
-    Runs runs;
-};
-
-__host__ __device__ inline int steps_of(int len) { return (len + kStep - 1) / kStep; }
-
-// Bytes of the plan in shared memory.
-__host__ __device__ inline int plan_bytes(int n_seqs) { return ((2 * n_seqs + 1) * 4 + 127) / 128 * 128; }
-
-// Built by every CTA from the lengths (a few KB from L2); all threads call it.
-template <int NT>
-__device__ Plan make_plan(const KvView& c, const Div& jobs, int warps, char* smem, unsigned int* err) {
-    int* pre = reinterpret_cast<int*>(smem);
-    int* lens = pre + c.n_seqs + 1;
-    __shared__ int wtot[NT / 32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int run = 0;
-    for (int b0 = 0; b0 < c.n_seqs; b0 += NT) {
-        const int b = b0 + tid;
-        int v = 0;
-        if (b < c.n_seqs) {
-            bool bad = false;
-            const int n = kv_length(c, b, &bad);
-            if (bad && err) atomicOr(err, kKvErrLen);
-            lens[b] = n;
-            v = steps_of(n);
-        }
-        int inc = v;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int t = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += t;
-        }
-        if (lane == 31) wtot[warp] = inc;
-        __syncthreads();
-        int before = run;
-        for (int w = 0; w < NT / 32; ++w) {
-            if (w < warp) before += wtot[w];
-            run += wtot[w];
-        }
-        if (b < c.n_seqs) pre[b] = before + inc - v;
-        __syncthreads();
-    }
-    if (tid == 0) pre[c.n_seqs] = run;
-    __syncthreads();
-    Plan p;
-    p.pre = pre;
-    p.len = lens;
-    p.jobs = jobs;
-    p.runs = Runs(run, c.n_seqs, jobs, warps);
-    return p;
-}
-
-// Where a step lies: sequence, its length, job and step of the job.
-struct StepAt {
-    int b, len, job, step;
-};
-
-__device__ __forceinline__ StepAt step_at(const Plan& p, int n_seqs, long long u) {
-    const int v = quotient(u, p.jobs);  // pre[b] <= v < pre[b + 1]: the last b with pre[b] <= v
-    int lo = 0, hi = n_seqs;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (p.pre[mid] <= v) lo = mid;
-        else hi = mid;
-    }
-    const int st = p.pre[lo + 1] - p.pre[lo];
-    const long long r = u - static_cast<long long>(p.pre[lo]) * p.jobs;
-    StepAt a;
-    a.b = lo;
-    a.len = p.len[lo];
-    a.job = static_cast<int>(quotient(r, static_cast<long long>(st)));
-    a.step = static_cast<int>(r - static_cast<long long>(a.job) * st);
-    return a;
-}
 
 // f16 pairs c 2^-24 of the nibbles at bits 0..3 and 16..19, c 2^-20 of those at bits 4..7 and 20..23.
 __device__ __forceinline__ uint32_t low_codes(uint32_t w) { return w & 0x000F000Fu; }
@@ -240,47 +101,6 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
     return r;
 }
 
-__device__ __forceinline__ float ex2(float v) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-    return r;
-}
-
-// Two FP32 operations in one instruction, on the pair of a lane's rows 2t, 2t + 1.
-struct f2 {
-    unsigned long long v;
-    __device__ __forceinline__ f2() {}
-    __device__ __forceinline__ f2(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
-    __device__ __forceinline__ explicit f2(float x) : f2(x, x) {}
-    __device__ __forceinline__ float x() const {
-        return __uint_as_float(static_cast<uint32_t>(v));
-    }
-    __device__ __forceinline__ float y() const {
-        return __uint_as_float(static_cast<uint32_t>(v >> 32));
-    }
-};
-__device__ __forceinline__ f2 operator+(f2 a, f2 b) {
-    f2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ f2 operator*(f2 a, f2 b) {
-    f2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-    f2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return r;
-}
-
-__device__ __forceinline__ uint32_t pack_f32(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
 __device__ __forceinline__ float lane_max_g(float v) {  // over the lanes g of one t
 #pragma unroll
     for (int o = 4; o <= 16; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -290,19 +110,6 @@ __device__ __forceinline__ float lane_sum_g(float v) {
 #pragma unroll
     for (int o = 4; o <= 16; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
-}
-
-// 1 / sum of a row's weights; 0 where it has seen no key, not a number where the sum is not.
-__device__ __forceinline__ float row_norm(float sum) {
-    return sum > 0.f ? __fdividef(1.f, sum) : (sum == 0.f ? 0.f : sum);  // sum < 2^31
-}
-
-// lse of a row, in log2 and natural.
-__device__ __forceinline__ void store_lse(const KvAttendArgs& a, int b, int tok, int head, float m, float sum) {
-    const size_t i = (static_cast<size_t>(b) * a.tokens + tok) * (a.c.heads * a.group) + head;
-    const float l2 = sum == 0.f ? -INFINITY : m + __log2f(sum);  // absolute error 2^-21
-    if (a.lse) a.lse[i] = l2 * 0.693147180559945309f;
-    if (a.lse2) a.lse2[i] = l2;
 }
 
 // B fragments of 8 NT query rows and what the scores need of them.
@@ -738,106 +545,6 @@ struct RowState {
     }
     __device__ __forceinline__ float top(int nt, int e) const { return -(e ? m[nt].y() : m[nt].x()); }
 };
-
-// Columns col .. col + N - 1 of row r of KV head h, normalised; the thread with column 0 stores the row's lse.
-template <int N>
-__device__ __forceinline__ void store_row(const KvAttendArgs& a, int b, int h, int r, int col, const float (&v)[N], float m,
-                                          float sum) {
-    const int tok = r / a.group, head = h * a.group + r - tok * a.group;
-    const float f = row_norm(sum);
-    uint16_t* dst = a.out + b * a.os[0] + tok * a.os[1] + head * a.os[2] + col;
-#pragma unroll
-    for (int i = 0; i < N; i += 8)
-        *reinterpret_cast<uint4*>(dst + i) =
-            make_uint4(pack_f32(v[i] * f, v[i + 1] * f), pack_f32(v[i + 2] * f, v[i + 3] * f),
-                       pack_f32(v[i + 4] * f, v[i + 5] * f), pack_f32(v[i + 6] * f, v[i + 7] * f));
-    if (col == 0) store_lse(a, b, tok, head, m, sum);
-}
-
-// The CTAs that share a job (c0 .. c0 + n - 1) and the workspace slot of the first; every later CTA begins
-// inside the job, which is its slot 0.
-struct Share {
-    long long c0;
-    int n, slot0;
-};
-
-template <int W>
-__device__ __forceinline__ Share share_of(const int* pre, int n_seqs, const Div& jobs, const Runs& runs, int b, int job) {
-    Share s{0, 0, 0};
-    const int p0 = pre[b], ul = pre[b + 1] - p0;
-    if (ul == 0) return s;
-    const long long u0 = static_cast<long long>(p0) * jobs + static_cast<long long>(ul) * job;
-    s.c0 = runs.warp_of(u0) / W;
-    s.n = static_cast<int>(runs.warp_of(u0 + ul - 1) / W - s.c0) + 1;
-    const long long start = runs.start(s.c0 * W);
-    if (s.n > 1 && u0 > start) {
-        // the job at the CTA's start has slot 0 if the border cuts it
-        const int v = quotient(start, jobs);
-        int lo = 0, hi = b + 1;  // pre[lo] <= v < pre[hi]
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (pre[mid] <= v) lo = mid;
-            else hi = mid;
-        }
-        const long long in = start - static_cast<long long>(pre[lo]) * jobs, st = pre[lo + 1] - pre[lo];
-        s.slot0 = in != quotient(in, st) * st ? 1 : 0;
-    }
-    return s;
-}
-
-// One warp joins row r's partial sums: maxima and sums a lane each, then the outputs eight partials at a time.
-template <int D, int NT>
-__device__ __forceinline__ void join_row(const KvAttendArgs& a, const Share& s, int b, int h, int rt, int r) {
-    constexpr int R = 8 * NT, V = D / 32, N = 8;  // V columns of a lane, side by side; partials at a time
-    const int lane = threadIdx.x & 31, rl = r - rt * R, first = s.slot0 * R;  // only the first CTA's may be its slot 1
-    const size_t row0 = static_cast<size_t>(s.c0) * 2 * R + rl;
-    const float2* ml0 = reinterpret_cast<const float2*>(a.part_ml) + row0;
-    const float* o0 = a.part + row0 * D + V * lane;
-    auto ml_at = [&](int i) { return i < s.n ? __ldcg(ml0 + (i == 0 ? first : i * 2 * R)) : make_float2(kNone, 0.f); };
-    float x[N][V];
-    auto fetch = [&](int i0) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const float* src = o0 + static_cast<size_t>(i0) * 2 * R * D + j * 2 * R * D + (i0 + j == 0 ? first * D : 0);
-            const bool on = i0 + j < s.n;
-            if constexpr (V == 4) {
-                const float4 y = on ? __ldcg(reinterpret_cast<const float4*>(src)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                x[j][0] = y.x; x[j][1] = y.y; x[j][2] = y.z; x[j][3] = y.w;
-            } else {
-                const float2 y = on ? __ldcg(reinterpret_cast<const float2*>(src)) : make_float2(0.f, 0.f);
-                x[j][0] = y.x; x[j][1] = y.y;
-            }
-        }
-    };
-    float2 ml = ml_at(lane);
-    fetch(0);
-    float m = ml.x, sum = 0.f, v[V];
-    for (int i = lane + 32; i < s.n; i += 32) m = fmaxf(m, ml_at(i).x);
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-#pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = 0.f;
-#pragma unroll 1
-    for (int i0 = 0; i0 < s.n; i0 += N) {
-        if (i0 > 0 && i0 % 32 == 0) ml = ml_at(i0 + lane);
-        const float f = ml.x > kNone ? ex2(ml.x - m) : (ml.x == kNone ? 0.f : ml.x);
-        if (i0 % 32 == 0) sum += ml.y * f;
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const float fj = __shfl_sync(0xffffffffu, f, i0 % 32 + j);
-#pragma unroll
-            for (int k = 0; k < V; ++k) v[k] = fmaf(x[j][k], fj, v[k]);
-        }
-        if (i0 + N < s.n) fetch(i0 + N);
-    }
-    sum = warp_sum(sum);
-    const int tok = r / a.group, head = h * a.group + r - tok * a.group;
-    const float f = row_norm(sum);
-    uint16_t* dst = a.out + b * a.os[0] + tok * a.os[1] + head * a.os[2] + V * lane;
-#pragma unroll
-    for (int k = 0; k < V; k += 2) *reinterpret_cast<uint32_t*>(dst + k) = pack_f32(v[k] * f, v[k + 1] * f);
-    if (lane == 0) store_lse(a, b, tok, head, m, sum);
-}
 
 // A piece of a job that its run cut: which job and which of its steps.
 struct Piece {
@@ -1335,6 +1042,24 @@ dq_status_t mass(KvAttendArgs& a, int sm_count, cudaStream_t stream) {
     return launch_pdl(kv_mass_kernel<D, NT>, dim3(sm_count * ms_ctas(NT)), 32 * ms_warps(NT), smem, stream, 1, a);
 }
 
+// The mass pass, from the kept scores or the keys.
+template <int D>
+dq_status_t weights(KvAttendArgs& a, int sm_count, cudaStream_t stream) {
+    const int rows = a.tokens * a.group;
+    a.jobs = Div(a.c.heads);
+    if (a.scores) {
+        const dim3 g(sm_count * 4);
+        const int threads = 32 * kSmWarps, bytes = plan_bytes(a.c.n_seqs);
+        switch (a.pitch) {
+            case 1: return launch_pdl(kv_score_mass_kernel<1>, g, threads, bytes, stream, 1, a);
+            case 2: return launch_pdl(kv_score_mass_kernel<2>, g, threads, bytes, stream, 1, a);
+            case 4: return launch_pdl(kv_score_mass_kernel<4>, g, threads, bytes, stream, 1, a);
+            default: return launch_pdl(kv_score_mass_kernel<8>, g, threads, bytes, stream, 1, a);
+        }
+    }
+    return rows <= 8 ? mass<D, 1>(a, sm_count, stream) : mass<D, 4>(a, sm_count, stream);
+}
+
 template <int D, int NT>
 dq_status_t attend(KvAttendArgs& a, cudaStream_t stream) {
     constexpr int W = at_warps(NT);
@@ -1358,19 +1083,11 @@ dq_status_t attend(KvAttendArgs& a, cudaStream_t stream) {
         st = launch_pdl(kv_combine_kernel<D, NT>, dim3(static_cast<unsigned>((items + kCbWarps - 1) / kCbWarps)),
                     32 * kCbWarps, 0, stream, 1, a, grid);
     if (st != DQ_OK || !a.lse2) return st;
-    a.jobs = Div(a.c.heads);
-    if (a.scores) {
-        const dim3 g(di.sm_count * 4);
-        const int threads = 32 * kSmWarps, bytes = plan_bytes(a.c.n_seqs);
-        switch (a.pitch) {
-            case 1: return launch_pdl(kv_score_mass_kernel<1>, g, threads, bytes, stream, 1, a);
-            case 2: return launch_pdl(kv_score_mass_kernel<2>, g, threads, bytes, stream, 1, a);
-            case 4: return launch_pdl(kv_score_mass_kernel<4>, g, threads, bytes, stream, 1, a);
-            default: return launch_pdl(kv_score_mass_kernel<8>, g, threads, bytes, stream, 1, a);
-        }
-    }
-    return rows <= 8 ? mass<D, 1>(a, di.sm_count, stream) : mass<D, 4>(a, di.sm_count, stream);
+    return weights<D>(a, di.sm_count, stream);
 }
+
+// Query rows of a KV head from which the tensor-memory kernel of dq_kv_chunk.cu takes the call.
+constexpr int kChunkMin = 64;
 
 // Row tiles of one warp: 8 rows when a KV head has no more, else 16.
 int row_tiles(int rows) { return rows <= 8 ? 1 : 2; }
@@ -1385,12 +1102,13 @@ struct AttendWs {
 };
 AttendWs attend_ws(const dq_kv_cache_t& c, int tokens, int q_heads, bool mass) {
     const int nt = row_tiles(tokens * (q_heads / c.kv_heads));
-    const size_t rows = static_cast<size_t>(kAtMaxWarps / at_warps(nt)) * 2 * 8 * nt;
+    const bool chunk = tokens * (q_heads / c.kv_heads) >= kChunkMin;
+    const size_t rows = chunk ? kv_chunk_part_rows() : static_cast<size_t>(kAtMaxWarps / at_warps(nt)) * 2 * 8 * nt;
     AttendWs w;
     w.part = 0;
     w.ml = align256(rows * c.head_dim * 4);
     w.first = w.ml + align256(rows * 8);
-    w.pre = w.first + align256(static_cast<size_t>(kAtMaxWarps) * 8 * nt * (c.head_dim + 2) * 4);
+    w.pre = w.first + (chunk ? 0 : align256(static_cast<size_t>(kAtMaxWarps) * 8 * nt * (c.head_dim + 2) * 4));
     w.lse2 = w.pre + align256((static_cast<size_t>(c.n_seqs) + 1) * 4);
     w.scores = w.lse2 + (mass ? align256(static_cast<size_t>(c.n_seqs) * tokens * q_heads * 4) : 0);
     const int group_rows = tokens * (q_heads / c.kv_heads);
@@ -1427,6 +1145,16 @@ dq_status_t launch_kv_attend(const dq_kv_cache_t& c, const dq_kv_attend_t& r, vo
     a.scores = w.total > w.scores ? reinterpret_cast<float*>(base + w.scores) : nullptr;
     const int rows = r.tokens * a.group, nt = row_tiles(rows);
     a.pitch = score_pitch(rows);
+    if (rows >= kChunkMin) {
+        KvAttendArgs b = a;
+        b.scale2 = r.scale * 1.44269504088896341f;  // its codes are whole numbers
+        const dq_status_t st = launch_kv_chunk(b, c.head_dim, stream);
+        if (st != DQ_OK || !a.lse2) return st;
+        DeviceInfo di;
+        const dq_status_t sd = device_info(&di);
+        if (sd != DQ_OK) return sd;
+        return c.head_dim == 128 ? weights<128>(a, di.sm_count, stream) : weights<64>(a, di.sm_count, stream);
+    }
     a.n_rt = Div((rows + 8 * nt - 1) / (8 * nt));
     a.jobs = Div(c.kv_heads * a.n_rt);
     if (c.head_dim == 128) return nt == 1 ? attend<128, 1>(a, stream) : attend<128, 2>(a, stream);

@@ -1,0 +1,603 @@
+// dq_kv_chunk.cu -- attention over the paged 4-bit KV cache for many query rows
+// per KV head (a prompt's chunk), on tcgen05 with the accumulators in tensor
+// memory.  The same softmax and the same result as dq_kv_attend.cu's kernel.
+//
+// A tile is 128 query rows (token, query head) of one KV head, a block 128
+// slots.  The (sequence, KV head, tile) jobs' blocks form one list cut into
+// equal runs, one per CTA (one CTA an SM); pieces of jobs that a border cuts are
+// joined by kv_chunk_combine_kernel.
+//
+// Roles of a CTA's nine warps, over the blocks i of its run:
+//   dequantizing (4)  wait for the block's units (bulk copies), turn codes into
+//                     f16 integers c - 8 in the MMA's shared-memory layout and
+//                     the scales into FP32 constants; ask for block i + 2
+//   MMA (1)           S(i) = Q K^T into one of two TMEM tiles, then, when the
+//                     weights of i - 1 are there, O += P(i-1) V
+//   softmax (4)       a thread per row: S(i) from TMEM, scores, weights, P(i)
+//                     back to TMEM as the A operand; at a job's end O
+// Everything hands over through mbarriers; every wait is bounded, and a CTA
+// whose wait gave up sets the error word and leaves.
+//
+// K rows keep their words' column order (c0 c4 c1 c5 c2 c6 c3 c7): a word
+// becomes one 16-byte chunk, and Q's columns are permuted alike.  V words hold
+// two neighbouring slots of a column, which is a K-major pair of V^T as it is.
+// Codes are exact in f16, scales and zeros are applied in FP32 around the
+// products as in dq_kv_attend.cu; p' = p s_v w is rounded to f16.
+#include "dq_kv_plan.cuh"
+
+namespace dq {
+
+namespace {
+
+__device__ unsigned int g_kv_chunk_error;
+
+constexpr int kBlk = 128;                  // slots of a block
+constexpr int kUnits = kBlk / kKvTokens;   // units of a block
+constexpr int kCkThreads = 9 * 32;
+constexpr int kTile = kChunkRows;
+
+// Shared memory, offsets from a 1024-byte boundary.  Operand tiles are 128-byte rows (64 f16 of K) in groups of
+// eight rows, the 16-byte chunks of row r xor-ed with r mod 8 (the 128-byte swizzle).
+template <int D>
+struct CkSmem {
+    static constexpr int kQ = 0;                                 // [D/64][128 rows]
+    static constexpr int kOp = D / 64 * kTile * 128;             // bytes of Q and of K
+    static constexpr int kK = kQ + kOp;                          // 2 x [D/64][128 slots]
+    static constexpr int kVBytes = kBlk / 64 * D * 128;
+    static constexpr int kV = kK + 2 * kOp;                      // 2 x [2][D columns], 64 slots a row
+    static constexpr int kRawBytes = kUnits * kv_unit_bytes(D);
+    static constexpr int kRaw = kV + 2 * kVBytes;                // 2 x the units of a block
+    static constexpr int kPar = kRaw + 2 * kRawBytes;            // 2 x [4][128]: - (z_k - 8), s_k, s_v, z_v - 8
+    static constexpr int kMisc = kPar + 2 * 4 * kBlk * 4;        // per buffer: 4 x largest s_v, 4 x slots there; found units
+    static constexpr int kBars = kMisc + 128;
+    static constexpr int kTotal = kBars + 128;
+};
+
+// Barriers (8 bytes each).
+enum { kRawFull = 0, kKvFull = 2, kKvFree = 4, kSFull = 6, kPFull = 8, kQFull = 10, kBarCount = 11 };
+
+// Tensor memory columns: two S tiles, O, two P tiles (f16 pairs).
+constexpr uint32_t kTmS = 0, kTmO = 256, kTmP = 384, kTmCols = 512;
+
+__device__ __forceinline__ void tm_alloc(uint32_t smem_dst, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tm_dealloc(uint32_t addr, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
+}
+__device__ __forceinline__ void tm_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tm_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// Arrives on the barrier when the MMAs issued so far have completed.
+__device__ __forceinline__ void tm_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// A K-major operand tile with the 128-byte swizzle: start address and the 1024 bytes between groups of eight rows in
+// units of 16 bytes, descriptor version 1, swizzle mode 2.
+__device__ __forceinline__ uint64_t operand(uint32_t addr) {
+    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (1ull << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) |
+           (2ull << 61);
+}
+// f16 x f16 -> f32, both operands K-major, M = 128, N = n.
+__host__ __device__ constexpr uint32_t mma_shape(int n) {
+    return (1u << 4) | (static_cast<uint32_t>(n / 8) << 17) | (static_cast<uint32_t>(kTile / 16) << 24);
+}
+__device__ __forceinline__ void tm_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(shape), "r"(add ? 1u : 0u)
+        : "memory");
+}
+__device__ __forceinline__ void tm_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t shape, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(shape), "r"(add ? 1u : 0u)
+        : "memory");
+}
+
+// 32 columns of the warp's 32 rows, one row a thread.
+__device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tm_st32(uint32_t addr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+
+__device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+
+// f16 pairs c - 8 of the nibbles at bits 0..3 / 16..19 and 4..7 / 20..23.
+__device__ __forceinline__ uint32_t low_f16(uint32_t w) {
+    return hsub2_u32(lop3_and_or(w, 0x000F000Fu, 0x64006400u), 0x64086408u);  // (1024 + c) - 1032
+}
+__device__ __forceinline__ uint32_t high_f16(uint32_t w) {
+    return hsub2_u32(lop3_and_or(w, 0x00F000F0u, 0x54005400u), 0x54805480u);  // (64 + c) - 72
+}
+
+__device__ __forceinline__ void sts_u32(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+// Walks the blocks of a CTA's run; every role keeps its own.
+struct Walk {
+    StepAt at;
+    int blocks;  // of the job
+
+    __device__ __forceinline__ void set(const Plan& p, int n_seqs, long long u) {
+        at = step_at(p, n_seqs, u);
+        blocks = steps_of<kBlk>(at.len);
+    }
+    // The next block; true when it begins another job.
+    __device__ __forceinline__ bool next(const Plan& p, int n_seqs, long long u) {
+        if (++at.step < blocks) return false;
+        if (at.job + 1 < static_cast<int>(p.jobs)) {
+            ++at.job;
+            at.step = 0;
+        } else {
+            set(p, n_seqs, u);
+        }
+        return true;
+    }
+};
+
+template <int D>
+__global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendArgs a) {
+    using S = CkSmem<D>;
+    extern __shared__ char dyn[];
+    __shared__ uint32_t tm_base;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const KvView& c = a.c;
+    const uint32_t smem0 = (smem_u32(dyn) + plan_bytes(c.n_seqs) + 1023u) & ~1023u;
+    const uint32_t bars = smem0 + S::kBars;
+    if (warp == 8) tm_alloc(smem_u32(&tm_base), kTmCols);
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bars + 8 * (kRawFull + i), 1);
+            mbar_init(bars + 8 * (kKvFull + i), 128);
+            mbar_init(bars + 8 * (kKvFree + i), 1);
+            mbar_init(bars + 8 * (kSFull + i), 1);
+            mbar_init(bars + 8 * (kPFull + i), 128);
+        }
+        mbar_init(bars + 8 * kQFull, 128);
+        fence_mbar_init();
+    }
+    tm_before_sync();
+    __syncthreads();
+    tm_after_sync();
+    const uint32_t tm = tm_base;
+    pdl_launch_dependents();
+    pdl_wait();
+    const Plan p = make_plan<kCkThreads, kBlk>(c, a.jobs, gridDim.x, dyn, blockIdx.x == 0 ? &g_kv_chunk_error : nullptr);
+    if (blockIdx.x == 0)
+        for (int b = tid; b <= c.n_seqs; b += kCkThreads) a.pre[b] = p.pre[b];
+    const long long u0 = p.runs.start(blockIdx.x);
+    const int n = static_cast<int>(p.runs.start(blockIdx.x + 1) - u0);
+    const int rows = a.tokens * a.group;
+    auto wait = [&](int bar, int parity) {
+        const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * bar, parity & 1));
+        if (!ok && lane == 0) atomicOr(&g_kv_chunk_error, kKvErrWait);
+        return ok;
+    };
+    Walk at;
+    if (n > 0) at.set(p, c.n_seqs, u0);
+
+    if (n > 0 && warp < 4) {
+        // ---- softmax: row tid of the tile
+        const uint32_t lanes = tm + (static_cast<uint32_t>(32 * warp) << 16);
+        float m = kNone, l = 0.f, zs = 0.f, vw = 0.f, qsum = 0.f;
+        int lim = 0, r = 0, first = 0, cuts = 0, jobs_done = 0;
+        bool begins = true;
+        auto load_q = [&]() {
+            const int h = at.at.job / a.n_rt, rt = at.at.job - h * a.n_rt;
+            r = rt * kTile + tid;
+            const int tok = r / a.group;
+            const int cnt = a.counts ? min(max(ld_l2(a.counts + at.at.b), 0), a.tokens) : a.tokens;
+            const bool on = r < rows && tok < cnt;
+            lim = on ? min(max(at.at.len - cnt + tok + 1, 0), at.at.len) : 0;
+            const uint16_t* src = a.q + at.at.b * a.qs[0] + tok * a.qs[1] + (h * a.group + r - tok * a.group) * a.qs[2];
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                const uint4 w = on ? ld_l2_v4(src + 8 * i) : make_uint4(0, 0, 0, 0);
+                const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s += h2f_bits(lo16(v[k])) + h2f_bits(hi16(v[k]));
+                sts_v4(smem0 + S::kQ + i / 8 * (kTile * 128) + tid * 128 + (((i % 8) ^ (tid & 7)) << 4),
+                       make_uint4(__byte_perm(w.x, w.z, 0x5410), __byte_perm(w.x, w.z, 0x7632),
+                                  __byte_perm(w.y, w.w, 0x5410), __byte_perm(w.y, w.w, 0x7632)));
+            }
+            qsum = s;
+            fence_async_smem();
+            mbar_arrive(bars + 8 * kQFull);
+        };
+        load_q();
+        first = at.at.step;
+        for (int i = 0; i < n; ++i) {
+            const int buf = i & 1, step = at.at.step;
+            if (!wait(kSFull + buf, i >> 1)) break;
+            tm_after_sync();
+            const uint32_t par = smem0 + S::kPar + buf * (4 * kBlk * 4), misc = smem0 + S::kMisc + buf * 64;
+            f2 s[kBlk / 2];
+            float top = -INFINITY;
+            const int left = lim - step * kBlk;  // slots of the block that the row sees
+            const uint4 there = lds_v4(misc + 16);
+            const bool all = left >= kBlk && (there.x & there.y & there.z & there.w) == 0xffffffffu;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t v[32];
+                tm_ld32(lanes + kTmS + buf * kBlk + 32 * k, v);
+                tm_wait_ld();
+                const uint32_t ok = k == 0 ? there.x : (k == 1 ? there.y : (k == 2 ? there.z : there.w));
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) {
+                    const uint4 z = lds_v4(par + 4 * (32 * k + j)), sc = lds_v4(par + 4 * (kBlk + 32 * k + j));
+                    f2 x = fma2(f2(__uint_as_float(z.x), __uint_as_float(z.y)), f2(qsum), f2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]))) *
+                           f2(__uint_as_float(sc.x), __uint_as_float(sc.y));
+                    f2 y = fma2(f2(__uint_as_float(z.z), __uint_as_float(z.w)), f2(qsum), f2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]))) *
+                           f2(__uint_as_float(sc.z), __uint_as_float(sc.w));
+                    if (!all) {
+                        const int e = 32 * k + j;
+                        x = f2(e < left && (ok >> j & 1u) ? x.x() : -INFINITY, e + 1 < left && (ok >> (j + 1) & 1u) ? x.y() : -INFINITY);
+                        y = f2(e + 2 < left && (ok >> (j + 2) & 1u) ? y.x() : -INFINITY, e + 3 < left && (ok >> (j + 3) & 1u) ? y.y() : -INFINITY);
+                    }
+                    s[16 * k + j / 2] = x;
+                    s[16 * k + j / 2 + 1] = y;
+                    top = fmaxf(top, fmaxf(fmaxf(x.x(), x.y()), fmaxf(y.x(), y.y())));
+                }
+            }
+            // a new maximum or a larger V scale (the same for all rows)
+            const uint4 bg = lds_v4(misc);
+            const float big = fmaxf(fmaxf(__uint_as_float(bg.x), __uint_as_float(bg.y)), fmaxf(__uint_as_float(bg.z), __uint_as_float(bg.w)));
+            if (begins) {
+                m = kNone;
+                l = zs = 0.f;
+                vw = 2147483648.0f;  // 2^31 brings the smallest FP16 scale, 2^-24, to 2^7
+            }
+            bool stop = false;
+            if (__any_sync(0xffffffffu, top > m + kLazy || big * vw > 128.f)) {
+                float ratio = 1.f;
+                if (big * vw > 128.f) {
+                    // 2^(7 - e) with 2^(e-1) <= big < 2^e
+                    const float nw = __uint_as_float((260u - (__float_as_uint(big) >> 23)) << 23);
+                    ratio = __uint_as_float(__float_as_uint(nw) - __float_as_uint(vw) + 0x3F800000u);  // nw / vw, powers of two
+                    vw = nw;
+                }
+                const float now = fmaxf(m, top), f = now == m ? 1.f : ex2(m - now), fr = f * ratio;
+                m = now;
+                l *= f;
+                zs *= fr;
+                if (!begins) {
+                    // O is this warp's alone once the last block's product is in it
+                    stop = !wait(kKvFree + (buf ^ 1), (i - 1) >> 1);
+                    if (stop) break;
+                    tm_after_sync();
+#pragma unroll
+                    for (int k = 0; k < D / 32; ++k) {
+                        uint32_t v[32];
+                        tm_ld32(lanes + kTmO + 32 * k, v);
+                        tm_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * fr);
+                        tm_st32(lanes + kTmO + 32 * k, v);
+                    }
+                    tm_wait_st();
+                }
+            }
+            f2 l2(0.f), z2(0.f);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t pk[16];
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) {
+                    const uint4 w4 = lds_v4(par + 4 * (2 * kBlk + 32 * k + j)), z4 = lds_v4(par + 4 * (3 * kBlk + 32 * k + j));
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const f2 d = s[16 * k + j / 2 + e] + f2(-m), x(ex2(d.x()), ex2(d.y()));
+                        const f2 w(__uint_as_float(e ? w4.z : w4.x), __uint_as_float(e ? w4.w : w4.y));
+                        const f2 z(__uint_as_float(e ? z4.z : z4.x), __uint_as_float(e ? z4.w : z4.y));
+                        const f2 pr = x * (w * f2(vw));
+                        l2 = l2 + x;
+                        z2 = fma2(pr, z, z2);
+                        pk[j / 2 + e] = pack_f32(pr.x(), pr.y());
+                    }
+                }
+                tm_st16(lanes + kTmP + buf * 64 + 16 * k, pk);
+            }
+            l += l2.x() + l2.y();
+            zs += z2.x() + z2.y();
+            tm_wait_st();
+            tm_before_sync();
+            mbar_arrive(bars + 8 * (kPFull + buf));
+            begins = false;
+            // the job's end, or the run's
+            const StepAt was = at.at;
+            const int blocks = at.blocks, row = r;
+            const bool last = i + 1 == n, turn = last || at.next(p, c.n_seqs, u0 + i + 1);
+            if (!turn) continue;
+            const float inv_w = __uint_as_float(0x7F000000u - __float_as_uint(vw));
+            if (!last) load_q();  // S of the old rows is done; the new ones' can start
+            if (!wait(kKvFree + buf, i >> 1)) break;
+            tm_after_sync();
+            const bool whole = first == 0 && was.step + 1 == blocks;
+            const int h = was.job / a.n_rt, slot = cuts;
+            const size_t pi = (static_cast<size_t>(blockIdx.x) * 2 + slot) * kTile + tid;
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k) {
+                uint32_t v[32];
+                tm_ld32(lanes + kTmO + 32 * k, v);
+                tm_wait_ld();
+                if (row < rows) {
+                    float o[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) o[j] = (__uint_as_float(v[j]) - zs) * inv_w;
+                    if (whole) {
+                        store_row(a, was.b, h, row, 32 * k, o, m, l);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4)
+                            *reinterpret_cast<float4*>(a.part + pi * D + 32 * k + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                        if (k == 0) *reinterpret_cast<float2*>(a.part_ml + pi * 2) = make_float2(m, l);
+                    }
+                }
+            }
+            tm_before_sync();
+            if (!whole) ++cuts;
+            ++jobs_done;
+            first = at.at.step;
+            begins = true;
+        }
+    } else if (n > 0 && warp < 8) {
+        // ---- dequantizing
+        const int dw = warp - 4;
+        bool absent = false;
+        Walk ahead = at;
+        auto request = [&](int i) {  // warp 4: the units of the block that `ahead` stands at
+            const int buf = i & 1, slot = ahead.at.step * kBlk + lane * kKvTokens;
+            int index = -1;
+            if (lane < kUnits && slot < ahead.at.len) {
+                const int page = kv_page(c, ahead.at.b, slot);
+                if (page >= 0) index = static_cast<int>((kv_line(c, page, ahead.at.job / a.n_rt) + slot % c.page_size) / kKvTokens);
+                else absent = true;
+            }
+            const uint32_t got = __ballot_sync(0xffffffffu, index >= 0), bar = bars + 8 * (kRawFull + buf);
+            if (lane == 0) {
+                sts_u32(smem0 + S::kMisc + 48 + buf * 64, got);
+                if (got) mbar_arrive_expect_tx(bar, __popc(got) * kv_unit_bytes(D));
+                else mbar_arrive(bar);
+            }
+            __syncwarp();
+            if (index >= 0)
+                bulk_g2s(smem0 + S::kRaw + buf * S::kRawBytes + lane * kv_unit_bytes(D),
+                         c.units + static_cast<size_t>(index) * kv_unit_bytes(D), kv_unit_bytes(D), bar);
+            ahead.next(p, c.n_seqs, u0 + i + 1 < u0 + n ? u0 + i + 1 : u0 + n - 1);
+        };
+        if (dw == 0)
+            for (int i = 0; i < min(2, n); ++i) request(i);
+        int i = 0;
+        for (; i < n; ++i) {
+            const int buf = i & 1;
+            if (!wait(kRawFull + buf, i >> 1)) break;
+            if (i >= 2 && !wait(kKvFree + buf, (i - 2) >> 1)) break;
+            const uint32_t got = lds_u32(smem0 + S::kMisc + 48 + buf * 64);
+            const uint32_t kb = smem0 + S::kK + buf * S::kOp, vb = smem0 + S::kV + buf * S::kVBytes;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int u = 2 * dw + e;
+                const uint32_t raw = smem0 + S::kRaw + buf * S::kRawBytes + u * kv_unit_bytes(D);
+                {
+                    // K: a lane half a row, a word a chunk
+                    const int row = lane & 15, half = lane >> 4, key = u * kKvTokens + row;
+                    constexpr int N = D / 16;  // words of a lane
+#pragma unroll
+                    for (int i4 = 0; i4 < N / 4; ++i4) {
+                        const uint4 w4 = lds_v4(raw + row * (D / 2) + half * (D / 4) + 16 * i4);
+                        const uint32_t ws[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t w = ws[j], x = w >> 8;
+                            const int ch = half * N + 4 * i4 + j;
+                            sts_v4(kb + ch / 8 * (kBlk * 128) + key * 128 + (((ch % 8) ^ (key & 7)) << 4),
+                                   make_uint4(low_f16(w), high_f16(w), low_f16(x), high_f16(x)));
+                        }
+                    }
+                }
+                {
+                    // V: a lane four column quads of a slot pair; which quad and column it stores when differs
+                    // among the lanes of a pair, so that a store's 32 words lie in 32 banks
+                    const int pr = lane >> 2, g = lane & 3;
+                    const int key = u * kKvTokens + 2 * pr;  // the pair's first slot
+                    const uint32_t dst = vb + key / 64 * (D * 128), byte = 2 * (key % 64);
+#pragma unroll
+                    for (int i4 = 0; i4 < D / 64; ++i4) {
+                        const int q0 = 4 * (4 * i4 + g);
+                        const uint4 w4 = lds_v4(raw + kv_v_offset(D) + pr * D + 4 * q0);
+                        const uint32_t ws[4] = {g & 1 ? w4.y : w4.x, g & 1 ? w4.x : w4.y, g & 1 ? w4.w : w4.z, g & 1 ? w4.z : w4.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t w = ws[k], x = w >> 8;
+                            const uint32_t h[4] = {low_f16(w), high_f16(w), low_f16(x), high_f16(x)};
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const int d = 4 * (q0 + (k ^ (g & 1))) + (j ^ (g & 2));
+                                sts_u32(dst + d * 128 + (byte ^ ((d & 7) << 4)), g & 2 ? h[j ^ 2] : h[j]);
+                            }
+                        }
+                    }
+                }
+            }
+            {
+                // scales and zeros, a lane a slot
+                const int u = 2 * dw + (lane >> 4), slot = 32 * dw + lane;
+                const bool on = (got >> u & 1u) && at.at.step * kBlk + slot < at.at.len;
+                const uint2 pw = lds_v2(smem0 + S::kRaw + buf * S::kRawBytes + u * kv_unit_bytes(D) + kv_param_offset(D) + 8 * (lane & 15));
+                const float sv = on ? h2f_bits(lo16(pw.y)) : 0.f;
+                const uint32_t par = smem0 + S::kPar + buf * (4 * kBlk * 4) + 4 * slot, misc = smem0 + S::kMisc + buf * 64;
+                sts_u32(par, __float_as_uint(on ? 8.f - h2f_bits(hi16(pw.x)) : 0.f));
+                sts_u32(par + 4 * kBlk, __float_as_uint(on ? h2f_bits(lo16(pw.x)) * a.scale2 : 0.f));
+                sts_u32(par + 8 * kBlk, __float_as_uint(sv));
+                sts_u32(par + 12 * kBlk, __float_as_uint(on ? h2f_bits(hi16(pw.y)) - 8.f : 0.f));
+                float big = sv;
+#pragma unroll
+                for (int o = 16; o >= 1; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                const uint32_t there = __ballot_sync(0xffffffffu, on);
+                if (lane == 0) {
+                    sts_u32(misc + 4 * dw, __float_as_uint(big));
+                    sts_u32(misc + 16 + 4 * dw, there);
+                }
+            }
+            fence_async_smem();
+            mbar_arrive(bars + 8 * (kKvFull + buf));
+            named_bar_sync(1, 128);  // all four warps have read the units
+            if (dw == 0 && i + 2 < n) request(i + 2);
+            if (i + 1 < n) at.next(p, c.n_seqs, u0 + i + 1);
+        }
+        if (i < n && dw == 0)  // gave up: the copies in flight must end before the shared memory goes
+            for (int j = i; j < min(i + 2, n); ++j) mbar_wait_bounded(bars + 8 * (kRawFull + (j & 1)), (j >> 1) & 1);
+        if (absent) atomicOr(&g_kv_chunk_error, kKvErrPage);
+    } else if (n > 0) {
+        // ---- MMA
+        int jobs = 0;
+        bool begins = true, begins_before = true;
+        auto output = [&](int i, bool start) {
+            const int buf = i & 1;
+            if (!wait(kPFull + buf, i >> 1)) return false;
+            tm_after_sync();
+            if (lane == 0) {
+                const uint32_t vb = smem0 + S::kV + buf * S::kVBytes;
+#pragma unroll
+                for (int k = 0; k < kBlk / 16; ++k)
+                    tm_mma_ts(tm + kTmO, tm + kTmP + buf * 64 + 8 * k, operand(vb + k / 4 * (D * 128) + 32 * (k % 4)), mma_shape(D),
+                              !(start && k == 0));
+                tm_commit(bars + 8 * (kKvFree + buf));
+            }
+            __syncwarp();
+            return true;
+        };
+        bool ok = true;
+        for (int i = 0; i < n && ok; ++i) {
+            const int buf = i & 1;
+            if (begins && !(ok = wait(kQFull, jobs))) break;
+            if (!(ok = wait(kKvFull + buf, i >> 1))) break;
+            tm_after_sync();
+            if (lane == 0) {
+                const uint32_t kb = smem0 + S::kK + buf * S::kOp;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+                    tm_mma_ss(tm + kTmS + buf * kBlk, operand(smem0 + S::kQ + k / 4 * (kTile * 128) + 32 * (k % 4)),
+                              operand(kb + k / 4 * (kBlk * 128) + 32 * (k % 4)), mma_shape(kBlk), k > 0);
+                tm_commit(bars + 8 * (kSFull + buf));
+            }
+            __syncwarp();
+            if (i > 0) ok = output(i - 1, begins_before);
+            begins_before = begins;
+            if (begins) ++jobs;
+            begins = i + 1 < n && at.next(p, c.n_seqs, u0 + i + 1);
+        }
+        if (ok) ok = output(n - 1, begins_before);
+        if (ok) wait(kKvFree + ((n - 1) & 1), (n - 1) >> 1);
+    }
+    // rows of sequences without slots
+    for (int b = blockIdx.x; b < c.n_seqs; b += gridDim.x) {
+        if (p.len[b] != 0) continue;
+        const int hq = c.heads * a.group;
+        for (int i = tid; i < a.tokens * hq * (D / 8); i += kCkThreads) {
+            const int x = i / (D / 8), tok = x / hq, head = x - tok * hq, col = 8 * (i % (D / 8));
+            *reinterpret_cast<uint4*>(a.out + b * a.os[0] + tok * a.os[1] + head * a.os[2] + col) = make_uint4(0, 0, 0, 0);
+            if (col == 0) store_lse(a, b, tok, head, 0.f, 0.f);
+        }
+    }
+    tm_before_sync();
+    __syncthreads();
+    if (warp == 8) {
+        tm_after_sync();
+        tm_dealloc(tm, kTmCols);
+    }
+}
+
+// Joins the partial sums of the jobs cut between CTAs: one warp per row.
+constexpr int kCcWarps = 4;
+
+template <int D>
+__global__ void __launch_bounds__(32 * kCcWarps) kv_chunk_combine_kernel(const KvAttendArgs a, const int ctas) {
+    const KvView& c = a.c;
+    const int hq = c.heads * a.group;
+    pdl_launch_dependents();
+    pdl_wait();
+    const long long item = static_cast<long long>(blockIdx.x) * kCcWarps + (threadIdx.x >> 5);
+    if (item >= static_cast<long long>(c.n_seqs) * a.tokens * hq) return;
+    const long long bt = item / hq;
+    const int head = static_cast<int>(item - bt * hq), b = static_cast<int>(bt / a.tokens);
+    const int tok = static_cast<int>(bt - static_cast<long long>(b) * a.tokens);
+    const int h = head / a.group, r = tok * a.group + head - h * a.group, rt = r / kTile;
+    const Runs runs(a.pre[c.n_seqs], c.n_seqs, a.jobs, ctas);
+    const Share s = share_of<1>(a.pre, c.n_seqs, a.jobs, runs, b, h * a.n_rt + rt);
+    if (s.n > 1) join_row<D, kTile / 8>(a, s, b, h, rt, r);  // else finished by its CTA, or empty
+}
+
+template <int D>
+dq_status_t chunk(const KvAttendArgs& a, cudaStream_t stream) {
+    DeviceInfo di;
+    dq_status_t st = device_info(&di);
+    if (st != DQ_OK) return st;
+    const int ctas = di.sm_count < 160 ? di.sm_count : 160;
+    const int smem = plan_bytes(a.c.n_seqs) + 1024 + CkSmem<D>::kTotal;
+    const cudaError_t e = cudaFuncSetAttribute(kv_chunk_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) { set_cuda_error(e); return DQ_ERR_CUDA; }
+    if ((st = launch_pdl(kv_chunk_kernel<D>, dim3(ctas), kCkThreads, smem, stream, 1, a)) != DQ_OK) return st;
+    const long long items = static_cast<long long>(a.c.n_seqs) * a.tokens * a.c.heads * a.group;
+    return launch_pdl(kv_chunk_combine_kernel<D>, dim3(static_cast<unsigned>((items + kCcWarps - 1) / kCcWarps)), 32 * kCcWarps, 0,
+                      stream, 1, a, ctas);
+}
+
+}  // namespace
+
+size_t kv_chunk_part_rows() { return size_t{160} * 2 * kTile; }
+
+dq_status_t launch_kv_chunk(KvAttendArgs a, int head_dim, cudaStream_t stream) {
+    const int rows = a.tokens * a.group;
+    a.n_rt = Div((rows + kTile - 1) / kTile);
+    a.jobs = Div(a.c.heads * a.n_rt);
+    return head_dim == 128 ? chunk<128>(a, stream) : chunk<64>(a, stream);
+}
+
+dq_status_t read_kv_chunk_error(uint32_t* word, bool clear) {
+    unsigned int v = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&v, g_kv_chunk_error, sizeof(v));
+    if (e == cudaSuccess && clear && v) {
+        const unsigned int zero = 0;
+        e = cudaMemcpyToSymbol(g_kv_chunk_error, &zero, sizeof(zero));
+    }
+    if (e != cudaSuccess) { set_cuda_error(e); return DQ_ERR_CUDA; }
+    *word = v;
+    return DQ_OK;
+}
+
+}  // namespace dq

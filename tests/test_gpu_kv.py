@@ -223,6 +223,52 @@ def test_attend_is_reproducible_and_ignores_what_lies_behind():
     assert torch.equal(cache.attend(q), a)
 
 
+@pytest.mark.parametrize("dim,heads,group,t,page,lens,counts", [
+    (128, 1, 1, 64, 64, [64], None),
+    (128, 1, 1, 128, 64, [128, 127, 129], [128, 127, 128]),
+    (64, 2, 8, 9, 16, [130, 9, 0, 300], None),
+    (128, 2, 4, 40, 16, [41, 700, 3], [40, 17, 40]),
+    (128, 1, 3, 90, 48, [1000, 260], None),
+    (64, 1, 16, 33, 32, [513, 40], [0, 33]),
+])
+def test_attend_many_rows(dim, heads, group, t, page, lens, counts):
+    """64 and more query rows per KV head: several tiles of 128, ragged counts, blocks that end inside a page."""
+    cache = R.make_cache(lens, heads, dim, page, seed=dim + t, mass=True)
+    q = R.queries(cache, t, group)
+    mass0 = cache.mass.clone()
+    out, lse = cache.attend(q, counts=None if counts is None else ints(*counts), accumulate=True, return_lse=True)
+    R.check_attend(out, lse, q, cache, dim ** -0.5, counts=counts, mass=cache.mass, mass0=mass0)
+    again, lse2 = cache.attend(q, counts=None if counts is None else ints(*counts), return_lse=True)
+    assert torch.equal(again, out) and torch.equal(lse2, lse)
+
+
+def test_attend_many_rows_of_very_different_size():
+    """The tensor-memory accumulator is rescaled when the maximum moves and when larger V rows come."""
+    cache = R.make_cache([0], 1, 128, 64, extra=600)
+    gen = torch.Generator().manual_seed(8)
+    k, v = (torch.randn(1, 600, 1, 128, generator=gen) for _ in range(2))
+    v *= 10.0 ** torch.linspace(-4, 2, 600).view(1, 600, 1, 1)
+    k *= torch.linspace(0.1, 8, 600).view(1, 600, 1, 1)
+    cache.append(k.half().cuda(), v.half().cuda())
+    q = R.queries(cache, 32, 3)
+    out, lse = cache.attend(q, return_lse=True)
+    R.check_attend(out, lse, q, cache, 128 ** -0.5)
+
+
+def test_attend_many_rows_page_outside_the_pool():
+    cache = R.make_cache([150], 1, 64, 16)
+    q = R.queries(cache, 70, 1)
+    cache.page_table[0, 3] = -5
+    out, lse = cache.attend(q, return_lse=True)
+    torch.cuda.synchronize()
+    assert _C.read_device_error(True) == 1 << 20
+    keep = [j for j in range(150) if j // 16 != 3]
+    cache.page_table[0, 3] = cache.page_table[0, 0]
+    line = {k: v[:, keep] for k, v in R.decode(cache.units, cache.page_table, 16, 0, 150).items()}
+    r = R.attend(q[0], line, len(keep), 64 ** -0.5, 70)
+    assert (np.abs(out[0].double().cpu().numpy() - r["out"]) <= r["tol"]).all()
+
+
 def test_attend_many_sequences_and_uneven_lengths():
     lens = [(i * 37) % 90 for i in range(300)]
     lens[7] = 1500
