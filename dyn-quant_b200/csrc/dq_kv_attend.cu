@@ -1092,7 +1092,8 @@ constexpr int kChunkMin = 64;
 // Row tiles of one warp: 8 rows when a KV head has no more, else 16.
 int row_tiles(int rows) { return rows <= 8 ? 1 : 2; }
 
-// Scores that the mass pass may keep in the workspace; a larger cache's keys are read a second time.
+// What the mass pass may keep in the workspace (scores of up to 8 rows, or a line of sums for each tile of 128);
+// without that room it reads the keys a second time.
 constexpr size_t kMaxScores = size_t{1} << 30;
 
 int score_pitch(int rows) { return rows <= 2 ? rows : (rows <= 4 ? 4 : 8); }
@@ -1112,8 +1113,9 @@ AttendWs attend_ws(const dq_kv_cache_t& c, int tokens, int q_heads, bool mass) {
     w.lse2 = w.pre + align256((static_cast<size_t>(c.n_seqs) + 1) * 4);
     w.scores = w.lse2 + (mass ? align256(static_cast<size_t>(c.n_seqs) * tokens * q_heads * 4) : 0);
     const int group_rows = tokens * (q_heads / c.kv_heads);
-    const size_t kept = static_cast<size_t>(c.n_pages) * c.kv_heads * c.page_size * score_pitch(group_rows) * sizeof(float);
-    w.total = w.scores + (mass && nt == 1 && group_rows > 0 && kept <= kMaxScores ? align256(kept) : 0);
+    const size_t line = static_cast<size_t>(c.n_pages) * c.kv_heads * c.page_size * sizeof(float);
+    const size_t kept = line * (chunk ? (group_rows + kChunkRows - 1) / kChunkRows : score_pitch(group_rows));
+    w.total = w.scores + (mass && (chunk || nt == 1) && group_rows > 0 && kept <= kMaxScores ? align256(kept) : 0);
     return w;
 }
 
@@ -1148,8 +1150,8 @@ dq_status_t launch_kv_attend(const dq_kv_cache_t& c, const dq_kv_attend_t& r, vo
     if (rows >= kChunkMin) {
         KvAttendArgs b = a;
         b.scale2 = r.scale * 1.44269504088896341f;  // its codes are whole numbers
-        const dq_status_t st = launch_kv_chunk(b, c.head_dim, stream);
-        if (st != DQ_OK || !a.lse2) return st;
+        const dq_status_t st = launch_kv_chunk(b, c.head_dim, a.scores, stream);
+        if (st != DQ_OK || !a.lse2 || a.scores) return st;
         DeviceInfo di;
         const dq_status_t sd = device_info(&di);
         if (sd != DQ_OK) return sd;

@@ -7,14 +7,16 @@
 // equal runs, one per CTA (one CTA an SM); pieces of jobs that a border cuts are
 // joined by kv_chunk_combine_kernel.
 //
-// Roles of a CTA's nine warps, over the blocks i of its run:
+// Roles of a CTA's thirteen warps, over the blocks i of its run:
 //   dequantizing (4)  wait for the block's units (bulk copies), turn codes into
 //                     f16 integers c - 8 in the MMA's shared-memory layout and
 //                     the scales into FP32 constants; ask for block i + 2
 //   MMA (1)           S(i) = Q K^T into one of two TMEM tiles, then, when the
 //                     weights of i - 1 are there, O += P(i-1) V
-//   softmax (4)       a thread per row: S(i) from TMEM, scores, weights, P(i)
-//                     back to TMEM as the A operand; at a job's end O
+//   softmax (8)       two threads per row, half of the block's slots (and of
+//                     the output's columns) each: S(i) from TMEM, scores,
+//                     weights, P(i) back to TMEM as the A operand; at a job's
+//                     end O
 // Everything hands over through mbarriers; every wait is bounded, and a CTA
 // whose wait gave up sets the error word and leaves.
 //
@@ -33,8 +35,10 @@ __device__ unsigned int g_kv_chunk_error;
 
 constexpr int kBlk = 128;                  // slots of a block
 constexpr int kUnits = kBlk / kKvTokens;   // units of a block
-constexpr int kCkThreads = 9 * 32;
+constexpr int kSoftWarps = 8, kSoft = 32 * kSoftWarps;  // two threads a row, half the columns each
+constexpr int kCkThreads = kSoft + 5 * 32;              // + four dequantizing warps, one for the MMAs
 constexpr int kTile = kChunkRows;
+constexpr int kChunkCtas = 160;            // bound on the grid (workspace sizing)
 
 // Shared memory, offsets from a 1024-byte boundary.  Operand tiles are 128-byte rows (64 f16 of K) in groups of
 // eight rows, the 16-byte chunks of row r xor-ed with r mod 8 (the 128-byte swizzle).
@@ -49,7 +53,10 @@ struct CkSmem {
     static constexpr int kRaw = kV + 2 * kVBytes;                // 2 x the units of a block
     static constexpr int kPar = kRaw + 2 * kRawBytes;            // 2 x [4][128]: - (z_k - 8), s_k, s_v, z_v - 8
     static constexpr int kMisc = kPar + 2 * 4 * kBlk * 4;        // per buffer: 4 x largest s_v, 4 x slots there; found units
-    static constexpr int kBars = kMisc + 128;
+    static constexpr int kTop = kMisc + 128;                     // 2 x [2 halves][128] largest score of a row's half
+    static constexpr int kSums = kTop + 4 * kTile * 4;           // [2 halves][128] x 2: sum of weights, of zeros' share
+    static constexpr int kQSum = kSums + 4 * kTile * 4;          // [2 halves][128] sums of q
+    static constexpr int kBars = kQSum + 2 * kTile * 4;
     static constexpr int kTotal = kBars + 128;
 };
 
@@ -168,6 +175,43 @@ struct Walk {
     }
 };
 
+// One unit's keys into the operand tile [D/64][128 slots]: a lane half a row, a word a chunk.
+template <int D>
+__device__ __forceinline__ void unpack_keys(const char* raw, char* tile, int u, int lane) {
+    constexpr int N = D / 16;  // words of a lane
+    const int row = lane & 15, half = lane >> 4;
+    char* to = tile + (half * N / 8) * (kBlk * 128) + (u * kKvTokens + row) * 128;
+#pragma unroll
+    for (int i4 = 0; i4 < N / 4; ++i4) {
+        const uint4 w4 = *reinterpret_cast<const uint4*>(raw + row * (D / 2) + half * (D / 4) + 16 * i4);
+        const uint32_t ws[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t w = ws[j], x = w >> 8;
+            *reinterpret_cast<uint4*>(to + ((((half * N + 4 * i4 + j) % 8) ^ (row & 7)) << 4)) =
+                make_uint4(low_f16(w), high_f16(w), low_f16(x), high_f16(x));
+        }
+    }
+}
+
+// Half of a query row's columns into the operand tile [D/64][128 rows], permuted as the keys' words are; their sum.
+template <int D>
+__device__ __forceinline__ float place_query(const uint16_t* src, bool on, char* tile, int row, int half) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+        const int ch = half * (D / 16) + i;
+        const uint4 w = on ? ld_l2_v4(src + half * (D / 2) + 8 * i) : make_uint4(0, 0, 0, 0);
+        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s += h2f_bits(lo16(v[k])) + h2f_bits(hi16(v[k]));
+        *reinterpret_cast<uint4*>(tile + ch / 8 * (kTile * 128) + row * 128 + (((ch % 8) ^ (row & 7)) << 4)) =
+            make_uint4(__byte_perm(w.x, w.z, 0x5410), __byte_perm(w.x, w.z, 0x7632), __byte_perm(w.y, w.w, 0x5410),
+                       __byte_perm(w.y, w.w, 0x7632));
+    }
+    return s;
+}
+
 template <int D>
 __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendArgs a) {
     using S = CkSmem<D>;
@@ -177,16 +221,16 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
     const KvView& c = a.c;
     const uint32_t smem0 = (smem_u32(dyn) + plan_bytes(c.n_seqs) + 1023u) & ~1023u;
     const uint32_t bars = smem0 + S::kBars;
-    if (warp == 8) tm_alloc(smem_u32(&tm_base), kTmCols);
+    if (warp == 12) tm_alloc(smem_u32(&tm_base), kTmCols);
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(bars + 8 * (kRawFull + i), 1);
             mbar_init(bars + 8 * (kKvFull + i), 128);
             mbar_init(bars + 8 * (kKvFree + i), 1);
             mbar_init(bars + 8 * (kSFull + i), 1);
-            mbar_init(bars + 8 * (kPFull + i), 128);
+            mbar_init(bars + 8 * (kPFull + i), kSoft);
         }
-        mbar_init(bars + 8 * kQFull, 128);
+        mbar_init(bars + 8 * kQFull, kSoft);
         fence_mbar_init();
     }
     tm_before_sync();
@@ -201,68 +245,67 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
     const long long u0 = p.runs.start(blockIdx.x);
     const int n = static_cast<int>(p.runs.start(blockIdx.x + 1) - u0);
     const int rows = a.tokens * a.group;
+    // A warp whose wait gave up waits no more but takes every other step of its loop, so that nobody stays behind
+    // at a barrier; the output is not valid then.
+    bool dead = false;
     auto wait = [&](int bar, int parity) {
-        const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * bar, parity & 1));
-        if (!ok && lane == 0) atomicOr(&g_kv_chunk_error, kKvErrWait);
-        return ok;
+        if (dead) return;
+        dead = !__all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * bar, parity & 1));
+        if (dead && lane == 0) atomicOr(&g_kv_chunk_error, kKvErrWait);
     };
     Walk at;
     if (n > 0) at.set(p, c.n_seqs, u0);
 
-    if (n > 0 && warp < 4) {
-        // ---- softmax: row tid of the tile
-        const uint32_t lanes = tm + (static_cast<uint32_t>(32 * warp) << 16);
+    if (n > 0 && warp < kSoftWarps) {
+        // ---- softmax
+        constexpr int H = kBlk / 2;
+        const int trow = 32 * (warp & 3) + lane, half = warp >> 2;
+        const uint32_t lanes = tm + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
+        char* const base = dyn + (smem0 - smem_u32(dyn));
+        auto word = [&](int off) -> float* { return reinterpret_cast<float*>(base + off); };
         float m = kNone, l = 0.f, zs = 0.f, vw = 0.f, qsum = 0.f;
-        int lim = 0, r = 0, first = 0, cuts = 0, jobs_done = 0;
+        int lim = 0, r = 0, cuts = 0;
         bool begins = true;
+        // the thread's half of the row's columns into the operand tile
         auto load_q = [&]() {
             const int h = at.at.job / a.n_rt, rt = at.at.job - h * a.n_rt;
-            r = rt * kTile + tid;
+            r = rt * kTile + trow;
             const int tok = r / a.group;
             const int cnt = a.counts ? min(max(ld_l2(a.counts + at.at.b), 0), a.tokens) : a.tokens;
             const bool on = r < rows && tok < cnt;
             lim = on ? min(max(at.at.len - cnt + tok + 1, 0), at.at.len) : 0;
             const uint16_t* src = a.q + at.at.b * a.qs[0] + tok * a.qs[1] + (h * a.group + r - tok * a.group) * a.qs[2];
-            float s = 0.f;
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                const uint4 w = on ? ld_l2_v4(src + 8 * i) : make_uint4(0, 0, 0, 0);
-                const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) s += h2f_bits(lo16(v[k])) + h2f_bits(hi16(v[k]));
-                sts_v4(smem0 + S::kQ + i / 8 * (kTile * 128) + tid * 128 + (((i % 8) ^ (tid & 7)) << 4),
-                       make_uint4(__byte_perm(w.x, w.z, 0x5410), __byte_perm(w.x, w.z, 0x7632),
-                                  __byte_perm(w.y, w.w, 0x5410), __byte_perm(w.y, w.w, 0x7632)));
-            }
-            qsum = s;
+            word(S::kQSum)[half * kTile + trow] = place_query<D>(src, on, base + S::kQ, trow, half);
             fence_async_smem();
             mbar_arrive(bars + 8 * kQFull);
+            named_bar_sync(2, kSoft);
+            qsum = word(S::kQSum)[trow] + word(S::kQSum)[kTile + trow];
         };
         load_q();
-        first = at.at.step;
+        int first = at.at.step;
         for (int i = 0; i < n; ++i) {
             const int buf = i & 1, step = at.at.step;
-            if (!wait(kSFull + buf, i >> 1)) break;
+            wait(kSFull + buf, i >> 1);
             tm_after_sync();
-            const uint32_t par = smem0 + S::kPar + buf * (4 * kBlk * 4), misc = smem0 + S::kMisc + buf * 64;
-            f2 s[kBlk / 2];
+            const float* par = word(S::kPar + buf * (4 * kBlk * 4)) + half * H;
+            const float* misc = word(S::kMisc + buf * 64);
+            f2 s[H / 2];
             float top = -INFINITY;
-            const int left = lim - step * kBlk;  // slots of the block that the row sees
-            const uint4 there = lds_v4(misc + 16);
-            const bool all = left >= kBlk && (there.x & there.y & there.z & there.w) == 0xffffffffu;
+            const int left = lim - step * kBlk - half * H;  // slots of the half block that the row sees
+            const uint2 there = *reinterpret_cast<const uint2*>(misc + 4 + 2 * half);
+            const bool all = left >= H && (there.x & there.y) == 0xffffffffu;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < 2; ++k) {
                 uint32_t v[32];
-                tm_ld32(lanes + kTmS + buf * kBlk + 32 * k, v);
+                tm_ld32(lanes + kTmS + buf * kBlk + half * H + 32 * k, v);
                 tm_wait_ld();
-                const uint32_t ok = k == 0 ? there.x : (k == 1 ? there.y : (k == 2 ? there.z : there.w));
+                const uint32_t ok = k == 0 ? there.x : there.y;
 #pragma unroll
                 for (int j = 0; j < 32; j += 4) {
-                    const uint4 z = lds_v4(par + 4 * (32 * k + j)), sc = lds_v4(par + 4 * (kBlk + 32 * k + j));
-                    f2 x = fma2(f2(__uint_as_float(z.x), __uint_as_float(z.y)), f2(qsum), f2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]))) *
-                           f2(__uint_as_float(sc.x), __uint_as_float(sc.y));
-                    f2 y = fma2(f2(__uint_as_float(z.z), __uint_as_float(z.w)), f2(qsum), f2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]))) *
-                           f2(__uint_as_float(sc.z), __uint_as_float(sc.w));
+                    const float4 z = *reinterpret_cast<const float4*>(par + 32 * k + j);
+                    const float4 sc = *reinterpret_cast<const float4*>(par + kBlk + 32 * k + j);
+                    f2 x = fma2(f2(z.x, z.y), f2(qsum), f2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]))) * f2(sc.x, sc.y);
+                    f2 y = fma2(f2(z.z, z.w), f2(qsum), f2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]))) * f2(sc.z, sc.w);
                     if (!all) {
                         const int e = 32 * k + j;
                         x = f2(e < left && (ok >> j & 1u) ? x.x() : -INFINITY, e + 1 < left && (ok >> (j + 1) & 1u) ? x.y() : -INFINITY);
@@ -273,15 +316,18 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
                     top = fmaxf(top, fmaxf(fmaxf(x.x(), x.y()), fmaxf(y.x(), y.y())));
                 }
             }
+            float* tops = word(S::kTop) + buf * 2 * kTile;
+            tops[half * kTile + trow] = top;
+            named_bar_sync(2, kSoft);
+            top = fmaxf(top, tops[(half ^ 1) * kTile + trow]);
             // a new maximum or a larger V scale (the same for all rows)
-            const uint4 bg = lds_v4(misc);
-            const float big = fmaxf(fmaxf(__uint_as_float(bg.x), __uint_as_float(bg.y)), fmaxf(__uint_as_float(bg.z), __uint_as_float(bg.w)));
+            const float4 bg = *reinterpret_cast<const float4*>(misc);
+            const float big = fmaxf(fmaxf(bg.x, bg.y), fmaxf(bg.z, bg.w));
             if (begins) {
                 m = kNone;
                 l = zs = 0.f;
                 vw = 2147483648.0f;  // 2^31 brings the smallest FP16 scale, 2^-24, to 2^7
             }
-            bool stop = false;
             if (__any_sync(0xffffffffu, top > m + kLazy || big * vw > 128.f)) {
                 float ratio = 1.f;
                 if (big * vw > 128.f) {
@@ -295,41 +341,40 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
                 l *= f;
                 zs *= fr;
                 if (!begins) {
-                    // O is this warp's alone once the last block's product is in it
-                    stop = !wait(kKvFree + (buf ^ 1), (i - 1) >> 1);
-                    if (stop) break;
+                    // O is the softmax warps' once the last block's product is in it
+                    wait(kKvFree + (buf ^ 1), (i - 1) >> 1);
                     tm_after_sync();
-#pragma unroll
-                    for (int k = 0; k < D / 32; ++k) {
+#pragma unroll 1
+                    for (int k = 0; k < D / 64; ++k) {
                         uint32_t v[32];
-                        tm_ld32(lanes + kTmO + 32 * k, v);
+                        const uint32_t o = lanes + kTmO + half * (D / 2) + 32 * k;
+                        tm_ld32(o, v);
                         tm_wait_ld();
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * fr);
-                        tm_st32(lanes + kTmO + 32 * k, v);
+                        tm_st32(o, v);
                     }
                     tm_wait_st();
                 }
             }
             f2 l2(0.f), z2(0.f);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < 2; ++k) {
                 uint32_t pk[16];
 #pragma unroll
                 for (int j = 0; j < 32; j += 4) {
-                    const uint4 w4 = lds_v4(par + 4 * (2 * kBlk + 32 * k + j)), z4 = lds_v4(par + 4 * (3 * kBlk + 32 * k + j));
+                    const float4 w4 = *reinterpret_cast<const float4*>(par + 2 * kBlk + 32 * k + j);
+                    const float4 z4 = *reinterpret_cast<const float4*>(par + 3 * kBlk + 32 * k + j);
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const f2 d = s[16 * k + j / 2 + e] + f2(-m), x(ex2(d.x()), ex2(d.y()));
-                        const f2 w(__uint_as_float(e ? w4.z : w4.x), __uint_as_float(e ? w4.w : w4.y));
-                        const f2 z(__uint_as_float(e ? z4.z : z4.x), __uint_as_float(e ? z4.w : z4.y));
-                        const f2 pr = x * (w * f2(vw));
+                        const f2 pr = x * (f2(e ? w4.z : w4.x, e ? w4.w : w4.y) * f2(vw));
                         l2 = l2 + x;
-                        z2 = fma2(pr, z, z2);
+                        z2 = fma2(pr, f2(e ? z4.z : z4.x, e ? z4.w : z4.y), z2);
                         pk[j / 2 + e] = pack_f32(pr.x(), pr.y());
                     }
                 }
-                tm_st16(lanes + kTmP + buf * 64 + 16 * k, pk);
+                tm_st16(lanes + kTmP + buf * 64 + half * 32 + 16 * k, pk);
             }
             l += l2.x() + l2.y();
             zs += z2.x() + z2.y();
@@ -342,44 +387,50 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
             const int blocks = at.blocks, row = r;
             const bool last = i + 1 == n, turn = last || at.next(p, c.n_seqs, u0 + i + 1);
             if (!turn) continue;
-            const float inv_w = __uint_as_float(0x7F000000u - __float_as_uint(vw));
+            float* sums = word(S::kSums);
+            sums[half * kTile + trow] = l;
+            sums[(2 + half) * kTile + trow] = zs;
             if (!last) load_q();  // S of the old rows is done; the new ones' can start
-            if (!wait(kKvFree + buf, i >> 1)) break;
+            else named_bar_sync(2, kSoft);
+            const float lsum = sums[trow] + sums[kTile + trow], zsum = sums[2 * kTile + trow] + sums[3 * kTile + trow];
+            const float inv_w = __uint_as_float(0x7F000000u - __float_as_uint(vw));
+            wait(kKvFree + buf, i >> 1);
             tm_after_sync();
             const bool whole = first == 0 && was.step + 1 == blocks;
-            const int h = was.job / a.n_rt, slot = cuts;
-            const size_t pi = (static_cast<size_t>(blockIdx.x) * 2 + slot) * kTile + tid;
-#pragma unroll
-            for (int k = 0; k < D / 32; ++k) {
+            const int h = was.job / a.n_rt;
+            const size_t pi = (static_cast<size_t>(blockIdx.x) * 2 + cuts) * kTile + trow;
+#pragma unroll 1
+            for (int k = 0; k < D / 64; ++k) {
                 uint32_t v[32];
-                tm_ld32(lanes + kTmO + 32 * k, v);
+                const int col = half * (D / 2) + 32 * k;
+                tm_ld32(lanes + kTmO + col, v);
                 tm_wait_ld();
                 if (row < rows) {
                     float o[32];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) o[j] = (__uint_as_float(v[j]) - zs) * inv_w;
+                    for (int j = 0; j < 32; ++j) o[j] = (__uint_as_float(v[j]) - zsum) * inv_w;
                     if (whole) {
-                        store_row(a, was.b, h, row, 32 * k, o, m, l);
+                        store_row(a, was.b, h, row, col, o, m, lsum);
                     } else {
 #pragma unroll
                         for (int j = 0; j < 32; j += 4)
-                            *reinterpret_cast<float4*>(a.part + pi * D + 32 * k + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-                        if (k == 0) *reinterpret_cast<float2*>(a.part_ml + pi * 2) = make_float2(m, l);
+                            *reinterpret_cast<float4*>(a.part + pi * D + col + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                        if (col == 0) *reinterpret_cast<float2*>(a.part_ml + pi * 2) = make_float2(m, lsum);
                     }
                 }
             }
             tm_before_sync();
             if (!whole) ++cuts;
-            ++jobs_done;
             first = at.at.step;
             begins = true;
         }
-    } else if (n > 0 && warp < 8) {
+    } else if (n > 0 && warp < kSoftWarps + 4) {
         // ---- dequantizing
-        const int dw = warp - 4;
+        const int dw = warp - kSoftWarps;
+        char* const base = dyn + (smem0 - smem_u32(dyn));
         bool absent = false;
         Walk ahead = at;
-        auto request = [&](int i) {  // warp 4: the units of the block that `ahead` stands at
+        auto request = [&](int i) {  // its first warp: the units of the block that `ahead` stands at
             const int buf = i & 1, slot = ahead.at.step * kBlk + lane * kKvTokens;
             int index = -1;
             if (lane < kUnits && slot < ahead.at.len) {
@@ -401,55 +452,43 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
         };
         if (dw == 0)
             for (int i = 0; i < min(2, n); ++i) request(i);
-        int i = 0;
-        for (; i < n; ++i) {
+        int asked = min(2, n);
+        for (int i = 0; i < n; ++i) {
             const int buf = i & 1;
-            if (!wait(kRawFull + buf, i >> 1)) break;
-            if (i >= 2 && !wait(kKvFree + buf, (i - 2) >> 1)) break;
+            wait(kRawFull + buf, i >> 1);
+            if (i >= 2) wait(kKvFree + buf, (i - 2) >> 1);
             const uint32_t got = lds_u32(smem0 + S::kMisc + 48 + buf * 64);
-            const uint32_t kb = smem0 + S::kK + buf * S::kOp, vb = smem0 + S::kV + buf * S::kVBytes;
-#pragma unroll
+            // V: a lane four column quads of a slot pair at a time; which quad (g1) and which two columns (g2)
+            // come first differs among the lanes of a pair, so that the 32 words of a store lie in 32 banks.
+            const int pr = lane >> 2, g = lane & 3, g1 = g & 1, g2 = g & 2;
+#pragma unroll 1
             for (int e = 0; e < 2; ++e) {
                 const int u = 2 * dw + e;
-                const uint32_t raw = smem0 + S::kRaw + buf * S::kRawBytes + u * kv_unit_bytes(D);
-                {
-                    // K: a lane half a row, a word a chunk
-                    const int row = lane & 15, half = lane >> 4, key = u * kKvTokens + row;
-                    constexpr int N = D / 16;  // words of a lane
+                const char* raw = base + S::kRaw + buf * S::kRawBytes + u * kv_unit_bytes(D);
+                unpack_keys<D>(raw, base + S::kK + buf * S::kOp, u, lane);
+                const int key = u * kKvTokens + 2 * pr, byte = 2 * (key % 64);  // the pair's first slot
+                char* vt = base + S::kV + buf * S::kVBytes + key / 64 * (D * 128) + 512 * 4 * g;
+                char* even[4];  // columns of quads g1, 2 + g1: in the order of their stores
+                char* odd[4];   // of quads 1 - g1, 3 - g1
 #pragma unroll
-                    for (int i4 = 0; i4 < N / 4; ++i4) {
-                        const uint4 w4 = lds_v4(raw + row * (D / 2) + half * (D / 4) + 16 * i4);
-                        const uint32_t ws[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint32_t w = ws[j], x = w >> 8;
-                            const int ch = half * N + 4 * i4 + j;
-                            sts_v4(kb + ch / 8 * (kBlk * 128) + key * 128 + (((ch % 8) ^ (key & 7)) << 4),
-                                   make_uint4(low_f16(w), high_f16(w), low_f16(x), high_f16(x)));
-                        }
-                    }
+                for (int j = 0; j < 4; ++j) {
+                    const int col = j ^ g2;
+                    even[j] = vt + 512 * g1 + 128 * col + (byte ^ ((4 * g1 + col) << 4));
+                    odd[j] = vt + 512 * (g1 ^ 1) + 128 * col + (byte ^ ((4 * (g1 ^ 1) + col) << 4));
                 }
-                {
-                    // V: a lane four column quads of a slot pair; which quad and column it stores when differs
-                    // among the lanes of a pair, so that a store's 32 words lie in 32 banks
-                    const int pr = lane >> 2, g = lane & 3;
-                    const int key = u * kKvTokens + 2 * pr;  // the pair's first slot
-                    const uint32_t dst = vb + key / 64 * (D * 128), byte = 2 * (key % 64);
 #pragma unroll
-                    for (int i4 = 0; i4 < D / 64; ++i4) {
-                        const int q0 = 4 * (4 * i4 + g);
-                        const uint4 w4 = lds_v4(raw + kv_v_offset(D) + pr * D + 4 * q0);
-                        const uint32_t ws[4] = {g & 1 ? w4.y : w4.x, g & 1 ? w4.x : w4.y, g & 1 ? w4.w : w4.z, g & 1 ? w4.z : w4.w};
+                for (int i4 = 0; i4 < D / 64; ++i4) {
+                    const uint4 w4 = *reinterpret_cast<const uint4*>(raw + kv_v_offset(D) + pr * D + 64 * i4 + 16 * g);
+                    const uint32_t ws[4] = {g1 ? w4.y : w4.x, g1 ? w4.x : w4.y, g1 ? w4.w : w4.z, g1 ? w4.z : w4.w};
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const uint32_t w = ws[k], x = w >> 8;
-                            const uint32_t h[4] = {low_f16(w), high_f16(w), low_f16(x), high_f16(x)};
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const int d = 4 * (q0 + (k ^ (g & 1))) + (j ^ (g & 2));
-                                sts_u32(dst + d * 128 + (byte ^ ((d & 7) << 4)), g & 2 ? h[j ^ 2] : h[j]);
-                            }
-                        }
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t w = ws[k] >> (g2 * 4), x = ws[k] >> (8 - g2 * 4);
+                        char* const* to = k & 1 ? odd : even;
+                        const int at4 = 512 * 16 * i4 + 1024 * (k >> 1);
+                        *reinterpret_cast<uint32_t*>(to[0] + at4) = low_f16(w);
+                        *reinterpret_cast<uint32_t*>(to[1] + at4) = high_f16(w);
+                        *reinterpret_cast<uint32_t*>(to[2] + at4) = low_f16(x);
+                        *reinterpret_cast<uint32_t*>(to[3] + at4) = high_f16(x);
                     }
                 }
             }
@@ -476,11 +515,14 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
             fence_async_smem();
             mbar_arrive(bars + 8 * (kKvFull + buf));
             named_bar_sync(1, 128);  // all four warps have read the units
-            if (dw == 0 && i + 2 < n) request(i + 2);
+            if (dw == 0 && i + 2 < n && !dead) {
+                request(i + 2);
+                asked = i + 3;
+            }
             if (i + 1 < n) at.next(p, c.n_seqs, u0 + i + 1);
         }
-        if (i < n && dw == 0)  // gave up: the copies in flight must end before the shared memory goes
-            for (int j = i; j < min(i + 2, n); ++j) mbar_wait_bounded(bars + 8 * (kRawFull + (j & 1)), (j >> 1) & 1);
+        if (dead && dw == 0)  // the copies in flight must end before the shared memory goes
+            for (int j = max(asked - 2, 0); j < asked; ++j) mbar_wait_bounded(bars + 8 * (kRawFull + (j & 1)), (j >> 1) & 1);
         if (absent) atomicOr(&g_kv_chunk_error, kKvErrPage);
     } else if (n > 0) {
         // ---- MMA
@@ -488,7 +530,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
         bool begins = true, begins_before = true;
         auto output = [&](int i, bool start) {
             const int buf = i & 1;
-            if (!wait(kPFull + buf, i >> 1)) return false;
+            wait(kPFull + buf, i >> 1);
             tm_after_sync();
             if (lane == 0) {
                 const uint32_t vb = smem0 + S::kV + buf * S::kVBytes;
@@ -499,13 +541,11 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
                 tm_commit(bars + 8 * (kKvFree + buf));
             }
             __syncwarp();
-            return true;
         };
-        bool ok = true;
-        for (int i = 0; i < n && ok; ++i) {
+        for (int i = 0; i < n; ++i) {
             const int buf = i & 1;
-            if (begins && !(ok = wait(kQFull, jobs))) break;
-            if (!(ok = wait(kKvFull + buf, i >> 1))) break;
+            if (begins) wait(kQFull, jobs);
+            wait(kKvFull + buf, i >> 1);
             tm_after_sync();
             if (lane == 0) {
                 const uint32_t kb = smem0 + S::kK + buf * S::kOp;
@@ -516,13 +556,13 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
                 tm_commit(bars + 8 * (kSFull + buf));
             }
             __syncwarp();
-            if (i > 0) ok = output(i - 1, begins_before);
+            if (i > 0) output(i - 1, begins_before);
             begins_before = begins;
             if (begins) ++jobs;
             begins = i + 1 < n && at.next(p, c.n_seqs, u0 + i + 1);
         }
-        if (ok) ok = output(n - 1, begins_before);
-        if (ok) wait(kKvFree + ((n - 1) & 1), (n - 1) >> 1);
+        output(n - 1, begins_before);
+        wait(kKvFree + ((n - 1) & 1), (n - 1) >> 1);
     }
     // rows of sequences without slots
     for (int b = blockIdx.x; b < c.n_seqs; b += gridDim.x) {
@@ -536,7 +576,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
     }
     tm_before_sync();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 12) {
         tm_after_sync();
         tm_dealloc(tm, kTmCols);
     }
@@ -562,30 +602,292 @@ __global__ void __launch_bounds__(32 * kCcWarps) kv_chunk_combine_kernel(const K
     if (s.n > 1) join_row<D, kTile / 8>(a, s, b, h, rt, r);  // else finished by its CTA, or empty
 }
 
+// ---------------------------------------------------------------------------
+// Accumulated weight for many rows: the keys once more, transposed.  S^T = K Q^T
+// has a slot a TMEM lane, so a thread adds its slot's weights over the tile's
+// rows (half of them each for two threads) by itself, with the rows' sums of q
+// and lse from shared memory.  Each row tile's sums go to their own line of the
+// workspace; kv_tile_mass_kernel adds them to mass in tile order.
+// ---------------------------------------------------------------------------
 template <int D>
-dq_status_t chunk(const KvAttendArgs& a, cudaStream_t stream) {
+struct CmSmem {
+    static constexpr int kOp = D / 64 * kTile * 128;
+    static constexpr int kQ = 0;
+    static constexpr int kK = kOp;                               // 2 x
+    static constexpr int kRawUnit = 8 * D + kKvTokens * 8;       // keys and parameters of a unit
+    static constexpr int kRaw = kK + 2 * kOp;                    // 2 x
+    static constexpr int kPar = kRaw + 2 * kUnits * kRawUnit;    // 2 x [2][128]: - (z_k - 8), s_k
+    static constexpr int kRow = kPar + 4 * kBlk * 4;             // [4][128]: sum of q (two halves), - lse, keys seen
+    static constexpr int kSum = kRow + 4 * kTile * 4;            // 2 x [128]: the other half's sums
+    static constexpr int kMisc = kSum + 2 * kBlk * 4;            // per buffer: 4 x slots there; found units
+    static constexpr int kBars = kMisc + 128;
+    static constexpr int kTotal = kBars + 128;
+};
+
+template <int D>
+__global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAttendArgs a, float* sums, const long long lines) {
+    using S = CmSmem<D>;
+    extern __shared__ char dyn[];
+    __shared__ uint32_t tm_base;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const KvView& c = a.c;
+    const uint32_t smem0 = (smem_u32(dyn) + plan_bytes(c.n_seqs) + 1023u) & ~1023u;
+    const uint32_t bars = smem0 + S::kBars;
+    char* const base = dyn + (smem0 - smem_u32(dyn));
+    auto word = [&](int off) -> float* { return reinterpret_cast<float*>(base + off); };
+    if (warp == 12) tm_alloc(smem_u32(&tm_base), 256);
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bars + 8 * (kRawFull + i), 1);
+            mbar_init(bars + 8 * (kKvFull + i), 128);
+            mbar_init(bars + 8 * (kSFull + i), 1);
+            mbar_init(bars + 8 * (kPFull + i), kSoft);  // S and the parameters have been read
+        }
+        mbar_init(bars + 8 * kQFull, kSoft);
+        fence_mbar_init();
+    }
+    tm_before_sync();
+    __syncthreads();
+    tm_after_sync();
+    const uint32_t tm = tm_base;
+    pdl_launch_dependents();
+    pdl_wait();
+    const Plan p = make_plan<kCkThreads, kBlk>(c, a.jobs, gridDim.x, dyn, nullptr);
+    const long long u0 = p.runs.start(blockIdx.x);
+    const int n = static_cast<int>(p.runs.start(blockIdx.x + 1) - u0);
+    const int rows = a.tokens * a.group;
+    bool dead = false;
+    auto wait = [&](int bar, int parity) {
+        if (dead) return;
+        dead = !__all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * bar, parity & 1));
+        if (dead && lane == 0) atomicOr(&g_kv_chunk_error, kKvErrWait);
+    };
+    Walk at;
+    if (n > 0) at.set(p, c.n_seqs, u0);
+
+    if (n > 0 && warp < kSoftWarps) {
+        const int trow = 32 * (warp & 3) + lane, half = warp >> 2;
+        const uint32_t lanes = tm + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
+        int least = 0;  // keys that every row of the tile sees
+        auto load_q = [&]() {
+            const int h = at.at.job / a.n_rt, rt = at.at.job - h * a.n_rt;
+            const int r = rt * kTile + trow, tok = r / a.group;
+            const int cnt = a.counts ? min(max(ld_l2(a.counts + at.at.b), 0), a.tokens) : a.tokens;
+            const bool on = r < rows && tok < cnt;
+            const int head = h * a.group + r - tok * a.group;
+            const uint16_t* src = a.q + at.at.b * a.qs[0] + tok * a.qs[1] + head * a.qs[2];
+            word(S::kRow)[half * kTile + trow] = place_query<D>(src, on, base + S::kQ, trow, half);
+            if (half == 0) {
+                // rows that are padding or see no key weigh nothing
+                float nl = -INFINITY;
+                int lim = 0;
+                if (on) {
+                    const float x = ld_l2(a.lse2 + (static_cast<size_t>(at.at.b) * a.tokens + tok) * (c.heads * a.group) + head);
+                    lim = min(max(at.at.len - cnt + tok + 1, 0), at.at.len);
+                    if (x != -INFINITY) nl = -x;
+                }
+                word(S::kRow)[2 * kTile + trow] = nl;
+                reinterpret_cast<int*>(word(S::kRow))[3 * kTile + trow] = on ? lim : at.at.len;
+            }
+            fence_async_smem();
+            mbar_arrive(bars + 8 * kQFull);
+            named_bar_sync(2, kSoft);
+            if (half == 0) word(S::kRow)[trow] += word(S::kRow)[kTile + trow];
+            int lim = reinterpret_cast<const int*>(word(S::kRow))[3 * kTile + trow];
+            lim = __reduce_min_sync(0xffffffffu, lim);
+            if (half == 0 && lane == 0) reinterpret_cast<int*>(word(S::kMisc))[24 + (warp & 3)] = lim;
+            named_bar_sync(2, kSoft);
+            const int4 l4 = *reinterpret_cast<const int4*>(word(S::kMisc) + 24);
+            least = min(min(l4.x, l4.y), min(l4.z, l4.w));
+        };
+        load_q();
+        for (int i = 0; i < n; ++i) {
+            const int buf = i & 1, slot = at.at.step * kBlk + trow;
+            wait(kSFull + buf, i >> 1);
+            tm_after_sync();
+            const float nz = word(S::kPar + buf * (2 * kBlk * 4))[trow], sk = word(S::kPar + buf * (2 * kBlk * 4))[kBlk + trow];
+            const bool there = reinterpret_cast<const uint32_t*>(word(S::kMisc + buf * 32))[warp & 3] >> lane & 1u;
+            const bool all = (at.at.step + 1) * kBlk <= least;
+            const float* row = word(S::kRow) + half * (kTile / 2);
+            f2 add(0.f);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                uint32_t v[32];
+                tm_ld32(lanes + buf * kTile + half * (kTile / 2) + 32 * k, v);
+                tm_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) {
+                    const float4 qs = *reinterpret_cast<const float4*>(row + 32 * k + j);
+                    const float4 nl = *reinterpret_cast<const float4*>(row + 2 * kTile + 32 * k + j);
+                    f2 x = fma2(fma2(f2(nz), f2(qs.x, qs.y), f2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]))), f2(sk), f2(nl.x, nl.y));
+                    f2 y = fma2(fma2(f2(nz), f2(qs.z, qs.w), f2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]))), f2(sk), f2(nl.z, nl.w));
+                    if (!all) {
+                        const int4 lim = *reinterpret_cast<const int4*>(row + 3 * kTile + 32 * k + j);
+                        x = f2(slot < lim.x ? x.x() : -INFINITY, slot < lim.y ? x.y() : -INFINITY);
+                        y = f2(slot < lim.z ? y.x() : -INFINITY, slot < lim.w ? y.y() : -INFINITY);
+                    }
+                    add = add + f2(ex2(x.x()), ex2(x.y()));
+                    add = add + f2(ex2(y.x()), ex2(y.y()));
+                }
+            }
+            const float sum = add.x() + add.y();
+            float* other = word(S::kSum) + buf * kBlk;
+            if (half == 1) other[trow] = sum;
+            tm_before_sync();
+            named_bar_sync(2, kSoft);
+            if (half == 0 && there) {
+                const int h = at.at.job / a.n_rt, rt = at.at.job - h * a.n_rt, page = kv_page(c, at.at.b, slot);
+                if (page >= 0) sums[rt * lines + static_cast<long long>(kv_line(c, page, h) + slot % c.page_size)] = sum + other[trow];
+            }
+            mbar_arrive(bars + 8 * (kPFull + buf));
+            if (i + 1 < n && at.next(p, c.n_seqs, u0 + i + 1)) load_q();  // S of the old rows is done
+        }
+    } else if (n > 0 && warp < kSoftWarps + 4) {
+        const int dw = warp - kSoftWarps;
+        Walk ahead = at;
+        auto request = [&](int i) {
+            const int buf = i & 1, slot = ahead.at.step * kBlk + lane * kKvTokens;
+            int index = -1;
+            if (lane < kUnits && slot < ahead.at.len) {
+                const int page = kv_page(c, ahead.at.b, slot);
+                if (page >= 0) index = static_cast<int>((kv_line(c, page, ahead.at.job / a.n_rt) + slot % c.page_size) / kKvTokens);
+            }
+            const uint32_t got = __ballot_sync(0xffffffffu, index >= 0), bar = bars + 8 * (kRawFull + buf);
+            if (lane == 0) {
+                sts_u32(smem0 + S::kMisc + 64 + buf * 4, got);
+                if (got) mbar_arrive_expect_tx(bar, __popc(got) * S::kRawUnit);
+                else mbar_arrive(bar);
+            }
+            __syncwarp();
+            if (index >= 0) {
+                const uint32_t dst = smem0 + S::kRaw + (buf * kUnits + lane) * S::kRawUnit;
+                const uint8_t* src = c.units + static_cast<size_t>(index) * kv_unit_bytes(D);
+                bulk_g2s(dst, src, 8 * D, bar);
+                bulk_g2s(dst + 8 * D, src + kv_param_offset(D), kKvTokens * 8, bar);
+            }
+            ahead.next(p, c.n_seqs, u0 + i + 1 < u0 + n ? u0 + i + 1 : u0 + n - 1);
+        };
+        if (dw == 0)
+            for (int i = 0; i < min(2, n); ++i) request(i);
+        int asked = min(2, n);
+        for (int i = 0; i < n; ++i) {
+            const int buf = i & 1;
+            wait(kRawFull + buf, i >> 1);
+            if (i >= 2) wait(kPFull + buf, (i - 2) >> 1);
+            const uint32_t got = reinterpret_cast<const uint32_t*>(word(S::kMisc))[16 + buf];
+            const char* raw = base + S::kRaw + buf * kUnits * S::kRawUnit;
+#pragma unroll 1
+            for (int e = 0; e < 2; ++e) unpack_keys<D>(raw + (2 * dw + e) * S::kRawUnit, base + S::kK + buf * S::kOp, 2 * dw + e, lane);
+            const int u = 2 * dw + (lane >> 4), slot = 32 * dw + lane;
+            const bool on = (got >> u & 1u) && at.at.step * kBlk + slot < at.at.len;
+            const uint32_t pw = *reinterpret_cast<const uint32_t*>(raw + u * S::kRawUnit + 8 * D + 8 * (lane & 15));
+            float* par = word(S::kPar + buf * (2 * kBlk * 4));
+            par[slot] = on ? 8.f - h2f_bits(hi16(pw)) : 0.f;
+            par[kBlk + slot] = on ? h2f_bits(lo16(pw)) * a.scale2 : 0.f;
+            const uint32_t there = __ballot_sync(0xffffffffu, on);
+            if (lane == 0) reinterpret_cast<uint32_t*>(word(S::kMisc + buf * 32))[dw] = there;
+            fence_async_smem();
+            mbar_arrive(bars + 8 * (kKvFull + buf));
+            named_bar_sync(1, 128);  // all four warps have read the units
+            if (dw == 0 && i + 2 < n && !dead) {
+                request(i + 2);
+                asked = i + 3;
+            }
+            if (i + 1 < n) at.next(p, c.n_seqs, u0 + i + 1);
+        }
+        if (dead && dw == 0)  // the copies in flight must end before the shared memory goes
+            for (int j = max(asked - 2, 0); j < asked; ++j) mbar_wait_bounded(bars + 8 * (kRawFull + (j & 1)), (j >> 1) & 1);
+    } else if (n > 0) {
+        int jobs = 0;
+        bool begins = true;
+        for (int i = 0; i < n; ++i) {
+            const int buf = i & 1;
+            if (begins) wait(kQFull, jobs++);
+            wait(kKvFull + buf, i >> 1);
+            if (i >= 2) wait(kPFull + buf, (i - 2) >> 1);
+            tm_after_sync();
+            if (lane == 0) {
+                const uint32_t kb = smem0 + S::kK + buf * S::kOp;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+                    tm_mma_ss(tm + buf * kTile, operand(kb + k / 4 * (kBlk * 128) + 32 * (k % 4)),
+                              operand(smem0 + S::kQ + k / 4 * (kTile * 128) + 32 * (k % 4)), mma_shape(kTile), k > 0);
+                tm_commit(bars + 8 * (kSFull + buf));
+            }
+            __syncwarp();
+            begins = i + 1 < n && at.next(p, c.n_seqs, u0 + i + 1);
+        }
+        wait(kSFull + ((n - 1) & 1), (n - 1) >> 1);
+    }
+    tm_before_sync();
+    __syncthreads();
+    if (warp == 12) {
+        tm_after_sync();
+        tm_dealloc(tm, 256);
+    }
+}
+
+constexpr int kTmWarps = 8;
+
+__global__ void __launch_bounds__(32 * kTmWarps) kv_tile_mass_kernel(const KvAttendArgs a, const float* sums, const long long lines) {
+    extern __shared__ char dyn[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_rt = a.n_rt;
+    const KvView& c = a.c;
+    pdl_launch_dependents();
+    pdl_wait();
+    const Plan p = make_plan<32 * kTmWarps>(c, a.jobs, gridDim.x * kTmWarps, dyn, nullptr);
+    const long long w = static_cast<long long>(blockIdx.x) * kTmWarps + warp, u0 = p.runs.start(w);
+    const int n = static_cast<int>(p.runs.start(w + 1) - u0);
+    if (n == 0) return;
+    StepAt at = step_at(p, c.n_seqs, u0);
+    for (int i = 0; i < n; ++i) {
+        const int slot = at.step * kStep + lane, page = slot < at.len ? kv_page(c, at.b, slot) : -1;
+        if (page >= 0) {
+            const long long line = static_cast<long long>(kv_line(c, page, at.job) + slot % c.page_size);
+            float add = 0.f;
+#pragma unroll 4
+            for (int rt = 0; rt < n_rt; ++rt) add += ld_l2(sums + rt * lines + line);
+            c.mass[line] = ld_l2(c.mass + line) + add;
+        }
+        if (++at.step == steps_of(at.len) && i + 1 < n) at = step_at(p, c.n_seqs, u0 + i + 1);
+    }
+}
+
+template <int D>
+dq_status_t chunk(KvAttendArgs a, float* sums, cudaStream_t stream) {
     DeviceInfo di;
     dq_status_t st = device_info(&di);
     if (st != DQ_OK) return st;
-    const int ctas = di.sm_count < 160 ? di.sm_count : 160;
-    const int smem = plan_bytes(a.c.n_seqs) + 1024 + CkSmem<D>::kTotal;
-    const cudaError_t e = cudaFuncSetAttribute(kv_chunk_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) { set_cuda_error(e); return DQ_ERR_CUDA; }
+    const int ctas = di.sm_count < kChunkCtas ? di.sm_count : kChunkCtas, plan = plan_bytes(a.c.n_seqs);
+    auto allow = [&](auto kernel, int smem) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) set_cuda_error(e);
+        return e == cudaSuccess ? DQ_OK : DQ_ERR_CUDA;
+    };
+    int smem = plan + 1024 + CkSmem<D>::kTotal;
+    if ((st = allow(kv_chunk_kernel<D>, smem)) != DQ_OK) return st;
     if ((st = launch_pdl(kv_chunk_kernel<D>, dim3(ctas), kCkThreads, smem, stream, 1, a)) != DQ_OK) return st;
     const long long items = static_cast<long long>(a.c.n_seqs) * a.tokens * a.c.heads * a.group;
-    return launch_pdl(kv_chunk_combine_kernel<D>, dim3(static_cast<unsigned>((items + kCcWarps - 1) / kCcWarps)), 32 * kCcWarps, 0,
-                      stream, 1, a, ctas);
+    st = launch_pdl(kv_chunk_combine_kernel<D>, dim3(static_cast<unsigned>((items + kCcWarps - 1) / kCcWarps)), 32 * kCcWarps, 0,
+                    stream, 1, a, ctas);
+    if (st != DQ_OK || !sums) return st;
+    const long long lines = static_cast<long long>(a.c.n_pages) * a.c.heads * a.c.page_size;
+    smem = plan + 1024 + CmSmem<D>::kTotal;
+    if ((st = allow(kv_chunk_mass_kernel<D>, smem)) != DQ_OK) return st;
+    if ((st = launch_pdl(kv_chunk_mass_kernel<D>, dim3(ctas), kCkThreads, smem, stream, 1, a, sums, lines)) != DQ_OK) return st;
+    a.jobs = Div(a.c.heads);
+    return launch_pdl(kv_tile_mass_kernel, dim3(di.sm_count * 4), 32 * kTmWarps, plan, stream, 1, a, sums, lines);
 }
 
 }  // namespace
 
-size_t kv_chunk_part_rows() { return size_t{160} * 2 * kTile; }
+size_t kv_chunk_part_rows() { return static_cast<size_t>(kChunkCtas) * 2 * kTile; }
 
-dq_status_t launch_kv_chunk(KvAttendArgs a, int head_dim, cudaStream_t stream) {
+dq_status_t launch_kv_chunk(KvAttendArgs a, int head_dim, float* sums, cudaStream_t stream) {
     const int rows = a.tokens * a.group;
     a.n_rt = Div((rows + kTile - 1) / kTile);
     a.jobs = Div(a.c.heads * a.n_rt);
-    return head_dim == 128 ? chunk<128>(a, stream) : chunk<64>(a, stream);
+    return head_dim == 128 ? chunk<128>(a, sums, stream) : chunk<64>(a, sums, stream);
 }
 
 dq_status_t read_kv_chunk_error(uint32_t* word, bool clear) {
