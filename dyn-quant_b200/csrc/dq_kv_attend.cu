@@ -1086,8 +1086,10 @@ dq_status_t attend(KvAttendArgs& a, cudaStream_t stream) {
     return weights<D>(a, di.sm_count, stream);
 }
 
-// Query rows of a KV head from which the tensor-memory kernel of dq_kv_chunk.cu takes the call.
-constexpr int kChunkMin = 64;
+// Query rows of a KV head from which the tensor-memory kernel of dq_kv_chunk.cu takes the call.  It costs about the
+// same for 1 to 128 rows, this file's kernels cost more for every 16: 32 KV heads with 8000 slots each take
+// 55 us (48 rows), 65 us (63) here and 58 us there with heads of 128; 45 us (63) here and 50 us there with 64.
+constexpr int chunk_min(int head_dim) { return head_dim == 128 ? 64 : 80; }
 
 // Row tiles of one warp: 8 rows when a KV head has no more, else 16.
 int row_tiles(int rows) { return rows <= 8 ? 1 : 2; }
@@ -1103,7 +1105,7 @@ struct AttendWs {
 };
 AttendWs attend_ws(const dq_kv_cache_t& c, int tokens, int q_heads, bool mass) {
     const int nt = row_tiles(tokens * (q_heads / c.kv_heads));
-    const bool chunk = tokens * (q_heads / c.kv_heads) >= kChunkMin;
+    const bool chunk = tokens * (q_heads / c.kv_heads) >= chunk_min(c.head_dim);
     const size_t rows = chunk ? kv_chunk_part_rows() : static_cast<size_t>(kAtMaxWarps / at_warps(nt)) * 2 * 8 * nt;
     AttendWs w;
     w.part = 0;
@@ -1147,7 +1149,7 @@ dq_status_t launch_kv_attend(const dq_kv_cache_t& c, const dq_kv_attend_t& r, vo
     a.scores = w.total > w.scores ? reinterpret_cast<float*>(base + w.scores) : nullptr;
     const int rows = r.tokens * a.group, nt = row_tiles(rows);
     a.pitch = score_pitch(rows);
-    if (rows >= kChunkMin) {
+    if (rows >= chunk_min(c.head_dim)) {
         KvAttendArgs b = a;
         b.scale2 = r.scale * 1.44269504088896341f;  // its codes are whole numbers
         const dq_status_t st = launch_kv_chunk(b, c.head_dim, a.scores, stream);

@@ -10,7 +10,9 @@
 // Roles of a CTA's thirteen warps, over the blocks i of its run:
 //   dequantizing (4)  wait for the block's units (bulk copies), turn codes into
 //                     f16 integers c - 8 in the MMA's shared-memory layout and
-//                     the scales into FP32 constants; ask for block i + 2
+//                     the scales into FP32 constants; ask for block i + 2.
+//                     K's tile is free again when S(i) is there, V's only
+//                     after the block's softmax, so they are filled apart
 //   MMA (1)           S(i) = Q K^T into one of two TMEM tiles, then, when the
 //                     weights of i - 1 are there, O += P(i-1) V
 //   softmax (8)       two threads per row, half of the block's slots (and of
@@ -51,17 +53,19 @@ struct CkSmem {
     static constexpr int kV = kK + 2 * kOp;                      // 2 x [2][D columns], 64 slots a row
     static constexpr int kRawBytes = kUnits * kv_unit_bytes(D);
     static constexpr int kRaw = kV + 2 * kVBytes;                // 2 x the units of a block
-    static constexpr int kPar = kRaw + 2 * kRawBytes;            // 2 x [4][128]: - (z_k - 8), s_k, s_v, z_v - 8
-    static constexpr int kMisc = kPar + 2 * 4 * kBlk * 4;        // per buffer: 4 x largest s_v, 4 x slots there; found units
-    static constexpr int kTop = kMisc + 128;                     // 2 x [2 halves][128] largest score of a row's half
+    static constexpr int kPar = kRaw + 2 * kRawBytes;            // 4 x [4][128]: - (z_k - 8), s_k, s_v, z_v - 8
+    static constexpr int kMisc = kPar + 4 * 4 * kBlk * 4;        // 4 x (4 x largest s_v, 4 x slots there)
+    static constexpr int kGot = kMisc + 128;                     // 2 x found units
+    static constexpr int kTop = kGot + 128;                      // 2 x [2 halves][128] largest score of a row's half
     static constexpr int kSums = kTop + 4 * kTile * 4;           // [2 halves][128] x 2: sum of weights, of zeros' share
     static constexpr int kQSum = kSums + 4 * kTile * 4;          // [2 halves][128] sums of q
     static constexpr int kBars = kQSum + 2 * kTile * 4;
     static constexpr int kTotal = kBars + 128;
 };
 
-// Barriers (8 bytes each).
-enum { kRawFull = 0, kKvFull = 2, kKvFree = 4, kSFull = 6, kPFull = 8, kQFull = 10, kBarCount = 11 };
+// Barriers (8 bytes each).  Each but the last is a pair, one for the even and one for the odd blocks.  S full also
+// says that K has been read, V free that the block's product is in O.
+enum { kRawFull = 0, kKFull = 2, kVFull = 4, kVFree = 6, kSFull = 8, kPFull = 10, kQFull = 12 };
 
 // Tensor memory columns: two S tiles, O, two P tiles (f16 pairs).
 constexpr uint32_t kTmS = 0, kTmO = 256, kTmP = 384, kTmCols = 512;
@@ -225,8 +229,9 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(bars + 8 * (kRawFull + i), 1);
-            mbar_init(bars + 8 * (kKvFull + i), 128);
-            mbar_init(bars + 8 * (kKvFree + i), 1);
+            mbar_init(bars + 8 * (kKFull + i), 128);
+            mbar_init(bars + 8 * (kVFull + i), 128);
+            mbar_init(bars + 8 * (kVFree + i), 1);
             mbar_init(bars + 8 * (kSFull + i), 1);
             mbar_init(bars + 8 * (kPFull + i), kSoft);
         }
@@ -287,8 +292,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
             const int buf = i & 1, step = at.at.step;
             wait(kSFull + buf, i >> 1);
             tm_after_sync();
-            const float* par = word(S::kPar + buf * (4 * kBlk * 4)) + half * H;
-            const float* misc = word(S::kMisc + buf * 64);
+            const float* par = word(S::kPar + (i & 3) * (4 * kBlk * 4)) + half * H;
+            const float* misc = word(S::kMisc + (i & 3) * 32);
             f2 s[H / 2];
             float top = -INFINITY;
             const int left = lim - step * kBlk - half * H;  // slots of the half block that the row sees
@@ -342,7 +347,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
                 zs *= fr;
                 if (!begins) {
                     // O is the softmax warps' once the last block's product is in it
-                    wait(kKvFree + (buf ^ 1), (i - 1) >> 1);
+                    wait(kVFree + (buf ^ 1), (i - 1) >> 1);
                     tm_after_sync();
 #pragma unroll 1
                     for (int k = 0; k < D / 64; ++k) {
@@ -394,7 +399,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
             else named_bar_sync(2, kSoft);
             const float lsum = sums[trow] + sums[kTile + trow], zsum = sums[2 * kTile + trow] + sums[3 * kTile + trow];
             const float inv_w = __uint_as_float(0x7F000000u - __float_as_uint(vw));
-            wait(kKvFree + buf, i >> 1);
+            wait(kVFree + buf, i >> 1);
             tm_after_sync();
             const bool whole = first == 0 && was.step + 1 == blocks;
             const int h = was.job / a.n_rt;
@@ -440,7 +445,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
             }
             const uint32_t got = __ballot_sync(0xffffffffu, index >= 0), bar = bars + 8 * (kRawFull + buf);
             if (lane == 0) {
-                sts_u32(smem0 + S::kMisc + 48 + buf * 64, got);
+                sts_u32(smem0 + S::kGot + buf * 4, got);
                 if (got) mbar_arrive_expect_tx(bar, __popc(got) * kv_unit_bytes(D));
                 else mbar_arrive(bar);
             }
@@ -456,16 +461,41 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
         for (int i = 0; i < n; ++i) {
             const int buf = i & 1;
             wait(kRawFull + buf, i >> 1);
-            if (i >= 2) wait(kKvFree + buf, (i - 2) >> 1);
-            const uint32_t got = lds_u32(smem0 + S::kMisc + 48 + buf * 64);
+            if (i >= 2) wait(kSFull + buf, (i - 2) >> 1);
+            const uint32_t got = lds_u32(smem0 + S::kGot + buf * 4);
+            const char* raws = base + S::kRaw + buf * S::kRawBytes;
+#pragma unroll 1
+            for (int e = 0; e < 2; ++e) unpack_keys<D>(raws + (2 * dw + e) * kv_unit_bytes(D), base + S::kK + buf * S::kOp, 2 * dw + e, lane);
+            {
+                // scales and zeros, a lane a slot
+                const int u = 2 * dw + (lane >> 4), slot = 32 * dw + lane;
+                const bool on = (got >> u & 1u) && at.at.step * kBlk + slot < at.at.len;
+                const uint2 pw = lds_v2(smem0 + S::kRaw + buf * S::kRawBytes + u * kv_unit_bytes(D) + kv_param_offset(D) + 8 * (lane & 15));
+                const float sv = on ? h2f_bits(lo16(pw.y)) : 0.f;
+                const uint32_t par = smem0 + S::kPar + (i & 3) * (4 * kBlk * 4) + 4 * slot, misc = smem0 + S::kMisc + (i & 3) * 32;
+                sts_u32(par, __float_as_uint(on ? 8.f - h2f_bits(hi16(pw.x)) : 0.f));
+                sts_u32(par + 4 * kBlk, __float_as_uint(on ? h2f_bits(lo16(pw.x)) * a.scale2 : 0.f));
+                sts_u32(par + 8 * kBlk, __float_as_uint(sv));
+                sts_u32(par + 12 * kBlk, __float_as_uint(on ? h2f_bits(hi16(pw.y)) - 8.f : 0.f));
+                float big = sv;
+#pragma unroll
+                for (int o = 16; o >= 1; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                const uint32_t there = __ballot_sync(0xffffffffu, on);
+                if (lane == 0) {
+                    sts_u32(misc + 4 * dw, __float_as_uint(big));
+                    sts_u32(misc + 16 + 4 * dw, there);
+                }
+            }
+            fence_async_smem();
+            mbar_arrive(bars + 8 * (kKFull + buf));
+            if (i >= 2) wait(kVFree + buf, (i - 2) >> 1);
             // V: a lane four column quads of a slot pair at a time; which quad (g1) and which two columns (g2)
             // come first differs among the lanes of a pair, so that the 32 words of a store lie in 32 banks.
             const int pr = lane >> 2, g = lane & 3, g1 = g & 1, g2 = g & 2;
 #pragma unroll 1
             for (int e = 0; e < 2; ++e) {
                 const int u = 2 * dw + e;
-                const char* raw = base + S::kRaw + buf * S::kRawBytes + u * kv_unit_bytes(D);
-                unpack_keys<D>(raw, base + S::kK + buf * S::kOp, u, lane);
+                const char* raw = raws + u * kv_unit_bytes(D);
                 const int key = u * kKvTokens + 2 * pr, byte = 2 * (key % 64);  // the pair's first slot
                 char* vt = base + S::kV + buf * S::kVBytes + key / 64 * (D * 128) + 512 * 4 * g;
                 char* even[4];  // columns of quads g1, 2 + g1: in the order of their stores
@@ -492,28 +522,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
                     }
                 }
             }
-            {
-                // scales and zeros, a lane a slot
-                const int u = 2 * dw + (lane >> 4), slot = 32 * dw + lane;
-                const bool on = (got >> u & 1u) && at.at.step * kBlk + slot < at.at.len;
-                const uint2 pw = lds_v2(smem0 + S::kRaw + buf * S::kRawBytes + u * kv_unit_bytes(D) + kv_param_offset(D) + 8 * (lane & 15));
-                const float sv = on ? h2f_bits(lo16(pw.y)) : 0.f;
-                const uint32_t par = smem0 + S::kPar + buf * (4 * kBlk * 4) + 4 * slot, misc = smem0 + S::kMisc + buf * 64;
-                sts_u32(par, __float_as_uint(on ? 8.f - h2f_bits(hi16(pw.x)) : 0.f));
-                sts_u32(par + 4 * kBlk, __float_as_uint(on ? h2f_bits(lo16(pw.x)) * a.scale2 : 0.f));
-                sts_u32(par + 8 * kBlk, __float_as_uint(sv));
-                sts_u32(par + 12 * kBlk, __float_as_uint(on ? h2f_bits(hi16(pw.y)) - 8.f : 0.f));
-                float big = sv;
-#pragma unroll
-                for (int o = 16; o >= 1; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-                const uint32_t there = __ballot_sync(0xffffffffu, on);
-                if (lane == 0) {
-                    sts_u32(misc + 4 * dw, __float_as_uint(big));
-                    sts_u32(misc + 16 + 4 * dw, there);
-                }
-            }
             fence_async_smem();
-            mbar_arrive(bars + 8 * (kKvFull + buf));
+            mbar_arrive(bars + 8 * (kVFull + buf));
             named_bar_sync(1, 128);  // all four warps have read the units
             if (dw == 0 && i + 2 < n && !dead) {
                 request(i + 2);
@@ -531,6 +541,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
         auto output = [&](int i, bool start) {
             const int buf = i & 1;
             wait(kPFull + buf, i >> 1);
+            wait(kVFull + buf, i >> 1);
             tm_after_sync();
             if (lane == 0) {
                 const uint32_t vb = smem0 + S::kV + buf * S::kVBytes;
@@ -538,14 +549,14 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
                 for (int k = 0; k < kBlk / 16; ++k)
                     tm_mma_ts(tm + kTmO, tm + kTmP + buf * 64 + 8 * k, operand(vb + k / 4 * (D * 128) + 32 * (k % 4)), mma_shape(D),
                               !(start && k == 0));
-                tm_commit(bars + 8 * (kKvFree + buf));
+                tm_commit(bars + 8 * (kVFree + buf));
             }
             __syncwarp();
         };
         for (int i = 0; i < n; ++i) {
             const int buf = i & 1;
             if (begins) wait(kQFull, jobs);
-            wait(kKvFull + buf, i >> 1);
+            wait(kKFull + buf, i >> 1);
             tm_after_sync();
             if (lane == 0) {
                 const uint32_t kb = smem0 + S::kK + buf * S::kOp;
@@ -562,7 +573,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
             begins = i + 1 < n && at.next(p, c.n_seqs, u0 + i + 1);
         }
         output(n - 1, begins_before);
-        wait(kKvFree + ((n - 1) & 1), (n - 1) >> 1);
+        wait(kVFree + ((n - 1) & 1), (n - 1) >> 1);
     }
     // rows of sequences without slots
     for (int b = blockIdx.x; b < c.n_seqs; b += gridDim.x) {
@@ -616,10 +627,10 @@ struct CmSmem {
     static constexpr int kK = kOp;                               // 2 x
     static constexpr int kRawUnit = 8 * D + kKvTokens * 8;       // keys and parameters of a unit
     static constexpr int kRaw = kK + 2 * kOp;                    // 2 x
-    static constexpr int kPar = kRaw + 2 * kUnits * kRawUnit;    // 2 x [2][128]: - (z_k - 8), s_k
-    static constexpr int kRow = kPar + 4 * kBlk * 4;             // [4][128]: sum of q (two halves), - lse, keys seen
+    static constexpr int kPar = kRaw + 2 * kUnits * kRawUnit;    // 4 x [2][128]: - (z_k - 8), s_k
+    static constexpr int kRow = kPar + 8 * kBlk * 4;             // [4][128]: sum of q (two halves), - lse, keys seen
     static constexpr int kSum = kRow + 4 * kTile * 4;            // 2 x [128]: the other half's sums
-    static constexpr int kMisc = kSum + 2 * kBlk * 4;            // per buffer: 4 x slots there; found units
+    static constexpr int kMisc = kSum + 2 * kBlk * 4;            // 4 x (4 x slots there); 2 x found units; 4 x keys seen
     static constexpr int kBars = kMisc + 128;
     static constexpr int kTotal = kBars + 128;
 };
@@ -639,7 +650,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(bars + 8 * (kRawFull + i), 1);
-            mbar_init(bars + 8 * (kKvFull + i), 128);
+            mbar_init(bars + 8 * (kKFull + i), 128);
             mbar_init(bars + 8 * (kSFull + i), 1);
             mbar_init(bars + 8 * (kPFull + i), kSoft);  // S and the parameters have been read
         }
@@ -705,8 +716,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
             const int buf = i & 1, slot = at.at.step * kBlk + trow;
             wait(kSFull + buf, i >> 1);
             tm_after_sync();
-            const float nz = word(S::kPar + buf * (2 * kBlk * 4))[trow], sk = word(S::kPar + buf * (2 * kBlk * 4))[kBlk + trow];
-            const bool there = reinterpret_cast<const uint32_t*>(word(S::kMisc + buf * 32))[warp & 3] >> lane & 1u;
+            const float nz = word(S::kPar + (i & 3) * (2 * kBlk * 4))[trow], sk = word(S::kPar + (i & 3) * (2 * kBlk * 4))[kBlk + trow];
+            const bool there = reinterpret_cast<const uint32_t*>(word(S::kMisc + (i & 3) * 16))[warp & 3] >> lane & 1u;
             const bool all = (at.at.step + 1) * kBlk <= least;
             const float* row = word(S::kRow) + half * (kTile / 2);
             f2 add(0.f);
@@ -773,7 +784,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
         for (int i = 0; i < n; ++i) {
             const int buf = i & 1;
             wait(kRawFull + buf, i >> 1);
-            if (i >= 2) wait(kPFull + buf, (i - 2) >> 1);
+            if (i >= 2) wait(kSFull + buf, (i - 2) >> 1);
             const uint32_t got = reinterpret_cast<const uint32_t*>(word(S::kMisc))[16 + buf];
             const char* raw = base + S::kRaw + buf * kUnits * S::kRawUnit;
 #pragma unroll 1
@@ -781,13 +792,13 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
             const int u = 2 * dw + (lane >> 4), slot = 32 * dw + lane;
             const bool on = (got >> u & 1u) && at.at.step * kBlk + slot < at.at.len;
             const uint32_t pw = *reinterpret_cast<const uint32_t*>(raw + u * S::kRawUnit + 8 * D + 8 * (lane & 15));
-            float* par = word(S::kPar + buf * (2 * kBlk * 4));
+            float* par = word(S::kPar + (i & 3) * (2 * kBlk * 4));
             par[slot] = on ? 8.f - h2f_bits(hi16(pw)) : 0.f;
             par[kBlk + slot] = on ? h2f_bits(lo16(pw)) * a.scale2 : 0.f;
             const uint32_t there = __ballot_sync(0xffffffffu, on);
-            if (lane == 0) reinterpret_cast<uint32_t*>(word(S::kMisc + buf * 32))[dw] = there;
+            if (lane == 0) reinterpret_cast<uint32_t*>(word(S::kMisc + (i & 3) * 16))[dw] = there;
             fence_async_smem();
-            mbar_arrive(bars + 8 * (kKvFull + buf));
+            mbar_arrive(bars + 8 * (kKFull + buf));
             named_bar_sync(1, 128);  // all four warps have read the units
             if (dw == 0 && i + 2 < n && !dead) {
                 request(i + 2);
@@ -803,7 +814,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
         for (int i = 0; i < n; ++i) {
             const int buf = i & 1;
             if (begins) wait(kQFull, jobs++);
-            wait(kKvFull + buf, i >> 1);
+            wait(kKFull + buf, i >> 1);
             if (i >= 2) wait(kPFull + buf, (i - 2) >> 1);
             tm_after_sync();
             if (lane == 0) {

@@ -226,7 +226,7 @@ def test_attend_is_reproducible_and_ignores_what_lies_behind():
 @pytest.mark.parametrize("dim,heads,group,t,page,lens,counts", [
     (128, 1, 1, 64, 64, [64], None),
     (128, 1, 1, 128, 64, [128, 127, 129], [128, 127, 128]),
-    (64, 2, 8, 9, 16, [130, 9, 0, 300], None),
+    (64, 2, 8, 12, 16, [130, 9, 0, 300], None),
     (128, 2, 4, 40, 16, [41, 700, 3], [40, 17, 40]),
     (128, 1, 3, 90, 48, [1000, 260], None),
     (64, 1, 16, 33, 32, [513, 40], [0, 33]),
