@@ -7,11 +7,11 @@
 // equal runs, one per CTA (one CTA an SM); pieces of jobs that a border cuts are
 // joined by kv_chunk_combine_kernel.
 //
-// Roles of a CTA's thirteen warps, over the blocks i of its run:
+// Roles of a CTA's fourteen warps, over the blocks i of its run:
+//   loading (1)       page lookups and bulk copies of the block's units
 //   dequantizing (4)  wait for the block's units (bulk copies), turn codes into
 //                     f16 integers c - 8 in the MMA's shared-memory layout and
-//                     the scales into FP32 constants; ask for block i + 2.
-//                     K's tile is free again when S(i) is there, V's only
+//                     the scales into FP32 constants.  K's tile is free again when S(i) is there, V's only
 //                     after the block's softmax, so they are filled apart
 //   MMA (1)           S(i) = Q K^T into one of two TMEM tiles, then, when the
 //                     weights of i - 1 are there, O += P(i-1) V
@@ -38,7 +38,8 @@ __device__ unsigned int g_kv_chunk_error;
 constexpr int kBlk = 128;                  // slots of a block
 constexpr int kUnits = kBlk / kKvTokens;   // units of a block
 constexpr int kSoftWarps = 8, kSoft = 32 * kSoftWarps;  // two threads a row, half the columns each
-constexpr int kCkThreads = kSoft + 5 * 32;              // + four dequantizing warps, one for the MMAs
+constexpr int kMmaWarp = kSoftWarps + 4, kLoadWarp = kMmaWarp + 1;
+constexpr int kCkThreads = 32 * (kLoadWarp + 1);
 constexpr int kTile = kChunkRows;
 constexpr int kChunkCtas = 160;            // bound on the grid (workspace sizing)
 
@@ -65,7 +66,7 @@ struct CkSmem {
 
 // Barriers (8 bytes each).  Each but the last is a pair, one for the even and one for the odd blocks.  S full also
 // says that K has been read, V free that the block's product is in O.
-enum { kRawFull = 0, kKFull = 2, kVFull = 4, kVFree = 6, kSFull = 8, kPFull = 10, kQFull = 12 };
+enum { kRawFull = 0, kKFull = 2, kVFull = 4, kVFree = 6, kSFull = 8, kPFull = 10, kRawFree = 12, kQFull = 14 };
 
 // Tensor memory columns: two S tiles, O, two P tiles (f16 pairs).
 constexpr uint32_t kTmS = 0, kTmO = 256, kTmP = 384, kTmCols = 512;
@@ -225,10 +226,11 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
     const KvView& c = a.c;
     const uint32_t smem0 = (smem_u32(dyn) + plan_bytes(c.n_seqs) + 1023u) & ~1023u;
     const uint32_t bars = smem0 + S::kBars;
-    if (warp == 12) tm_alloc(smem_u32(&tm_base), kTmCols);
+    if (warp == kMmaWarp) tm_alloc(smem_u32(&tm_base), kTmCols);
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(bars + 8 * (kRawFull + i), 1);
+            mbar_init(bars + 8 * (kRawFree + i), 128);
             mbar_init(bars + 8 * (kKFull + i), 128);
             mbar_init(bars + 8 * (kVFull + i), 128);
             mbar_init(bars + 8 * (kVFree + i), 1);
@@ -294,36 +296,38 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
             tm_after_sync();
             const float* par = word(S::kPar + (i & 3) * (4 * kBlk * 4)) + half * H;
             const float* misc = word(S::kMisc + (i & 3) * 32);
+            uint32_t va[32], vb[32];
+            tm_ld32(lanes + kTmS + buf * kBlk + half * H, va);
+            tm_ld32(lanes + kTmS + buf * kBlk + half * H + 32, vb);
             f2 s[H / 2];
             float top = -INFINITY;
-            const int left = lim - step * kBlk - half * H;  // slots of the half block that the row sees
-            const uint2 there = *reinterpret_cast<const uint2*>(misc + 4 + 2 * half);
-            const bool all = left >= H && (there.x & there.y) == 0xffffffffu;
+            tm_wait_ld();
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                uint32_t v[32];
-                tm_ld32(lanes + kTmS + buf * kBlk + half * H + 32 * k, v);
-                tm_wait_ld();
-                const uint32_t ok = k == 0 ? there.x : there.y;
+                const uint32_t (&v)[32] = k == 0 ? va : vb;
 #pragma unroll
                 for (int j = 0; j < 32; j += 4) {
                     const float4 z = *reinterpret_cast<const float4*>(par + 32 * k + j);
                     const float4 sc = *reinterpret_cast<const float4*>(par + kBlk + 32 * k + j);
-                    f2 x = fma2(f2(z.x, z.y), f2(qsum), f2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]))) * f2(sc.x, sc.y);
-                    f2 y = fma2(f2(z.z, z.w), f2(qsum), f2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]))) * f2(sc.z, sc.w);
-                    if (!all) {
-                        const int e = 32 * k + j;
-                        x = f2(e < left && (ok >> j & 1u) ? x.x() : -INFINITY, e + 1 < left && (ok >> (j + 1) & 1u) ? x.y() : -INFINITY);
-                        y = f2(e + 2 < left && (ok >> (j + 2) & 1u) ? y.x() : -INFINITY, e + 3 < left && (ok >> (j + 3) & 1u) ? y.y() : -INFINITY);
-                    }
-                    s[16 * k + j / 2] = x;
-                    s[16 * k + j / 2 + 1] = y;
-                    top = fmaxf(top, fmaxf(fmaxf(x.x(), x.y()), fmaxf(y.x(), y.y())));
+                    s[16 * k + j / 2] = fma2(f2(z.x, z.y), f2(qsum), f2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]))) * f2(sc.x, sc.y);
+                    s[16 * k + j / 2 + 1] =
+                        fma2(f2(z.z, z.w), f2(qsum), f2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]))) * f2(sc.z, sc.w);
                 }
             }
+            const int left = lim - step * kBlk - half * H;  // slots of the half block that the row sees
+            const uint2 there = *reinterpret_cast<const uint2*>(misc + 4 + 2 * half);
+            if (left < H || (there.x & there.y) != 0xffffffffu) {
+#pragma unroll
+                for (int j = 0; j < H; j += 2) {
+                    const uint32_t ok = (j < 32 ? there.x : there.y) >> (j & 31);
+                    s[j / 2] = f2(j < left && (ok & 1u) ? s[j / 2].x() : -INFINITY, j + 1 < left && (ok & 2u) ? s[j / 2].y() : -INFINITY);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < H / 2; ++j) top = fmaxf(top, fmaxf(s[j].x(), s[j].y()));
             float* tops = word(S::kTop) + buf * 2 * kTile;
             tops[half * kTile + trow] = top;
-            named_bar_sync(2, kSoft);
+            named_bar_sync(3 + (warp & 3), 64);  // the two warps of these rows
             top = fmaxf(top, tops[(half ^ 1) * kTile + trow]);
             // a new maximum or a larger V scale (the same for all rows)
             const float4 bg = *reinterpret_cast<const float4*>(misc);
@@ -429,35 +433,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
             first = at.at.step;
             begins = true;
         }
-    } else if (n > 0 && warp < kSoftWarps + 4) {
+    } else if (n > 0 && warp < kMmaWarp) {
         // ---- dequantizing
         const int dw = warp - kSoftWarps;
         char* const base = dyn + (smem0 - smem_u32(dyn));
-        bool absent = false;
-        Walk ahead = at;
-        auto request = [&](int i) {  // its first warp: the units of the block that `ahead` stands at
-            const int buf = i & 1, slot = ahead.at.step * kBlk + lane * kKvTokens;
-            int index = -1;
-            if (lane < kUnits && slot < ahead.at.len) {
-                const int page = kv_page(c, ahead.at.b, slot);
-                if (page >= 0) index = static_cast<int>((kv_line(c, page, ahead.at.job / a.n_rt) + slot % c.page_size) / kKvTokens);
-                else absent = true;
-            }
-            const uint32_t got = __ballot_sync(0xffffffffu, index >= 0), bar = bars + 8 * (kRawFull + buf);
-            if (lane == 0) {
-                sts_u32(smem0 + S::kGot + buf * 4, got);
-                if (got) mbar_arrive_expect_tx(bar, __popc(got) * kv_unit_bytes(D));
-                else mbar_arrive(bar);
-            }
-            __syncwarp();
-            if (index >= 0)
-                bulk_g2s(smem0 + S::kRaw + buf * S::kRawBytes + lane * kv_unit_bytes(D),
-                         c.units + static_cast<size_t>(index) * kv_unit_bytes(D), kv_unit_bytes(D), bar);
-            ahead.next(p, c.n_seqs, u0 + i + 1 < u0 + n ? u0 + i + 1 : u0 + n - 1);
-        };
-        if (dw == 0)
-            for (int i = 0; i < min(2, n); ++i) request(i);
-        int asked = min(2, n);
         for (int i = 0; i < n; ++i) {
             const int buf = i & 1;
             wait(kRawFull + buf, i >> 1);
@@ -524,17 +503,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
             }
             fence_async_smem();
             mbar_arrive(bars + 8 * (kVFull + buf));
-            named_bar_sync(1, 128);  // all four warps have read the units
-            if (dw == 0 && i + 2 < n && !dead) {
-                request(i + 2);
-                asked = i + 3;
-            }
+            mbar_arrive(bars + 8 * (kRawFree + buf));
             if (i + 1 < n) at.next(p, c.n_seqs, u0 + i + 1);
         }
-        if (dead && dw == 0)  // the copies in flight must end before the shared memory goes
-            for (int j = max(asked - 2, 0); j < asked; ++j) mbar_wait_bounded(bars + 8 * (kRawFull + (j & 1)), (j >> 1) & 1);
-        if (absent) atomicOr(&g_kv_chunk_error, kKvErrPage);
-    } else if (n > 0) {
+    } else if (n > 0 && warp == kMmaWarp) {
         // ---- MMA
         int jobs = 0;
         bool begins = true, begins_before = true;
@@ -574,6 +546,38 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
         }
         output(n - 1, begins_before);
         wait(kVFree + ((n - 1) & 1), (n - 1) >> 1);
+    } else if (n > 0) {
+        // ---- loading: a lane a unit
+        bool absent = false;
+        int asked = 0;
+        for (int i = 0; i < n; ++i) {
+            const int buf = i & 1, slot = at.at.step * kBlk + lane * kKvTokens;
+            int index = -1;
+            if (lane < kUnits && slot < at.at.len) {
+                const int page = kv_page(c, at.at.b, slot);
+                if (page >= 0) index = static_cast<int>((kv_line(c, page, at.at.job / a.n_rt) + slot % c.page_size) / kKvTokens);
+                else absent = true;
+            }
+            if (i >= 2) wait(kRawFree + buf, (i - 2) >> 1);
+            if (dead) break;
+            asked = i + 1;
+            const uint32_t got = __ballot_sync(0xffffffffu, index >= 0), bar = bars + 8 * (kRawFull + buf);
+            if (lane == 0) {
+                sts_u32(smem0 + S::kGot + buf * 4, got);
+                if (got) mbar_arrive_expect_tx(bar, __popc(got) * kv_unit_bytes(D));
+                else mbar_arrive(bar);
+            }
+            __syncwarp();
+            if (index >= 0) {
+                bulk_g2s(smem0 + S::kRaw + buf * S::kRawBytes + lane * kv_unit_bytes(D),
+                         c.units + static_cast<size_t>(index) * kv_unit_bytes(D), kv_unit_bytes(D), bar);
+            }
+            if (i + 1 < n) at.next(p, c.n_seqs, u0 + i + 1);
+        }
+        // given up: the copies in flight must end before the shared memory goes
+        if (dead)
+            for (int j = max(asked - 2, 0); j < asked; ++j) mbar_wait_bounded(bars + 8 * (kRawFull + (j & 1)), (j >> 1) & 1);
+        if (absent) atomicOr(&g_kv_chunk_error, kKvErrPage);
     }
     // rows of sequences without slots
     for (int b = blockIdx.x; b < c.n_seqs; b += gridDim.x) {
@@ -587,7 +591,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
     }
     tm_before_sync();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == kMmaWarp) {
         tm_after_sync();
         tm_dealloc(tm, kTmCols);
     }
@@ -646,10 +650,11 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
     const uint32_t bars = smem0 + S::kBars;
     char* const base = dyn + (smem0 - smem_u32(dyn));
     auto word = [&](int off) -> float* { return reinterpret_cast<float*>(base + off); };
-    if (warp == 12) tm_alloc(smem_u32(&tm_base), 256);
+    if (warp == kMmaWarp) tm_alloc(smem_u32(&tm_base), 256);
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(bars + 8 * (kRawFull + i), 1);
+            mbar_init(bars + 8 * (kRawFree + i), 128);
             mbar_init(bars + 8 * (kKFull + i), 128);
             mbar_init(bars + 8 * (kSFull + i), 1);
             mbar_init(bars + 8 * (kPFull + i), kSoft);  // S and the parameters have been read
@@ -721,11 +726,13 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
             const bool all = (at.at.step + 1) * kBlk <= least;
             const float* row = word(S::kRow) + half * (kTile / 2);
             f2 add(0.f);
+            uint32_t va[32], vb[32];
+            tm_ld32(lanes + buf * kTile + half * (kTile / 2), va);
+            tm_ld32(lanes + buf * kTile + half * (kTile / 2) + 32, vb);
+            tm_wait_ld();
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                uint32_t v[32];
-                tm_ld32(lanes + buf * kTile + half * (kTile / 2) + 32 * k, v);
-                tm_wait_ld();
+                const uint32_t (&v)[32] = k == 0 ? va : vb;
 #pragma unroll
                 for (int j = 0; j < 32; j += 4) {
                     const float4 qs = *reinterpret_cast<const float4*>(row + 32 * k + j);
@@ -753,34 +760,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
             mbar_arrive(bars + 8 * (kPFull + buf));
             if (i + 1 < n && at.next(p, c.n_seqs, u0 + i + 1)) load_q();  // S of the old rows is done
         }
-    } else if (n > 0 && warp < kSoftWarps + 4) {
+    } else if (n > 0 && warp < kMmaWarp) {
         const int dw = warp - kSoftWarps;
-        Walk ahead = at;
-        auto request = [&](int i) {
-            const int buf = i & 1, slot = ahead.at.step * kBlk + lane * kKvTokens;
-            int index = -1;
-            if (lane < kUnits && slot < ahead.at.len) {
-                const int page = kv_page(c, ahead.at.b, slot);
-                if (page >= 0) index = static_cast<int>((kv_line(c, page, ahead.at.job / a.n_rt) + slot % c.page_size) / kKvTokens);
-            }
-            const uint32_t got = __ballot_sync(0xffffffffu, index >= 0), bar = bars + 8 * (kRawFull + buf);
-            if (lane == 0) {
-                sts_u32(smem0 + S::kMisc + 64 + buf * 4, got);
-                if (got) mbar_arrive_expect_tx(bar, __popc(got) * S::kRawUnit);
-                else mbar_arrive(bar);
-            }
-            __syncwarp();
-            if (index >= 0) {
-                const uint32_t dst = smem0 + S::kRaw + (buf * kUnits + lane) * S::kRawUnit;
-                const uint8_t* src = c.units + static_cast<size_t>(index) * kv_unit_bytes(D);
-                bulk_g2s(dst, src, 8 * D, bar);
-                bulk_g2s(dst + 8 * D, src + kv_param_offset(D), kKvTokens * 8, bar);
-            }
-            ahead.next(p, c.n_seqs, u0 + i + 1 < u0 + n ? u0 + i + 1 : u0 + n - 1);
-        };
-        if (dw == 0)
-            for (int i = 0; i < min(2, n); ++i) request(i);
-        int asked = min(2, n);
         for (int i = 0; i < n; ++i) {
             const int buf = i & 1;
             wait(kRawFull + buf, i >> 1);
@@ -799,16 +780,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
             if (lane == 0) reinterpret_cast<uint32_t*>(word(S::kMisc + (i & 3) * 16))[dw] = there;
             fence_async_smem();
             mbar_arrive(bars + 8 * (kKFull + buf));
-            named_bar_sync(1, 128);  // all four warps have read the units
-            if (dw == 0 && i + 2 < n && !dead) {
-                request(i + 2);
-                asked = i + 3;
-            }
+            mbar_arrive(bars + 8 * (kRawFree + buf));
             if (i + 1 < n) at.next(p, c.n_seqs, u0 + i + 1);
         }
-        if (dead && dw == 0)  // the copies in flight must end before the shared memory goes
-            for (int j = max(asked - 2, 0); j < asked; ++j) mbar_wait_bounded(bars + 8 * (kRawFull + (j & 1)), (j >> 1) & 1);
-    } else if (n > 0) {
+    } else if (n > 0 && warp == kMmaWarp) {
         int jobs = 0;
         bool begins = true;
         for (int i = 0; i < n; ++i) {
@@ -829,10 +804,41 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
             begins = i + 1 < n && at.next(p, c.n_seqs, u0 + i + 1);
         }
         wait(kSFull + ((n - 1) & 1), (n - 1) >> 1);
+    } else if (n > 0) {
+        // ---- loading: a lane a unit
+        int asked = 0;
+        for (int i = 0; i < n; ++i) {
+            const int buf = i & 1, slot = at.at.step * kBlk + lane * kKvTokens;
+            int index = -1;
+            if (lane < kUnits && slot < at.at.len) {
+                const int page = kv_page(c, at.at.b, slot);
+                if (page >= 0) index = static_cast<int>((kv_line(c, page, at.at.job / a.n_rt) + slot % c.page_size) / kKvTokens);
+            }
+            if (i >= 2) wait(kRawFree + buf, (i - 2) >> 1);
+            if (dead) break;
+            asked = i + 1;
+            const uint32_t got = __ballot_sync(0xffffffffu, index >= 0), bar = bars + 8 * (kRawFull + buf);
+            if (lane == 0) {
+                sts_u32(smem0 + S::kMisc + 64 + buf * 4, got);
+                if (got) mbar_arrive_expect_tx(bar, __popc(got) * S::kRawUnit);
+                else mbar_arrive(bar);
+            }
+            __syncwarp();
+            if (index >= 0) {
+                const uint32_t dst = smem0 + S::kRaw + (buf * kUnits + lane) * S::kRawUnit;
+                const uint8_t* src = c.units + static_cast<size_t>(index) * kv_unit_bytes(D);
+                bulk_g2s(dst, src, 8 * D, bar);
+                bulk_g2s(dst + 8 * D, src + kv_param_offset(D), kKvTokens * 8, bar);
+            }
+            if (i + 1 < n) at.next(p, c.n_seqs, u0 + i + 1);
+        }
+        // given up: the copies in flight must end before the shared memory goes
+        if (dead)
+            for (int j = max(asked - 2, 0); j < asked; ++j) mbar_wait_bounded(bars + 8 * (kRawFull + (j & 1)), (j >> 1) & 1);
     }
     tm_before_sync();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == kMmaWarp) {
         tm_after_sync();
         tm_dealloc(tm, 256);
     }
