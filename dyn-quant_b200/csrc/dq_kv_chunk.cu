@@ -180,6 +180,18 @@ struct Walk {
     }
 };
 
+// Copies a block's units, the index of each in its lane (negative: none; `got` has the others' bits), one copy for
+// units side by side in memory: a copy's issue takes some 80 cycles of the loading warp whatever its size.
+template <int D>
+__device__ __forceinline__ void copy_units(const KvView& c, uint32_t dst, int index, uint32_t got, int lane, uint32_t bar) {
+    const int before = __shfl_up_sync(0xffffffffu, index, 1);
+    const bool begins = index >= 0 && (lane == 0 || before + 1 != index || before < 0);
+    const uint32_t ends = __ballot_sync(0xffffffffu, begins) | ~got;
+    if (begins)
+        bulk_g2s(dst + lane * kv_unit_bytes(D), c.units + static_cast<size_t>(index) * kv_unit_bytes(D),
+                 __ffs(ends >> (lane + 1)) * kv_unit_bytes(D), bar);
+}
+
 // One unit's keys into the operand tile [D/64][128 slots]: a lane half a row, a word a chunk.
 template <int D>
 __device__ __forceinline__ void unpack_keys(const char* raw, char* tile, int u, int lane) {
@@ -547,7 +559,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
         output(n - 1, begins_before);
         wait(kVFree + ((n - 1) & 1), (n - 1) >> 1);
     } else if (n > 0) {
-        // ---- loading: a lane a unit
+        // ---- loading: a lane a unit, a copy a run of units of one page
         bool absent = false;
         int asked = 0;
         for (int i = 0; i < n; ++i) {
@@ -568,10 +580,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
                 else mbar_arrive(bar);
             }
             __syncwarp();
-            if (index >= 0) {
-                bulk_g2s(smem0 + S::kRaw + buf * S::kRawBytes + lane * kv_unit_bytes(D),
-                         c.units + static_cast<size_t>(index) * kv_unit_bytes(D), kv_unit_bytes(D), bar);
-            }
+            copy_units<D>(c, smem0 + S::kRaw + buf * S::kRawBytes, index, got, lane, bar);
             if (i + 1 < n) at.next(p, c.n_seqs, u0 + i + 1);
         }
         // given up: the copies in flight must end before the shared memory goes
@@ -629,15 +638,21 @@ struct CmSmem {
     static constexpr int kOp = D / 64 * kTile * 128;
     static constexpr int kQ = 0;
     static constexpr int kK = kOp;                               // 2 x
-    static constexpr int kRawUnit = 8 * D + kKvTokens * 8;       // keys and parameters of a unit
-    static constexpr int kRaw = kK + 2 * kOp;                    // 2 x
-    static constexpr int kPar = kRaw + 2 * kUnits * kRawUnit;    // 4 x [2][128]: - (z_k - 8), s_k
-    static constexpr int kRow = kPar + 8 * kBlk * 4;             // [4][128]: sum of q (two halves), - lse, keys seen
-    static constexpr int kSum = kRow + 4 * kTile * 4;            // 2 x [128]: the other half's sums
-    static constexpr int kMisc = kSum + 2 * kBlk * 4;            // 4 x (4 x slots there); 2 x found units; 4 x keys seen
+    static constexpr int kRawBytes = kUnits * kv_unit_bytes(D);
+    static constexpr int kRaw = kK + 2 * kOp;                    // 4 x the units of a block
+    static constexpr int kPar = kRaw + 4 * kRawBytes;            // 8 x [2][128]: - (z_k - 8), s_k
+    static constexpr int kRow = kPar + 16 * kBlk * 4;            // [4][128]: sum of q (two halves), - lse, keys seen
+    static constexpr int kIndex = kRow + 4 * kTile * 4;          // 16 x the block's units
+    static constexpr int kThere = kIndex + 16 * kUnits * 4;      // 8 x (4 x slots there)
+    static constexpr int kMisc = kThere + 8 * 16;                // 4 x found units; 4 x keys seen
     static constexpr int kBars = kMisc + 128;
-    static constexpr int kTotal = kBars + 128;
+    static constexpr int kTotal = kBars + 256;
 };
+
+// Barriers: four for the units' buffers and for the S tiles, two for K's tiles.  S full also says that K has been read,
+// and a block's constants are kept until its S is free: the warps that fill them are at most six blocks ahead of those
+// that read them, the loading warp ten.
+enum { kCmRawFull = 0, kCmRawFree = 4, kCmSFull = 8, kCmSFree = 12, kCmKFull = 16, kCmQFull = 18 };
 
 template <int D>
 __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAttendArgs a, float* sums, const long long lines) {
@@ -650,16 +665,16 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
     const uint32_t bars = smem0 + S::kBars;
     char* const base = dyn + (smem0 - smem_u32(dyn));
     auto word = [&](int off) -> float* { return reinterpret_cast<float*>(base + off); };
-    if (warp == kMmaWarp) tm_alloc(smem_u32(&tm_base), 256);
+    if (warp == kMmaWarp) tm_alloc(smem_u32(&tm_base), kTmCols);
     if (tid == 0) {
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(bars + 8 * (kRawFull + i), 1);
-            mbar_init(bars + 8 * (kRawFree + i), 128);
-            mbar_init(bars + 8 * (kKFull + i), 128);
-            mbar_init(bars + 8 * (kSFull + i), 1);
-            mbar_init(bars + 8 * (kPFull + i), kSoft);  // S and the parameters have been read
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(bars + 8 * (kCmRawFull + i), 1);
+            mbar_init(bars + 8 * (kCmRawFree + i), 128);
+            mbar_init(bars + 8 * (kCmSFull + i), 1);
+            mbar_init(bars + 8 * (kCmSFree + i), kTile);  // S and the block's constants have been read
         }
-        mbar_init(bars + 8 * kQFull, kSoft);
+        for (int i = 0; i < 2; ++i) mbar_init(bars + 8 * (kCmKFull + i), 128);
+        mbar_init(bars + 8 * kCmQFull, kSoft);
         fence_mbar_init();
     }
     tm_before_sync();
@@ -706,81 +721,87 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
                 reinterpret_cast<int*>(word(S::kRow))[3 * kTile + trow] = on ? lim : at.at.len;
             }
             fence_async_smem();
-            mbar_arrive(bars + 8 * kQFull);
+            mbar_arrive(bars + 8 * kCmQFull);
             named_bar_sync(2, kSoft);
             if (half == 0) word(S::kRow)[trow] += word(S::kRow)[kTile + trow];
             int lim = reinterpret_cast<const int*>(word(S::kRow))[3 * kTile + trow];
             lim = __reduce_min_sync(0xffffffffu, lim);
-            if (half == 0 && lane == 0) reinterpret_cast<int*>(word(S::kMisc))[24 + (warp & 3)] = lim;
+            if (half == 0 && lane == 0) reinterpret_cast<int*>(word(S::kMisc))[4 + (warp & 3)] = lim;
             named_bar_sync(2, kSoft);
-            const int4 l4 = *reinterpret_cast<const int4*>(word(S::kMisc) + 24);
+            const int4 l4 = *reinterpret_cast<const int4*>(word(S::kMisc) + 4);
             least = min(min(l4.x, l4.y), min(l4.z, l4.w));
         };
         load_q();
         for (int i = 0; i < n; ++i) {
-            const int buf = i & 1, slot = at.at.step * kBlk + trow;
-            wait(kSFull + buf, i >> 1);
-            tm_after_sync();
-            const float nz = word(S::kPar + (i & 3) * (2 * kBlk * 4))[trow], sk = word(S::kPar + (i & 3) * (2 * kBlk * 4))[kBlk + trow];
-            const bool there = reinterpret_cast<const uint32_t*>(word(S::kMisc + (i & 3) * 16))[warp & 3] >> lane & 1u;
-            const bool all = (at.at.step + 1) * kBlk <= least;
-            const float* row = word(S::kRow) + half * (kTile / 2);
-            f2 add(0.f);
-            uint32_t va[32], vb[32];
-            tm_ld32(lanes + buf * kTile + half * (kTile / 2), va);
-            tm_ld32(lanes + buf * kTile + half * (kTile / 2) + 32, vb);
-            tm_wait_ld();
+            if ((i & 1) == half) {
+                const int buf = i & 3, slot = at.at.step * kBlk + trow;
+                wait(kCmSFull + buf, i >> 2);
+                tm_after_sync();
+                const float* par = word(S::kPar + (i & 7) * (2 * kBlk * 4));
+                const float nz = par[trow], sk = par[kBlk + trow];
+                const bool there = reinterpret_cast<const uint32_t*>(word(S::kThere + (i & 7) * 16))[warp & 3] >> lane & 1u;
+                const int unit = reinterpret_cast<const int*>(word(S::kIndex + (i & 15) * (kUnits * 4)))[trow / kKvTokens];
+                const bool all = (at.at.step + 1) * kBlk <= least;
+                f2 add(0.f);
+                uint32_t v[2][32];
+                tm_ld32(lanes + buf * kTile, v[0]);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const uint32_t (&v)[32] = k == 0 ? va : vb;
+                for (int k = 0; k < kTile / 32; ++k) {
+                    const float* row = word(S::kRow) + 32 * k;
+                    const uint32_t (&x)[32] = v[k & 1];
+                    f2 s[16];
+                    tm_wait_ld();
+                    if (k + 1 < kTile / 32) tm_ld32(lanes + buf * kTile + 32 * (k + 1), v[(k + 1) & 1]);
 #pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                    const float4 qs = *reinterpret_cast<const float4*>(row + 32 * k + j);
-                    const float4 nl = *reinterpret_cast<const float4*>(row + 2 * kTile + 32 * k + j);
-                    f2 x = fma2(fma2(f2(nz), f2(qs.x, qs.y), f2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]))), f2(sk), f2(nl.x, nl.y));
-                    f2 y = fma2(fma2(f2(nz), f2(qs.z, qs.w), f2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]))), f2(sk), f2(nl.z, nl.w));
-                    if (!all) {
-                        const int4 lim = *reinterpret_cast<const int4*>(row + 3 * kTile + 32 * k + j);
-                        x = f2(slot < lim.x ? x.x() : -INFINITY, slot < lim.y ? x.y() : -INFINITY);
-                        y = f2(slot < lim.z ? y.x() : -INFINITY, slot < lim.w ? y.y() : -INFINITY);
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 qs = *reinterpret_cast<const float4*>(row + j);
+                        const float4 nl = *reinterpret_cast<const float4*>(row + 2 * kTile + j);
+                        s[j / 2] = fma2(fma2(f2(nz), f2(qs.x, qs.y), f2(__uint_as_float(x[j]), __uint_as_float(x[j + 1]))), f2(sk), f2(nl.x, nl.y));
+                        s[j / 2 + 1] =
+                            fma2(fma2(f2(nz), f2(qs.z, qs.w), f2(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3]))), f2(sk), f2(nl.z, nl.w));
                     }
-                    add = add + f2(ex2(x.x()), ex2(x.y()));
-                    add = add + f2(ex2(y.x()), ex2(y.y()));
+                    if (!all) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            const int4 lim = *reinterpret_cast<const int4*>(row + 3 * kTile + j);
+                            s[j / 2] = f2(slot < lim.x ? s[j / 2].x() : -INFINITY, slot < lim.y ? s[j / 2].y() : -INFINITY);
+                            s[j / 2 + 1] = f2(slot < lim.z ? s[j / 2 + 1].x() : -INFINITY, slot < lim.w ? s[j / 2 + 1].y() : -INFINITY);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) add = add + f2(ex2(s[j].x()), ex2(s[j].y()));
                 }
+                tm_before_sync();
+                mbar_arrive(bars + 8 * (kCmSFree + buf));
+                if (there)
+                    sums[(at.at.job - at.at.job / a.n_rt * a.n_rt) * lines + static_cast<long long>(unit) * kKvTokens + trow % kKvTokens] = add.x() + add.y();
             }
-            const float sum = add.x() + add.y();
-            float* other = word(S::kSum) + buf * kBlk;
-            if (half == 1) other[trow] = sum;
-            tm_before_sync();
-            named_bar_sync(2, kSoft);
-            if (half == 0 && there) {
-                const int h = at.at.job / a.n_rt, rt = at.at.job - h * a.n_rt, page = kv_page(c, at.at.b, slot);
-                if (page >= 0) sums[rt * lines + static_cast<long long>(kv_line(c, page, h) + slot % c.page_size)] = sum + other[trow];
+            if (i + 1 < n && at.next(p, c.n_seqs, u0 + i + 1)) {
+                named_bar_sync(2, kSoft);  // all have read the old rows' constants; S of them is done
+                load_q();
             }
-            mbar_arrive(bars + 8 * (kPFull + buf));
-            if (i + 1 < n && at.next(p, c.n_seqs, u0 + i + 1)) load_q();  // S of the old rows is done
         }
     } else if (n > 0 && warp < kMmaWarp) {
         const int dw = warp - kSoftWarps;
         for (int i = 0; i < n; ++i) {
-            const int buf = i & 1;
-            wait(kRawFull + buf, i >> 1);
-            if (i >= 2) wait(kSFull + buf, (i - 2) >> 1);
-            const uint32_t got = reinterpret_cast<const uint32_t*>(word(S::kMisc))[16 + buf];
-            const char* raw = base + S::kRaw + buf * kUnits * S::kRawUnit;
+            const int buf = i & 1, from = i & 3;
+            wait(kCmRawFull + from, i >> 2);
+            if (i >= 2) wait(kCmSFull + ((i - 2) & 3), (i - 2) >> 2);
+            const uint32_t got = reinterpret_cast<const uint32_t*>(word(S::kMisc))[from];
+            const char* raw = base + S::kRaw + from * S::kRawBytes;
 #pragma unroll 1
-            for (int e = 0; e < 2; ++e) unpack_keys<D>(raw + (2 * dw + e) * S::kRawUnit, base + S::kK + buf * S::kOp, 2 * dw + e, lane);
+            for (int e = 0; e < 2; ++e) unpack_keys<D>(raw + (2 * dw + e) * kv_unit_bytes(D), base + S::kK + buf * S::kOp, 2 * dw + e, lane);
             const int u = 2 * dw + (lane >> 4), slot = 32 * dw + lane;
             const bool on = (got >> u & 1u) && at.at.step * kBlk + slot < at.at.len;
-            const uint32_t pw = *reinterpret_cast<const uint32_t*>(raw + u * S::kRawUnit + 8 * D + 8 * (lane & 15));
-            float* par = word(S::kPar + (i & 3) * (2 * kBlk * 4));
+            const uint32_t pw = *reinterpret_cast<const uint32_t*>(raw + u * kv_unit_bytes(D) + kv_param_offset(D) + 8 * (lane & 15));
+            float* par = word(S::kPar + (i & 7) * (2 * kBlk * 4));
             par[slot] = on ? 8.f - h2f_bits(hi16(pw)) : 0.f;
             par[kBlk + slot] = on ? h2f_bits(lo16(pw)) * a.scale2 : 0.f;
             const uint32_t there = __ballot_sync(0xffffffffu, on);
-            if (lane == 0) reinterpret_cast<uint32_t*>(word(S::kMisc + (i & 3) * 16))[dw] = there;
+            if (lane == 0) reinterpret_cast<uint32_t*>(word(S::kThere + (i & 7) * 16))[dw] = there;
             fence_async_smem();
-            mbar_arrive(bars + 8 * (kKFull + buf));
-            mbar_arrive(bars + 8 * (kRawFree + buf));
+            mbar_arrive(bars + 8 * (kCmKFull + buf));
+            mbar_arrive(bars + 8 * (kCmRawFree + from));
             if (i + 1 < n) at.next(p, c.n_seqs, u0 + i + 1);
         }
     } else if (n > 0 && warp == kMmaWarp) {
@@ -788,59 +809,56 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
         bool begins = true;
         for (int i = 0; i < n; ++i) {
             const int buf = i & 1;
-            if (begins) wait(kQFull, jobs++);
-            wait(kKFull + buf, i >> 1);
-            if (i >= 2) wait(kPFull + buf, (i - 2) >> 1);
+            if (begins) wait(kCmQFull, jobs++);
+            wait(kCmKFull + buf, i >> 1);
+            if (i >= 4) wait(kCmSFree + (i & 3), (i - 4) >> 2);
             tm_after_sync();
             if (lane == 0) {
                 const uint32_t kb = smem0 + S::kK + buf * S::kOp;
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
-                    tm_mma_ss(tm + buf * kTile, operand(kb + k / 4 * (kBlk * 128) + 32 * (k % 4)),
+                    tm_mma_ss(tm + (i & 3) * kTile, operand(kb + k / 4 * (kBlk * 128) + 32 * (k % 4)),
                               operand(smem0 + S::kQ + k / 4 * (kTile * 128) + 32 * (k % 4)), mma_shape(kTile), k > 0);
-                tm_commit(bars + 8 * (kSFull + buf));
+                tm_commit(bars + 8 * (kCmSFull + (i & 3)));
             }
             __syncwarp();
             begins = i + 1 < n && at.next(p, c.n_seqs, u0 + i + 1);
         }
-        wait(kSFull + ((n - 1) & 1), (n - 1) >> 1);
+        wait(kCmSFull + ((n - 1) & 3), (n - 1) >> 2);
     } else if (n > 0) {
-        // ---- loading: a lane a unit
+        // ---- loading, as above
         int asked = 0;
         for (int i = 0; i < n; ++i) {
-            const int buf = i & 1, slot = at.at.step * kBlk + lane * kKvTokens;
+            const int buf = i & 3, slot = at.at.step * kBlk + lane * kKvTokens;
             int index = -1;
             if (lane < kUnits && slot < at.at.len) {
                 const int page = kv_page(c, at.at.b, slot);
                 if (page >= 0) index = static_cast<int>((kv_line(c, page, at.at.job / a.n_rt) + slot % c.page_size) / kKvTokens);
             }
-            if (i >= 2) wait(kRawFree + buf, (i - 2) >> 1);
+            if (i >= 4) wait(kCmRawFree + buf, (i - 4) >> 2);
             if (dead) break;
             asked = i + 1;
-            const uint32_t got = __ballot_sync(0xffffffffu, index >= 0), bar = bars + 8 * (kRawFull + buf);
+            const uint32_t got = __ballot_sync(0xffffffffu, index >= 0), bar = bars + 8 * (kCmRawFull + buf);
+            if (lane < kUnits) sts_u32(smem0 + S::kIndex + ((i & 15) * kUnits + lane) * 4, static_cast<uint32_t>(index));
+            __syncwarp();
             if (lane == 0) {
-                sts_u32(smem0 + S::kMisc + 64 + buf * 4, got);
-                if (got) mbar_arrive_expect_tx(bar, __popc(got) * S::kRawUnit);
+                sts_u32(smem0 + S::kMisc + buf * 4, got);
+                if (got) mbar_arrive_expect_tx(bar, __popc(got) * kv_unit_bytes(D));
                 else mbar_arrive(bar);
             }
             __syncwarp();
-            if (index >= 0) {
-                const uint32_t dst = smem0 + S::kRaw + (buf * kUnits + lane) * S::kRawUnit;
-                const uint8_t* src = c.units + static_cast<size_t>(index) * kv_unit_bytes(D);
-                bulk_g2s(dst, src, 8 * D, bar);
-                bulk_g2s(dst + 8 * D, src + kv_param_offset(D), kKvTokens * 8, bar);
-            }
+            copy_units<D>(c, smem0 + S::kRaw + buf * S::kRawBytes, index, got, lane, bar);
             if (i + 1 < n) at.next(p, c.n_seqs, u0 + i + 1);
         }
         // given up: the copies in flight must end before the shared memory goes
         if (dead)
-            for (int j = max(asked - 2, 0); j < asked; ++j) mbar_wait_bounded(bars + 8 * (kRawFull + (j & 1)), (j >> 1) & 1);
+            for (int j = max(asked - 4, 0); j < asked; ++j) mbar_wait_bounded(bars + 8 * (kCmRawFull + (j & 3)), (j >> 2) & 1);
     }
     tm_before_sync();
     __syncthreads();
     if (warp == kMmaWarp) {
         tm_after_sync();
-        tm_dealloc(tm, 256);
+        tm_dealloc(tm, kTmCols);
     }
 }
 
