@@ -34,6 +34,10 @@
 // The 8 is the same for all columns: one MMA a unit with a constant A collects
 // 8 sum p' and every 8 steps it is taken off all of O, which keeps the running
 // sums (FP32, and the rounding of p' in them) at the size of the centred values.
+// An MMA cuts its terms off below the largest (a subnormal counts as 2^-14), and
+// codes all have one sign: the output of 128K slots, a thousandth of a value's
+// size, leaned by 2e-4 of it.  So the second unit of a step is taken the other
+// way round, -p' with 15 - c, and the errors cancel (1% of the time).
 // p' is the only rounding to FP16 besides the output's: p <= 2^8 (the maximum
 // is taken again only when a score passes it by 8) and w is the power of two
 // that brings the largest s_v seen to at most 2^7, so p' <= 2^15 and small
@@ -57,6 +61,12 @@ __host__ __device__ constexpr int at_ctas(int nt) { return nt == 1 ? 2 : 1; }
 // f16 pairs c 2^-24 of the nibbles at bits 0..3 and 16..19, c 2^-20 of those at bits 4..7 and 20..23.
 __device__ __forceinline__ uint32_t low_codes(uint32_t w) { return w & 0x000F000Fu; }
 __device__ __forceinline__ uint32_t high_codes(uint32_t w) { return w & 0x00F000F0u; }
+// mask & ~w, the codes 15 - c, in one instruction (left to itself, ~w would be one of its own)
+__device__ __forceinline__ uint32_t and_not(uint32_t mask, uint32_t w) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %1, 0x30;" : "=r"(r) : "r"(mask), "r"(w));
+    return r;
+}
 
 // mma_16816 that the compiler may move (it has no effect besides its result).
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -358,7 +368,7 @@ struct StepStream {
 // The running softmax of one job in one warp: rows 2t, 2t + 1 of each row tile.
 template <int D, int NT>
 struct RowState {
-    float o[NT][D / 16][4], c8[NT][4], vw;  // c8: - 8 sum p' since the last settle(), in either scale of o
+    float o[NT][D / 16][4], c8[NT][4], vw;  // c8: -+ 8 sum p' since the last settle(), in either scale of o
     f2 m[NT], l[NT], zs[NT];  // m: minus the running maximum
 
     __device__ __forceinline__ void clear() {
@@ -377,8 +387,9 @@ struct RowState {
     }
 
     // Scores and weights of U units from slot j of the sequence on, the weights as the B operands of their
-    // output product, and the units' V codes.  found: bit u set where unit u is there.
-    template <int U, bool kScores>
+    // output product, and the units' V codes.  found: bit u set where unit u is there.  kFirst: the first unit's
+    // place in its step.
+    template <int U, int kFirst, bool kScores>
     __device__ __forceinline__ void weigh(const QueryTile<D, NT>& q, int unit, int j, int len, uint32_t found, float scale2,
                                           uint32_t (&pf)[U][NT][2], uint32_t (&v)[U][2][D / 32], float* scores, int pitch,
                                           int2 index) {
@@ -394,7 +405,8 @@ struct RowState {
                 const uint2 p = smem_at<uint2>(pa + 64 * x);
                 const f2 sk(h2f_bits(lo16(p.x)) * scale2), zk(h2f_bits(hi16(p.x)));
                 sv[u][x] = h2f_bits(lo16(p.y));
-                zv[u][x] = h2f_bits(hi16(p.y)) - 8.f;
+                // -p' (15 - c) + 8 p' - p' = p' (c - 8)
+                zv[u][x] = (u + kFirst) % 2 ? 7.f - h2f_bits(hi16(p.y)) : h2f_bits(hi16(p.y)) - 8.f;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) s[u][nt][x] = fma2(zk, q.sum[nt], s[u][nt][x]) * sk;
             }
@@ -457,7 +469,7 @@ struct RowState {
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                const f2 w(sv[u][x] * vw), z(zv[u][x]);
+                const f2 w((u + kFirst) % 2 ? -(sv[u][x] * vw) : sv[u][x] * vw), z(zv[u][x]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     const f2 d = s[u][nt][x] + m[nt], e(ex2(d.x()), ex2(d.y())), p = e * w;
@@ -470,11 +482,13 @@ struct RowState {
 
     // The output product of what weigh() left.  Rows g of an MMA are columns of low nibbles, rows g + 8 of
     // high ones; the constants are -8 in either.
-    template <int U>
+    template <int U, int kFirst>
     __device__ __forceinline__ void output(const uint32_t (&pf)[U][NT][2], const uint32_t (&v)[U][2][D / 32]) {
         constexpr uint32_t kLow8 = 0x80088008u, kHigh8 = 0x80808080u;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+            auto lows = [&](uint32_t w) { return (u + kFirst) % 2 ? and_not(0x000F000Fu, w) : low_codes(w); };
+            auto highs = [&](uint32_t w) { return (u + kFirst) % 2 ? and_not(0x00F000F0u, w) : high_codes(w); };
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma(c8[nt], kLow8, kHigh8, kLow8, kHigh8, pf[u][nt][0], pf[u][nt][1]);
 #pragma unroll
@@ -483,8 +497,8 @@ struct RowState {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     const uint32_t b0 = pf[u][nt][0], b1 = pf[u][nt][1];
-                    mma(o[nt][2 * k], low_codes(w0), high_codes(w0), low_codes(w1), high_codes(w1), b0, b1);
-                    mma(o[nt][2 * k + 1], low_codes(y0), high_codes(y0), low_codes(y1), high_codes(y1), b0, b1);
+                    mma(o[nt][2 * k], lows(w0), highs(w0), lows(w1), highs(w1), b0, b1);
+                    mma(o[nt][2 * k + 1], lows(y0), highs(y0), lows(y1), highs(y1), b0, b1);
                 }
             }
         }
@@ -645,19 +659,19 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
                         uint32_t pf[2][NT][2], v[2][2][D / 32];
                         int2 index = make_int2(-1, -1);
                         if (kScores) index = st.unit_index();
-                        rs.template weigh<2, kScores>(q, st.unit(), j, len, found, a.scale2, pf, v, a.scores, a.pitch, index);
+                        rs.template weigh<2, 0, kScores>(q, st.unit(), j, len, found, a.scale2, pf, v, a.scores, a.pitch, index);
                         st.next(a, p);
-                        rs.template output<2>(pf, v);
+                        rs.template output<2, 0>(pf, v);
                     } else {
                         uint32_t pf[1][NT][2], v[1][2][D / 32];
-                        rs.template weigh<1, false>(q, st.unit(), j, len, found & 1u, a.scale2, pf, v, nullptr, 0, make_int2(-1, -1));
-                        rs.template output<1>(pf, v);
+                        rs.template weigh<1, 0, false>(q, st.unit(), j, len, found & 1u, a.scale2, pf, v, nullptr, 0, make_int2(-1, -1));
+                        rs.template output<1, 0>(pf, v);
                         const bool second = j + kKvTokens < q.max_lim;
                         if (second)
-                            rs.template weigh<1, false>(q, st.unit() + kv_unit_bytes(D), j + kKvTokens, len, found >> 1, a.scale2, pf, v,
+                            rs.template weigh<1, 1, false>(q, st.unit() + kv_unit_bytes(D), j + kKvTokens, len, found >> 1, a.scale2, pf, v,
                                                  nullptr, 0, make_int2(-1, -1));
                         st.next(a, p);
-                        if (second) rs.template output<1>(pf, v);
+                        if (second) rs.template output<1, 1>(pf, v);
                     }
                 } else {
                     st.next(a, p);
