@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
                 }
                 const float now = fmaxf(m, top), f = now == m ? 1.f : ex2(m - now), fr = f * ratio;
                 m = now;
-                l *= f;
+                l *= fr;
                 zs *= fr;
                 if (!begins) {
                     // O is the softmax warps' once the last block's product is in it
@@ -378,6 +378,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
                     tm_wait_st();
                 }
             }
+            // 2^(s - m) w at once: l too is in units of 1 / w
+            const f2 shift(static_cast<float>(static_cast<int>(__float_as_uint(vw) >> 23) - 127) - m);
             f2 l2(0.f), z2(0.f);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -388,8 +390,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
                     const float4 z4 = *reinterpret_cast<const float4*>(par + 3 * kBlk + 32 * k + j);
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const f2 d = s[16 * k + j / 2 + e] + f2(-m), x(ex2(d.x()), ex2(d.y()));
-                        const f2 pr = x * (f2(e ? w4.z : w4.x, e ? w4.w : w4.y) * f2(vw));
+                        const f2 d = s[16 * k + j / 2 + e] + shift, x(ex2(d.x()), ex2(d.y()));
+                        const f2 pr = x * f2(e ? w4.z : w4.x, e ? w4.w : w4.y);
                         l2 = l2 + x;
                         z2 = fma2(pr, f2(e ? z4.z : z4.x, e ? z4.w : z4.y), z2);
                         pk[j / 2 + e] = pack_f32(pr.x(), pr.y());
@@ -413,8 +415,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
             sums[(2 + half) * kTile + trow] = zs;
             if (!last) load_q();  // S of the old rows is done; the new ones' can start
             else named_bar_sync(2, kSoft);
-            const float lsum = sums[trow] + sums[kTile + trow], zsum = sums[2 * kTile + trow] + sums[3 * kTile + trow];
             const float inv_w = __uint_as_float(0x7F000000u - __float_as_uint(vw));
+            const float lsum = (sums[trow] + sums[kTile + trow]) * inv_w, zsum = sums[2 * kTile + trow] + sums[3 * kTile + trow];
             wait(kVFree + buf, i >> 1);
             tm_after_sync();
             const bool whole = first == 0 && was.step + 1 == blocks;
