@@ -108,6 +108,7 @@ public:
             out = out_in->dim() == 3 ? out_in->unsqueeze(1) : *out_in;
             TORCH_CHECK(direct(out), "out needs head_dim contiguous, strides multiples of 8 and a 16-byte aligned start");
             TORCH_CHECK(apart(out), "out must not overlap itself");
+            TORCH_CHECK(!meet(out, q), "out must not lie among q's rows: rows are read after others are written");
         } else {
             out = torch::empty({q.size(0), q.size(1), q.size(2), q.size(3)}, q.options());
         }
@@ -168,6 +169,16 @@ private:
             extent = (t.size(i) - 1) * t.stride(i) + extent;
         }
         return true;
+    }
+    // Whether the memory between two tensors' first and last values overlaps.
+    static bool meet(const torch::Tensor& a, const torch::Tensor& b) {
+        if (a.numel() == 0 || b.numel() == 0) return false;
+        auto end = [](const torch::Tensor& t) {
+            int64_t last = 0;
+            for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+            return h16(t) + last + 1;
+        };
+        return h16(a) < end(b) && h16(b) < end(a);
     }
     // [n_seqs, T, heads, head_dim] float16, readable in place (heads 0: any number)
     torch::Tensor rows(const torch::Tensor& t_in, const char* name, int64_t heads) const {

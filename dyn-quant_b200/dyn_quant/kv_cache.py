@@ -10,7 +10,10 @@ layers on either side of the attention; dyn_quant.attention.Int4Attention joins
 them.
 
 A decode step issues kernel launches only (lengths live on the device), so it
-can be captured in a CUDA graph; calls on one cache must be stream-ordered.
+can be captured in a CUDA graph; calls on one cache must be stream-ordered.  Pages
+may be shared by sequences with a common beginning, but only to be read: append,
+evict and accumulated weights need pages that one sequence owns.  There are no
+gradients.
 """
 from __future__ import annotations
 
@@ -151,7 +154,7 @@ class Int4KVCache:
                         the rows of the others are zero, their lse -inf.
             accumulate: add each slot's attention weight, summed over query tokens
                         and the KV head's query heads, to `mass`.
-            out:        tensor to write into, of q's shape.
+            out:        tensor to write into, of q's shape, not among q's memory.
             return_lse: also return log(sum(exp(scores))), float32, without head_dim.
 
         Returns:
@@ -165,7 +168,8 @@ class Int4KVCache:
         """Cut every sequence of more than `keep` slots to `keep`, head by head:
         the last `recent` and the first `sink` positions stay, and of the other
         slots those with the largest `mass` (equal ones: lowest slot first).
-        Kept slots beyond `keep` move into the freed ones below (one kernel)."""
+        Kept slots beyond `keep` move into the freed ones below (one kernel, two
+        when more than 256 slots of a head may have to move)."""
         self._h.evict(keep, recent, sink)
 
     def read(self, seq: int):

@@ -65,14 +65,17 @@ def attend(q, line, n, scale, count=None):
             terms = abs(scale) * line["ks"][e, :seen] * (np.abs(q[i, a]) @ line["kc"][e, :seen].T
                                                          + np.abs(line["kz"][e, :seen]) * np.abs(q[i, a]).sum())
             rel = 2 * (24 * 2.0 ** -23 * terms.max() + 2.0 ** -22 + 2.0 ** -22 * np.abs(s).max()) + 2.0 ** -20
-            # Output: p' = p s w is rounded to FP16 once (2^-11 of p s |c - 8|; below 2^-14 half of 2^-24, with
-            # 1 / w <= 2^-6 max s), the sums are FP32 (one truncation per unit), the result is rounded to FP16.
+            # Output: p' = p s w is rounded to FP16 once (2^-11 of p s |c - 8| or, in units counted from 15, of
+            # p s |c - 7|; below 2^-14 half of 2^-24, with 1 / w <= 2^-6 max s), the sums are FP32 (one truncation
+            # per unit), the result is rounded to FP16.  Within an MMA the 16 terms and the sum are cut off 2^-23 below
+            # the largest, where a code's subnormal c 2^-24 counts as 2^-14: 17 times 2^-13 of the unit's largest p s.
             sv = line["vs"][e, :seen]
-            s8 = (p * sv) @ np.abs(line["vc"][e, :seen] - 8)
+            s8 = (p * sv) @ (np.abs(line["vc"][e, :seen] - 7.5) + 0.5)
+            cut = 17 * 2.0 ** -13 * np.pad(p * sv, (0, -seen % 16)).reshape(-1, 16).max(1).sum()
             sz = (p * sv) @ np.abs(line["vz"][e, :seen] - 8)
             sums = (seen / 16 + 64) * 2.0 ** -23
             tol[i, a] = (H16 * (np.abs(out[i, a]) + s8) + 2.0 ** -25 + rel * (p @ np.abs(v[e, :seen]) + s8 + sz)
-                         + sums * (s8 + sz) + 8 * seen * sv.max() * 2.0 ** -31)
+                         + sums * (s8 + sz) + 8 * seen * sv.max() * 2.0 ** -31 + cut)
             lse_tol[i, a] = rel + 2.0 ** -22 * abs(lse[i, a])
             mass_err[e, :seen] += rel * p
     return {"out": out, "tol": tol, "lse": lse, "lse_tol": lse_tol, "mass": mass, "mass_tol": mass_err}

@@ -242,6 +242,62 @@ def test_attend_many_rows(dim, heads, group, t, page, lens, counts):
     assert torch.equal(again, out) and torch.equal(lse2, lse)
 
 
+def test_attend_many_rows_in_long_runs():
+    """Some twenty blocks of a CTA's run in a row, over job borders: every buffer of the pipelines comes round."""
+    lens, t, group = [6000, 3500], 40, 16
+    cache = R.make_cache(lens, 8, 128, 64, seed=21)
+    q = R.queries(cache, t, group)
+    out, lse = cache.attend(q, accumulate=True, return_lse=True)
+    table = cache.page_table.cpu().numpy()
+    for b, n in enumerate(lens):
+        line = R.decode(cache.units, cache.page_table, 64, b, n)
+        gain = cache.mass.double().cpu().numpy()[table[b, np.arange(n) // 64], :, np.arange(n) % 64]
+        for e in (0, 5, 7):
+            one = {k: v[e:e + 1] for k, v in line.items()}
+            heads = slice(e * group, (e + 1) * group)
+            for at in (0, t - 2):  # the first and the last tile's tokens at, at + 1
+                seen = n - t + at + 2
+                r = R.attend(q[b, at:at + 2, heads], {k: v[:, :seen] for k, v in one.items()}, seen, 128 ** -0.5)
+                assert (np.abs(out[b, at:at + 2, heads].double().cpu().numpy() - r["out"]) <= r["tol"]).all()
+                assert (np.abs(lse[b, at:at + 2, heads].double().cpu().numpy() - r["lse"]) <= r["lse_tol"]).all()
+            # a row's weights sum to 1, each off by what its lse allows
+            assert abs(gain[:, e].sum() - t * group) <= t * group * (r["lse_tol"].max() + n * 2.0 ** -24)
+
+
+def test_attend_many_rows_of_most_sequences():
+    """1024 sequences, a third of them empty: the plan of the most sequences beside the largest tiles."""
+    lens = [(i * 29) % 60 if i % 3 else 0 for i in range(1024)]
+    lens[500] = 700
+    cache = R.make_cache(lens, 1, 128, 16, seed=22, mass=True)
+    q = R.queries(cache, 16, 4)
+    mass0 = cache.mass.clone()
+    out, lse = cache.attend(q, accumulate=True, return_lse=True)
+    R.check_attend(out, lse, q, cache, 128 ** -0.5, mass=cache.mass, mass0=mass0)
+
+
+def test_attend_many_rows_replayed():
+    cache = R.make_cache([900, 150], 2, 128, 16, seed=23, mass=True)
+    q = R.queries(cache, 24, 4)
+    mass0 = cache.mass.clone()
+    want = cache.attend(q, accumulate=True)
+    gain = cache.mass - mass0
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = cache.attend(q, accumulate=True)
+        cache.mass.copy_(mass0)
+        for _ in range(2):
+            graph.replay()
+            assert torch.equal(out, want)
+    stream.synchronize()
+    # two passes of the same weights, each step half a unit at most: the gain's own sum and difference count twice,
+    # the two running sums once
+    want2 = mass0.double() + 2 * gain.double()
+    assert ((cache.mass.double() - want2).abs() <= 6 * 2.0 ** -24 * (mass0.abs() + 2 * gain.abs()).double()).all()
+
+
 def test_attend_many_rows_of_very_different_size():
     """The tensor-memory accumulator is rescaled when the maximum moves and when larger V rows come."""
     cache = R.make_cache([0], 1, 128, 64, extra=600)
@@ -525,6 +581,9 @@ def test_refusals():
     bad(cache.attend, q, out=torch.empty_like(q[:, :, :2]))
     bad(cache.attend, q, out=torch.empty(1, 1, 4, 128, dtype=torch.float16, device="cuda").expand(2, 1, 4, 128))
     bad(cache.attend, q, out=torch.empty(2, 1, 128, 4, dtype=torch.float16, device="cuda").transpose(2, 3))
+    bad(cache.attend, q, out=q)
+    wide = torch.empty(2, 1, 8, 128, dtype=torch.float16, device="cuda")
+    bad(cache.attend, wide[:, :, :4], out=wide[:, :, 4:])
     bad(cache.append, k, k[:, :, :1])
     bad(cache.append, k[:, :, :1], k[:, :, :1])
     bad(cache.append, k.cpu(), k.cpu())
