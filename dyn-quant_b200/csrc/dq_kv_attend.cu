@@ -42,6 +42,14 @@
 // is taken again only when a score passes it by 8) and w is the power of two
 // that brings the largest s_v seen to at most 2^7, so p' <= 2^15 and small
 // weights keep their 11 bits down to 2^-29 of the largest.
+//
+// Measured: 64 sequences of 2000 to 4096 slots with 32 heads of 128 and one row
+// each, 850 MB, 176 us, 4.8 TB/s (75% of a copy's; 55% of the issue slots, the
+// tensor pipe 31%); 16 sequences of 1000 to 4100 slots with 8 heads of 8 rows,
+// 48 MB, 26 us; 131071 slots with 8 heads of 8 rows, 143 MB, 45 us; 8 sequences of
+// 200 to 8000 slots with 8 heads of 64 and 20 rows, 22 MB, 35 us with the join.
+// The smaller ones are bound by the chain lengths, pages, units, join: 77 slots of
+// 32 heads take 9 us.
 #include "dq_kv_plan.cuh"
 
 namespace dq {
@@ -831,7 +839,8 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
 
 // ---------------------------------------------------------------------------
 // Joins the partial sums of the jobs cut between CTAs when a KV head's rows fill
-// several tiles (their jobs have no arrival counters).  One warp per row.
+// several tiles (their jobs have no arrival counters).  One warp per row.  Bound
+// by its chain of loads: 5 us of the 35 of 1280 rows of 64 columns.
 // ---------------------------------------------------------------------------
 constexpr int kCbWarps = 4;
 
@@ -858,7 +867,8 @@ __global__ void __launch_bounds__(32 * kCbWarps) kv_combine_kernel(const KvAtten
 // every row's lse is known.  Up to 8 rows stay in registers for a whole job;
 // more are taken 32 at a time over up to four steps that wait in the ring, so a
 // tile of queries is arranged once for 128 slots.  A slot's sum is one lane
-// group's, in row order.
+// group's, in row order.  Where the first pass has kept the scores they are read
+// instead (12 us of 43 for 16 sequences of 2000 to 4100 slots, 8 heads of 8 rows).
 // ---------------------------------------------------------------------------
 __host__ __device__ constexpr int ms_warps(int nt) { return nt == 1 ? 8 : 12; }
 __host__ __device__ constexpr int ms_ctas(int nt) { return nt == 1 ? 2 : 1; }
