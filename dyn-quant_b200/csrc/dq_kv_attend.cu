@@ -840,7 +840,7 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
 // ---------------------------------------------------------------------------
 // Joins the partial sums of the jobs cut between CTAs when a KV head's rows fill
 // several tiles (their jobs have no arrival counters).  One warp per row.  Bound
-// by its chain of loads: 5 us of the 35 of 1280 rows of 64 columns.
+// by its chain of loads: 7 us by itself for 1280 rows of 64 columns.
 // ---------------------------------------------------------------------------
 constexpr int kCbWarps = 4;
 
@@ -868,7 +868,8 @@ __global__ void __launch_bounds__(32 * kCbWarps) kv_combine_kernel(const KvAtten
 // more are taken 32 at a time over up to four steps that wait in the ring, so a
 // tile of queries is arranged once for 128 slots.  A slot's sum is one lane
 // group's, in row order.  Where the first pass has kept the scores they are read
-// instead (12 us of 43 for 16 sequences of 2000 to 4100 slots, 8 heads of 8 rows).
+// instead (16 sequences of 2000 to 4100 slots, 8 heads of 8 rows: 15 us by itself,
+// 43 with the attention).
 // ---------------------------------------------------------------------------
 __host__ __device__ constexpr int ms_warps(int nt) { return nt == 1 ? 8 : 12; }
 __host__ __device__ constexpr int ms_ctas(int nt) { return nt == 1 ? 2 : 1; }
@@ -1118,8 +1119,8 @@ constexpr int chunk_min(int head_dim) { return head_dim == 128 ? 64 : 80; }
 // Row tiles of one warp: 8 rows when a KV head has no more, else 16.
 int row_tiles(int rows) { return rows <= 8 ? 1 : 2; }
 
-// What the mass pass may keep in the workspace (scores of up to 8 rows, or a line of sums for each tile of 128);
-// without that room it reads the keys a second time.
+// What the mass pass may keep in the workspace (scores of up to 8 rows, or a line of sums for each of several tiles of
+// 128); without that room kv_mass_kernel reads the keys a second time.
 constexpr size_t kMaxScores = size_t{1} << 30;
 
 int score_pitch(int rows) { return rows <= 2 ? rows : (rows <= 4 ? 4 : 8); }
@@ -1140,7 +1141,8 @@ AttendWs attend_ws(const dq_kv_cache_t& c, int tokens, int q_heads, bool mass) {
     w.scores = w.lse2 + (mass ? align256(static_cast<size_t>(c.n_seqs) * tokens * q_heads * 4) : 0);
     const int group_rows = tokens * (q_heads / c.kv_heads);
     const size_t line = static_cast<size_t>(c.n_pages) * c.kv_heads * c.page_size * sizeof(float);
-    const size_t kept = line * (chunk ? (group_rows + kChunkRows - 1) / kChunkRows : score_pitch(group_rows));
+    const size_t tiles = (group_rows + kChunkRows - 1) / kChunkRows;
+    const size_t kept = line * (chunk ? (tiles > 1 ? tiles : 0) : score_pitch(group_rows));
     w.total = w.scores + (mass && (chunk || nt == 1) && group_rows > 0 && kept <= kMaxScores ? align256(kept) : 0);
     return w;
 }
@@ -1176,8 +1178,9 @@ dq_status_t launch_kv_attend(const dq_kv_cache_t& c, const dq_kv_attend_t& r, vo
     if (rows >= chunk_min(c.head_dim)) {
         KvAttendArgs b = a;
         b.scale2 = r.scale * 1.44269504088896341f;  // its codes are whole numbers
-        const dq_status_t st = launch_kv_chunk(b, c.head_dim, a.scores, stream);
-        if (st != DQ_OK || !a.lse2 || a.scores) return st;
+        const bool there = a.lse2 && (a.scores || rows <= kChunkRows);
+        const dq_status_t st = launch_kv_chunk(b, c.head_dim, there, a.scores, stream);
+        if (st != DQ_OK || !a.lse2 || there) return st;
         DeviceInfo di;
         const dq_status_t sd = device_info(&di);
         if (sd != DQ_OK) return sd;

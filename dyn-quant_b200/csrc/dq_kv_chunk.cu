@@ -640,8 +640,10 @@ __global__ void __launch_bounds__(32 * kCcWarps) kv_chunk_combine_kernel(const K
 // Accumulated weight for many rows: the keys once more, transposed.  S^T = K Q^T
 // has a slot a TMEM lane, so a thread adds its slot's weights over the tile's
 // rows by itself, with the rows' sums of q
-// and lse from shared memory.  Each row tile's sums go to their own line of the
-// workspace; kv_tile_mass_kernel adds them to mass in tile order.  The two halves
+// and lse from shared memory.  One row tile's sums are added to mass at once; those
+// of several go to lines of their own in the workspace, which kv_tile_mass_kernel
+// adds to mass in tile order (two sequences of 8000 slots, 8 heads of 128 rows:
+// the call takes 51 us, 60 with the lines).  The two halves
 // of the softmax warps take the blocks in turn, a slot's 128 rows a thread, and
 // four S tiles keep the MMAs ahead of them: 41 us where one block at a time, its
 // rows split over two threads, took 51.
@@ -786,8 +788,12 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
                 }
                 tm_before_sync();
                 mbar_arrive(bars + 8 * (kCmSFree + buf));
-                if (there)
-                    sums[(at.at.job - at.at.job / a.n_rt * a.n_rt) * lines + static_cast<long long>(unit) * kKvTokens + trow % kKvTokens] = add.x() + add.y();
+                if (there) {
+                    const long long line = static_cast<long long>(unit) * kKvTokens + trow % kKvTokens;
+                    const float sum = add.x() + add.y();
+                    if (a.n_rt == 1) atomicAdd(c.mass + line, sum);  // the slot's only one: no order, and nothing waits for it
+                    else sums[(at.at.job - at.at.job / a.n_rt * a.n_rt) * lines + line] = sum;
+                }
             }
             if (i + 1 < n && at.next(p, c.n_seqs, u0 + i + 1)) {
                 named_bar_sync(2, kSoft);  // all have read the old rows' constants; S of them is done
@@ -902,7 +908,7 @@ __global__ void __launch_bounds__(32 * kTmWarps) kv_tile_mass_kernel(const KvAtt
 }
 
 template <int D>
-dq_status_t chunk(KvAttendArgs a, float* sums, cudaStream_t stream) {
+dq_status_t chunk(KvAttendArgs a, bool weights, float* sums, cudaStream_t stream) {
     DeviceInfo di;
     dq_status_t st = device_info(&di);
     if (st != DQ_OK) return st;
@@ -918,11 +924,12 @@ dq_status_t chunk(KvAttendArgs a, float* sums, cudaStream_t stream) {
     const long long items = static_cast<long long>(a.c.n_seqs) * a.tokens * a.c.heads * a.group;
     st = launch_pdl(kv_chunk_combine_kernel<D>, dim3(static_cast<unsigned>((items + kCcWarps - 1) / kCcWarps)), 32 * kCcWarps, 0,
                     stream, 1, a, ctas);
-    if (st != DQ_OK || !sums) return st;
+    if (st != DQ_OK || !weights) return st;
     const long long lines = static_cast<long long>(a.c.n_pages) * a.c.heads * a.c.page_size;
     smem = plan + 1024 + CmSmem<D>::kTotal;
     if ((st = allow(kv_chunk_mass_kernel<D>, smem)) != DQ_OK) return st;
-    if ((st = launch_pdl(kv_chunk_mass_kernel<D>, dim3(ctas), kCkThreads, smem, stream, 1, a, sums, lines)) != DQ_OK) return st;
+    st = launch_pdl(kv_chunk_mass_kernel<D>, dim3(ctas), kCkThreads, smem, stream, 1, a, sums, lines);
+    if (st != DQ_OK || a.n_rt == 1) return st;
     a.jobs = Div(a.c.heads);
     return launch_pdl(kv_tile_mass_kernel, dim3(di.sm_count * 4), 32 * kTmWarps, plan, stream, 1, a, sums, lines);
 }
@@ -931,11 +938,11 @@ dq_status_t chunk(KvAttendArgs a, float* sums, cudaStream_t stream) {
 
 size_t kv_chunk_part_rows() { return static_cast<size_t>(kChunkCtas) * 2 * kTile; }
 
-dq_status_t launch_kv_chunk(KvAttendArgs a, int head_dim, float* sums, cudaStream_t stream) {
+dq_status_t launch_kv_chunk(KvAttendArgs a, int head_dim, bool weights, float* sums, cudaStream_t stream) {
     const int rows = a.tokens * a.group;
     a.n_rt = Div((rows + kTile - 1) / kTile);
     a.jobs = Div(a.c.heads * a.n_rt);
-    return head_dim == 128 ? chunk<128>(a, sums, stream) : chunk<64>(a, sums, stream);
+    return head_dim == 128 ? chunk<128>(a, weights, sums, stream) : chunk<64>(a, weights, sums, stream);
 }
 
 dq_status_t read_kv_chunk_error(uint32_t* word, bool clear) {

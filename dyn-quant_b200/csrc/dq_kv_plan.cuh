@@ -32,8 +32,8 @@ struct KvAttendArgs {
 // Attention of many query rows per KV head (dq_kv_chunk.cu): workspace rows, and the launch (a's lse2 filled in too).
 constexpr int kChunkRows = 128;  // query rows of a tile
 size_t kv_chunk_part_rows();     // rows of part / part_ml
-// sums: room for the mass pass, [row tiles][n_pages][kv_heads][page_size], or null: no mass pass.
-dq_status_t launch_kv_chunk(KvAttendArgs a, int head_dim, float* sums, cudaStream_t stream);
+// weights: run the mass pass.  sums: its room, [row tiles][n_pages][kv_heads][page_size], for more tiles than one.
+dq_status_t launch_kv_chunk(KvAttendArgs a, int head_dim, bool weights, float* sums, cudaStream_t stream);
 
 namespace {
 

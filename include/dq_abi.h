@@ -471,7 +471,7 @@ DQ_API size_t dq_kv_attend_workspace_bytes(const dq_kv_cache_t* cache, int32_t t
  * word.  Slots behind lengths[b] are not read into any result.  Results are
  * bit-reproducible.  One kernel when a KV head has at most 16 query rows (query
  * tokens times its query heads), else two; one more with accumulate, two more
- * from 64 rows on (80 with head_dim 64).  out must not overlap q.  With
+ * beyond 128 rows.  out must not overlap q.  With
  * accumulate the workspace keeps scores or partial sums of up to 1 GiB, and
  * where they would be more the keys are read once more instead.
  */
