@@ -239,7 +239,7 @@ __device__ __forceinline__ void score_mma(int unit, const QueryTile<D, NT>& q, f
 
 // A warp's run of steps through its ring: lane i % 32 of each 32 steps looks
 // the step's pages up and issues its copies.
-template <int D, bool kKeysOnly>
+template <int D>
 struct StepStream {
     static constexpr int kUnit = kv_unit_bytes(D);
     static constexpr int kSlot = 2 * kUnit;
@@ -273,7 +273,7 @@ struct StepStream {
         StepAt x{0, 0, 0, 0};
         if (i < n) {
             x = step_at(p, a.c.n_seqs, u0 + i);
-            const int h = kKeysOnly ? x.job : x.job / a.n_rt;
+            const int h = x.job / a.n_rt;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int s = x.step * kStep + e * kKvTokens;
@@ -293,7 +293,7 @@ struct StepStream {
         if ((threadIdx.x & 31) == 0) {
             const uint32_t bar = base() + bars + 8 * s, dst = base() + ring + s * kSlot;
             asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(base() + units + 8 * s), "r"(i0), "r"(i1) : "memory");
-            if (!kKeysOnly && i0 >= 0 && i1 == i0 + 1) {
+            if (i0 >= 0 && i1 == i0 + 1) {
                 mbar_arrive_expect_tx(bar, kSlot);
                 bulk_g2s(dst, a.c.units + static_cast<size_t>(i0) * kUnit, kSlot, bar);
             } else {
@@ -302,26 +302,15 @@ struct StepStream {
         }
         ++issued;
     }
-    // A step's units one by one: from different pages, one of them missing, or their keys alone.
+    // A step's units one by one: from different pages, or one of them missing.
     __device__ __forceinline__ void issue_units(const KvAttendArgs& a, uint32_t bar, uint32_t dst, int i0, int i1) {
-        constexpr uint32_t kBytes = kKeysOnly ? 8 * D + kKvTokens * 8 : kUnit;
         if (i0 < 0 && i1 < 0) {
             mbar_arrive(bar);
             return;
         }
-        mbar_arrive_expect_tx(bar, (i0 >= 0 ? kBytes : 0u) + (i1 >= 0 ? kBytes : 0u));
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int i = e ? i1 : i0;
-            if (i < 0) continue;
-            const uint8_t* from = a.c.units + static_cast<size_t>(i) * kUnit;
-            if (kKeysOnly) {
-                bulk_g2s(dst + e * kUnit, from, 8 * D, bar);
-                bulk_g2s(dst + e * kUnit + kv_param_offset(D), from + kv_param_offset(D), kKvTokens * 8, bar);
-            } else {
-                bulk_g2s(dst + e * kUnit, from, kUnit, bar);
-            }
-        }
+        mbar_arrive_expect_tx(bar, (i0 >= 0 ? kUnit : 0) + (i1 >= 0 ? kUnit : 0));
+        if (i0 >= 0) bulk_g2s(dst, a.c.units + static_cast<size_t>(i0) * kUnit, kUnit, bar);
+        if (i1 >= 0) bulk_g2s(dst + kUnit, a.c.units + static_cast<size_t>(i1) * kUnit, kUnit, bar);
     }
     // Where the run begins; then fill() asks for its first steps.
     __device__ __forceinline__ StepAt start(const KvAttendArgs& a, const Plan& p, long long first, int count) {
@@ -340,16 +329,11 @@ struct StepStream {
         const int m = min(depth, n);
         for (int i = 0; i < m; ++i) issue(a, p, i);
     }
-    // Wait for the step `ahead` slots on; false when the bounded wait gave up.
-    __device__ __forceinline__ bool wait(int ahead = 0) {
-        const bool wrap = slot + ahead >= depth;
-        const bool got = mbar_wait_bounded(base() + bars + 8 * (slot + ahead - (wrap ? depth : 0)), parity ^ (wrap ? 1 : 0));
-        return __all_sync(0xffffffffu, got);
+    // Wait for the step's copies; false when the bounded wait gave up.
+    __device__ __forceinline__ bool wait() {
+        return __all_sync(0xffffffffu, mbar_wait_bounded(base() + bars + 8 * slot, parity));
     }
     __device__ __forceinline__ int unit() const { return ring + slot * kSlot; }
-    __device__ __forceinline__ int unit(int ahead) const {
-        return ring + (slot + ahead - (slot + ahead >= depth ? depth : 0)) * kSlot;
-    }
     // The step's units in the pool, -1: not copied.
     __device__ __forceinline__ int2 unit_index() const { return smem_at<int2>(units + 8 * slot); }
     // Bit e: unit e of the step was copied (only asked for when some unit of the run is absent).
@@ -588,7 +572,7 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
     __shared__ Share share[2];
     __shared__ bool join[2];
     __shared__ int kept, place[W];
-    StepStream<D, false> st;
+    StepStream<D> st;
     st.init(plan_bytes(c.n_seqs), W, warp, a.depth);
     // A piece is a row of D + 2 floats for each row of the job: output, maximum, sum.  A warp's last piece
     // takes its ring, which has run dry by then; one of a job that ends inside the run takes one of the
@@ -597,7 +581,7 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
     if (threadIdx.x == 0) kept = 0;
     auto piece_at = [&](int k) {
         const int i = k >> 1;
-        if (k & 1) return reinterpret_cast<float*>(smem + plan_bytes(c.n_seqs) + i * a.depth * StepStream<D, false>::kSlot);
+        if (k & 1) return reinterpret_cast<float*>(smem + plan_bytes(c.n_seqs) + i * a.depth * StepStream<D>::kSlot);
         if (place[i] < a.places) return reinterpret_cast<float*>(smem + a.first_off) + place[i] * piece;
         return a.first + (static_cast<size_t>(blockIdx.x) * W + i) * piece;
     };
@@ -771,7 +755,7 @@ __global__ void __launch_bounds__(32 * at_warps(NT), at_ctas(NT)) kv_attend_kern
             if (rl >= min(R, rows - rt * R)) continue;
             // the warps' last pieces with loads that do not wait for one another; first pieces are few
             float m = kNone, sum = 0.f, v[C], pm[W];
-            const int ring0 = plan_bytes(c.n_seqs) + rl * (D + 2) * 4, ring_step = a.depth * StepStream<D, false>::kSlot;
+            const int ring0 = plan_bytes(c.n_seqs) + rl * (D + 2) * 4, ring_step = a.depth * StepStream<D>::kSlot;
             constexpr uint32_t kFirst = 0x55555555u;
 #pragma unroll
             for (int i = 0; i < W; ++i) {
@@ -862,120 +846,11 @@ __global__ void __launch_bounds__(32 * kCbWarps) kv_combine_kernel(const KvAtten
 }
 
 // ---------------------------------------------------------------------------
-// Accumulated weight: mass_j += sum over the rows of exp2(score - lse), a second
-// pass over the keys alone (8 D + 128 of a unit's 16 D + 128 bytes) now that
-// every row's lse is known.  Up to 8 rows stay in registers for a whole job;
-// more are taken 32 at a time over up to four steps that wait in the ring, so a
-// tile of queries is arranged once for 128 slots.  A slot's sum is one lane
-// group's, in row order.  Where the first pass has kept the scores they are read
-// instead (16 sequences of 2000 to 4100 slots, 8 heads of 8 rows: 15 us by itself,
-// 43 with the attention).
+// Accumulated weight: mass_j += sum over the rows of exp2(score - lse), from the
+// scores that the pass over the cache has kept: a lane a slot, 32 slots a step, a
+// slot's sum in row order.  16 sequences of 2000 to 4100 slots, 8 heads of 8 rows:
+// 15 us by itself, 43 with the attention.
 // ---------------------------------------------------------------------------
-__host__ __device__ constexpr int ms_warps(int nt) { return nt == 1 ? 8 : 12; }
-__host__ __device__ constexpr int ms_ctas(int nt) { return nt == 1 ? 2 : 1; }
-
-template <int D, int NT>
-__global__ void __launch_bounds__(32 * ms_warps(NT), ms_ctas(NT)) kv_mass_kernel(const KvAttendArgs a) {
-    constexpr int W = ms_warps(NT), G = NT == 1 ? 1 : 4, U = NT == 1 ? 2 : 1;
-    extern __shared__ __align__(128) char smem[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const KvView& c = a.c;
-    StepStream<D, true> st;
-    st.init(plan_bytes(c.n_seqs), W, warp, a.depth);
-    pdl_launch_dependents();
-    pdl_wait();
-    const Plan p = make_plan<32 * W>(c, a.jobs, gridDim.x * W, smem, nullptr);
-    const long long w = static_cast<long long>(blockIdx.x) * W + warp;
-    const long long u0 = p.runs.start(w);
-    const int n = static_cast<int>(p.runs.start(w + 1) - u0);
-    if (n == 0) return;
-    const int rows = a.tokens * a.group, n_rt = (rows + 8 * NT - 1) / (8 * NT);
-    StepAt at = st.start(a, p, u0, n);
-    st.fill(a, p);
-    QueryTile<D, NT> q;
-    f2 lse[NT];  // minus the rows' lse
-    bool fresh = true;
-    for (int done = 0; done < n;) {
-        const int ul = steps_of(at.len), take = min(min(G, a.depth), min(ul - at.step, n - done));
-        for (int e = 0; e < take; ++e)
-            if (!st.wait(e)) { st.drain(done); return; }
-        float add[G][2][2];
-#pragma unroll
-        for (int e = 0; e < G; ++e) add[e][0][0] = add[e][0][1] = add[e][1][0] = add[e][1][1] = 0.f;
-        for (int rt = 0; rt < n_rt; ++rt) {
-            if (n_rt > 1 || fresh) {
-                q.load(a, at.b, at.job, rt, at.len);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float v[2];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int row = (rt * NT + nt) * 8 + 2 * t + e;
-                        v[e] = -INFINITY;  // padding rows and rows without keys weigh nothing
-                        if (row < rows) {
-                            const int tok = row / a.group, head = at.job * a.group + row - tok * a.group;
-                            const float x = ld_l2(a.lse2 + (static_cast<size_t>(at.b) * a.tokens + tok) * (c.heads * a.group) + head);
-                            if (x != -INFINITY) v[e] = -x;
-                        }
-                    }
-                    lse[nt] = f2(v[0], v[1]);
-                }
-                fresh = false;
-            }
-#pragma unroll
-            for (int e = 0; e < G; ++e) {
-                if (e >= take || (at.step + e) * kStep >= q.max_lim) continue;
-#pragma unroll
-                for (int y0 = 0; y0 < 2; y0 += U) {
-                    const int unit = st.unit(e) + y0 * kv_unit_bytes(D);
-                    f2 s[U][NT][2];
-                    score_mma<D, NT, U>(unit, q, s);
-#pragma unroll
-                    for (int y = 0; y < U; ++y)
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const uint2 pr = smem_at<uint2>(unit + y * kv_unit_bytes(D) + kv_param_offset(D) + 8 * g + 64 * x);
-                            const f2 zk(h2f_bits(hi16(pr.x))), sk(h2f_bits(lo16(pr.x)) * a.scale2);
-                            const int j = (at.step + e) * kStep + (y0 + y) * kKvTokens + g + 8 * x;
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                const f2 d = fma2(zk, q.sum[nt], s[y][nt][x]) * sk + lse[nt];
-                                if (j < q.lim[nt][0]) add[e][y0 + y][x] += ex2(d.x());
-                                if (j < q.lim[nt][1]) add[e][y0 + y][x] += ex2(d.y());
-                            }
-                        }
-                }
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < G; ++e) {
-            if (e >= take) continue;
-            const uint32_t found = st.found();
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                float add0 = add[e][y][0], add1 = add[e][y][1];
-                add0 += __shfl_xor_sync(0xffffffffu, add0, 1);
-                add1 += __shfl_xor_sync(0xffffffffu, add1, 1);
-                add0 += __shfl_xor_sync(0xffffffffu, add0, 2);
-                add1 += __shfl_xor_sync(0xffffffffu, add1, 2);
-                const int s0 = (at.step + e) * kStep + y * kKvTokens, j = s0 + g + 8 * t;
-                if ((found >> y & 1u) && t < 2 && j < at.len) {
-                    const int page = kv_page(c, at.b, s0);
-                    if (page >= 0) c.mass[kv_line(c, page, at.job) + j % c.page_size] += t == 0 ? add0 : add1;
-                }
-            }
-            st.next(a, p);
-        }
-        done += take;
-        at.step += take;
-        if (at.step == ul && done < n) {
-            at = step_at(p, c.n_seqs, u0 + done);
-            fresh = true;
-        }
-    }
-}
-
-// The same from the scores that the pass over the cache has kept: a lane a slot, 32 slots a step.
 constexpr int kSmWarps = 8;
 
 template <int P>
@@ -1047,43 +922,9 @@ int ring_depth(int n_seqs, int warps, int ctas, int fixed, int* smem) {
     return depth;
 }
 
-template <class K>
-dq_status_t allow_smem(K kernel, int smem) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) { set_cuda_error(e); return DQ_ERR_CUDA; }
-    return DQ_OK;
-}
-
 // Shared memory for pieces of jobs that end inside a run: two of eight rows, all of a CTA's with one row (where
 // nearly every warp has one).  Room for eight of eight rows would take a slot of every ring.
 constexpr int kKeptBytes = 8448;
-
-template <int D, int NT>
-dq_status_t mass(KvAttendArgs& a, int sm_count, cudaStream_t stream) {
-    int smem = 0;
-    a.depth = ring_depth<StepStream<D, true>>(a.c.n_seqs, ms_warps(NT), ms_ctas(NT), 0, &smem);
-    const dq_status_t st = allow_smem(kv_mass_kernel<D, NT>, smem);
-    if (st != DQ_OK) return st;
-    return launch_pdl(kv_mass_kernel<D, NT>, dim3(sm_count * ms_ctas(NT)), 32 * ms_warps(NT), smem, stream, 1, a);
-}
-
-// The mass pass, from the kept scores or the keys.
-template <int D>
-dq_status_t weights(KvAttendArgs& a, int sm_count, cudaStream_t stream) {
-    const int rows = a.tokens * a.group;
-    a.jobs = Div(a.c.heads);
-    if (a.scores) {
-        const dim3 g(sm_count * 4);
-        const int threads = 32 * kSmWarps, bytes = plan_bytes(a.c.n_seqs);
-        switch (a.pitch) {
-            case 1: return launch_pdl(kv_score_mass_kernel<1>, g, threads, bytes, stream, 1, a);
-            case 2: return launch_pdl(kv_score_mass_kernel<2>, g, threads, bytes, stream, 1, a);
-            case 4: return launch_pdl(kv_score_mass_kernel<4>, g, threads, bytes, stream, 1, a);
-            default: return launch_pdl(kv_score_mass_kernel<8>, g, threads, bytes, stream, 1, a);
-        }
-    }
-    return rows <= 8 ? mass<D, 1>(a, sm_count, stream) : mass<D, 4>(a, sm_count, stream);
-}
 
 template <int D, int NT>
 dq_status_t attend(KvAttendArgs& a, cudaStream_t stream) {
@@ -1095,10 +936,10 @@ dq_status_t attend(KvAttendArgs& a, cudaStream_t stream) {
     if (grid * W > kAtMaxWarps) grid = kAtMaxWarps / W;
     const int rows = a.tokens * a.group, piece = (rows < 8 * NT ? rows : 8 * NT) * (D + 2) * 4;
     a.places = kKeptBytes / piece < W ? kKeptBytes / piece : W;
-    a.depth = ring_depth<StepStream<D, false>>(a.c.n_seqs, W, at_ctas(NT), (a.places * piece + 127) / 128 * 128, &smem);
+    a.depth = ring_depth<StepStream<D>>(a.c.n_seqs, W, at_ctas(NT), (a.places * piece + 127) / 128 * 128, &smem);
     a.first_off = smem - (a.places * piece + 127) / 128 * 128;
     // a piece fits in a ring of two slots
-    static_assert(8 * NT * (D + 2) * 4 <= 2 * StepStream<D, false>::kSlot, "ring too small for a piece");
+    static_assert(8 * NT * (D + 2) * 4 <= 2 * StepStream<D>::kSlot, "ring too small for a piece");
     if (a.depth < 2) return DQ_ERR_UNSUPPORTED;
     const auto kernel = NT == 1 && a.scores ? kv_attend_kernel<D, NT, NT == 1> : kv_attend_kernel<D, NT, false>;
     if ((st = allow_smem(kernel, smem)) != DQ_OK) return st;
@@ -1107,8 +948,23 @@ dq_status_t attend(KvAttendArgs& a, cudaStream_t stream) {
     if (a.n_rt > 1)
         st = launch_pdl(kv_combine_kernel<D, NT>, dim3(static_cast<unsigned>((items + kCbWarps - 1) / kCbWarps)),
                     32 * kCbWarps, 0, stream, 1, a, grid);
-    if (st != DQ_OK || !a.lse2) return st;
-    return weights<D>(a, di.sm_count, stream);
+    return st;
+}
+
+// The mass pass over kept scores of up to 8 rows.
+dq_status_t score_mass(KvAttendArgs& a, cudaStream_t stream) {
+    DeviceInfo di;
+    const dq_status_t st = device_info(&di);
+    if (st != DQ_OK) return st;
+    a.jobs = Div(a.c.heads);
+    const dim3 g(di.sm_count * 4);
+    const int threads = 32 * kSmWarps, bytes = plan_bytes(a.c.n_seqs);
+    switch (a.pitch) {
+        case 1: return launch_pdl(kv_score_mass_kernel<1>, g, threads, bytes, stream, 1, a);
+        case 2: return launch_pdl(kv_score_mass_kernel<2>, g, threads, bytes, stream, 1, a);
+        case 4: return launch_pdl(kv_score_mass_kernel<4>, g, threads, bytes, stream, 1, a);
+        default: return launch_pdl(kv_score_mass_kernel<8>, g, threads, bytes, stream, 1, a);
+    }
 }
 
 // Query rows of a KV head from which the tensor-memory kernel of dq_kv_chunk.cu takes the call.  It costs about the
@@ -1119,8 +975,8 @@ constexpr int chunk_min(int head_dim) { return head_dim == 128 ? 64 : 80; }
 // Row tiles of one warp: 8 rows when a KV head has no more, else 16.
 int row_tiles(int rows) { return rows <= 8 ? 1 : 2; }
 
-// What the mass pass may keep in the workspace (scores of up to 8 rows, or a line of sums for each of several tiles of
-// 128); without that room kv_mass_kernel reads the keys a second time.
+// What the mass pass may keep in the workspace: scores of up to 8 rows, or a line of sums for each of several tiles
+// of 128.  Without that room it reads the keys a second time, a tile a launch.
 constexpr size_t kMaxScores = size_t{1} << 30;
 
 int score_pitch(int rows) { return rows <= 2 ? rows : (rows <= 4 ? 4 : 8); }
@@ -1163,7 +1019,8 @@ dq_status_t launch_kv_attend(const dq_kv_cache_t& c, const dq_kv_attend_t& r, vo
     a.counts = r.counts;
     a.tokens = r.tokens;
     a.group = Div(r.q_heads / c.kv_heads);
-    a.scale2 = r.scale * (1.44269504088896341f * kCode);
+    const float scale2 = r.scale * 1.44269504088896341f;
+    a.scale2 = scale2 * kCode;
     a.done = c.arrivals + c.n_seqs;
     const AttendWs w = attend_ws(c, r.tokens, r.q_heads, r.accumulate != 0);
     char* base = static_cast<char*>(workspace);
@@ -1175,21 +1032,19 @@ dq_status_t launch_kv_attend(const dq_kv_cache_t& c, const dq_kv_attend_t& r, vo
     a.scores = w.total > w.scores ? reinterpret_cast<float*>(base + w.scores) : nullptr;
     const int rows = r.tokens * a.group, nt = row_tiles(rows);
     a.pitch = score_pitch(rows);
+    KvAttendArgs whole = a;  // for dq_kv_chunk.cu, whose codes are whole numbers
+    whole.scale2 = scale2;
+    dq_status_t st;
     if (rows >= chunk_min(c.head_dim)) {
-        KvAttendArgs b = a;
-        b.scale2 = r.scale * 1.44269504088896341f;  // its codes are whole numbers
-        const bool there = a.lse2 && (a.scores || rows <= kChunkRows);
-        const dq_status_t st = launch_kv_chunk(b, c.head_dim, there, a.scores, stream);
-        if (st != DQ_OK || !a.lse2 || there) return st;
-        DeviceInfo di;
-        const dq_status_t sd = device_info(&di);
-        if (sd != DQ_OK) return sd;
-        return c.head_dim == 128 ? weights<128>(a, di.sm_count, stream) : weights<64>(a, di.sm_count, stream);
+        st = launch_kv_chunk(whole, c.head_dim, stream);
+    } else {
+        a.n_rt = Div((rows + 8 * nt - 1) / (8 * nt));
+        a.jobs = Div(c.kv_heads * a.n_rt);
+        if (c.head_dim == 128) st = nt == 1 ? attend<128, 1>(a, stream) : attend<128, 2>(a, stream);
+        else st = nt == 1 ? attend<64, 1>(a, stream) : attend<64, 2>(a, stream);
     }
-    a.n_rt = Div((rows + 8 * nt - 1) / (8 * nt));
-    a.jobs = Div(c.kv_heads * a.n_rt);
-    if (c.head_dim == 128) return nt == 1 ? attend<128, 1>(a, stream) : attend<128, 2>(a, stream);
-    return nt == 1 ? attend<64, 1>(a, stream) : attend<64, 2>(a, stream);
+    if (st != DQ_OK || !a.lse2) return st;
+    return nt == 1 && a.scores ? score_mass(a, stream) : launch_kv_chunk_mass(whole, c.head_dim, whole.scores, stream);
 }
 
 dq_status_t read_kv_attend_error(uint32_t* word, bool clear) {

@@ -637,16 +637,18 @@ __global__ void __launch_bounds__(32 * kCcWarps) kv_chunk_combine_kernel(const K
 }
 
 // ---------------------------------------------------------------------------
-// Accumulated weight for many rows: the keys once more, transposed.  S^T = K Q^T
-// has a slot a TMEM lane, so a thread adds its slot's weights over the tile's
-// rows by itself, with the rows' sums of q
-// and lse from shared memory.  One row tile's sums are added to mass at once; those
-// of several go to lines of their own in the workspace, which kv_tile_mass_kernel
-// adds to mass in tile order (two sequences of 8000 slots, 8 heads of 128 rows:
-// the call takes 51 us, 60 with the lines).  The two halves
-// of the softmax warps take the blocks in turn, a slot's 128 rows a thread, and
-// four S tiles keep the MMAs ahead of them: 41 us where one block at a time, its
-// rows split over two threads, took 51.
+// Accumulated weight: mass_j += sum over the rows of exp2(score - lse), from the
+// keys once more now that every row's lse is known (the scores of up to 8 rows
+// are kept by the pass over the cache instead, see dq_kv_attend.cu).  S^T = K Q^T
+// has a slot a TMEM lane, so a thread adds its slot's weights over the tile's rows
+// by itself, with the rows' sums of q and lse from shared memory.  One row tile's
+// sums are added to mass at once; those of several go to lines of their own in the
+// workspace, which kv_tile_mass_kernel adds to mass in tile order (two sequences
+// of 8000 slots, 8 heads of 128 rows: the call takes 51 us, 60 with the lines), or,
+// where the lines would be too many, to mass by a launch a tile.  The two halves of
+// the softmax warps take the blocks in turn, a slot's 128 rows a thread, and four S
+// tiles keep the MMAs ahead of them: 41 us for the case above where one block at a
+// time, its rows split over two threads, took 51.
 // ---------------------------------------------------------------------------
 template <int D>
 struct CmSmem {
@@ -670,7 +672,8 @@ struct CmSmem {
 enum { kCmRawFull = 0, kCmRawFree = 4, kCmSFull = 8, kCmSFree = 12, kCmKFull = 16, kCmQFull = 18 };
 
 template <int D>
-__global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAttendArgs a, float* sums, const long long lines) {
+__global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAttendArgs a, float* sums, const long long lines,
+                                                                      const int rt0) {
     using S = CmSmem<D>;
     extern __shared__ char dyn[];
     __shared__ uint32_t tm_base;
@@ -717,7 +720,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
         int least = 0;  // keys that every row of the tile sees
         auto load_q = [&]() {
             const int h = at.at.job / a.n_rt, rt = at.at.job - h * a.n_rt;
-            const int r = rt * kTile + trow, tok = r / a.group;
+            const int r = (rt0 + rt) * kTile + trow, tok = r / a.group;
             const int cnt = a.counts ? min(max(ld_l2(a.counts + at.at.b), 0), a.tokens) : a.tokens;
             const bool on = r < rows && tok < cnt;
             const int head = h * a.group + r - tok * a.group;
@@ -907,42 +910,60 @@ __global__ void __launch_bounds__(32 * kTmWarps) kv_tile_mass_kernel(const KvAtt
     }
 }
 
+int chunk_ctas(const DeviceInfo& di) { return di.sm_count < kChunkCtas ? di.sm_count : kChunkCtas; }
+
 template <int D>
-dq_status_t chunk(KvAttendArgs a, bool weights, float* sums, cudaStream_t stream) {
+dq_status_t chunk(KvAttendArgs& a, cudaStream_t stream) {
     DeviceInfo di;
     dq_status_t st = device_info(&di);
     if (st != DQ_OK) return st;
-    const int ctas = di.sm_count < kChunkCtas ? di.sm_count : kChunkCtas, plan = plan_bytes(a.c.n_seqs);
-    auto allow = [&](auto kernel, int smem) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) set_cuda_error(e);
-        return e == cudaSuccess ? DQ_OK : DQ_ERR_CUDA;
-    };
-    int smem = plan + 1024 + CkSmem<D>::kTotal;
-    if ((st = allow(kv_chunk_kernel<D>, smem)) != DQ_OK) return st;
+    const int ctas = chunk_ctas(di), smem = plan_bytes(a.c.n_seqs) + 1024 + CkSmem<D>::kTotal;
+    if ((st = allow_smem(kv_chunk_kernel<D>, smem)) != DQ_OK) return st;
     if ((st = launch_pdl(kv_chunk_kernel<D>, dim3(ctas), kCkThreads, smem, stream, 1, a)) != DQ_OK) return st;
     const long long items = static_cast<long long>(a.c.n_seqs) * a.tokens * a.c.heads * a.group;
-    st = launch_pdl(kv_chunk_combine_kernel<D>, dim3(static_cast<unsigned>((items + kCcWarps - 1) / kCcWarps)), 32 * kCcWarps, 0,
-                    stream, 1, a, ctas);
-    if (st != DQ_OK || !weights) return st;
+    return launch_pdl(kv_chunk_combine_kernel<D>, dim3(static_cast<unsigned>((items + kCcWarps - 1) / kCcWarps)), 32 * kCcWarps, 0,
+                      stream, 1, a, ctas);
+}
+
+template <int D>
+dq_status_t chunk_mass(KvAttendArgs& a, float* sums, cudaStream_t stream) {
+    DeviceInfo di;
+    dq_status_t st = device_info(&di);
+    if (st != DQ_OK) return st;
+    const int ctas = chunk_ctas(di), plan = plan_bytes(a.c.n_seqs), smem = plan + 1024 + CmSmem<D>::kTotal;
     const long long lines = static_cast<long long>(a.c.n_pages) * a.c.heads * a.c.page_size;
-    smem = plan + 1024 + CmSmem<D>::kTotal;
-    if ((st = allow(kv_chunk_mass_kernel<D>, smem)) != DQ_OK) return st;
-    st = launch_pdl(kv_chunk_mass_kernel<D>, dim3(ctas), kCkThreads, smem, stream, 1, a, sums, lines);
-    if (st != DQ_OK || a.n_rt == 1) return st;
+    if ((st = allow_smem(kv_chunk_mass_kernel<D>, smem)) != DQ_OK) return st;
+    const int tiles = a.n_rt;
+    if (tiles > 1 && sums) {
+        if ((st = launch_pdl(kv_chunk_mass_kernel<D>, dim3(ctas), kCkThreads, smem, stream, 1, a, sums, lines, 0)) != DQ_OK) return st;
+        a.jobs = Div(a.c.heads);
+        return launch_pdl(kv_tile_mass_kernel, dim3(di.sm_count * 4), 32 * kTmWarps, plan, stream, 1, a, sums, lines);
+    }
+    a.n_rt = Div(1);
     a.jobs = Div(a.c.heads);
-    return launch_pdl(kv_tile_mass_kernel, dim3(di.sm_count * 4), 32 * kTmWarps, plan, stream, 1, a, sums, lines);
+    for (int rt = 0; rt < tiles && st == DQ_OK; ++rt)
+        st = launch_pdl(kv_chunk_mass_kernel<D>, dim3(ctas), kCkThreads, smem, stream, 1, a, sums, lines, rt);
+    return st;
+}
+
+// The jobs of tiles of 128 rows.
+void tile_jobs(KvAttendArgs& a) {
+    a.n_rt = Div((a.tokens * a.group + kTile - 1) / kTile);
+    a.jobs = Div(a.c.heads * a.n_rt);
 }
 
 }  // namespace
 
 size_t kv_chunk_part_rows() { return static_cast<size_t>(kChunkCtas) * 2 * kTile; }
 
-dq_status_t launch_kv_chunk(KvAttendArgs a, int head_dim, bool weights, float* sums, cudaStream_t stream) {
-    const int rows = a.tokens * a.group;
-    a.n_rt = Div((rows + kTile - 1) / kTile);
-    a.jobs = Div(a.c.heads * a.n_rt);
-    return head_dim == 128 ? chunk<128>(a, weights, sums, stream) : chunk<64>(a, weights, sums, stream);
+dq_status_t launch_kv_chunk(KvAttendArgs a, int head_dim, cudaStream_t stream) {
+    tile_jobs(a);
+    return head_dim == 128 ? chunk<128>(a, stream) : chunk<64>(a, stream);
+}
+
+dq_status_t launch_kv_chunk_mass(KvAttendArgs a, int head_dim, float* sums, cudaStream_t stream) {
+    tile_jobs(a);
+    return head_dim == 128 ? chunk_mass<128>(a, sums, stream) : chunk_mass<64>(a, sums, stream);
 }
 
 dq_status_t read_kv_chunk_error(uint32_t* word, bool clear) {

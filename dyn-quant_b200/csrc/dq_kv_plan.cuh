@@ -32,8 +32,9 @@ struct KvAttendArgs {
 // Attention of many query rows per KV head (dq_kv_chunk.cu): workspace rows, and the launch (a's lse2 filled in too).
 constexpr int kChunkRows = 128;  // query rows of a tile
 size_t kv_chunk_part_rows();     // rows of part / part_ml
-// weights: run the mass pass.  sums: its room, [row tiles][n_pages][kv_heads][page_size], for more tiles than one.
-dq_status_t launch_kv_chunk(KvAttendArgs a, int head_dim, bool weights, float* sums, cudaStream_t stream);
+dq_status_t launch_kv_chunk(KvAttendArgs a, int head_dim, cudaStream_t stream);
+// The mass pass for any number of rows, from lse2.  sums: [row tiles][n_pages][kv_heads][page_size], or null.
+dq_status_t launch_kv_chunk_mass(KvAttendArgs a, int head_dim, float* sums, cudaStream_t stream);
 
 namespace {
 
@@ -310,6 +311,13 @@ __device__ __forceinline__ void join_row(const KvAttendArgs& a, const Share& s, 
 #pragma unroll
     for (int k = 0; k < V; k += 2) *reinterpret_cast<uint32_t*>(dst + k) = pack_f32(v[k] * f, v[k + 1] * f);
     if (lane == 0) store_lse(a, b, tok, head, m, sum);
+}
+
+template <class K>
+dq_status_t allow_smem(K kernel, int smem) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) { set_cuda_error(e); return DQ_ERR_CUDA; }
+    return DQ_OK;
 }
 
 }  // namespace

@@ -472,8 +472,8 @@ DQ_API size_t dq_kv_attend_workspace_bytes(const dq_kv_cache_t* cache, int32_t t
  * bit-reproducible.  One kernel when a KV head has at most 16 query rows (query
  * tokens times its query heads), else two; one more with accumulate, two more
  * beyond 128 rows.  out must not overlap q.  With
- * accumulate the workspace keeps scores or partial sums of up to 1 GiB, and
- * where they would be more the keys are read once more instead.
+ * accumulate the workspace keeps scores or partial sums of up to 1 GiB; where
+ * they would be more, each 128 rows are one more kernel that reads the keys.
  */
 DQ_API dq_status_t dq_kv_attend(const dq_kv_cache_t* cache, const dq_kv_attend_t* args, void* workspace,
                                 size_t workspace_bytes, void* stream);

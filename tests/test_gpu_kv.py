@@ -350,6 +350,30 @@ def test_attend_pool_beyond_4_gb():
     R.check_attend(out, lse, q, small, 128 ** -0.5, mass=cache.mass[first:], mass0=mass0[first:])
 
 
+@pytest.mark.parametrize("group,t", [(8, 1), (8, 128)])
+def test_accumulate_over_a_pool_too_large_to_keep_scores(group, t):
+    """Scores of 8 rows, or sums of 8 tiles of rows, would take more than 1 GiB: the keys are read again instead."""
+    cache = R.make_cache([150, 139], 8, 128, 64, big_pages=72000)
+    q = R.queries(cache, t, group)
+    mass0 = cache.mass.clone()
+    out, lse = cache.attend(q, return_lse=True, accumulate=True)
+    table = cache.page_table.clone()
+    first = 72000 - 8
+    assert int(table[table >= 0].min()) >= first
+    small = Int4KVCache(2, 8, 8, 128, 64, max_pages=table.shape[1], units=cache.units[first:].contiguous(),
+                        page_table=torch.where(table >= 0, table - first, table))
+    small.lengths.copy_(cache.lengths)
+    assert not (cache.mass[:first] != mass0[:first]).any()
+    if t == 1:
+        R.check_attend(out, lse, q, small, 128 ** -0.5, mass=cache.mass[first:], mass0=mass0[first:])
+    else:  # against the pass with lines of sums: the same weights, added in another order (9 roundings of at most all)
+        small.mass.copy_(mass0[first:])
+        again = small.attend(q, accumulate=True)
+        assert torch.equal(again, out)
+        a, b = cache.mass[first:].double(), small.mass.double()
+        assert ((a - b).abs() <= 2 * 9 * 2.0 ** -24 * b.abs()).all()
+
+
 def test_attend_page_outside_the_pool_is_absent():
     """Its slots count as not there and the device error word says so."""
     cache = R.make_cache([60], 2, 128, 16)
