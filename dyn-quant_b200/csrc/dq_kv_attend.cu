@@ -855,6 +855,7 @@ constexpr int kSmWarps = 8;
 
 template <int P>
 __global__ void __launch_bounds__(32 * kSmWarps) kv_score_mass_kernel(const KvAttendArgs a) {
+    constexpr int B = P == 8 ? 2 : 4;
     extern __shared__ __align__(128) char smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const KvView& c = a.c;
@@ -879,30 +880,42 @@ __global__ void __launch_bounds__(32 * kSmWarps) kv_score_mass_kernel(const KvAt
                 if (x != -INFINITY) lse[r] = x;
             }
         }
-#pragma unroll 2
-        for (int i = 0; i < take; ++i) {
-            const int slot = (at.step + i) * kStep + lane;
-            if (slot >= at.len || none) continue;
-            const int page = kv_page(c, at.b, slot);
-            if (page < 0) continue;
-            const size_t line = kv_line(c, page, at.job) + slot % c.page_size;
-            float s[P];
-            if constexpr (P >= 4) {
+        // several steps' loads at once: pages, then scores and sums
+        for (int i0 = 0; i0 < take; i0 += B) {
+            long long line[B];
+            float s[B][P], was[B];
 #pragma unroll
-                for (int r = 0; r < P; r += 4) {
-                    const uint4 x = ld_l2_v4(a.scores + line * P + r);
-                    s[r] = __uint_as_float(x.x); s[r + 1] = __uint_as_float(x.y);
-                    s[r + 2] = __uint_as_float(x.z); s[r + 3] = __uint_as_float(x.w);
-                }
-            } else {
-#pragma unroll
-                for (int r = 0; r < P; ++r) s[r] = ld_l2(a.scores + line * P + r);
+            for (int i = 0; i < B; ++i) {
+                const int slot = (at.step + i0 + i) * kStep + lane;
+                const bool on = i0 + i < take && slot < at.len && !none;
+                const int page = on ? kv_page(c, at.b, slot) : -1;
+                line[i] = page >= 0 ? static_cast<long long>(kv_line(c, page, at.job) + slot % c.page_size) : -1;
             }
-            float add = 0.f;
 #pragma unroll
-            for (int r = 0; r < P; ++r)
-                if (r < rows) add += ex2(s[r] - lse[r]);
-            c.mass[line] = ld_l2(c.mass + line) + add;
+            for (int i = 0; i < B; ++i) {
+                const float* src = a.scores + (line[i] >= 0 ? line[i] : 0) * P;
+                const bool on = line[i] >= 0;
+                if constexpr (P >= 4) {
+#pragma unroll
+                    for (int r = 0; r < P; r += 4) {
+                        const uint4 x = on ? ld_l2_v4(src + r) : make_uint4(0, 0, 0, 0);
+                        s[i][r] = __uint_as_float(x.x); s[i][r + 1] = __uint_as_float(x.y);
+                        s[i][r + 2] = __uint_as_float(x.z); s[i][r + 3] = __uint_as_float(x.w);
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < P; ++r) s[i][r] = on ? ld_l2(src + r) : 0.f;
+                }
+                was[i] = on ? ld_l2(c.mass + line[i]) : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                float add = 0.f;
+#pragma unroll
+                for (int r = 0; r < P; ++r)
+                    if (r < rows) add += ex2(s[i][r] - lse[r]);
+                if (line[i] >= 0) c.mass[line[i]] = was[i] + add;
+            }
         }
         done += take;
         if (done < n) at = step_at(p, c.n_seqs, u0 + done);
