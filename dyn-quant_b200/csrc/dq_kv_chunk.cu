@@ -643,9 +643,8 @@ __global__ void __launch_bounds__(32 * kCcWarps) kv_chunk_combine_kernel(const K
 // has a slot a TMEM lane, so a thread adds its slot's weights over the tile's rows
 // by itself, with the rows' sums of q and lse from shared memory.  One row tile's
 // sums are added to mass at once; those of several go to lines of their own in the
-// workspace, which kv_tile_mass_kernel adds to mass in tile order (two sequences
-// of 8000 slots, 8 heads of 128 rows: the call takes 51 us, 60 with the lines), or,
-// where the lines would be too many, to mass by a launch a tile.  The two halves of
+// workspace, which kv_tile_mass_kernel (7 us by itself) adds to mass in tile order,
+// or, where the lines would be too many, to mass by a launch a tile.  The two halves of
 // the softmax warps take the blocks in turn, a slot's 128 rows a thread, and four S
 // tiles keep the MMAs ahead of them: 41 us for the case above where one block at a
 // time, its rows split over two threads, took 51.
@@ -919,16 +918,28 @@ __global__ void __launch_bounds__(32 * kTmWarps) kv_tile_mass_kernel(const KvAtt
     const int n = static_cast<int>(p.runs.start(w + 1) - u0);
     if (n == 0) return;
     StepAt at = step_at(p, c.n_seqs, u0);
-    for (int i = 0; i < n; ++i) {
-        const int slot = at.step * kStep + lane, page = slot < at.len ? kv_page(c, at.b, slot) : -1;
-        if (page >= 0) {
-            const long long line = static_cast<long long>(kv_line(c, page, at.job) + slot % c.page_size);
-            float add = 0.f;
-#pragma unroll 4
-            for (int rt = 0; rt < n_rt; ++rt) add += ld_l2(sums + rt * lines + line);
-            c.mass[line] = ld_l2(c.mass + line) + add;
+    constexpr int B = 4;  // steps at once: their pages, then their sums
+    for (int i0 = 0; i0 < n; i0 += B) {
+        long long line[B];
+        float was[B], add[B];
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            const int slot = at.step * kStep + lane, page = i0 + i < n && slot < at.len ? kv_page(c, at.b, slot) : -1;
+            line[i] = page >= 0 ? static_cast<long long>(kv_line(c, page, at.job) + slot % c.page_size) : -1;
+            if (++at.step == steps_of(at.len) && i0 + i + 1 < n) at = step_at(p, c.n_seqs, u0 + i0 + i + 1);
         }
-        if (++at.step == steps_of(at.len) && i + 1 < n) at = step_at(p, c.n_seqs, u0 + i + 1);
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            was[i] = line[i] >= 0 ? ld_l2(c.mass + line[i]) : 0.f;
+            add[i] = 0.f;
+        }
+#pragma unroll 2
+        for (int rt = 0; rt < n_rt; ++rt)
+#pragma unroll
+            for (int i = 0; i < B; ++i) add[i] += line[i] >= 0 ? ld_l2(sums + rt * lines + line[i]) : 0.f;
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+            if (line[i] >= 0) c.mass[line[i]] = was[i] + add[i];
     }
 }
 
