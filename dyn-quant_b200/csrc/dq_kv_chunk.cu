@@ -633,7 +633,7 @@ __global__ void __launch_bounds__(32 * kCcWarps) kv_chunk_combine_kernel(const K
     const int h = head / a.group, r = tok * a.group + head - h * a.group, rt = r / kTile;
     const Runs runs(a.pre[c.n_seqs], c.n_seqs, a.jobs, ctas);
     const Share s = share_of<1>(a.pre, c.n_seqs, a.jobs, runs, b, h * a.n_rt + rt);
-    if (s.n > 1) join_row<D, kTile / 8>(a, s, b, h, rt, r);  // else finished by its CTA, or empty
+    if (s.n > 1) join_row<D, kTile / 8, 4>(a, s, b, h, rt, r);  // else finished by its CTA, or empty
 }
 
 // ---------------------------------------------------------------------------

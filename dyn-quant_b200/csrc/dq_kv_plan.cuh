@@ -259,10 +259,11 @@ __device__ __forceinline__ Share share_of(const int* pre, int n_seqs, const Div&
     return s;
 }
 
-// One warp joins row r's partial sums: maxima and sums a lane each, then the outputs eight partials at a time.
-template <int D, int NT>
+// One warp joins row r's partial sums: maxima and sums a lane each, then the outputs N partials at a time (eight where
+// a job is cut between many warps; four leave room for all of dq_kv_chunk.cu's rows at once: 9 us for 10).
+template <int D, int NT, int N = 8>
 __device__ __forceinline__ void join_row(const KvAttendArgs& a, const Share& s, int b, int h, int rt, int r) {
-    constexpr int R = 8 * NT, V = D / 32, N = 8;  // V columns of a lane, side by side; partials at a time
+    constexpr int R = 8 * NT, V = D / 32;  // V columns of a lane, side by side; N partials at a time
     const int lane = threadIdx.x & 31, rl = r - rt * R, first = s.slot0 * R;  // only the first CTA's may be its slot 1
     const size_t row0 = static_cast<size_t>(s.c0) * 2 * R + rl;
     const float2* ml0 = reinterpret_cast<const float2*>(a.part_ml) + row0;
