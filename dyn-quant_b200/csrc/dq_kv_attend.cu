@@ -44,12 +44,12 @@
 // weights keep their 11 bits down to 2^-29 of the largest.
 //
 // Measured: 64 sequences of 2000 to 4096 slots with 32 heads of 128 and one row
-// each, 850 MB, 176 us, 4.8 TB/s (75% of a copy's; 55% of the issue slots, the
-// tensor pipe 31%); 16 sequences of 1000 to 4100 slots with 8 heads of 8 rows,
-// 48 MB, 26 us; 131071 slots with 8 heads of 8 rows, 143 MB, 45 us; 8 sequences of
-// 200 to 8000 slots with 8 heads of 64 and 20 rows, 22 MB, 35 us with the join.
-// The smaller ones are bound by the chain lengths, pages, units, join: 77 slots of
-// 32 heads take 9 us.
+// each, 850 MB, 165 to 176 us, 4.8 to 5.1 TB/s (75 to 80% of a copy's; 55% of the
+// issue slots, the tensor pipe 31%); 16 sequences of 1000 to 4100 slots with 8
+// heads of 8 rows, 48 MB, 26 us; 131071 slots with 8 heads of 8 rows, 143 MB, 45
+// us; 8 sequences of 200 to 8000 slots with 8 heads of 64 and 20 rows, 22 MB, 35
+// us with the join.  The smaller ones are bound by the chain lengths, pages, units,
+// join: 77 slots of 32 heads take 9 us.
 #include "dq_kv_plan.cuh"
 
 namespace dq {
@@ -849,7 +849,7 @@ __global__ void __launch_bounds__(32 * kCbWarps) kv_combine_kernel(const KvAtten
 // Accumulated weight: mass_j += sum over the rows of exp2(score - lse), from the
 // scores that the pass over the cache has kept: a lane a slot, 32 slots a step, a
 // slot's sum in row order.  16 sequences of 2000 to 4100 slots, 8 heads of 8 rows:
-// 15 us by itself, 43 with the attention.
+// 14 us by itself, 41 with the attention.
 // ---------------------------------------------------------------------------
 constexpr int kSmWarps = 8;
 

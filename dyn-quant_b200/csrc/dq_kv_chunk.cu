@@ -30,7 +30,7 @@
 // products as in dq_kv_attend.cu; p' = p s_v w is rounded to f16.
 //
 // Measured: two sequences of 6000 and 8000 slots, 8 KV heads of 128 with 512 rows
-// each, 31 GFLOP: 74 us, 0.42 PFLOP/s, and 10 us for the join.  A block takes 3900
+// each, 31 GFLOP: 73 us, 0.42 PFLOP/s, and 9 us for the join.  A block takes 3900
 // cycles, of which the exponentials are 1024, the MMAs 800; the softmax warps'
 // other instructions and latencies bound it (45% of the issue slots are busy).
 // Dequantizing and loading keep ahead of them.  Masks are applied after the loop
