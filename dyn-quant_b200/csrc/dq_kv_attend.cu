@@ -981,9 +981,10 @@ dq_status_t score_mass(KvAttendArgs& a, cudaStream_t stream) {
 }
 
 // Query rows of a KV head from which the tensor-memory kernel of dq_kv_chunk.cu takes the call.  It costs about the
-// same for 1 to 128 rows, this file's kernels cost more for every 16: 32 KV heads with 8000 slots each take
-// 55 us (48 rows), 65 us (63) here and 58 us there with heads of 128; 45 us (63) here and 50 us there with 64.
-constexpr int chunk_min(int head_dim) { return head_dim == 128 ? 64 : 80; }
+// same for 1 to 128 rows, this file's kernels cost more for every 16.  Here and there, in us, for 1 sequence of 8000
+// slots and 32 KV heads, 4 of 2000 and 8, 16 of 4000 and 8: heads of 128 43, 28, 69 (32 rows), 54, 29, 92 (33) and
+// 54, 23, 96; heads of 64 44, 23, 76 (64 rows), 51, 23, 91 (79) and 48, 21, 85.
+constexpr int chunk_min(int head_dim) { return head_dim == 128 ? 33 : 65; }
 
 // Row tiles of one warp: 8 rows when a KV head has no more, else 16.
 int row_tiles(int rows) { return rows <= 8 ? 1 : 2; }

@@ -230,9 +230,13 @@ def test_attend_is_reproducible_and_ignores_what_lies_behind():
     (128, 2, 4, 40, 16, [41, 700, 3], [40, 17, 40]),
     (128, 1, 3, 90, 48, [1000, 260], None),
     (64, 1, 16, 33, 32, [513, 40], [0, 33]),
+    (128, 2, 1, 32, 32, [32, 700], [32, 5]),
+    (128, 2, 3, 11, 32, [11, 700], [11, 2]),
+    (64, 1, 8, 8, 16, [400, 3], None),
+    (64, 1, 5, 13, 16, [400, 3], None),
 ])
 def test_attend_many_rows(dim, heads, group, t, page, lens, counts):
-    """64 and more query rows per KV head: several tiles of 128, ragged counts, blocks that end inside a page."""
+    """Many query rows per KV head: several tiles of 128, ragged counts, blocks that end inside a page."""
     cache = R.make_cache(lens, heads, dim, page, seed=dim + t, mass=True)
     q = R.queries(cache, t, group)
     mass0 = cache.mass.clone()
