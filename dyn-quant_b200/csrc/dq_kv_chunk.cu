@@ -580,7 +580,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
                 if (page >= 0) index = static_cast<int>((kv_line(c, page, at.at.job / a.n_rt) + slot % c.page_size) / kKvTokens);
                 else absent = true;
             }
-            if (i >= 2) wait(kRawFree + buf, (i - 2) >> 1);
+            if (i >= 2) {
+                wait(kRawFree + buf, (i - 2) >> 1);
+                wait(kRawFull + buf, (i - 2) >> 1);  // long ago, unless its readers gave up
+            }
             if (dead) break;
             asked = i + 1;
             const uint32_t got = __ballot_sync(0xffffffffu, index >= 0), bar = bars + 8 * (kRawFull + buf);
@@ -593,9 +596,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
             copy_units<D>(c, smem0 + S::kRaw + buf * S::kRawBytes, index, got, lane, bar);
             if (i + 1 < n) at.next(p, c.n_seqs, u0 + i + 1);
         }
-        // given up: the copies in flight must end before the shared memory goes
-        if (dead)
-            for (int j = max(asked - 2, 0); j < asked; ++j) mbar_wait_bounded(bars + 8 * (kRawFull + (j & 1)), (j >> 1) & 1);
+        // the copies must end before the shared memory goes, whatever their readers have done
+        for (int j = max(asked - 2, 0); j < asked; ++j) mbar_wait_bounded(bars + 8 * (kRawFull + (j & 1)), (j >> 1) & 1);
         if (absent) atomicOr(&g_kv_chunk_error, kKvErrPage);
     }
     // rows of sequences without slots
@@ -878,7 +880,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
                 const int page = kv_page(c, at.at.b, slot);
                 if (page >= 0) index = static_cast<int>((kv_line(c, page, at.at.job / a.n_rt) + slot % c.page_size) / kKvTokens);
             }
-            if (i >= 4) wait(kCmRawFree + buf, (i - 4) >> 2);
+            if (i >= 4) {
+                wait(kCmRawFree + buf, (i - 4) >> 2);
+                wait(kCmRawFull + buf, (i - 4) >> 2);
+            }
             if (dead) break;
             asked = i + 1;
             const uint32_t got = __ballot_sync(0xffffffffu, index >= 0), bar = bars + 8 * (kCmRawFull + buf);
@@ -893,9 +898,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
             copy_units<D>(c, smem0 + S::kRaw + buf * S::kRawBytes, index, got, lane, bar);
             if (i + 1 < n) at.next(p, c.n_seqs, u0 + i + 1);
         }
-        // given up: the copies in flight must end before the shared memory goes
-        if (dead)
-            for (int j = max(asked - 4, 0); j < asked; ++j) mbar_wait_bounded(bars + 8 * (kCmRawFull + (j & 3)), (j >> 2) & 1);
+        for (int j = max(asked - 4, 0); j < asked; ++j) mbar_wait_bounded(bars + 8 * (kCmRawFull + (j & 3)), (j >> 2) & 1);
     }
     tm_before_sync();
     __syncthreads();
