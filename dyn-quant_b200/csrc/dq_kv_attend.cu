@@ -412,6 +412,15 @@ struct RowState {
                 for (int x = 0; x < 2; ++x) {
                     const int jj = j + u * kKvTokens + g + 8 * x;
                     const bool there = jj < len && (found >> u & 1u);
+                    if (there && !(fabsf(sv[u][x]) + fabsf(zv[u][x]) < INFINITY)) {
+                        // a value row that is not finite: the outputs of the rows that see it are not either, and it
+                        // must not meet the zero weights of those that do not
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            zs[nt] = zs[nt] + f2(jj < q.lim[nt][0] ? NAN : 0.f, jj < q.lim[nt][1] ? NAN : 0.f);
+                        sv[u][x] = 0.f;
+                        zv[u][x] = 0.f;
+                    }
                     if (!there) { sv[u][x] = 0.f; zv[u][x] = 0.f; }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)

@@ -63,8 +63,9 @@ struct CkSmem {
     static constexpr int kRawBytes = kUnits * kv_unit_bytes(D);
     static constexpr int kRaw = kV + 2 * kVBytes;                // 2 x the units of a block
     static constexpr int kPar = kRaw + 2 * kRawBytes;            // 4 x [4][128]: - (z_k - 8), s_k, s_v, z_v - 8
-    static constexpr int kMisc = kPar + 4 * 4 * kBlk * 4;        // 4 x (4 x largest s_v, 4 x slots there)
-    static constexpr int kGot = kMisc + 128;                     // 2 x found units
+    static constexpr int kMiscBytes = 48;
+    static constexpr int kMisc = kPar + 4 * 4 * kBlk * 4;        // 4 x (4 x largest s_v, 4 x slots there, 4 x not finite)
+    static constexpr int kGot = kMisc + 256;                     // 2 x found units
     static constexpr int kTop = kGot + 128;                      // 2 x [2 halves][128] largest score of a row's half
     static constexpr int kSums = kTop + 4 * kTile * 4;           // [2 halves][128] x 2: sum of weights, of zeros' share
     static constexpr int kQSum = kSums + 4 * kTile * 4;          // [2 halves][128] sums of q
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
             wait(kSFull + buf, i >> 1);
             tm_after_sync();
             const float* par = word(S::kPar + (i & 3) * (4 * kBlk * 4)) + half * H;
-            const float* misc = word(S::kMisc + (i & 3) * 32);
+            const float* misc = word(S::kMisc + (i & 3) * S::kMiscBytes);
             uint32_t va[32], vb[32];
             tm_ld32(lanes + kTmS + buf * kBlk + half * H, va);
             tm_ld32(lanes + kTmS + buf * kBlk + half * H + 32, vb);
@@ -356,6 +357,13 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
                 m = kNone;
                 l = zs = 0.f;
                 vw = 2147483648.0f;  // 2^31 brings the smallest FP16 scale, 2^-24, to 2^7
+            }
+            // value rows that are not finite (their scales and zeros are 0 here): the output of a row that sees one
+            // is not either
+            const uint2 odd = *reinterpret_cast<const uint2*>(misc + 8 + 2 * half);
+            if ((odd.x | odd.y) != 0) {
+                const unsigned long long sees = left >= H ? ~0ull : (1ull << max(left, 0)) - 1ull;
+                if (((static_cast<unsigned long long>(odd.y) << 32 | odd.x) & sees) != 0) zs = NAN;
             }
             if (__any_sync(0xffffffffu, top > m + kLazy || big * vw > 128.f)) {
                 float ratio = 1.f;
@@ -472,19 +480,22 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
                 const int u = 2 * dw + (lane >> 4), slot = 32 * dw + lane;
                 const bool on = (got >> u & 1u) && at.at.step * kBlk + slot < at.at.len;
                 const uint2 pw = lds_v2(smem0 + S::kRaw + buf * S::kRawBytes + u * kv_unit_bytes(D) + kv_param_offset(D) + 8 * (lane & 15));
-                const float sv = on ? h2f_bits(lo16(pw.y)) : 0.f;
-                const uint32_t par = smem0 + S::kPar + (i & 3) * (4 * kBlk * 4) + 4 * slot, misc = smem0 + S::kMisc + (i & 3) * 32;
+                float sv = on ? h2f_bits(lo16(pw.y)) : 0.f, zv = on ? h2f_bits(hi16(pw.y)) - 8.f : 0.f;
+                const bool finite = fabsf(sv) + fabsf(zv) < INFINITY;
+                if (!finite) sv = zv = 0.f;
+                const uint32_t par = smem0 + S::kPar + (i & 3) * (4 * kBlk * 4) + 4 * slot, misc = smem0 + S::kMisc + (i & 3) * S::kMiscBytes;
                 sts_u32(par, __float_as_uint(on ? 8.f - h2f_bits(hi16(pw.x)) : 0.f));
                 sts_u32(par + 4 * kBlk, __float_as_uint(on ? h2f_bits(lo16(pw.x)) * a.scale2 : 0.f));
                 sts_u32(par + 8 * kBlk, __float_as_uint(sv));
-                sts_u32(par + 12 * kBlk, __float_as_uint(on ? h2f_bits(hi16(pw.y)) - 8.f : 0.f));
+                sts_u32(par + 12 * kBlk, __float_as_uint(zv));
                 float big = sv;
 #pragma unroll
                 for (int o = 16; o >= 1; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-                const uint32_t there = __ballot_sync(0xffffffffu, on);
+                const uint32_t there = __ballot_sync(0xffffffffu, on), odd = __ballot_sync(0xffffffffu, !finite);
                 if (lane == 0) {
                     sts_u32(misc + 4 * dw, __float_as_uint(big));
                     sts_u32(misc + 16 + 4 * dw, there);
+                    sts_u32(misc + 32 + 4 * dw, odd);
                 }
             }
             fence_async_smem();

@@ -1,0 +1,61 @@
+"""The 4-bit KV cache where values, pages and arguments are at their edges."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+import kv_ref as R  # noqa: E402
+from dyn_quant import _C  # noqa: E402
+from dyn_quant.kv_cache import Int4KVCache  # noqa: E402
+
+I32 = dict(dtype=torch.int32, device="cuda")
+
+
+@pytest.fixture(autouse=True)
+def no_device_error():
+    yield
+    assert _C.read_device_error(True) == 0
+
+
+def ints(*v):
+    return torch.tensor(v, **I32)
+
+
+def slots(cache, b, n):
+    """Page and offset of the first n slots of sequence b (numpy)."""
+    j = np.arange(n)
+    return cache.page_table.cpu().numpy()[b, j // cache.page_size], j % cache.page_size
+
+
+# ---------------------------------------------------------------------------
+# values that are not finite
+# ---------------------------------------------------------------------------
+# query heads a KV head, new tokens: 8 rows, 16 and 32 (mma.sync; 32 of heads of 128 too), 48 and 160 (tensor memory,
+# one tile and two; 48 of heads of 64 are mma.sync), 8 of one token
+ROWS = [(2, 4), (4, 4), (8, 4), (8, 6), (16, 10), (8, 1)]
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group,t", ROWS)
+@pytest.mark.parametrize("value", [float("inf"), float("-inf")])
+def test_a_value_that_is_not_finite_reaches_only_queries_that_see_it(dim, group, t, value):
+    """A new token's value has an infinity: queries before it do not see it, and get what they would get without it,
+    bit for bit (the weights' power of two may differ, which no rounding feels); the others' outputs are not finite.
+    Weights and their sums are the keys' alone."""
+    lens, at = [70, 300], 3 if t > 1 else 0  # the at-th of the t new tokens
+    caches = [R.make_cache(lens, 2, dim, 16, seed=5, extra=t, mass=True) for _ in range(2)]
+    gen = torch.Generator().manual_seed(6)
+    k, v = (torch.randn(2, t, 2, dim, generator=gen).half().cuda() for _ in range(2))
+    q = R.queries(caches[0], t, group)
+    v1 = v.clone()
+    v1[:, at, 0, 5] = value
+    caches[0].append(k, v)
+    caches[1].append(k, v1)
+    (want, want_lse), (got, got_lse) = (c.attend(q, accumulate=True, return_lse=True) for c in caches)
+    assert torch.isfinite(want).all()
+    assert torch.equal(got[:, :at], want[:, :at])
+    assert torch.equal(got[:, :, group:], want[:, :, group:])  # the other KV head
+    assert not torch.isfinite(got[:, at:, :group]).any()
+    assert torch.equal(got_lse, want_lse) and torch.equal(caches[1].mass, caches[0].mass)
