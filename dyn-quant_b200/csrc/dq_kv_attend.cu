@@ -921,8 +921,8 @@ __global__ void __launch_bounds__(32 * kSmWarps, 4) kv_score_mass_kernel(const K
             for (int i = 0; i < B; ++i) {
                 float add = 0.f;
 #pragma unroll
-                for (int r = 0; r < P; ++r)
-                    if (r < rows) add += ex2(s[i][r] - lse[r]);
+                for (int r = 0; r < P; ++r)  // (a row whose lse is not a number gives nothing to the slots that it does not see)
+                    if (r < rows && s[i][r] != -INFINITY) add += ex2(s[i][r] - lse[r]);
                 if (line[i] >= 0) c.mass[line[i]] = was[i] + add;
             }
         }

@@ -59,3 +59,25 @@ def test_a_value_that_is_not_finite_reaches_only_queries_that_see_it(dim, group,
     assert torch.equal(got[:, :, group:], want[:, :, group:])  # the other KV head
     assert not torch.isfinite(got[:, at:, :group]).any()
     assert torch.equal(got_lse, want_lse) and torch.equal(caches[1].mass, caches[0].mass)
+
+
+@pytest.mark.parametrize("group,t", ROWS[:-1])
+def test_weights_of_a_query_that_is_not_finite_stay_with_the_slots_it_sees(group, t):
+    """An early query is not a number, so the weights it gives are not either; the slots behind it, which it does not
+    see, keep what the other queries give them."""
+    cache, clean = (R.make_cache([150, 70], 2, 64, 16, seed=5, mass=True) for _ in range(2))
+    q = R.queries(cache, t, group)
+    clean.attend(q, accumulate=True)
+    mass0 = cache.mass.clone()
+    q[:, 1, 0] = float("nan")
+    out, lse = cache.attend(q, accumulate=True, return_lse=True)
+    assert torch.isnan(out[:, 1, 0]).all() and torch.isnan(lse[:, 1, 0]).all()
+    assert int(torch.isnan(lse).sum()) == 2
+    for b, n in enumerate(cache.lengths.tolist()):
+        page, off = slots(cache, b, n)
+        seen = n - t + 2  # slots that query 1 sees
+        assert torch.isnan(cache.mass[page, 0, off][:seen]).all()
+        # the other rows' weights, summed in the same order without one that is zero
+        assert torch.equal(cache.mass[page, 0, off][seen:], clean.mass[page, 0, off][seen:])
+        assert torch.equal(cache.mass[page, 1, off], clean.mass[page, 1, off])
+        assert not torch.equal(cache.mass[page, 1, off], mass0[page, 1, off])
