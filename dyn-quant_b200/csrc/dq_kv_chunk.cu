@@ -754,7 +754,9 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
                     if (x != -INFINITY) nl = -x;
                 }
                 word(S::kRow)[2 * kTile + trow] = nl;
-                reinterpret_cast<int*>(word(S::kRow))[3 * kTile + trow] = on ? lim : at.at.len;
+                // (padding sees all, so that it costs no masks, but nothing where the sequence has no query at all:
+                // 0 times a key that is not finite is not 0)
+                reinterpret_cast<int*>(word(S::kRow))[3 * kTile + trow] = on ? lim : (cnt > 0 ? at.at.len : 0);
             }
             fence_async_smem();
             mbar_arrive(bars + 8 * kCmQFull);

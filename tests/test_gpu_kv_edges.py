@@ -81,3 +81,21 @@ def test_weights_of_a_query_that_is_not_finite_stay_with_the_slots_it_sees(group
         assert torch.equal(cache.mass[page, 0, off][seen:], clean.mass[page, 0, off][seen:])
         assert torch.equal(cache.mass[page, 1, off], clean.mass[page, 1, off])
         assert not torch.equal(cache.mass[page, 1, off], mass0[page, 1, off])
+
+
+@pytest.mark.parametrize("group,t", ROWS)
+@pytest.mark.parametrize("value", [float("inf"), float("-inf")])
+def test_a_sequence_without_queries_gains_no_weight(group, t, value):
+    """Whatever its keys hold: here a row that is not finite."""
+    cache = R.make_cache([150, 70], 2, 128, 16, seed=5, extra=1, mass=True)
+    k = torch.randn(2, 1, 2, 128, generator=torch.Generator().manual_seed(3)).half().cuda()
+    k[1, :, :, 9] = value
+    cache.append(k, k.nan_to_num(0, 0, 0))
+    q = R.queries(cache, t, group)
+    mass0 = cache.mass.clone()
+    out, lse = cache.attend(q, counts=ints(t, 0), accumulate=True, return_lse=True)
+    assert not out[1].any() and torch.isinf(lse[1]).all() and torch.isfinite(out[0]).all()
+    page, off = slots(cache, 1, 71)
+    assert torch.equal(cache.mass[page, :, off], mass0[page, :, off])
+    page, off = slots(cache, 0, 151)
+    assert (cache.mass[page, :, off] > mass0[page, :, off]).all()
