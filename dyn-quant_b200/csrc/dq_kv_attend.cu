@@ -406,21 +406,32 @@ struct RowState {
         if (j + U * kKvTokens > q.min_lim || found != (1u << U) - 1u) {
             // the end of the sequence or of a query token's keys, or an absent page: slots behind a
             // row's keys are taken out, and what lies behind the last token is never multiplied
+            bool odd = false;
+#pragma unroll
+            for (int u = 0; u < U; ++u) odd |= !(fabsf(sv[u][0]) + fabsf(sv[u][1]) + fabsf(zv[u][0]) + fabsf(zv[u][1]) < INFINITY);
+            if (__any_sync(0xffffffffu, odd)) {
+                // a value row that is not finite (or is not there): the outputs of the rows that see it are not either,
+                // and it must not meet the zero weights of those that do not
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int jj = j + u * kKvTokens + g + 8 * x;
+                        if (fabsf(sv[u][x]) + fabsf(zv[u][x]) < INFINITY) continue;
+                        const bool there = jj < len && (found >> u & 1u);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            zs[nt] = zs[nt] + f2(there && jj < q.lim[nt][0] ? NAN : 0.f, there && jj < q.lim[nt][1] ? NAN : 0.f);
+                        sv[u][x] = 0.f;
+                        zv[u][x] = 0.f;
+                    }
+            }
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     const int jj = j + u * kKvTokens + g + 8 * x;
                     const bool there = jj < len && (found >> u & 1u);
-                    if (there && !(fabsf(sv[u][x]) + fabsf(zv[u][x]) < INFINITY)) {
-                        // a value row that is not finite: the outputs of the rows that see it are not either, and it
-                        // must not meet the zero weights of those that do not
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-                            zs[nt] = zs[nt] + f2(jj < q.lim[nt][0] ? NAN : 0.f, jj < q.lim[nt][1] ? NAN : 0.f);
-                        sv[u][x] = 0.f;
-                        zv[u][x] = 0.f;
-                    }
                     if (!there) { sv[u][x] = 0.f; zv[u][x] = 0.f; }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
