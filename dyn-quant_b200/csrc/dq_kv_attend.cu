@@ -24,20 +24,24 @@
 // A decode step has at most 8 rows per KV head, so nothing of an MMA is idle,
 // and a lane's S values (slots g, g + 8; rows 2t, 2t + 1) lie in the lanes that
 // hold its O columns' rows: maxima, sums and rescaling stay in the lane.
-// Codes are used as they lie: a nibble at bits 0..3 or 4..7 of a half word is the
-// subnormal f16 number c 2^-24 or c 2^-20, which an MMA multiplies exactly, so a
-// word of eight codes costs one shift and four masks.  Scores keep the two
-// weights in two accumulators; in the output they lie in different rows of the
-// MMA and are set right at the end.  Scales and zeros are applied in FP32:
+// A nibble at bits 0..3 or 4..7 of a half word is the subnormal f16 number c 2^-24
+// or c 2^-20, which an MMA multiplies exactly, so a word of eight codes costs one
+// shift and four masks.  But an MMA cuts its terms off below the largest, for which
+// a subnormal counts as 2^-14.  Scores are not to feel that (with one column of q at
+// 4000 and the rest below 1 they were off by 0.5 in units of a code, 200 times what
+// normal numbers give): keys are brought to c 2^-14 by one multiplication a pair
+// (64 sequences of 2000 to 4096 slots with 32 heads: 166 -> 171.5 us; 131071 slots
+// with 8 heads of 8 rows: 46.0 -> 46.9).  In the output the values' codes are used as they
+// lie: the two weights lie in different rows of the MMA and are set right at the
+// end.  Scales and zeros are applied in FP32:
 //   S   = s_k (D - z_k sum q),  D the MMAs' sum of q c
 //   O   = sum p' (c - 8) - sum p' (z_v - 8),  p' = p s_v w
 // The 8 is the same for all columns: one MMA a unit with a constant A collects
 // 8 sum p' and every 8 steps it is taken off all of O, which keeps the running
 // sums (FP32, and the rounding of p' in them) at the size of the centred values.
-// An MMA cuts its terms off below the largest (a subnormal counts as 2^-14), and
-// codes all have one sign: the output of 128K slots, a thousandth of a value's
-// size, leaned by 2e-4 of it.  So the second unit of a step is taken the other
-// way round, -p' with 15 - c, and the errors cancel (1% of the time).
+// Codes all have one sign, so what is cut off adds up: the output of 128K slots, a
+// thousandth of a value's size, leaned by 2e-4 of it.  So the second unit of a step
+// is taken the other way round, -p' with 15 - c, and the errors cancel (1% of the time).
 // p' is the only rounding to FP16 besides the output's: p <= 2^8 (the maximum
 // is taken again only when a score passes it by 8) and w is the power of two
 // that brings the largest s_v seen to at most 2^7, so p' <= 2^15 and small
@@ -59,7 +63,8 @@ namespace {
 __device__ unsigned int g_kv_attend_error;
 
 constexpr int kAtMaxWarps = 2560;     // bound on the grid's warps (workspace sizing)
-constexpr float kCode = 16777216.0f;  // 2^24: a masked code is c / kCode
+constexpr float kCode = 16777216.0f;  // 2^24: a masked low code is c / kCode
+constexpr float kKey = 16384.0f;      // 2^14: a key's code in its product is c / kKey
 
 // Warps of a CTA and CTAs of an SM for row tiles of 8 NT rows: two row tiles
 // need about 200 registers a thread, one tile 128.
@@ -69,6 +74,14 @@ __host__ __device__ constexpr int at_ctas(int nt) { return nt == 1 ? 2 : 1; }
 // f16 pairs c 2^-24 of the nibbles at bits 0..3 and 16..19, c 2^-20 of those at bits 4..7 and 20..23.
 __device__ __forceinline__ uint32_t low_codes(uint32_t w) { return w & 0x000F000Fu; }
 __device__ __forceinline__ uint32_t high_codes(uint32_t w) { return w & 0x00F000F0u; }
+// Both as c 2^-14, normal numbers (exact).
+__device__ __forceinline__ uint32_t times(uint32_t w, uint32_t pow2) {
+    uint32_t r;
+    asm("mul.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(pow2));
+    return r;
+}
+__device__ __forceinline__ uint32_t low_keys(uint32_t w) { return times(low_codes(w), 0x64006400u); }
+__device__ __forceinline__ uint32_t high_keys(uint32_t w) { return times(high_codes(w), 0x54005400u); }
 // mask & ~w, the codes 15 - c, in one instruction (left to itself, ~w would be one of its own)
 __device__ __forceinline__ uint32_t and_not(uint32_t mask, uint32_t w) {
     uint32_t r;
@@ -134,7 +147,7 @@ __device__ __forceinline__ float lane_sum_g(float v) {
 template <int D, int NT>
 struct QueryTile {
     uint32_t f[NT][D / 8];  // per 8-column word: (0,4), (1,5), (2,6), (3,7)
-    f2 sum[NT];             // - sum of q over the columns / kCode, rows 2t and 2t + 1
+    f2 sum[NT];             // - sum of q over the columns / kKey, rows 2t and 2t + 1
     int lim[NT][2];         // keys that rows 2t and 2t + 1 see
     int min_lim, max_lim;   // over the tile's rows
 
@@ -184,7 +197,7 @@ struct QueryTile {
                 lo = min(lo, l);
                 hi = max(hi, l);
             }
-            s *= -1.f / kCode;
+            s *= -1.f / kKey;
             sum[nt] = f2(__shfl_sync(0xffffffffu, s, 8 * t), __shfl_sync(0xffffffffu, s, 8 * t + 4));
 #pragma unroll
             for (int e = 0; e < 2; ++e) lim[nt][e] = __shfl_sync(0xffffffffu, l, 8 * t + 4 * e);
@@ -199,7 +212,7 @@ struct QueryTile {
     }
 };
 
-// D / kCode of U units: the MMAs' sums of q c for slots g, g + 8 and rows 2t, 2t + 1.
+// D / kKey of U units, D the MMAs' sums of q c for slots g, g + 8 and rows 2t, 2t + 1.
 template <int D, int NT, int U>
 __device__ __forceinline__ void score_mma(int unit, const QueryTile<D, NT>& q, f2 (&s)[U][NT][2]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -219,11 +232,11 @@ __device__ __forceinline__ void score_mma(int unit, const QueryTile<D, NT>& q, f
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 if (i == 0) {
-                    mma_first(lo[u][nt], low_codes(w0), low_codes(w1), low_codes(x0), low_codes(x1), q.f[nt][0], q.f[nt][2]);
-                    mma_first(hi[u][nt], high_codes(w0), high_codes(w1), high_codes(x0), high_codes(x1), q.f[nt][1], q.f[nt][3]);
+                    mma_first(lo[u][nt], low_keys(w0), low_keys(w1), low_keys(x0), low_keys(x1), q.f[nt][0], q.f[nt][2]);
+                    mma_first(hi[u][nt], high_keys(w0), high_keys(w1), high_keys(x0), high_keys(x1), q.f[nt][1], q.f[nt][3]);
                 } else {
-                    mma(lo[u][nt], low_codes(w0), low_codes(w1), low_codes(x0), low_codes(x1), q.f[nt][4 * i], q.f[nt][4 * i + 2]);
-                    mma(hi[u][nt], high_codes(w0), high_codes(w1), high_codes(x0), high_codes(x1), q.f[nt][4 * i + 1],
+                    mma(lo[u][nt], low_keys(w0), low_keys(w1), low_keys(x0), low_keys(x1), q.f[nt][4 * i], q.f[nt][4 * i + 2]);
+                    mma(hi[u][nt], high_keys(w0), high_keys(w1), high_keys(x0), high_keys(x1), q.f[nt][4 * i + 1],
                         q.f[nt][4 * i + 3]);
                 }
             }
@@ -234,7 +247,7 @@ __device__ __forceinline__ void score_mma(int unit, const QueryTile<D, NT>& q, f
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int x = 0; x < 2; ++x)
-                s[u][nt][x] = fma2(f2(hi[u][nt][2 * x], hi[u][nt][2 * x + 1]), f2(0.0625f), f2(lo[u][nt][2 * x], lo[u][nt][2 * x + 1]));
+                s[u][nt][x] = f2(hi[u][nt][2 * x], hi[u][nt][2 * x + 1]) + f2(lo[u][nt][2 * x], lo[u][nt][2 * x + 1]);
 }
 
 // A warp's run of steps through its ring: lane i % 32 of each 32 steps looks
@@ -1054,7 +1067,7 @@ dq_status_t launch_kv_attend(const dq_kv_cache_t& c, const dq_kv_attend_t& r, vo
     a.tokens = r.tokens;
     a.group = Div(r.q_heads / c.kv_heads);
     const float scale2 = r.scale * 1.44269504088896341f;
-    a.scale2 = scale2 * kCode;
+    a.scale2 = scale2 * kKey;
     a.done = c.arrivals + c.n_seqs;
     const AttendWs w = attend_ws(c, r.tokens, r.q_heads, r.accumulate != 0);
     char* base = static_cast<char*>(workspace);

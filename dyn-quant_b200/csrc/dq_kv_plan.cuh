@@ -24,7 +24,7 @@ struct KvAttendArgs {
     uint32_t* done;          // [n_seqs][heads] CTAs of a cut job that have arrived (one row tile)
     int tokens;              // query tokens
     Div group, n_rt, jobs;   // query heads per KV head, row tiles, jobs of a sequence
-    float scale2;            // scale * log2(e) * kCode
+    float scale2;            // scale * log2(e), times 2^14 where the codes are c 2^-14
     int depth;               // ring slots per warp
     int first_off, places;   // shared memory for some of those pieces: its offset, how many
 };

@@ -99,3 +99,63 @@ def test_a_sequence_without_queries_gains_no_weight(group, t, value):
     assert torch.equal(cache.mass[page, :, off], mass0[page, :, off])
     page, off = slots(cache, 0, 151)
     assert (cache.mass[page, :, off] > mass0[page, :, off]).all()
+
+
+# ---------------------------------------------------------------------------
+# scores
+# ---------------------------------------------------------------------------
+def definition(cache, q, b, scale):
+    """attend() of sequence b in float64 on the GPU: scores [T, KV heads, group, n], lse [T, q_heads], mass
+    [KV heads, n], and K's codes, scales, zeros [KV heads, n, ...]."""
+    h, d, size, n = cache.n_kv_heads, cache.head_dim, cache.page_size, int(cache.lengths[b])
+    u = cache.units[cache.page_table[b, :-(-n // size)].long()].transpose(0, 1).reshape(h, -1, 16 * d + 128)
+    par = u[..., 16 * d:].contiguous().view(torch.float16).view(h, -1, 4).double()[:, :n]
+    raw = u[..., :8 * d].reshape(h, -1, d // 2)[:, :n]
+    code = torch.stack([raw & 15, raw >> 4], -1).flatten(-2).double()
+    t = q.shape[1]
+    qq = q[b].double().view(t, h, -1, d)
+    s = scale * torch.einsum("thgd,hnd->thgn", qq, par[..., :1] * (code - par[..., 1:2]))
+    late = torch.arange(n, device="cuda") > n - t + torch.arange(t, device="cuda")[:, None]
+    s = s.masked_fill(late[:, None, None], float("-inf"))
+    l = torch.logsumexp(s, -1)
+    return s, l.reshape(t, -1), torch.exp(s - l[..., None]).sum((0, 2)), code, par[..., 0], par[..., 1]
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("large", [20, 21])
+@pytest.mark.parametrize("group,t", [(1, 1), (8, 1), (8, 2), (8, 4), (8, 9)])
+def test_scores_of_queries_with_one_large_column(dim, group, t, large):
+    """One column of the query is 4000, the rest lie in [0, 1), and the keys' codes of that column are 0 or 1: the small
+    columns' share of a score is not lost.
+    A score's error, in code units (the score is scale s_k times that):
+      - FP32 sums of q c: each of the D/16 MMAs cuts its 17 terms off 2^-23 below the largest, at most sum |q| c;
+      - sum q, D/4 additions and two shuffles deep at most, and its product with z: (D/4 + 4) 2^-24 |z| sum |q|;
+      - joining the two halves of D, the zero's part and the scale: 3 x 2^-24 x (sum |q| c + |z| sum |q|).
+    lse: the largest score error, 2^-20 for the sum of weights (an exponential 2^-22, a lane's some hundred additions),
+    2^-22 of the largest score, 2^-21 for the logarithm."""
+    lens = [5000, 1300]
+    cache = R.make_cache([0, 0], 2, dim, 64, seed=7, extra=5000)
+    gen = torch.Generator().manual_seed(8)
+    k = torch.rand(2, 5000, 2, dim, generator=gen) * 3.75
+    k[..., large] = torch.randint(0, 2, k.shape[:-1], generator=gen) * 0.25
+    k[..., 3], k[..., 4] = 0.0, 3.75
+    cache.append(k.half().cuda(), k.half().cuda(), counts=ints(*lens))
+    q = torch.rand(2, t, 2 * group, dim, generator=gen)
+    q[..., large] = 4000.0
+    q = q.half().cuda()
+    scale = 2e-3
+    out, lse = cache.attend(q, scale=scale, accumulate=True, return_lse=True)
+    for b, n in enumerate(lens):
+        s, l, mass, code, ks, kz = definition(cache, q, b, scale)
+        qa = q[b].double().abs().view(t, 2, group, dim)
+        total = qa.sum(-1)[..., None]
+        terms = torch.einsum("thgd,hnd->thgn", qa, code)
+        zeros = kz.abs()[:, None] * total
+        err = (dim // 16 * 17 * 2.0 ** -23 * terms + (dim // 4 + 4) * 2.0 ** -24 * zeros
+               + 3 * 2.0 ** -24 * (terms + zeros)) * scale * ks[:, None]
+        tol = err.amax(-1).reshape(t, -1) + 2.0 ** -20 + 2.0 ** -22 * s.masked_fill(s.isinf(), 0).abs().max() + 2.0 ** -21
+        assert ((lse[b].double() - l).abs() <= tol).all()
+        # a slot's weights: its scores' errors and the lse's, the exponential, one addition a row
+        page, at = slots(cache, b, n)
+        gain = cache.mass[page, :, at].double().T
+        assert ((gain - mass).abs() <= (err.amax((0, 2)) + tol.max() + 2.0 ** -21 + t * group * 2.0 ** -24) * mass).all()
