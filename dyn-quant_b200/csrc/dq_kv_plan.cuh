@@ -3,6 +3,8 @@
 // the lengths), the exchange of partial results, and small arithmetic.
 #pragma once
 
+#include <cfloat>
+
 #include "dq_kv.cuh"
 
 namespace dq {
@@ -38,7 +40,7 @@ dq_status_t launch_kv_chunk_mass(KvAttendArgs a, int head_dim, float* sums, cuda
 
 namespace {
 
-constexpr float kNone = -1e30f;       // running maximum of a row that has seen no key
+constexpr float kNone = -FLT_MAX;     // running maximum of a row that has seen no key
 constexpr float kLazy = 8.0f;         // a score passes the running maximum by this much (log2) before it moves
 constexpr int kStep = 2 * kKvTokens;  // slots of one step of a run
 
