@@ -73,9 +73,9 @@ struct CkSmem {
     static constexpr int kTotal = kBars + 128;
 };
 
-// Barriers (8 bytes each).  Each but the last is a pair, one for the even and one for the odd blocks.  S full also
-// says that K has been read, V free that the block's product is in O.
-enum { kRawFull = 0, kKFull = 2, kVFull = 4, kVFree = 6, kSFull = 8, kPFull = 10, kRawFree = 12, kQFull = 14 };
+// Barriers (8 bytes each).  Each but the last two is a pair, one for the even and one for the odd blocks.  S full also
+// says that K has been read, V free that the block's product is in O, done that every product has ended.
+enum { kRawFull = 0, kKFull = 2, kVFull = 4, kVFree = 6, kSFull = 8, kPFull = 10, kRawFree = 12, kQFull = 14, kDone = 15 };
 
 // Tensor memory columns: two S tiles, O, two P tiles (f16 pairs).
 constexpr uint32_t kTmS = 0, kTmO = 256, kTmP = 384, kTmCols = 512;
@@ -259,6 +259,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
             mbar_init(bars + 8 * (kPFull + i), kSoft);
         }
         mbar_init(bars + 8 * kQFull, kSoft);
+        mbar_init(bars + 8 * kDone, 1);
         fence_mbar_init();
     }
     tm_before_sync();
@@ -280,6 +281,13 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
         if (dead) return;
         dead = !__all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * bar, parity & 1));
         if (dead && lane == 0) atomicOr(&g_kv_chunk_error, kKvErrWait);
+    };
+    // The MMA warp's end: tensor and shared memory are let go only when its products have ended, also after a wait that
+    // gave up (a barrier of its own, since the others' phases may then lie behind).
+    auto drain = [&](int bar) {
+        if (lane == 0) tm_commit(bars + 8 * bar);
+        __syncwarp();
+        if (!mbar_wait_bounded(bars + 8 * bar, 0) && lane == 0) atomicOr(&g_kv_chunk_error, kKvErrWait);
     };
     Walk at;
     if (n > 0) at.set(p, c.n_seqs, u0);
@@ -578,7 +586,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_kernel(const KvAttendA
             begins = i + 1 < n && at.next(p, c.n_seqs, u0 + i + 1);
         }
         output(n - 1, begins_before);
-        wait(kVFree + ((n - 1) & 1), (n - 1) >> 1);
+        drain(kDone);
     } else if (n > 0) {
         // ---- loading: a lane a unit, a copy a run of units of one page
         bool absent = false;
@@ -681,7 +689,7 @@ struct CmSmem {
 // Barriers: four for the units' buffers and for the S tiles, two for K's tiles.  S full also says that K has been read,
 // and a block's constants are kept until its S is free: the warps that fill them are at most six blocks ahead of those
 // that read them, the loading warp ten.
-enum { kCmRawFull = 0, kCmRawFree = 4, kCmSFull = 8, kCmSFree = 12, kCmKFull = 16, kCmQFull = 18 };
+enum { kCmRawFull = 0, kCmRawFree = 4, kCmSFull = 8, kCmSFree = 12, kCmKFull = 16, kCmQFull = 18, kCmDone = 19 };
 
 template <int D>
 __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAttendArgs a, float* sums, const long long lines,
@@ -705,6 +713,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
         }
         for (int i = 0; i < 2; ++i) mbar_init(bars + 8 * (kCmKFull + i), 128);
         mbar_init(bars + 8 * kCmQFull, kSoft);
+        mbar_init(bars + 8 * kCmDone, 1);
         fence_mbar_init();
     }
     tm_before_sync();
@@ -722,6 +731,13 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
         if (dead) return;
         dead = !__all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * bar, parity & 1));
         if (dead && lane == 0) atomicOr(&g_kv_chunk_error, kKvErrWait);
+    };
+    // The MMA warp's end: tensor and shared memory are let go only when its products have ended, also after a wait that
+    // gave up (a barrier of its own, since the others' phases may then lie behind).
+    auto drain = [&](int bar) {
+        if (lane == 0) tm_commit(bars + 8 * bar);
+        __syncwarp();
+        if (!mbar_wait_bounded(bars + 8 * bar, 0) && lane == 0) atomicOr(&g_kv_chunk_error, kKvErrWait);
     };
     Walk at;
     if (n > 0) at.set(p, c.n_seqs, u0);
@@ -882,7 +898,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv_chunk_mass_kernel(const KvAt
             __syncwarp();
             begins = i + 1 < n && at.next(p, c.n_seqs, u0 + i + 1);
         }
-        wait(kCmSFull + ((n - 1) & 3), (n - 1) >> 2);
+        drain(kCmDone);
     } else if (n > 0) {
         // ---- loading, as above
         int asked = 0;
