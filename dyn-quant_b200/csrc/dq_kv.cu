@@ -342,53 +342,58 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_kernel(const KvEvictArgs 
     const int len = kv_length(c, b, &bad);
     const int gone = ld_l2(c.evicted + b);
     if (bad && tid == 0) atomicOr(&g_kv_error, kKvErrLen);
-    const bool work = len > a.keep;
+    bool work = len > a.keep;
     int n_moves = 0;
-    if (work) {
-        const int newest = gone + len;
-        const int units = (len + kKvTokens - 1) / kKvTokens, share = (units + cs - 1) / cs, rounds = (share + kEvThreads - 1) / kEvThreads;
-        uint32_t k[kKvTokens];
-        int n = 0, slot0 = 0;  // this thread's unit of the round: its slots in use, the first of them
-        auto fetch = [&](int round) {
-            const int i = round * kEvThreads + tid;
-            slot0 = (rank * share + i) * kKvTokens;
-            n = i >= share || len - slot0 < 0 ? 0 : (len - slot0 > kKvTokens ? kKvTokens : len - slot0);
-            const int page = n > 0 ? kv_page(c, b, slot0) : 0;
-            if (n > 0 && page < 0) {
-                page_ok = false;  // the slots of an absent page weigh least
+    const int newest = gone + len;
+    const int units = (len + kKvTokens - 1) / kKvTokens, share = (units + cs - 1) / cs, rounds = (share + kEvThreads - 1) / kEvThreads;
+    uint32_t k[kKvTokens];
+    int n = 0, slot0 = 0;  // this thread's unit of the round: its slots in use, the first of them
+    auto fetch = [&](int round) {
+        const int i = round * kEvThreads + tid;
+        slot0 = (rank * share + i) * kKvTokens;
+        n = i >= share || len - slot0 < 0 ? 0 : (len - slot0 > kKvTokens ? kKvTokens : len - slot0);
+        const int page = n > 0 ? kv_page(c, b, slot0) : -1;
 #pragma unroll
-                for (int j = 0; j < kKvTokens; ++j) k[j] = 0u;
-            } else if (n > 0) {
-                const size_t line = kv_line(c, page, h) + slot0 % c.page_size;
-                uint32_t w[kKvTokens], p[kKvTokens];
-                const bool wide = ((reinterpret_cast<uintptr_t>(c.mass) | reinterpret_cast<uintptr_t>(c.pos)) & 15u) == 0;
+        for (int j = 0; j < kKvTokens; ++j) k[j] = 0u;
+        if (page >= 0) {
+            const size_t line = kv_line(c, page, h) + slot0 % c.page_size;
+            uint32_t w[kKvTokens], p[kKvTokens];
+            const bool wide = ((reinterpret_cast<uintptr_t>(c.mass) | reinterpret_cast<uintptr_t>(c.pos)) & 15u) == 0;
 #pragma unroll
-                for (int j = 0; j < kKvTokens; j += 4) {
-                    if (wide) {
-                        const uint4 x = ld_l2_v4(c.mass + line + j), y = ld_l2_v4(c.pos + line + j);
-                        w[j] = x.x; w[j + 1] = x.y; w[j + 2] = x.z; w[j + 3] = x.w;
-                        p[j] = y.x; p[j + 1] = y.y; p[j + 2] = y.z; p[j + 3] = y.w;
-                    } else {
+            for (int j = 0; j < kKvTokens; j += 4) {
+                if (wide) {
+                    const uint4 x = ld_l2_v4(c.mass + line + j), y = ld_l2_v4(c.pos + line + j);
+                    w[j] = x.x; w[j + 1] = x.y; w[j + 2] = x.z; w[j + 3] = x.w;
+                    p[j] = y.x; p[j + 1] = y.y; p[j + 2] = y.z; p[j + 3] = y.w;
+                } else {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            w[j + e] = __float_as_uint(ld_l2(c.mass + line + j + e));
-                            p[j + e] = static_cast<uint32_t>(ld_l2(c.pos + line + j + e));
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        w[j + e] = __float_as_uint(ld_l2(c.mass + line + j + e));
+                        p[j + e] = static_cast<uint32_t>(ld_l2(c.pos + line + j + e));
                     }
                 }
-#pragma unroll
-                for (int j = 0; j < kKvTokens; ++j) {
-                    uint32_t u = __float_as_uint(__fadd_rn(__uint_as_float(w[j]), 0.f));  // -0 counts as 0
-                    u ^= (u >> 31) ? 0xFFFFFFFFu : 0x80000000u;
-                    const int at = static_cast<int>(p[j]);
-                    k[j] = (at >= newest - a.recent || at < a.sink) ? 0xFFFFFFFFu : (u < 0xFFFFFFFEu ? u : 0xFFFFFFFEu);
-                }
             }
-        };
+#pragma unroll
+            for (int j = 0; j < kKvTokens; ++j) {
+                uint32_t u = __float_as_uint(__fadd_rn(__uint_as_float(w[j]), 0.f));  // -0 counts as 0
+                u ^= (u >> 31) ? 0xFFFFFFFFu : 0x80000000u;
+                const int at = static_cast<int>(p[j]);
+                k[j] = (at >= newest - a.recent || at < a.sink) ? 0xFFFFFFFFu : (u < 0xFFFFFFFEu ? u : 0xFFFFFFFEu);
+            }
+        }
+    };
+    if (work) {
         for (int i = 4 * tid; i < 2 * kEvRadix; i += 4 * kEvThreads) *reinterpret_cast<uint4*>(&local[0][0] + i) = make_uint4(0, 0, 0, 0);
         for (int i = 4 * tid; i < 3 * kEvRadix; i += 4 * kEvThreads) *reinterpret_cast<uint4*>(&hists[0][0] + i) = make_uint4(0, 0, 0, 0);
+        // A sequence with a page outside the pool is left as it is: a slot that is not there can neither be ranked nor
+        // take a survivor.  Every CTA looks at all of its pages, so that they agree.
+        bool there = true;
+        for (int i = tid; i * c.page_size < len; i += kEvThreads) there &= kv_page(c, b, i * c.page_size) >= 0;
         if (rounds == 1) fetch(0);
-        meet();
+        if (cs > 1) cluster.sync();
+        work = page_ok = __syncthreads_and(there);
+    }
+    if (work) {
         // the keep-th largest key
         uint32_t prefix = 0, mask = 0;
         int need = a.keep;

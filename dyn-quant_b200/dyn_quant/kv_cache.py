@@ -169,7 +169,8 @@ class Int4KVCache:
         the last `recent` and the first `sink` positions stay, and of the other
         slots those with the largest `mass` (equal ones: lowest slot first).
         Kept slots beyond `keep` move into the freed ones below (one kernel, two
-        when more than 256 slots of a head may have to move)."""
+        when more than 256 slots of a head may have to move).  A sequence with a
+        page missing is left as it is and reported in the device error word."""
         self._h.evict(keep, recent, sink)
 
     def read(self, seq: int):

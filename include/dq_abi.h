@@ -488,8 +488,10 @@ DQ_API size_t dq_kv_evict_workspace_bytes(const dq_kv_cache_t* cache, int32_t ke
  * ones lowest slot first.  Survivors below slot `keep` stay where they are; the
  * k-th survivor beyond moves into the k-th freed slot below, with its mass and
  * position.  evicted[b] grows by what lengths[b] loses; slots from `keep` on are
- * left as they were.  Attention does not depend on the order of slots.  One
- * kernel, two where a sequence may lose more than 256 slots at once.
+ * left as they were.  Attention does not depend on the order of slots.  A
+ * sequence one of whose slots lies in a page outside the pool is left as it is
+ * and sets a bit of the device error word.  One kernel, two where a sequence may
+ * lose more than 256 slots at once.
  */
 DQ_API dq_status_t dq_kv_evict(const dq_kv_cache_t* cache, int32_t keep, int32_t recent, int32_t sink,
                                void* workspace, size_t workspace_bytes, void* stream);

@@ -186,3 +186,81 @@ def test_scores_below_minus_1e30(group, t):
         off = (out[b].double() - want.double()).abs()
         assert (off <= 2.0 ** -10 * want.double().abs() + 17 * 2.0 ** -14)[clear].all()
         assert ((lse[b].double() - two.values[..., 0].reshape(t, -1)).abs() <= 1.3e31 + 2.0 ** -22 * 4e35).all()
+
+
+# ---------------------------------------------------------------------------
+# evict
+# ---------------------------------------------------------------------------
+def raw_cache(lens, heads, dim, page, ties, seed=1):
+    """A cache of random bytes (evict moves them unread), weights and positions, pages in any order, two of them
+    nobody's."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    need = [max(1, -(-n // page)) for n in lens]
+    cache = Int4KVCache(len(lens), sum(need) + 2, heads, dim, page, max_pages=max(need))
+    cache.units.random_(0, 256, generator=gen)
+    cache.mass.uniform_(0, 4 if ties else 1, generator=gen)
+    if ties:
+        cache.mass.floor_()
+    order = torch.randperm(cache.n_pages, generator=torch.Generator().manual_seed(seed)).tolist()
+    for b, m in enumerate(need):
+        cache.assign(b, order[:m])
+        del order[:m]
+        page_of, off = slots(cache, b, m * page)
+        for h in range(heads):
+            cache.pos[page_of, h, off] = torch.randperm(m * page, generator=gen, device="cuda").int() + 3
+    cache.lengths.copy_(ints(*lens))
+    cache.evicted.fill_(3)
+    return cache
+
+
+def lines(cache, b):
+    """Every slot of a sequence as one row of bytes, with its weight and position: [heads, slots, head_dim + 16]."""
+    d, h = cache.head_dim, cache.n_kv_heads
+    pages = cache.page_table[b]
+    pages = pages[pages >= 0].long()
+    u = cache.units[pages].transpose(0, 1).reshape(h, -1, 16 * d + 128)
+    k = u[..., :8 * d].reshape(h, -1, d // 2)
+    v = u[..., 8 * d:16 * d].reshape(h, -1, 8, d // 4, 2, 2).transpose(3, 4).reshape(h, -1, d // 2)
+    rest = [x[pages].transpose(0, 1).reshape(h, -1, 1).contiguous().view(torch.uint8) for x in (cache.mass, cache.pos)]
+    return torch.cat([k, v, u[..., 16 * d:].reshape(h, -1, 8), *rest], -1).cpu().numpy()
+
+
+def evicted_lines(cache, b, keep, recent, sink):
+    """What lines(cache, b) has to be after evict, and how many slots move."""
+    want, n, moves = lines(cache, b), int(cache.lengths[b]), 0
+    if n <= keep:
+        return want, 0
+    page, off = slots(cache, b, n)
+    mass, pos = cache.mass.cpu().numpy(), cache.pos.cpu().numpy()
+    seen = n + int(cache.evicted[b])
+    for h in range(cache.n_kv_heads):
+        w, p = mass[page, h, off].astype(np.float64), pos[page, h, off]
+        w[(p >= seen - recent) | (p < sink)] = np.inf
+        kept = np.zeros(n, bool)
+        kept[np.lexsort((np.arange(n), -w))[:keep]] = True
+        to, src = np.flatnonzero(~kept[:keep]), keep + np.flatnonzero(kept[keep:])
+        want[h, to] = want[h, src]
+        moves += len(to)
+    return want, moves
+
+
+@pytest.mark.parametrize("lens,keep", [([200, 150], 100), ([700, 690], 400), ([9000, 8990], 5000)])
+@pytest.mark.parametrize("below", [True, False])
+def test_evict_leaves_a_sequence_with_a_missing_page_as_it_is(lens, keep, below):
+    """A page outside the pool, below `keep` or beyond: nothing of its sequence moves or is lost, the device error word
+    says so, and the other sequences are cut."""
+    cache = raw_cache(lens, 2, 64, 16, False)
+    gone = 2 if below else lens[0] // 16 - 1
+    page = int(cache.page_table[0, gone])
+    want = lines(cache, 0), evicted_lines(cache, 1, keep, 8, 2)[0]
+    cache.page_table[0, gone] = cache.n_pages if below else -1
+    cache.evict(keep, recent=8, sink=2)
+    torch.cuda.synchronize()
+    assert _C.read_device_error(True) == 1 << 16
+    cache.page_table[0, gone] = page
+    assert cache.lengths.tolist() == [lens[0], keep] and cache.evicted.tolist() == [3, 3 + lens[1] - keep]
+    for b in range(2):
+        assert np.array_equal(lines(cache, b), want[b]), f"sequence {b}"
+    assert not cache._arrivals.any()
+    cache.evict(keep, recent=8, sink=2)  # with its page again
+    assert cache.lengths.tolist() == [keep, keep]
