@@ -244,6 +244,38 @@ def evicted_lines(cache, b, keep, recent, sink):
     return want, moves
 
 
+# (cluster, rounds) is what the kernel takes on 148 SMs: CTAs a head, turns of 4096 slots of each
+EVICT = [
+    (64, 2, 64, [9000], 5000, 100, 7),              # (4, 1)
+    (128, 2, 48, [9000, 300], 8850, 100, 7),        # (4, 1), moves made by the selecting kernel
+    (128, 1, 64, [20000], 10000, 0, 0),             # (8, 1)
+    (64, 2, 64, [20000, 20010], 19900, 19000, 900),  # (8, 1), moves made by the selecting kernel, most slots protected
+    (64, 8, 64, [4900 - 37 * i for i in range(38)], 3600, 64, 5),  # (1, 2) and, below 4097 slots, (1, 1)
+    (64, 8, 64, [4900 - 7 * i for i in range(38)], 4700, 64, 5),   # the same, moves made by the selecting kernel
+    (64, 1, 16, [40000, 33000], 21000, 512, 4),     # (8, 2)
+    (128, 1, 64, [70000], 200, 100, 4),             # (8, 3), moves made by the selecting kernel
+]
+
+
+@pytest.mark.parametrize("dim,heads,page,lens,keep,recent,sink", EVICT)
+@pytest.mark.parametrize("ties", [False, True])
+def test_evict_over_clusters_and_rounds(dim, heads, page, lens, keep, recent, sink, ties):
+    """Few weights that many slots share: the threshold's ties span the CTAs and the rounds."""
+    cache = raw_cache(lens, heads, dim, page, ties)
+    want = [evicted_lines(cache, b, keep, recent, sink) for b in range(len(lens))]
+    mine = torch.zeros(cache.n_pages, dtype=torch.bool, device="cuda")
+    mine[cache.page_table[cache.page_table >= 0].long()] = True
+    rest = cache.units[~mine].clone()
+    cache.evict(keep, recent=recent, sink=sink)
+    assert cache.lengths.tolist() == [min(n, keep) for n in lens]
+    assert cache.evicted.tolist() == [3 + max(0, n - keep) for n in lens]
+    for b, (rows, moves) in enumerate(want):
+        assert lens[b] <= keep or moves > 0
+        assert np.array_equal(lines(cache, b), rows), f"sequence {b}"
+    assert torch.equal(cache.units[~mine], rest)
+    assert not cache._arrivals.any()
+
+
 @pytest.mark.parametrize("lens,keep", [([200, 150], 100), ([700, 690], 400), ([9000, 8990], 5000)])
 @pytest.mark.parametrize("below", [True, False])
 def test_evict_leaves_a_sequence_with_a_missing_page_as_it_is(lens, keep, below):
