@@ -67,7 +67,21 @@ __device__ __forceinline__ KvRow kv_quant_row(uint4& raw) {
     uint32_t mm = min_h2(__byte_perm(lo2, hi2, 0x5410), __byte_perm(lo2, hi2, 0x7632));  // (min, -max)
 #pragma unroll
     for (int o = LPR / 2; o >= 1; o >>= 1) mm = min_h2(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-    const float lo = h2f_bits(lo16(mm)), range = __fsub_rn(-h2f_bits(hi16(mm)), lo);
+    float lo = h2f_bits(lo16(mm));
+    const float range = __fsub_rn(-h2f_bits(hi16(mm)), lo);
+    if (__any_sync(0xffffffffu, lo == 0.f)) {
+        // zeros of both signs: the quantizer's minimum is the row's first one, whose sign the zero-point shows
+        uint32_t first = 2;  // this lane's first zero: its sign, 2 where it has none
+#pragma unroll
+        for (int i = 7; i >= 0; --i) {
+            const uint32_t v = i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xFFFFu;
+            if ((v & 0x7FFFu) == 0) first = v >> 15;
+        }
+        const int row = (threadIdx.x & 31) & ~(LPR - 1);  // the row's first lane
+        const uint32_t has = __ballot_sync(0xffffffffu, first != 2) >> row & ((1u << LPR) - 1u);
+        const uint32_t negative = __ballot_sync(0xffffffffu, first == 1) >> row;
+        if (lo == 0.f) lo = (has & (0u - has) & negative) != 0 ? -0.f : 0.f;
+    }
     const float step = (range < 1e-8f) ? 1.0f : __fdiv_rn(range, 15.0f);
     const float inv = __fdiv_rn(1.0f, step);
     KvRow r;

@@ -6,6 +6,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
+import dyn_quant  # noqa: E402
 import kv_ref as R  # noqa: E402
 from dyn_quant import _C  # noqa: E402
 from dyn_quant.kv_cache import Int4KVCache  # noqa: E402
@@ -296,3 +297,35 @@ def test_evict_leaves_a_sequence_with_a_missing_page_as_it_is(lens, keep, below)
     assert not cache._arrivals.any()
     cache.evict(keep, recent=8, sink=2)  # with its page again
     assert cache.lengths.tolist() == [keep, keep]
+
+
+# ---------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dim", [64, 128])
+def test_append_equals_quantize_where_the_minimum_is_a_zero_of_either_sign(dim):
+    """The zero-point's sign bit is that of the row's first zero."""
+    gen = torch.Generator().manual_seed(9)
+    n = 400
+    x = torch.rand(n, dim, generator=gen) * torch.randint(0, 2, (n, 1), generator=gen)  # every other row is flat
+    x[torch.rand(n, dim, generator=gen) < 0.2 * torch.rand(n, 1, generator=gen)] = 0.0
+    x = torch.where(torch.rand(n, dim, generator=gen) < 0.5, x, torch.where(x == 0, -0.0, x))
+    x[7] = 0.0
+    x[8] = -0.0
+    x[9] -= 0.5
+    x = x.half().cuda()
+    cache = R.make_cache([0], 2, dim, 16, extra=n // 2)
+    kv, vv = cache.append(x.view(1, -1, 2, dim), x.flip(0).view(1, -1, 2, dim), values=True)
+    # a row of 64 twice over is a group of 128 with the same minimum, maximum and first zero
+    packed, s, z, _ = dyn_quant.quantize(x if dim == 128 else torch.cat([x, x], 1).contiguous())
+    codes = torch.stack([packed & 15, packed >> 4], -1).flatten(1)[:, :dim]
+    page, off = slots(cache, 0, n // 2)
+    par = cache.units.view(torch.float16)[..., 8 * dim:].unflatten(-1, (16, 4))[page, :, off // 16, off % 16]
+    bits = torch.cat([s, z], 1).view(torch.int16)  # [n, 2]
+    assert ((x.amin(1) == 0) & (bits[:, 1] == 0)).any() and (bits[:, 1] == -32768).any()
+    assert torch.equal(par.reshape(n, 4)[:, :2].contiguous().view(torch.int16), bits)
+    assert torch.equal(par.reshape(n, 4)[:, 2:].contiguous().view(torch.int16), bits.flip(0))
+    line = R.decode(cache.units, cache.page_table, 16, 0, n // 2)
+    assert np.array_equal(line["kc"].transpose(1, 0, 2).reshape(n, dim), codes.cpu().numpy())
+    want = (s.float() * (codes.float() - z.float())).half()
+    assert torch.equal(kv.view(n, dim), want) and torch.equal(vv.view(n, dim), want.flip(0))
