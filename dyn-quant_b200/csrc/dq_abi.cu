@@ -420,6 +420,7 @@ dq_status_t dq_kv_append(const dq_kv_cache_t* cache, const uint16_t* k, const in
     const dq_status_t st = check_kv_cache(cache);
     if (st != DQ_OK) return st;
     if (tokens < 0) return DQ_ERR_SHAPE;
+    if (static_cast<long long>(tokens) * cache->kv_heads > (1ll << 26)) return DQ_ERR_UNSUPPORTED;
     if (cache->n_seqs == 0 || tokens == 0) return DQ_OK;
     if (!k || !v || !k_stride || !v_stride || (k_values == nullptr) != (v_values == nullptr))
         return DQ_ERR_INVALID_ARGUMENT;
@@ -433,7 +434,8 @@ dq_status_t dq_kv_append(const dq_kv_cache_t* cache, const uint16_t* k, const in
 
 static dq_status_t check_kv_rows(const dq_kv_cache_t* c, int32_t tokens, int32_t q_heads) {
     if (tokens < 0 || q_heads <= 0 || q_heads % c->kv_heads != 0) return DQ_ERR_SHAPE;
-    if (static_cast<long long>(tokens) * q_heads > (1ll << 26)) return DQ_ERR_UNSUPPORTED;
+    const long long rows = static_cast<long long>(tokens) * q_heads;
+    if (rows > (1ll << 26) || rows * c->n_seqs > (1ll << 32)) return DQ_ERR_UNSUPPORTED;  // (a row is a warp of a join)
     return DQ_OK;
 }
 

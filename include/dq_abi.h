@@ -435,7 +435,7 @@ DQ_API size_t dq_kv_unit_bytes(int32_t head_dim);
  * cache now holds, scale * (code - zero) rounded to f16, zero for i >= counts[b].
  * A start outside the pages leaves the sequence as it is, tokens past its last
  * page are dropped, a page index outside the pool drops its tokens; each sets a
- * bit of the device error word.  One kernel.
+ * bit of the device error word.  tokens * kv_heads <= 2^26.  One kernel.
  */
 DQ_API dq_status_t dq_kv_append(const dq_kv_cache_t* cache, const uint16_t* k, const int64_t k_stride[3],
                                 const uint16_t* v, const int64_t v_stride[3], int32_t tokens,
@@ -450,7 +450,7 @@ typedef struct dq_kv_attend_t {
     int64_t out_stride[3];
     float* lse;             /* [n_seqs][tokens][q_heads] natural log of the softmax's sum, or NULL */
     const int32_t* counts;  /* [n_seqs] query tokens of each sequence, or NULL: all of them */
-    int32_t tokens;
+    int32_t tokens;         /* tokens * q_heads <= 2^26, n_seqs * tokens * q_heads <= 2^32 */
     int32_t q_heads;        /* a multiple of kv_heads; query heads g h .. g h + g - 1 read KV head h */
     float scale;            /* of the scores, e.g. 1 / sqrt(head_dim) */
     int32_t accumulate;     /* != 0: add each slot's weight, summed over query tokens and heads, to mass */
