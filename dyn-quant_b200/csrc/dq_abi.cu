@@ -421,7 +421,13 @@ dq_status_t dq_kv_append(const dq_kv_cache_t* cache, const uint16_t* k, const in
     if (st != DQ_OK) return st;
     if (tokens < 0) return DQ_ERR_SHAPE;
     if (static_cast<long long>(tokens) * cache->kv_heads > (1ll << 26)) return DQ_ERR_UNSUPPORTED;
-    if (cache->n_seqs == 0 || tokens == 0) return DQ_OK;
+    if (cache->n_seqs == 0 || (tokens == 0 && !at)) return DQ_OK;
+    const int64_t none[3] = {0, 0, 0};
+    if (tokens == 0) {  // no rows: the sequences' lengths become at
+        if (!aligned4(counts) || !aligned4(at)) return DQ_ERR_ALIGNMENT;
+        return launch_kv_append(*cache, nullptr, none, nullptr, none, 0, counts, at, nullptr, nullptr,
+                                static_cast<cudaStream_t>(stream));
+    }
     if (!k || !v || !k_stride || !v_stride || (k_values == nullptr) != (v_values == nullptr))
         return DQ_ERR_INVALID_ARGUMENT;
     if (!strides_ok(k_stride) || !strides_ok(v_stride)) return DQ_ERR_ALIGNMENT;

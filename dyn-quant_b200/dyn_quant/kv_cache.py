@@ -55,7 +55,8 @@ class Int4KVCache:
         meta        one int32 buffer behind mass, pos, lengths and evicted.
 
     Pages hold 16-slot units, so new pages need no clearing: nothing behind
-    `lengths` is read into a result.
+    `lengths` is read into a result (append with `at` above a length moves it past
+    slots that then are).
     """
 
     def __init__(self, n_seqs: int, n_pages: int, n_kv_heads: int, head_dim: int = 128, page_size: int = 64,
@@ -130,11 +131,14 @@ class Int4KVCache:
                     n_kv_heads, head_dim] for one token each; slices of a fused
                     projection's output are read in place.
             counts: int32 [n_seqs], new tokens of each sequence (default: T each;
-                    0 leaves a sequence as it is).
+                    0 leaves a sequence as it is, unless `at` moves its end).
             at:     int32 [n_seqs], the slot of each sequence's first new token
-                    (default: its length).  Below the length it rewinds the
-                    sequence, e.g. past rejected draft tokens; not below what an
-                    eviction has rearranged.
+                    (default: its length).  The length becomes at + counts, also
+                    for 0 tokens.  Below the length it rewinds the sequence, e.g.
+                    past rejected draft tokens; not below what an eviction has
+                    rearranged.  Above the length the slots between count as in
+                    use and must hold rows already, e.g. a prefix copied into
+                    `units`, `mass` and `pos`.
             values: return (k, v) as the cache now holds them, float16, zero for
                     padding tokens.
         """

@@ -426,9 +426,11 @@ DQ_API size_t dq_kv_unit_bytes(int32_t head_dim);
  * Quantize new keys and values into the cache: for every sequence b the tokens
  * k[b][i], v[b][i], i < counts[b] (counts NULL: all `tokens`), go to slots
  * at[b] + i (at NULL: lengths[b] + i), mass 0, pos evicted[b] + slot, and
- * lengths[b] becomes at[b] + counts[b].  at below lengths rewinds the sequence
- * (drafted tokens that were rejected); it must not reach below what an eviction
- * has rearranged.  Bytes and scales are those of dq_quantize for rows of 128.
+ * lengths[b] becomes at[b] + counts[b], also with 0 tokens.  at below lengths
+ * rewinds the sequence (drafted tokens that were rejected); it must not reach
+ * below what an eviction has rearranged.  at above lengths takes the slots
+ * between as the caller has left them (a prefix copied in with its mass and
+ * pos); they must hold rows.  Bytes and scales are those of dq_quantize for rows of 128.
  * k, v: f16, 16-byte aligned, head_dim values contiguous, strides (sequence,
  * token, head) in values, multiples of 8.  k_values, v_values: both NULL, or
  * f16 [n_seqs][tokens][kv_heads][head_dim], which receive the values that the

@@ -329,3 +329,23 @@ def test_append_equals_quantize_where_the_minimum_is_a_zero_of_either_sign(dim):
     assert np.array_equal(line["kc"].transpose(1, 0, 2).reshape(n, dim), codes.cpu().numpy())
     want = (s.float() * (codes.float() - z.float())).half()
     assert torch.equal(kv.view(n, dim), want) and torch.equal(vv.view(n, dim), want.flip(0))
+
+
+def test_append_of_no_tokens_moves_the_ends_to_at():
+    """As with some tokens: the length becomes at + counts."""
+    cache = R.make_cache([30, 40, 7], 2, 64, 16)
+    units, mass = cache.units.clone(), cache.mass.clone()
+    k = torch.randn(3, 4, 2, 64).half().cuda()
+    cache.append(k[:, :0], k[:, :0])
+    assert cache.lengths.tolist() == [30, 40, 7]
+    cache.append(k[:, :0], k[:, :0], at=ints(28, 40, 0))
+    assert cache.lengths.tolist() == [28, 40, 0]
+    kv, vv = cache.append(k[:, :0], k[:, :0], counts=ints(0, 0, 0), at=ints(27, 3, 0), values=True)
+    assert cache.lengths.tolist() == [27, 3, 0] and kv.shape == vv.shape == (3, 0, 2, 64)
+    cache.append(k, k, counts=ints(0, 0, 0), at=ints(25, 2, 0))  # the same with tokens, none of them real
+    assert cache.lengths.tolist() == [25, 2, 0]
+    assert torch.equal(cache.units, units) and torch.equal(cache.mass, mass) and not cache._arrivals.any()
+    cache.append(k[:, :0], k[:, :0], at=ints(-1, 2, 10 ** 6))  # outside the pages: left as they are
+    torch.cuda.synchronize()
+    assert _C.read_device_error(True) == 2 << 16
+    assert cache.lengths.tolist() == [25, 2, 0]
