@@ -110,6 +110,8 @@ class Int4KVCache:
             raise RuntimeError(f"{len(pages)} pages for a sequence, at most {self.max_pages}")
         if any(not 0 <= p < self.n_pages for p in pages):
             raise RuntimeError("page index outside the pool")
+        if len(set(pages)) != len(pages):
+            raise RuntimeError("a sequence cannot have a page twice")
         row = torch.full((self.max_pages,), -1, dtype=torch.int32)
         row[:len(pages)] = torch.tensor(pages, dtype=torch.int32)
         self.page_table[seq].copy_(row)

@@ -349,3 +349,19 @@ def test_append_of_no_tokens_moves_the_ends_to_at():
     torch.cuda.synchronize()
     assert _C.read_device_error(True) == 2 << 16
     assert cache.lengths.tolist() == [25, 2, 0]
+
+
+# ---------------------------------------------------------------------------
+# the Python class
+# ---------------------------------------------------------------------------
+def test_assign_refuses_a_page_twice():
+    """Two runs of slots would share its memory."""
+    cache = Int4KVCache(2, 6, 1, 64, 16, max_pages=4)
+    cache.assign(0, [1, 2])
+    for pages in ([3, 3], [0, 4, 5, 0]):
+        with pytest.raises(RuntimeError):
+            cache.assign(0, pages)
+    assert cache.page_table[0].tolist() == [1, 2, -1, -1]
+    cache.assign(1, [1, 3])  # shared by two sequences: a common beginning
+    cache.assign(0, [])
+    assert cache.page_table.tolist() == [[-1] * 4, [1, 3, -1, -1]]
