@@ -183,7 +183,11 @@ class Int4KVCache:
         """(k, v) of one sequence as the cache holds them, float16 [length,
         n_kv_heads, head_dim] each, in slot order (for inspection; synchronises)."""
         n, d, size = int(self.lengths[seq]), self.head_dim, self.page_size
+        if not 0 <= n <= self.max_pages * size:
+            raise RuntimeError(f"sequence {seq} has a length of {n}, outside its pages")
         pages = self.page_table[seq, :-(-n // size)].long()
+        if bool(((pages < 0) | (pages >= self.n_pages)).any()):
+            raise RuntimeError(f"sequence {seq} has slots in a page outside the pool")
         u = self.units[pages].transpose(0, 1).reshape(self.n_kv_heads, -1, unit_bytes(d))
         par = u[..., 16 * d:].contiguous().view(torch.float16).view(self.n_kv_heads, -1, 4).float()
         rows = (u[..., :8 * d].reshape(self.n_kv_heads, -1, d // 2),

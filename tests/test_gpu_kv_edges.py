@@ -365,3 +365,20 @@ def test_assign_refuses_a_page_twice():
     cache.assign(1, [1, 3])  # shared by two sequences: a common beginning
     cache.assign(0, [])
     assert cache.page_table.tolist() == [[-1] * 4, [1, 3, -1, -1]]
+
+
+def test_read_refuses_slots_that_are_not_there():
+    cache = R.make_cache([40, 5], 2, 64, 16)
+    assert cache.read(1)[0].shape == (5, 2, 64)
+    page = int(cache.page_table[0, 1])
+    for bad in (-1, cache.n_pages):
+        cache.page_table[0, 1] = bad
+        with pytest.raises(RuntimeError):
+            cache.read(0)
+    cache.page_table[0, 1] = page
+    for n in (-3, cache.max_pages * 16 + 1):
+        cache.lengths[0] = n
+        with pytest.raises(RuntimeError):
+            cache.read(0)
+    cache.lengths[0] = 0
+    assert cache.read(0)[0].shape == (0, 2, 64)
