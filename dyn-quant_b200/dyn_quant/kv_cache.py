@@ -10,7 +10,8 @@ layers on either side of the attention; dyn_quant.attention.Int4Attention joins
 them.
 
 A decode step issues kernel launches only (lengths live on the device), so it
-can be captured in a CUDA graph; calls on one cache must be stream-ordered.  Pages
+can be captured in a CUDA graph; what does not fit the pages is reported in the
+device error word (Int4KVCache.check); calls on one cache must be stream-ordered.  Pages
 may be shared by sequences with a common beginning, but only to be read: append,
 evict and accumulated weights need pages that one sequence owns.  There are no
 gradients.
@@ -25,6 +26,10 @@ import torch
 import dyn_quant
 
 UNIT_TOKENS = 16  # slots of one unit
+
+# Bits 16 .. 18 (append, evict) and 20 .. 22 (attend) of the device error word
+_ERRORS = ("a page outside the pool", "a length, count or start outside the sequence's pages",
+           "a wait for the kernel's own copies or products gave up")
 
 
 def unit_bytes(head_dim: int) -> int:
@@ -176,8 +181,21 @@ class Int4KVCache:
         slots those with the largest `mass` (equal ones: lowest slot first).
         Kept slots beyond `keep` move into the freed ones below (one kernel, two
         when more than 256 slots of a head may have to move).  A sequence with a
-        page missing is left as it is and reported in the device error word."""
+        page missing is left as it is (see check)."""
         self._h.evict(keep, recent, sink)
+
+    def check(self) -> None:
+        """Raise RuntimeError if a call on this device has reported an error since the last check: slots in a page
+        outside the pool (not written, not read), a length, count or `at` outside a sequence's pages (tokens that do
+        not fit are dropped), a wait that gave up.  The calls themselves only launch kernels and never raise for
+        these.  Synchronises; clears the device error word, which all kernels of the library share."""
+        with torch.cuda.device(self.units.device):
+            torch.cuda.synchronize()
+            word = dyn_quant._C.read_device_error(True)
+        if word:
+            what = [f"{call}: {text}" for shift, call in ((16, "append or evict"), (20, "attend"))
+                    for bit, text in enumerate(_ERRORS) if word >> (shift + bit) & 1]
+            raise RuntimeError(f"device error word {word:#x} ({'; '.join(what) or 'not of a KV cache call'})")
 
     def read(self, seq: int):
         """(k, v) of one sequence as the cache holds them, float16 [length,

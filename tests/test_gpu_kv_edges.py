@@ -382,3 +382,22 @@ def test_read_refuses_slots_that_are_not_there():
             cache.read(0)
     cache.lengths[0] = 0
     assert cache.read(0)[0].shape == (0, 2, 64)
+
+
+def test_check_raises_for_what_the_kernels_reported():
+    cache = R.make_cache([30, 5], 2, 64, 16)
+    cache.check()
+    k = torch.zeros(2, 70, 2, 64, dtype=torch.float16, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        cache.append(k, k)  # tokens beyond the last page are dropped
+    with pytest.raises(RuntimeError, match="append or evict: a length"):
+        cache.check()
+    cache.check()
+    cache.lengths.copy_(ints(30, 5))
+    cache.page_table[0, 0] = -1
+    cache.attend(R.queries(cache, 1, 2))
+    with pytest.raises(RuntimeError, match="attend: a page"):
+        cache.check()
+    cache.check()
