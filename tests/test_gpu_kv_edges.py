@@ -401,3 +401,52 @@ def test_check_raises_for_what_the_kernels_reported():
     with pytest.raises(RuntimeError, match="attend: a page"):
         cache.check()
     cache.check()
+
+
+# ---------------------------------------------------------------------------
+# jobs over many CTAs; pages that are not there
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dim,n,group,t", [
+    (128, 40000, 8, 1),   # one row tile: the last CTA joins
+    (64, 40000, 3, 2),
+    (128, 50000, 8, 2),   # two row tiles, joined by a kernel
+    (64, 10000, 7, 10),   # tensor memory
+    (128, 10000, 6, 8),
+])
+def test_attend_joins_a_job_of_more_than_32_ctas(dim, n, group, t):
+    """One KV head of one sequence: 39 CTAs or more (of the mma.sync kernels 8 or 10 runs of four steps of 32 slots, of
+    the tensor-memory kernel a block of 128), more partial sums than a warp has lanes."""
+    cache = R.make_cache([n], 1, dim, 64, seed=31)
+    q = R.queries(cache, t, group)
+    out, lse = cache.attend(q, return_lse=True)
+    R.check_attend(out, lse, q, cache, dim ** -0.5)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group,t", [(4, 1), (4, 2), (8, 2), (10, 7), (20, 8)])
+def test_weights_where_a_page_is_missing(dim, group, t):
+    """Up to 8 rows (kept scores), 16 (the keys again), one tile of 128 and two: the slots that are there gain the
+    weights of an attention over them alone, nothing else changes."""
+    cache = R.make_cache([150, 90], 2, dim, 16, seed=5, mass=True, spare=2)
+    q = R.queries(cache, t, group)
+    mass0 = cache.mass.clone()
+    pages = cache.page_table.clone()
+    cache.page_table[0, 3] = cache.n_pages + 7
+    cache.page_table[1, 0] = -1
+    out, lse = cache.attend(q, accumulate=True, return_lse=True)
+    torch.cuda.synchronize()
+    assert _C.read_device_error(True) == 1 << 20
+    cache.page_table.copy_(pages)
+    touched = torch.zeros_like(cache.mass, dtype=torch.bool)
+    for b, (n, gone) in enumerate(((150, 3), (90, 0))):
+        keep = [j for j in range(n) if j // 16 != gone]
+        line = {k: v[:, keep] for k, v in R.decode(cache.units, cache.page_table, 16, b, n).items()}
+        r = R.attend(q[b], line, len(keep), dim ** -0.5)
+        assert (np.abs(out[b].double().cpu().numpy() - r["out"]) <= r["tol"]).all()
+        assert (np.abs(lse[b].double().cpu().numpy() - r["lse"]) <= r["lse_tol"]).all()
+        page, off = (x[keep] for x in slots(cache, b, n))
+        z = mass0[page, :, off].double().cpu().numpy().T
+        gain = cache.mass[page, :, off].double().cpu().numpy().T - z
+        assert (np.abs(gain - r["mass"]) <= r["mass_tol"] + 2.0 ** -23 * (z + r["mass"]) + 1e-30).all()
+        touched[page, :, off] = True
+    assert torch.equal(cache.mass[~touched], mass0[~touched])
