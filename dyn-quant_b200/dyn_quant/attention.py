@@ -35,6 +35,11 @@ class Int4Attention(torch.nn.Module):
         self.wo = DynQuantLinear(n_heads * head_dim, d_model, outlier_k)
 
     def load_weights(self, wq: torch.Tensor, wk: torch.Tensor, wv: torch.Tensor, wo: torch.Tensor) -> None:
+        q, kv = self.n_heads * self.head_dim, self.n_kv_heads * self.head_dim
+        for name, w, shape in (("wq", wq, (q, self.d_model)), ("wk", wk, (kv, self.d_model)),
+                               ("wv", wv, (kv, self.d_model)), ("wo", wo, (self.d_model, q))):
+            if tuple(w.shape) != shape:
+                raise RuntimeError(f"{name} must be {list(shape)}, got {list(w.shape)}")
         self.wqkv.load_weight(torch.cat([wq, wk, wv]).contiguous())
         self.wo.load_weight(wo)
 

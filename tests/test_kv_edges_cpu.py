@@ -1,7 +1,11 @@
 """The KV cache's C entry points on a host without a GPU, where sizes are at their edges."""
 import ctypes as C
 
+import pytest
+import torch
+
 from dyn_quant import _lib
+from dyn_quant.attention import Int4Attention
 from test_kv_cpu import S3, append, attend, cache
 
 
@@ -15,3 +19,12 @@ def test_calls_beyond_the_grids_are_refused():
     assert _lib.lib().dq_kv_attend_workspace_bytes(C.byref(many), 1 << 20, 64, 0) == 0
     assert _lib.lib().dq_kv_attend_workspace_bytes(C.byref(many), 1 << 16, 64, 0) > 0
     assert attend(many, tokens=1 << 16, q_heads=64, q_stride=S3(0, 0, 128), ws_bytes=8) == _lib.DQ_ERR_WORKSPACE
+
+
+def test_attention_layer_refuses_projections_of_other_shapes():
+    """Also where the stacked matrix would have the right size: wq and wk exchanged."""
+    layer = Int4Attention(256, 4, 2, 64)
+    wq, wk, wo = torch.zeros(256, 256), torch.zeros(128, 256), torch.zeros(256, 256)
+    for w in ((wk, wq, wk, wo), (wk, wk, wq, wo), (wq, wk, wk[:64], wo), (wq, wk, wk, wo[:128]), (wq[:, :128], wk, wk, wo)):
+        with pytest.raises(RuntimeError, match="must be"):
+            layer.load_weights(*w)
