@@ -458,7 +458,8 @@ dq_status_t dq_kv_attend(const dq_kv_cache_t* cache, const dq_kv_attend_t* r, vo
     if ((st = check_kv_rows(cache, r->tokens, r->q_heads)) != DQ_OK) return st;
     if (cache->n_seqs == 0 || r->tokens == 0) return DQ_OK;
     if (!r->q || !r->out) return DQ_ERR_INVALID_ARGUMENT;
-    if (!(r->scale == r->scale) || r->scale - r->scale != 0.f) return DQ_ERR_INVALID_ARGUMENT;  // NaN, infinity
+    // times log2(e), 2^14 and a key's scale it has to be a number
+    if (!(r->scale <= 1e29f && r->scale >= -1e29f)) return DQ_ERR_INVALID_ARGUMENT;
     if (!strides_ok(r->q_stride) || !strides_ok(r->out_stride)) return DQ_ERR_ALIGNMENT;
     if (!aligned16(r->q) || !aligned16(r->out) || !aligned4(r->lse) || !aligned4(r->counts)) return DQ_ERR_ALIGNMENT;
     if (!workspace || workspace_bytes < kv_attend_workspace(*cache, r->tokens, r->q_heads, r->accumulate != 0))

@@ -454,7 +454,7 @@ typedef struct dq_kv_attend_t {
     const int32_t* counts;  /* [n_seqs] query tokens of each sequence, or NULL: all of them */
     int32_t tokens;         /* tokens * q_heads <= 2^26, n_seqs * tokens * q_heads <= 2^32 */
     int32_t q_heads;        /* a multiple of kv_heads; query heads g h .. g h + g - 1 read KV head h */
-    float scale;            /* of the scores, e.g. 1 / sqrt(head_dim) */
+    float scale;            /* of the scores, e.g. 1 / sqrt(head_dim); at most 1e29 in size */
     int32_t accumulate;     /* != 0: add each slot's weight, summed over query tokens and heads, to mass */
 } dq_kv_attend_t;
 

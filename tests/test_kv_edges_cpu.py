@@ -28,3 +28,13 @@ def test_attention_layer_refuses_projections_of_other_shapes():
     for w in ((wk, wq, wk, wo), (wk, wk, wq, wo), (wq, wk, wk[:64], wo), (wq, wk, wk, wo[:128]), (wq[:, :128], wk, wk, wo)):
         with pytest.raises(RuntimeError, match="must be"):
             layer.load_weights(*w)
+
+
+def test_attend_refuses_scales_whose_products_overflow():
+    """1e29 times log2(e), 2^14 and the largest f16 scale is below the largest FP32 number."""
+    c = cache()
+    assert 1e29 * 1.4427 * 2 ** 14 * 65504 < 3.4e38
+    for scale in (1.01e29, -1e30, 3e38):
+        assert attend(c, scale=scale) == _lib.DQ_ERR_INVALID_ARGUMENT
+    for scale in (1e29, -1e29, 0.0):
+        assert attend(c, scale=scale, ws_bytes=8) == _lib.DQ_ERR_WORKSPACE
