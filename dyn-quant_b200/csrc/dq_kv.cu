@@ -219,14 +219,16 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const KvAppendArgs a, co
 // 16-byte loads.  Slots are ranked by an order-preserving integer of their
 // weight (protected slots first), kept in registers.  The keep-th largest is
 // found by three radix passes of 11, 11 and 10 bits over shared-memory
-// histograms, summed over the cluster through distributed shared memory; ties
+// histograms, summed over the cluster through distributed shared memory (beyond
+// 4096 slots a CTA in several rounds, which read weights and positions again); ties
 // stay in slot order (a scan of the threads' counts).  Survivors keep their slot
 // unless it lies at keep or beyond: the k-th of those moves into the k-th hole
 // below keep.  Sources and holes are disjoint, so the moves need no order among
 // themselves, and a step that drops one slot moves at most one.  Few moves (a
 // step at the cache's bound) are made by the cluster itself, many by a second
-// kernel over the whole GPU.  Bound by the chain of passes (128 heads of 2049
-// slots: 16 us), then by the moves' pieces of 2 to 16 bytes (32 heads of 9000 to
+// kernel over the whole GPU; which it is goes by what a sequence's pages could hold,
+// min(keep, capacity - keep).  Bound by the chain of passes (128 heads of 2049
+// slots: 17 us; one CTA a head, half of its threads with a unit), then by the moves' pieces of 2 to 16 bytes (32 heads of 9000 to
 // 32768 slots cut to 16384: 25 us and 31 us for 43 MB).
 // ---------------------------------------------------------------------------
 constexpr int kEvThreads = 256;

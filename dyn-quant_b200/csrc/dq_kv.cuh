@@ -62,8 +62,8 @@ inline KvView kv_view(const dq_kv_cache_t& c) {
                   c.n_seqs, c.n_pages, c.max_pages, c.kv_heads, Div(c.page_size)};
 }
 
-// Loads from L2 of what earlier kernels or other CTAs wrote.  Unlike the volatile forms of dq_common.cuh the
-// compiler may move them past one another, so a run of them is in flight at once.
+// Loads from L2 of what earlier kernels or other CTAs wrote.  They keep the order of the source: those that are to be
+// in flight at once stand together there, before the first use of any.
 __device__ __forceinline__ int ld_l2(const int* p) { return __ldcg(p); }
 __device__ __forceinline__ uint32_t ld_l2(const uint32_t* p) { return __ldcg(p); }
 __device__ __forceinline__ float ld_l2(const float* p) { return __ldcg(p); }

@@ -44,16 +44,17 @@
 // is taken the other way round, -p' with 15 - c, and the errors cancel (1% of the time).
 // p' is the only rounding to FP16 besides the output's: p <= 2^8 (the maximum
 // is taken again only when a score passes it by 8) and w is the power of two
-// that brings the largest s_v seen to at most 2^7, so p' <= 2^15 and small
-// weights keep their 11 bits down to 2^-29 of the largest.
+// that brings the largest s_v seen to at most 2^7, so p' <= 2^15.  Weights keep their
+// 11 bits down to about 2^-20 of the largest (p' of 2^-14, where that has 2^6 to 2^7;
+// 2^-28 where the maximum lags by its 8), below it they lose one a halving.
 //
 // Measured: 64 sequences of 2000 to 4096 slots with 32 heads of 128 and one row
-// each, 850 MB, 165 to 176 us, 4.8 to 5.1 TB/s (75 to 80% of a copy's; 55% of the
-// issue slots, the tensor pipe 31%); 16 sequences of 1000 to 4100 slots with 8
-// heads of 8 rows, 48 MB, 26 us; 131071 slots with 8 heads of 8 rows, 143 MB, 45
-// us; 8 sequences of 200 to 8000 slots with 8 heads of 64 and 20 rows, 22 MB, 35
+// each, 850 MB, 171 to 183 us, 4.6 to 5.0 TB/s (72 to 77% of a copy's; 59% of the
+// issue slots, the tensor pipe 30%); 16 sequences of 1000 to 4100 slots with 8
+// heads of 8 rows, 48 MB, 26 us; 131071 slots with 8 heads of 8 rows, 143 MB, 47
+// us; 8 sequences of 200 to 8000 slots with 8 heads of 64 and 20 rows, 22 MB, 38
 // us with the join.  The smaller ones are bound by the chain lengths, pages, units,
-// join: 77 slots of 32 heads take 9 us.
+// join: 77 slots of 32 heads take 9.2 us.
 #include "dq_kv_plan.cuh"
 
 namespace dq {
@@ -66,8 +67,8 @@ constexpr int kAtMaxWarps = 2560;     // bound on the grid's warps (workspace si
 constexpr float kCode = 16777216.0f;  // 2^24: a masked low code is c / kCode
 constexpr float kKey = 16384.0f;      // 2^14: a key's code in its product is c / kKey
 
-// Warps of a CTA and CTAs of an SM for row tiles of 8 NT rows: two row tiles
-// need about 200 registers a thread, one tile 128.
+// Warps of a CTA and CTAs of an SM for row tiles of 8 NT rows: with one tile a thread
+// has 128 registers, with two 168, of which heads of 128 spill some 250 bytes.
 __host__ __device__ constexpr int at_warps(int nt) { return nt == 1 ? 8 : 10; }
 __host__ __device__ constexpr int at_ctas(int nt) { return nt == 1 ? 2 : 1; }
 
@@ -882,7 +883,7 @@ __global__ void __launch_bounds__(32 * kCbWarps) kv_combine_kernel(const KvAtten
 // Accumulated weight: mass_j += sum over the rows of exp2(score - lse), from the
 // scores that the pass over the cache has kept: a lane a slot, 32 slots a step, a
 // slot's sum in row order.  16 sequences of 2000 to 4100 slots, 8 heads of 8 rows:
-// 14 us by itself, 41 with the attention.
+// 14 us by itself, 43 with the attention.
 // ---------------------------------------------------------------------------
 constexpr int kSmWarps = 8;
 
@@ -1015,8 +1016,8 @@ dq_status_t score_mass(KvAttendArgs& a, cudaStream_t stream) {
 
 // Query rows of a KV head from which the tensor-memory kernel of dq_kv_chunk.cu takes the call.  It costs about the
 // same for 1 to 128 rows, this file's kernels cost more for every 16.  Here and there, in us, for 1 sequence of 8000
-// slots and 32 KV heads, 4 of 2000 and 8, 16 of 4000 and 8: heads of 128 43, 28, 69 (32 rows), 54, 29, 92 (33) and
-// 54, 23, 96; heads of 64 44, 23, 76 (64 rows), 51, 23, 91 (79) and 48, 21, 85.
+// slots and 32 KV heads, 4 of 2000 and 8, 16 of 4000 and 8: heads of 128 46, 29, 75 (32 rows), 58, 30, 102 (33) and
+// 54, 22, 95; heads of 64 46, 23, 79 (64 rows), 54, 23, 95 (79) and 49, 20, 87.
 constexpr int chunk_min(int head_dim) { return head_dim == 128 ? 33 : 65; }
 
 // Row tiles of one warp: 8 rows when a KV head has no more, else 16.

@@ -668,7 +668,7 @@ __global__ void __launch_bounds__(32 * kCcWarps) kv_chunk_combine_kernel(const K
 // or, where the lines would be too many, to mass by a launch a tile.  The two halves of
 // the softmax warps take the blocks in turn, a slot's 128 rows a thread, and four S
 // tiles keep the MMAs ahead of them: 41 us for the case above where one block at a
-// time, its rows split over two threads, took 51.
+// time, its rows split over two threads, took 55.
 // ---------------------------------------------------------------------------
 template <int D>
 struct CmSmem {

@@ -204,7 +204,7 @@ __device__ __forceinline__ uint32_t pack_f32(float lo, float hi) {
 
 // 1 / sum of a row's weights; 0 where it has seen no key, not a number where the sum is not.
 __device__ __forceinline__ float row_norm(float sum) {
-    return sum > 0.f ? __fdividef(1.f, sum) : (sum == 0.f ? 0.f : sum);  // sum < 2^31
+    return sum > 0.f ? __fdividef(1.f, sum) : (sum == 0.f ? 0.f : sum);  // sum <= 2^38: weights of 2^8, 2^30 slots
 }
 
 // lse of a row, in log2 and natural.

@@ -164,7 +164,8 @@ class Int4KVCache:
             counts:     int32 [n_seqs], query tokens of each sequence (default: T);
                         the rows of the others are zero, their lse -inf.
             accumulate: add each slot's attention weight, summed over query tokens
-                        and the KV head's query heads, to `mass`.
+                        and the KV head's query heads, to `mass` (with scores of
+                        the whole pool, up to 1 GiB, in a temporary buffer).
             out:        tensor to write into, of q's shape, not among q's memory.
             return_lse: also return log(sum(exp(scores))), float32, without head_dim.
 
@@ -179,9 +180,11 @@ class Int4KVCache:
         """Cut every sequence of more than `keep` slots to `keep`, head by head:
         the last `recent` and the first `sink` positions stay, and of the other
         slots those with the largest `mass` (equal ones: lowest slot first).
-        Kept slots beyond `keep` move into the freed ones below (one kernel, two
-        when more than 256 slots of a head may have to move).  A sequence with a
-        page missing is left as it is (see check)."""
+        Kept slots beyond `keep` move into the freed ones below.  One kernel, two
+        when min(keep, capacity - keep) is above 256, with lists that grow with
+        it; the capacity is max_pages * page_size, so a max_pages close to what a
+        sequence needs keeps a step at the cache's bound in one kernel.  A
+        sequence with a page missing is left as it is (see check)."""
         self._h.evict(keep, recent, sink)
 
     def check(self) -> None:

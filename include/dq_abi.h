@@ -468,7 +468,9 @@ DQ_API size_t dq_kv_attend_workspace_bytes(const dq_kv_cache_t* cache, int32_t t
  * 0 .. lengths[b] - counts[b] + i.  out = softmax(scale q K^T) V; scores, the
  * softmax's maximum and sum and the output are FP32, the weights times the V
  * scales are rounded to f16 for the product.  Rows without keys (an empty
- * sequence, i >= counts[b]) give out 0 and lse -infinity.  Units of a page
+ * sequence, i >= counts[b]) give out 0 and lse -infinity; counts outside
+ * 0 .. tokens are taken as the nearest of them.  A value row that is not finite
+ * makes the outputs of the queries that see it not finite, and no others.  Units of a page
  * index outside the pool count as absent and set a bit of the device error
  * word.  Slots behind lengths[b] are not read into any result.  Results are
  * bit-reproducible.  One kernel when a KV head has at most 16 query rows (query
@@ -492,8 +494,10 @@ DQ_API size_t dq_kv_evict_workspace_bytes(const dq_kv_cache_t* cache, int32_t ke
  * position.  evicted[b] grows by what lengths[b] loses; slots from `keep` on are
  * left as they were.  Attention does not depend on the order of slots.  A
  * sequence one of whose slots lies in a page outside the pool is left as it is
- * and sets a bit of the device error word.  One kernel, two where a sequence may
- * lose more than 256 slots at once.
+ * and sets a bit of the device error word.  A mass that is not a number counts as
+ * the largest.  One kernel, two where min(keep, capacity - keep) > 256 (capacity =
+ * max_pages * page_size: the path goes by the page table's size, not the lengths);
+ * none where keep >= capacity.
  */
 DQ_API dq_status_t dq_kv_evict(const dq_kv_cache_t* cache, int32_t keep, int32_t recent, int32_t sink,
                                void* workspace, size_t workspace_bytes, void* stream);
